@@ -3,6 +3,8 @@ pinned ring, the CUDA stream handle, and dtype checks.  PyTorch is used only
 for device memory and streams."""
 from __future__ import annotations
 
+import contextlib
+
 import numpy as np
 import torch
 
@@ -73,3 +75,16 @@ def upload_static(arr: np.ndarray, device) -> torch.Tensor:
     b = np.ascontiguousarray(arr).view(np.uint8).reshape(-1)
     t = torch.from_numpy(b.copy())
     return t.to(device)
+
+
+def raw_stream(device) -> int:
+    """The current stream of `device`, as the C entry points take it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which `device` is the current one (free when it is already)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)

@@ -15,7 +15,7 @@ import numpy as np
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libadvopt.so")
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # ---- constants mirrored from include/advopt.h ----
 DT_F32, DT_BF16 = 0, 1
@@ -156,6 +156,13 @@ class MuonArgs(ctypes.Structure):
     ]
 
 
+# advopt_dropout_spec, advopt_fp8_quant_args, advopt_fp8_gemm_args: packed per
+# call with struct.Struct (fp8.py, dropout.py), which costs a tenth of filling
+# a ctypes structure field by field
+DROPOUT_SPEC_BYTES = 32
+FP8_QUANT_ARGS_BYTES = 152
+FP8_GEMM_ARGS_BYTES = 192
+
 _LIB = None
 _LOCK = threading.Lock()
 
@@ -209,6 +216,10 @@ def lib():
             "advopt_ipc_close": ([P], ctypes.c_int),
             "advopt_enable_peer": ([I32], ctypes.c_int),
             "advopt_copy_async": ([P, P, U64, P], ctypes.c_int),
+            "advopt_dropout": ([P, P, P, ctypes.c_int64, I32, P, P], ctypes.c_int),
+            "advopt_fp8_quantize": ([P, P], ctypes.c_int),
+            "advopt_col_sum": ([P, P, ctypes.c_int64, ctypes.c_int64, I32, P], ctypes.c_int),
+            "advopt_fp8_gemm": ([P, P], ctypes.c_int),
             "advopt_spectral_step": ([ctypes.POINTER(AdamLaunch), P, P, I32, P, I32, P], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
@@ -221,7 +232,8 @@ def lib():
                             (2, ctypes.sizeof(AdamLaunch)), (3, LION_TENSOR_DT.itemsize),
                             (4, ctypes.sizeof(MuonArgs)), (5, ctypes.sizeof(KourkoutasArgs)),
                             (6, PRODIGY_DEV_BYTES), (7, ctypes.sizeof(ProdigyScalarArgs)),
-                            (8, ctypes.sizeof(ProdigyDArgs)), (9, SPECTRAL_TENSOR_DT.itemsize)):
+                            (8, ctypes.sizeof(ProdigyDArgs)), (9, SPECTRAL_TENSOR_DT.itemsize),
+                            (10, DROPOUT_SPEC_BYTES), (11, FP8_QUANT_ARGS_BYTES), (12, FP8_GEMM_ARGS_BYTES)):
             got = L.advopt_sizeof(which)
             if got != size:
                 raise AdvOptError(f"struct layout mismatch (#{which}: C {got} bytes, Python {size})")
@@ -243,7 +255,8 @@ def exported_symbols():
             "advopt_noise_fill", "advopt_ns_chain", "advopt_kourkoutas_prepare", "advopt_kourkoutas_accumulate",
             "advopt_prodigy_scalars", "advopt_prodigy_update_d", "advopt_lr_sketch", "advopt_lr_gemm",
             "advopt_lr_qr_work", "advopt_lr_qr", "advopt_ipc_get_handle", "advopt_ipc_open", "advopt_ipc_close",
-            "advopt_enable_peer", "advopt_copy_async", "advopt_spectral_step"]
+            "advopt_enable_peer", "advopt_copy_async", "advopt_spectral_step", "advopt_dropout",
+            "advopt_fp8_quantize", "advopt_col_sum", "advopt_fp8_gemm"]
 
 
 _OCC_CACHE = {}

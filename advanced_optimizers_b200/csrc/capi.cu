@@ -36,6 +36,9 @@ extern "C" size_t advopt_sizeof(int which) {
     case 7: return sizeof(advopt_prodigy_scalar_args);
     case 8: return sizeof(advopt_prodigy_d_args);
     case 9: return sizeof(advopt_spectral_tensor);
+    case 10: return sizeof(advopt_dropout_spec);
+    case 11: return sizeof(advopt_fp8_quant_args);
+    case 12: return sizeof(advopt_fp8_gemm_args);
     default: return 0;
   }
 }

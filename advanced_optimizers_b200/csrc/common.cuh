@@ -102,7 +102,7 @@ __device__ __forceinline__ U4 philox4x32_10_k(U4 c, const PhiloxKeys& K) {
 }
 
 // Noise streams (counter word y carries the stream id in its top byte).
-enum NoiseStream : uint32_t { kNoiseV = 0, kNoiseM = 1, kNoiseP = 2, kNoiseAux = 3 };
+enum NoiseStream : uint32_t { kNoiseV = 0, kNoiseM = 1, kNoiseP = 2, kNoiseAux = 3, kNoiseDrop = 4 };
 
 // Eight 16-bit uniform integers in [0, 65536) for elements k0 .. k0+7 of a
 // tensor (k0 a multiple of 8), the same values the injected-noise path reads

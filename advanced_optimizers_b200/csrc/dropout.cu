@@ -1,0 +1,69 @@
+// y = residual + keep * x * scale with the mask drawn on the fly (drop.cuh).
+//
+// Bound: HBM.  bf16 with a residual moves 6 bytes per element; the Philox
+// rounds are 2.5 wide multiplies per element.
+#include "advopt.h"
+#include "capi_internal.h"
+#include "common.cuh"
+#include "drop.cuh"
+
+namespace advopt {
+namespace {
+
+template <bool BF16, bool RES>
+__global__ void __launch_bounds__(256)
+    dropout_kernel(void* y, const void* x, const void* res, int64_t n, bool vec, DropSpec d) {
+  const uint32_t step = drop_step(d);
+  const int64_t groups = (n + 7) >> 3;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += stride) {
+    const int64_t k0 = g << 3;
+    const int nv = n - k0 < 8 ? (int)(n - k0) : 8;
+    const bool v = vec && nv == 8;
+    float a[8], r[8];
+    load8<BF16>(x, k0, nv, v, a);
+    if (RES) load8<BF16>(res, k0, nv, v, r);
+    const uint32_t keep = d.threshold ? drop_keep<8>(d, step, (uint64_t)k0) : 0xFFu;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = (keep >> e) & 1u ? __fmul_rn(a[e], d.scale) : 0.0f;
+      a[e] = RES ? __fadd_rn(r[e], t) : t;
+    }
+    if (BF16) {
+      uint32_t u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = f_to_bf16_rne(a[e]);
+      store8_bf16(y, k0, nv, v, u);
+    } else {
+      store8_f32(y, k0, nv, v, a);
+    }
+  }
+}
+
+template <bool BF16>
+void launch(void* y, const void* x, const void* res, int64_t n, const DropSpec& d, cudaStream_t s) {
+  const int64_t groups = (n + 7) >> 3;
+  const int64_t blocks = (groups + 255) / 256;
+  const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
+  const bool vec = ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(res)) & 15) == 0;
+  if (res) dropout_kernel<BF16, true><<<grid, 256, 0, s>>>(y, x, res, n, vec, d);
+  else dropout_kernel<BF16, false><<<grid, 256, 0, s>>>(y, x, res, n, vec, d);
+}
+
+}  // namespace
+}  // namespace advopt
+
+using namespace advopt;
+
+extern "C" int advopt_dropout(void* y, const void* x, const void* residual, int64_t n, int32_t dtype,
+                              const advopt_dropout_spec* spec, void* stream) {
+  if (n < 0 || !spec || (n > 0 && (!x || !y))) return set_error(ADVOPT_E_INVALID, "advopt_dropout: bad arguments");
+  if (dtype != ADVOPT_DT_F32 && dtype != ADVOPT_DT_BF16)
+    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_dropout: float32 and bfloat16 tensors are supported");
+  if (const char* why = drop_check(*spec)) return set_error(ADVOPT_E_INVALID, why);
+  if (n == 0) return ADVOPT_OK;
+  const DropSpec d = drop_spec(*spec);
+  if (dtype == ADVOPT_DT_BF16) launch<true>(y, x, residual, n, d, static_cast<cudaStream_t>(stream));
+  else launch<false>(y, x, residual, n, d, static_cast<cudaStream_t>(stream));
+  return check_cuda(cudaGetLastError(), "advopt_dropout");
+}

@@ -1,0 +1,554 @@
+// Block-scaled 8-bit product for sm_100a:
+//   D = residual + dropout(sum_b 2^(sa + sb) sum_{k in block b} A B^T + bias)
+//
+// Operands are K-major e4m3 / e5m2 with one power-of-two scale (E8M0) for
+// each 128 elements along K; the tensor cores apply the scales themselves
+// (tcgen05.mma kind::mxf8f6f4 with block scales), so the accumulator never
+// leaves tensor memory until the product is done.  The hardware's scale
+// granule is 32 elements: one 32-bit scale word per row holds the scales of
+// four consecutive 128-blocks, and the four K = 32 instructions of a block all
+// name that block's byte, so no scale is replicated in memory.
+//
+// One CTA computes a 128 x BN tile: "rows" come from one operand (the
+// accumulator's 128 lanes), "columns" from the other.  With few tokens the
+// operands trade places (`swap`): the weights fill the 128 lanes and BN
+// shrinks to the tokens.  With few tiles, S CTAs of a cluster split K and add
+// their accumulators through distributed shared memory, in rank order.
+//   * warp 0 (one lane): TMA loads of 128-byte wide K blocks, 128B swizzle;
+//   * warp 1 (one lane): copies scale words to tensor memory (tcgen05.cp) and
+//     issues the MMAs;
+//   * warp 2: gathers the scale words of four blocks at a time;
+//   * warps 4..7: the epilogue.
+// Every wait is bounded and gives up when another role has; the CTA then
+// waits (bounded) for its copies and MMAs in flight, frees its tensor memory
+// and reports through *err.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "advopt.h"
+#include "capi_internal.h"
+#include "common.cuh"
+#include "drop.cuh"
+
+namespace advopt {
+namespace fp8 {
+
+constexpr int BM = 128, BK = 128;
+constexpr int THREADS = 256;
+constexpr int SF_SLOTS = 4;                   // scale words of 4 x 4 blocks in flight
+constexpr int SF_SLOT_BYTES = 512 * 3;        // rows, columns 0..127, columns 128..255
+
+// One operand as the kernel sees it.
+struct Side {
+  const uint8_t* scales;
+  int64_t ld;
+  int64_t extent;     // rows
+  int shift;          // 7: a scale row per 128 rows, 0: per row
+  int code;
+};
+
+struct GemmArgs {
+  Side p, q;          // accumulator lanes / columns
+  void* d;
+  const void* bias;
+  const void* residual;
+  int64_t ldd, ldres, n;
+  int kblocks;
+  int swap;           // D[q][p] instead of D[p][q]
+  int vec;            // rows of D and the residual are 16-byte aligned
+  int drop;
+  int32_t* err;
+};
+
+template <int BN>
+struct Cfg {
+  static constexpr int STAGES = BN >= 256 ? 4 : 6;
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int SF_OFF = STAGES * STAGE_BYTES;
+  static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
+  // scale buffers in tensor memory: buffer b is written only after the MMAs
+  // that read it are known to be done, because the data stage waited for at
+  // that point was itself freed by MMAs of a later group
+  static constexpr int SF_BUFS = STAGES <= 4 ? 2 : 3;
+  static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
+  static constexpr int USED = BN + SF_BUFS * SF_COLS;
+  static constexpr uint32_t TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+};
+
+// Shared-memory matrix descriptor: start, stride between 8-row groups, version 1.
+__device__ __forceinline__ uint64_t desc_of(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint64_t swizzle) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
+         ((uint64_t)1 << 46) | (swizzle << 61);
+}
+
+// Instruction descriptor of kind::mxf8f6f4 with E8M0 scales, K-major operands.
+__device__ __forceinline__ uint32_t instr_desc(int rows, int cols, int a_code, int b_code, uint32_t sf_id) {
+  return (sf_id << 4) | ((uint32_t)a_code << 7) | ((uint32_t)b_code << 10) | ((uint32_t)(cols >> 3) << 17) |
+         (1u << 23) | ((uint32_t)(rows >> 4) << 24) | (sf_id << 29);
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                           uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of 16 bytes -> 4 tensor-memory columns, repeated for the four lane quarters.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded wait that also gives up once another role of the CTA has.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *abort_flag) return false;
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+  return v;
+}
+
+// Scale word (four consecutive K blocks) of row r; rows outside get 1.
+__device__ __forceinline__ uint32_t scale_word(const Side& s, int64_t r, int group) {
+  if (r >= s.extent) return 0x7F7F7F7Fu;
+  return __ldg(reinterpret_cast<const uint32_t*>(s.scales + (r >> s.shift) * s.ld) + group);
+}
+
+// W accumulator values of lane p, columns q0 .. q0 + W - 1, through bias, dropout and residual into D.
+template <bool BF16, int W>
+__device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint32_t step, int64_t p, int64_t q0,
+                                     float (&v)[W]) {
+  if (p >= g.p.extent || q0 >= g.q.extent) return;
+  const int w = g.q.extent - q0 < W ? (int)(g.q.extent - q0) : W;
+  const uint16_t* bias_h = static_cast<const uint16_t*>(g.bias);
+  const float* bias_f = static_cast<const float*>(g.bias);
+  if (g.swap) {
+    const float b = !g.bias ? 0.0f : BF16 ? bf16_to_f(bias_h[p]) : bias_f[p];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if (j >= w) break;
+      float x = __fadd_rn(v[j], b);
+      if (g.drop) x = drop_keep1(d, step, (uint64_t)((q0 + j) * g.n + p)) ? __fmul_rn(x, d.scale) : 0.0f;
+      if (g.residual)
+        x = __fadd_rn(x, BF16 ? bf16_to_f(static_cast<const uint16_t*>(g.residual)[(q0 + j) * g.ldres + p])
+                              : static_cast<const float*>(g.residual)[(q0 + j) * g.ldres + p]);
+      if (BF16) static_cast<uint16_t*>(g.d)[(q0 + j) * g.ldd + p] = (uint16_t)f_to_bf16_rne(x);
+      else static_cast<float*>(g.d)[(q0 + j) * g.ldd + p] = x;
+    }
+    return;
+  }
+  if (g.bias) {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (j < w) v[j] = __fadd_rn(v[j], BF16 ? bf16_to_f(bias_h[q0 + j]) : bias_f[q0 + j]);
+  }
+  if (g.drop) {
+    const uint32_t keep = drop_keep<W>(d, step, (uint64_t)(p * g.n + q0));
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = (keep >> j) & 1u ? __fmul_rn(v[j], d.scale) : 0.0f;
+  }
+#pragma unroll
+  for (int c = 0; c < W; c += 8) {
+    constexpr int STEP = W < 8 ? W : 8;
+    const int left = w - c;
+    if (left <= 0) break;
+    const bool vec = STEP == 8 && g.vec && left >= 8;
+    if (g.residual) {
+      float r[8];
+      load8<BF16>(g.residual, p * g.ldres + q0 + c, left < STEP ? left : STEP, vec, r);
+#pragma unroll
+      for (int e = 0; e < STEP; ++e) v[c + e] = __fadd_rn(v[c + e], r[e]);
+    }
+    if (BF16) {
+      uint32_t u[8];
+#pragma unroll
+      for (int e = 0; e < STEP; ++e) u[e] = f_to_bf16_rne(v[c + e]);
+      store8_bf16(g.d, p * g.ldd + q0 + c, left < STEP ? left : STEP, vec, u);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < STEP; ++e) x[e] = v[c + e];
+      store8_f32(g.d, p * g.ldd + q0 + c, left < STEP ? left : STEP, vec, x);
+    }
+  }
+}
+
+// Tile blockIdx.y (columns) x blockIdx.z... of one cluster of S CTAs along x.
+template <int BN, int S, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, GemmArgs g,
+                DropSpec d) {
+  using C = Cfg<BN>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag, loads_issued;
+  volatile int* abort_v = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const uint32_t rank = S > 1 ? cluster_rank() : 0u;
+  const int64_t tile = blockIdx.x / S;
+  const int64_t p_tiles = (g.p.extent + BM - 1) / BM;
+  const int64_t p0 = (tile % p_tiles) * BM, q0 = (tile / p_tiles) * BN;
+  // this CTA's K blocks: whole groups of four, so that scale words are not split
+  const int groups = (g.kblocks + 3) / 4;
+  const int kb0 = 4 * (int)((int64_t)groups * rank / S);
+  const int kb1 = min(g.kblocks, 4 * (int)((int64_t)groups * (rank + 1) / S));
+  const int nkb = kb1 > kb0 ? kb1 - kb0 : 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < SF_SLOTS; ++s) {
+      mbar_init(&sf_full[s], 32);
+      mbar_init(&sf_empty[s], 1);
+    }
+    mbar_init(&acc_full, 1);
+    abort_flag = 0;
+    loads_issued = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(C::TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_base;
+
+  bool have = false;   // the epilogue warps: the accumulator is ready
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % C::STAGES;
+        if (i >= C::STAGES && !wait_or_abort(&empty[s], (uint32_t)(i / C::STAGES - 1) & 1u, abort_v)) {
+          abort_flag = 1;
+          break;
+        }
+        unsigned char* sp = smem + s * C::STAGE_BYTES;
+        mbar_arrive_tx(&full[s], C::STAGE_BYTES);
+        tma_load_2d(sp, &map_p, (kb0 + i) * BK, (int)p0, &full[s]);
+        tma_load_2d(sp + C::A_BYTES, &map_q, (kb0 + i) * BK, (int)q0, &full[s]);
+        issued = i + 1;
+      }
+      loads_issued = issued;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = 0; i < nkb && ok; ++i) {
+        const int grp = i >> 2, buf = grp % C::SF_BUFS, slot = grp % SF_SLOTS;
+        const uint32_t sfp = tmem + BN + buf * C::SF_COLS, sfq = sfp + 4;
+        const int s = i % C::STAGES;
+        ok = wait_or_abort(&full[s], (uint32_t)(i / C::STAGES) & 1u, abort_v);
+        if (ok && (i & 3) == 0) {
+          ok = wait_or_abort(&sf_full[slot], (uint32_t)(grp / SF_SLOTS) & 1u, abort_v);
+          if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = smem_u32(smem + C::SF_OFF + slot * SF_SLOT_BYTES);
+            copy_scales(sfp, desc_of(src, 0, 128, 0));
+            copy_scales(sfq, desc_of(src + 512, 0, 128, 0));
+            if (BN > 128) copy_scales(sfq + 4, desc_of(src + 1024, 0, 128, 0));
+            mma_commit(&sf_empty[slot]);
+          }
+        }
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t sp = smem_u32(smem + s * C::STAGE_BYTES), sq = sp + C::A_BYTES;
+        const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code, (uint32_t)(i & 3));
+#pragma unroll
+        for (int k = 0; k < BK / 32; ++k)
+          mma_scaled(tmem, desc_of(sp + k * 32, 16, 1024, 2), desc_of(sq + k * 32, 16, 1024, 2), idesc, sfp, sfq,
+                     (i > 0 || k > 0) ? 1u : 0u);
+        mma_commit(&empty[s]);
+      }
+      if (!ok) abort_flag = 1;
+      // also when giving up: the commit tells when everything issued is done
+      mma_commit(&acc_full);
+    }
+  } else if (warp == 2) {
+    bool ok = true;
+    for (int i = 0; i < nkb; i += 4) {
+      const int grp = i >> 2, slot = grp % SF_SLOTS;
+      if (grp >= SF_SLOTS) ok = wait_or_abort(&sf_empty[slot], (uint32_t)(grp / SF_SLOTS - 1) & 1u, abort_v);
+      if (!__all_sync(0xffffffffu, ok)) {
+        abort_flag = 1;
+        break;
+      }
+      const int kg = (kb0 >> 2) + grp;
+      unsigned char* dst = smem + C::SF_OFF + slot * SF_SLOT_BYTES + lane * 16;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = scale_word(g.p, p0 + 32 * e + lane, kg);
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int c = 0; c < (BN + 127) / 128; ++c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = scale_word(g.q, q0 + 128 * c + 32 * e + lane, kg);
+        *reinterpret_cast<uint4*>(dst + 512 * (c + 1)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(&sf_full[slot]);
+    }
+  } else if (warp >= 4) {
+    have = wait_or_abort(&acc_full, 0, abort_v);
+    if (!have) abort_flag = 1;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  }
+
+  const uint32_t step = g.drop ? drop_step(d) : 0u;
+  const int quarter = warp & 3, row = quarter * 32 + lane;
+  const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16);
+  if (S == 1) {
+    if (warp >= 4 && have) {
+      for (int c = 0; c < BN; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c, r);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]);
+        emit<BF16, 16>(g, d, step, p0 + row, q0 + c, v);
+      }
+    }
+  } else {
+    // the ring is drained once the accumulator is complete: [column][row] floats over it
+    float* acc = reinterpret_cast<float*>(smem);
+    if (warp >= 4 && have) {
+      for (int c = 0; c < BN; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c, r);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[(c + e) * BM + row] = nkb ? __uint_as_float(r[e]) : 0.0f;
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 4 && have) {
+      constexpr int PER = BN / S, W = PER < 16 ? PER : 16;
+#pragma unroll 1
+      for (int c = 0; c < PER; c += W) {
+        float v[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const uint32_t at = smem_u32(acc + (rank * PER + c + e) * BM + row);
+          v[e] = peer_float(at, 0);
+#pragma unroll
+          for (int o = 1; o < S; ++o) v[e] = __fadd_rn(v[e], peer_float(at, o));
+        }
+        emit<BF16, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync();   // no CTA leaves while its shared memory is read
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (abort_flag) {
+    // wait (bounded) for the loads and MMAs in flight before memory is given back
+    if (threadIdx.x == 0) {
+      for (int i = loads_issued > C::STAGES ? loads_issued - C::STAGES : 0; i < loads_issued; ++i)
+        mbar_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, 1u << 20);
+      mbar_wait(&acc_full, 0, 1u << 20);
+      if (g.err) *reinterpret_cast<volatile int32_t*>(g.err) = 1;
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+  }
+}
+
+// ---- host ----
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+int encode_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  if (!g_encode) return set_error(ADVOPT_E_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  if (g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: cuTensorMapEncodeTiled rejected an operand");
+  return ADVOPT_OK;
+}
+
+struct Launch {
+  const void *p, *q;
+  int64_t ldp, ldq, k;
+  GemmArgs g;
+  DropSpec d;
+  cudaStream_t stream;
+};
+
+template <int BN, int S, bool BF16>
+int launch_t(const Launch& L) {
+  using C = Cfg<BN>;
+  CUtensorMap mp, mq;
+  int rc = encode_map(&mp, L.p, L.g.p.extent, L.k, L.ldp, BM);
+  if (rc == ADVOPT_OK) rc = encode_map(&mq, L.q, L.g.q.extent, L.k, L.ldq, BN);
+  if (rc != ADVOPT_OK) return rc;
+  const auto kernel = gemm_kernel<BN, S, BF16>;
+  // per call, not once: the attribute belongs to the current device
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
+  const int64_t tiles = ((L.g.p.extent + BM - 1) / BM) * ((L.g.q.extent + BN - 1) / BN);
+  if (tiles * S > 0x7fffffff) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * S));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = L.stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = S;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, L.g, L.d);
+  return check_cuda(e, "advopt_fp8_gemm");
+}
+
+template <int BN, bool BF16>
+int launch_s(const Launch& L, int split) {
+  switch (split) {
+    case 8: return launch_t<BN, 8, BF16>(L);
+    case 4: return launch_t<BN, 4, BF16>(L);
+    case 2: return launch_t<BN, 2, BF16>(L);
+    default: return launch_t<BN, 1, BF16>(L);
+  }
+}
+
+template <bool BF16>
+int launch_n(const Launch& L, int bn, int split) {
+  switch (bn) {
+    case 32: return launch_s<32, BF16>(L, split);
+    case 64: return launch_s<64, BF16>(L, split);
+    case 128: return launch_s<128, BF16>(L, split);
+    default: return launch_s<256, BF16>(L, split);
+  }
+}
+
+}  // namespace fp8
+}  // namespace advopt
+
+using namespace advopt;
+
+extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
+  if (!a || a->m < 0 || a->n < 0 || a->k <= 0) return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: bad shape");
+  if (a->d_dtype != ADVOPT_DT_F32 && a->d_dtype != ADVOPT_DT_BF16)
+    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: float32 and bfloat16 outputs are supported");
+  if ((a->a_code & ~1) || (a->b_code & ~1)) return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: unknown code type");
+  if (const char* why = drop_check(a->drop)) return set_error(ADVOPT_E_INVALID, why);
+  if (a->m == 0 || a->n == 0) return ADVOPT_OK;
+  if (!a->a || !a->b || !a->sa || !a->sb || !a->d) return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: null operand");
+  if ((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b)) % 16 || a->lda % 16 || a->ldb % 16 ||
+      a->lda < a->k || a->ldb < a->k)
+    return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: operands must be 16-byte aligned with pitches of whole 16 bytes");
+  const int64_t nb = (a->k + 127) / 128;
+  if ((reinterpret_cast<uintptr_t>(a->sa) | reinterpret_cast<uintptr_t>(a->sb)) % 4 || a->ldsa % 4 || a->ldsb % 4 ||
+      a->ldsa < nb || a->ldsb < nb)
+    return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: scales must be 4-byte aligned with pitches of whole 4 bytes");
+  if (a->ldd < a->n || (a->residual && a->ldres < a->n))
+    return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: a row pitch is smaller than a row");
+  const int64_t top = 0x7fffff00;
+  if (a->m > top || a->n > top || a->k > top) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: extents are at most 2^31 - 256");
+
+  fp8::Launch L;
+  const fp8::Side A{a->sa, a->ldsa, a->m, a->a_tile ? 7 : 0, a->a_code};
+  const fp8::Side B{a->sb, a->ldsb, a->n, a->b_tile ? 7 : 0, a->b_code};
+  const bool swap = a->m <= 128 && a->n > a->m;
+  fp8::GemmArgs& g = L.g;
+  g.p = swap ? B : A;
+  g.q = swap ? A : B;
+  L.p = swap ? a->b : a->a;
+  L.q = swap ? a->a : a->b;
+  L.ldp = swap ? a->ldb : a->lda;
+  L.ldq = swap ? a->lda : a->ldb;
+  L.k = a->k;
+  g.d = a->d;
+  g.bias = a->bias;
+  g.residual = a->residual;
+  g.ldd = a->ldd;
+  g.ldres = a->ldres;
+  g.n = a->n;
+  g.kblocks = (int)nb;
+  g.swap = swap;
+  const int64_t es = a->d_dtype == ADVOPT_DT_BF16 ? 2 : 4;
+  g.vec = reinterpret_cast<uintptr_t>(a->d) % 16 == 0 && a->ldd * es % 16 == 0 &&
+          (!a->residual || (reinterpret_cast<uintptr_t>(a->residual) % 16 == 0 && a->ldres * es % 16 == 0));
+  g.drop = a->drop.threshold > 0;
+  g.err = a->err;
+  L.d = drop_spec(a->drop);
+  L.stream = static_cast<cudaStream_t>(stream);
+  const int64_t q = g.q.extent;
+  const int bn = q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256;
+  const int64_t tiles = ((g.p.extent + 127) / 128) * ((q + bn - 1) / bn);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= 148 && nb >= 8 * split) split *= 2;
+  return a->d_dtype == ADVOPT_DT_BF16 ? fp8::launch_n<true>(L, bn, split) : fp8::launch_n<false>(L, bn, split);
+}

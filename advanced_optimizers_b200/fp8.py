@@ -1,0 +1,312 @@
+"""Matrix products in 8-bit floating point with a scale for each block of 128.
+
+A block is 1 x 128 along the contraction (activations, gradients) or
+128 x 128 (weights); its scale is a power of two, so quantising rounds each
+value once, a 128 x 128 block may be read in both directions, and the tensor
+cores apply the scales themselves.  `quantize_fp8` makes the operands,
+`fp8_matmul` multiplies them, `fp8_linear` is a training layer of both with
+its gradients, optional bias, residual and dropout.
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib as L
+from ._device import dtype_code, on_device, raw_stream
+from .dropout import NO_DROP, drop_fields
+
+_CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+_E8M0 = torch.float8_e8m0fnu
+
+# advopt_fp8_quant_args, advopt_fp8_gemm_args (each ends in an advopt_dropout_spec)
+_QUANT = struct.Struct("<QqqqQqQqQqQqQiiiiQQIIIf")
+_GEMM = struct.Struct("<QqQqQqQqQqQQqqqqiiiiiiQQQIIIf")
+
+
+class _ErrorWord:
+    """The word that a kernel's bounded wait sets when it gives up: pinned host
+    memory that the kernels write directly, so that every call can look at it
+    without waiting for the GPU."""
+
+    def __init__(self):
+        self.word = None
+
+    def pointer(self) -> int:
+        if self.word is None:
+            if torch.cuda.is_current_stream_capturing():
+                return 0   # no allocation of pinned memory during a capture
+            self.word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            self.view = self.word.numpy()
+        elif self.view[0]:
+            self.raise_()
+        return self.word.data_ptr()
+
+    def raise_(self):
+        self.view[0] = 0
+        raise L.AdvOptError("an earlier fp8 product gave up waiting for its copies (bounded wait); its result is not valid")
+
+
+_ERR = _ErrorWord()
+
+
+def check_fp8_errors():
+    """Waits for the GPU and raises if an fp8 product's bounded wait gave up
+    (a guard that is not expected to fire; otherwise the next call raises)."""
+    torch.cuda.synchronize()
+    if _ERR.word is not None and _ERR.view[0]:
+        _ERR.raise_()
+
+
+def _round_up(n, to):
+    return (n + to - 1) // to * to
+
+
+def _empty_codes(rows, k, dtype, device):
+    t = torch.empty((rows, _round_up(k, 16)), dtype=dtype, device=device)
+    return t if t.shape[1] == k else t[:, :k]
+
+
+def _empty_scales(rows, nb, device):
+    t = torch.empty((rows, _round_up(nb, 4)), dtype=_E8M0, device=device)
+    return t if t.shape[1] == nb else t[:, :nb]
+
+
+class Fp8Blocks:
+    """A matrix [rows][k] quantised along k.
+
+    codes   [rows][k], torch.float8_e4m3fn or torch.float8_e5m2
+    scales  torch.float8_e8m0fnu, [rows][ceil(k / 128)] (1 x 128 blocks) or
+            [ceil(rows / 128)][ceil(k / 128)] (128 x 128 blocks)
+
+    Element (i, j) stands for codes[i, j] * scales[i or i // 128, j // 128].
+    Codes whose rows do not start at whole 16 bytes, and scales whose rows do
+    not hold whole 4 bytes, are copied once into such a layout here."""
+
+    __slots__ = ("codes", "scales", "rows", "k", "square", "ld", "lds")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype not in _CODE or scales.dtype != _E8M0:
+            raise NotImplementedError("Fp8Blocks: codes are float8_e4m3fn or float8_e5m2, scales float8_e8m0fnu "
+                                      f"(got {codes.dtype}, {scales.dtype})")
+        if not codes.is_cuda or scales.device != codes.device:
+            raise NotImplementedError("Fp8Blocks: codes and scales must live on one CUDA device (no CPU fallback)")
+        if codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError("Fp8Blocks: codes and scales are matrices")
+        rows, k = codes.shape
+        nb = (k + 127) // 128
+        if tuple(scales.shape) == (rows, nb):
+            square = False
+        elif tuple(scales.shape) == ((rows + 127) // 128, nb):
+            square = True
+        else:
+            raise ValueError(f"Fp8Blocks: codes {rows} x {k} need scales {rows} x {nb} or {(rows + 127) // 128} x {nb}, "
+                             f"got {tuple(scales.shape)}")
+        if rows and k:
+            ld = codes.stride(0) if rows > 1 else _round_up(k, 16)
+            if codes.data_ptr() % 16 or ld % 16 or ld < k or (k > 1 and codes.stride(1) != 1):
+                own = _empty_codes(rows, k, codes.dtype, codes.device)
+                own.view(torch.uint8).copy_(codes.view(torch.uint8))
+                codes, ld = own, _round_up(k, 16)
+            lds = scales.stride(0) if scales.shape[0] > 1 else _round_up(nb, 4)
+            if scales.data_ptr() % 4 or lds % 4 or lds < nb or (nb > 1 and scales.stride(1) != 1) or (
+                    nb % 4 and scales.untyped_storage().nbytes() <
+                    scales.storage_offset() + (scales.shape[0] - 1) * lds + _round_up(nb, 4)):
+                own = _empty_scales(scales.shape[0], nb, scales.device)
+                own.view(torch.uint8).copy_(scales.view(torch.uint8))
+                scales, lds = own, _round_up(nb, 4)
+            self.ld, self.lds = ld, lds
+        else:
+            self.ld, self.lds = _round_up(k, 16), _round_up(nb, 4)
+        self.codes, self.scales, self.rows, self.k, self.square = codes, scales, rows, k, square
+
+    @property
+    def block(self):
+        return (128, 128) if self.square else (1, 128)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _blocks(codes, scales, rows, k, square, ld, lds):
+    """An Fp8Blocks of tensors this module laid out itself."""
+    b = object.__new__(Fp8Blocks)
+    b.codes, b.scales, b.rows, b.k, b.square, b.ld, b.lds = codes, scales, rows, k, square, ld, lds
+    return b
+
+
+def _quantize(x, square, dtype, rows, cols, sums=False, drop=NO_DROP):
+    """(blocks of x or None, blocks of x^T or None, column sums of 128-row slabs or None)."""
+    R, C = x.shape
+    dev = x.device
+    if C > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < C:
+        x = x.contiguous()
+    ldx = x.stride(0) if R > 1 else C
+    nr, nc = (R + 127) // 128, (C + 127) // 128
+    br = bc = partial = None
+    args_r = args_c = (0, 0, 0, 0)
+    if rows:
+        br = _blocks(_empty_codes(R, C, dtype, dev), _empty_scales(nr if square else R, nc, dev), R, C, square,
+                     _round_up(C, 16), _round_up(nc, 4))
+        args_r = (br.codes.data_ptr(), br.ld, br.scales.data_ptr(), br.lds)
+    if cols:
+        bc = _blocks(_empty_codes(C, R, dtype, dev), _empty_scales(nc if square else C, nr, dev), C, R, square,
+                     _round_up(R, 16), _round_up(nr, 4))
+        args_c = (bc.codes.data_ptr(), bc.ld, bc.scales.data_ptr(), bc.lds)
+    if sums:
+        partial = torch.empty((nr, C), dtype=torch.float32, device=dev)
+    with on_device(dev):
+        L.check(L.lib().advopt_fp8_quantize(
+            _QUANT.pack(x.data_ptr(), ldx, R, C, *args_r, *args_c, partial.data_ptr() if sums else 0,
+                        dtype_code(x.dtype), 1 if square else 0, _CODE[dtype], 0, *drop), raw_stream(dev)),
+            "advopt_fp8_quantize")
+    return br, bc, partial
+
+
+def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.float8_e4m3fn, layout: str = "rows"):
+    """Quantises a matrix [R][C] (float32 or bfloat16, rows of any pitch).
+
+    For each block the scale is the least power of two that brings the largest
+    finite magnitude into the type's range (1 for a block of zeros, never below
+    2^-127), and a code is the nearest value of the type, ties to even.
+    Infinities and NaN become NaN codes and do not enter a scale.
+
+    layout  "rows": Fp8Blocks of x, quantised along its columns' index
+            "cols": Fp8Blocks of x^T [C][R], quantised along the rows' index
+            "both": the pair, from one pass over x
+    block   (1, 128), or (128, 128): then both layouts hold the same codes"""
+    if block not in ((1, 128), (128, 128)):
+        raise NotImplementedError(f"quantize_fp8: blocks of (1, 128) and (128, 128) are supported, got {block}")
+    if dtype not in _CODE:
+        raise NotImplementedError(f"quantize_fp8: codes are float8_e4m3fn or float8_e5m2, got {dtype}")
+    if layout not in ("rows", "cols", "both"):
+        raise ValueError(f"quantize_fp8: layout is 'rows', 'cols' or 'both', got {layout!r}")
+    if x.dim() != 2:
+        raise ValueError("quantize_fp8 takes a matrix")
+    if not x.is_cuda:
+        raise NotImplementedError("quantize_fp8: tensors must live on a CUDA device (no CPU fallback)")
+    dtype_code(x.dtype)
+    r, c, _ = _quantize(x.detach(), block[0] == 128, dtype, layout != "cols", layout != "rows")
+    return (r, c) if layout == "both" else r if layout == "rows" else c
+
+
+def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP):
+    m, n = out.shape
+    dev = out.device
+    with on_device(dev):
+        L.check(L.lib().advopt_fp8_gemm(
+            _GEMM.pack(a.codes.data_ptr(), a.ld, a.scales.data_ptr(), a.lds,
+                       b.codes.data_ptr(), b.ld, b.scales.data_ptr(), b.lds, out.data_ptr(), n,
+                       0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n,
+                       m, n, a.k, _CODE[a.codes.dtype], _CODE[b.codes.dtype], a.square, b.square,
+                       dtype_code(out.dtype), 0, _ERR.pointer(), *drop), raw_stream(dev)),
+            "advopt_fp8_gemm")
+    return out
+
+
+def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a @ b^T [a.rows][b.rows]: products of the values that the codes and
+    scales stand for, summed in float32 and rounded once to `out_dtype`
+    (bfloat16 or float32).  The operands may differ in code type and block
+    shape.  Its gradients are products of the same kind (see `fp8_linear`)."""
+    if a.k != b.k:
+        raise ValueError(f"fp8_matmul: the operands are quantised along {a.k} and {b.k} elements")
+    if a.codes.device != b.codes.device:
+        raise ValueError(f"fp8_matmul: operands on {a.device} and {b.device}")
+    dtype_code(out_dtype)
+    if a.k == 0:
+        return torch.zeros((a.rows, b.rows), dtype=out_dtype, device=a.device)
+    return _gemm(a, b, torch.empty((a.rows, b.rows), dtype=out_dtype, device=a.codes.device))
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, w_rows, w_cols, step_tensor, drop):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        e4m3 = torch.float8_e4m3fn
+        xr, xc, _ = _quantize(x, False, e4m3, True, need_w)
+        if w_rows is None:
+            w_rows, w_cols, _ = _quantize(weight, True, e4m3, True, need_x)
+        y = torch.empty((x.shape[0], weight.shape[0]), dtype=x.dtype, device=x.device)
+        _gemm(xr, w_rows, y, bias, residual, drop)
+        ctx.drop, ctx.w_dtype, ctx.x_dtype = drop, weight.dtype, x.dtype
+        ctx.xc, ctx.wc = xc if need_w else None, w_cols if need_x else None
+        ctx.save_for_backward(*(() if step_tensor is None else (step_tensor,)))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        _ = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        dev = dy.device
+        T, N = dy.shape
+        if need_x or need_w or need_b:
+            # g = mask * dy / q once, for every gradient that reads it
+            gr, gc, sums = _quantize(dy, False, torch.float8_e4m3fn, need_x or not need_w, need_w, need_b, ctx.drop)
+            if need_x:
+                dx = torch.empty((T, ctx.wc.rows), dtype=ctx.x_dtype, device=dev)
+                _gemm(gr, ctx.wc, dx)
+            if need_w:
+                dw = torch.empty((N, ctx.xc.rows), dtype=ctx.w_dtype, device=dev)
+                _gemm(gc, ctx.xc, dw)
+            if need_b:
+                db = torch.empty((N,), dtype=dy.dtype, device=dev)
+                with on_device(dev):
+                    L.check(L.lib().advopt_col_sum(db.data_ptr(), sums.data_ptr(), sums.shape[0], N,
+                                                   dtype_code(db.dtype), raw_stream(dev)), "advopt_col_sum")
+        return dx, dw, db, (dy if need_r else None), None, None, None, None
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+               residual: torch.Tensor | None = None, dropout_p: float = 0.0, seed: int = 42, site: int = 0, step=0,
+               weight_blocks=None) -> torch.Tensor:
+    """y = residual + dropout(x @ weight^T + bias), the products in block-scaled
+    e4m3 with float32 accumulation, bias, dropout and residual in the product's
+    epilogue (float32, one rounding to x's dtype).
+
+    x [..., K] and weight [N][K] are quantised in the call: x in 1 x 128
+    blocks, the weight in 128 x 128 ones.  Gradients: with g = dropout's mask and
+    scale applied to dy (the mask of `philox_dropout` with these `seed`,
+    `site`, `step`, over y's elements; it is drawn again, never stored),
+      dx = Q(g) Q(weight),  dweight = Q(g^T) Q(x^T)^T,  dbias = sum of g,
+      dresidual = dy,
+    where Q quantises along the contraction (g in 1 x 128 blocks of its rows
+    for dx, of its columns for dweight; x in blocks of its columns).  What is
+    kept for the backward pass is x's and the weight's transposed codes, one
+    byte per element, not x.
+
+    x, bias and residual share a dtype (float32 or bfloat16), the weight may
+    have the other one; dweight has the weight's.  `weight_blocks` takes
+    quantize_fp8(weight, (128, 128), layout="both") made before, for weights
+    that do not change between calls (accumulation, evaluation)."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"fp8_linear: x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    for t in (x, weight, bias, residual):
+        if t is not None and (not t.is_cuda or t.device != x.device):
+            raise NotImplementedError("fp8_linear: tensors must live on one CUDA device (no CPU fallback)")
+    dtype_code(x.dtype), dtype_code(weight.dtype)
+    N, K = weight.shape
+    if bias is not None and (bias.shape != (N,) or bias.dtype != x.dtype):
+        raise ValueError(f"fp8_linear: bias must be [{N}] in x's dtype")
+    if residual is not None and (residual.shape != (*x.shape[:-1], N) or residual.dtype != x.dtype):
+        raise ValueError("fp8_linear: the residual must have the result's shape and dtype")
+    if N == 0 or K == 0:
+        raise ValueError("fp8_linear: the weight is empty")
+    drop = drop_fields(dropout_p, seed, site, step, x.device)
+    w_rows = w_cols = None
+    if weight_blocks is not None:
+        w_rows, w_cols = weight_blocks
+        if not (w_rows.square and w_cols.square and (w_rows.rows, w_rows.k) == (N, K) == (w_cols.k, w_cols.rows)
+                and w_rows.device == x.device == w_cols.device):
+            raise ValueError("fp8_linear: weight_blocks is quantize_fp8(weight, (128, 128), layout='both')")
+    if x.numel() == 0:   # no tokens: no products, and gradients of zeros
+        y = x.new_zeros((*x.shape[:-1], N)) if residual is None else residual.clone()
+        return y + 0.0 * (x.sum() + weight.sum(dtype=x.dtype) + (0.0 if bias is None else bias.sum()))
+    y = _Fp8Linear.apply(x.reshape(-1, K), weight, None if bias is None else bias.contiguous(),
+                         None if residual is None else residual.reshape(-1, N).contiguous(), w_rows, w_cols,
+                         step if isinstance(step, torch.Tensor) else None, drop)
+    return y.view(*x.shape[:-1], N)

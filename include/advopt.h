@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define ADVOPT_ABI_VERSION 5
+#define ADVOPT_ABI_VERSION 6
 
 /* ---- error codes ---- */
 #define ADVOPT_OK 0
@@ -573,8 +573,106 @@ int advopt_ns_chain(void* x, void* c, void* a, void* b, int32_t m_pad, int32_t n
                     double coef_a, double coef_b, double coef_c, double cns_lower_bound, void** final_x,
                     int32_t* err, void* stream);
 
+/* ---- Counter-based dropout ----
+ * y_k = residual_k + (keep_k ? x_k * scale : 0) in float32, rounded once.
+ * keep_k = (r_k >= threshold), r_k the 16-bit value advopt_noise_fill gives
+ * element k for (seed, tensor_id = site, step, stream 4): the mask is a pure
+ * function of these and is stored nowhere.  scale is 65536 / (65536 -
+ * threshold), the inverse of the probability that is really drawn.  The
+ * gradient is the same call on dy without a residual. */
+typedef struct advopt_dropout_spec {
+  uint64_t seed;
+  const int64_t* step_dev;  /* not NULL: the step is read on the device       */
+  uint32_t site;
+  uint32_t step;
+  uint32_t threshold;       /* 0 .. 65536; 0: nothing is dropped              */
+  float scale;
+} advopt_dropout_spec;
+
+/* x, y, residual (may be NULL): n contiguous elements of `dtype` (ADVOPT_DT_*);
+ * y may be x or residual. */
+int advopt_dropout(void* y, const void* x, const void* residual, int64_t n, int32_t dtype,
+                   const advopt_dropout_spec* spec, void* stream);
+
+/* ---- 8-bit floating point with a scale for each block of 128 ----
+ * A block is 1 x 128 (along the contraction) or 128 x 128; its scale is a
+ * power of two, stored as its biased exponent (E8M0: byte b is 2^(b - 127)). */
+#define ADVOPT_FP8_E4M3 0
+#define ADVOPT_FP8_E5M2 1
+
+/* Quantises x [rows][cols] (row pitch ldx, elements): with a the largest
+ * finite magnitude of a block, the scale is the least power of two (not below
+ * 2^-127; 1 when a = 0) with a <= fmax * scale (fmax 448 for E4M3, 57344 for
+ * E5M2), the code x / scale rounded to nearest even; an infinity or NaN
+ * becomes NaN.  Either or both layouts (NULL codes: not written):
+ *   codes_r [rows][cols], scales_r [rows or ceil(rows/128)][ceil(cols/128)]
+ *   codes_c [cols][rows], scales_c [cols or ceil(cols/128)][ceil(rows/128)]: x^T in blocks
+ * With drop.threshold > 0, x is dropped out first (element index row * cols +
+ * col; the product stays in float32).  col_partial (or NULL) receives the
+ * float32 column sums of each 128-row slab of what was quantised,
+ * [ceil(rows/128)][cols], for advopt_col_sum. */
+typedef struct advopt_fp8_quant_args {
+  const void* x;
+  int64_t ldx;
+  int64_t rows;
+  int64_t cols;
+  uint8_t* codes_r;
+  int64_t ld_r;             /* bytes, a multiple of 16; codes 16-byte aligned  */
+  uint8_t* scales_r;
+  int64_t ld_sr;            /* bytes                                           */
+  uint8_t* codes_c;
+  int64_t ld_c;
+  uint8_t* scales_c;
+  int64_t ld_sc;
+  float* col_partial;
+  int32_t x_dtype;          /* ADVOPT_DT_*                                     */
+  int32_t tile;             /* 0: 1 x 128 blocks, 1: 128 x 128                 */
+  int32_t code;             /* ADVOPT_FP8_*                                    */
+  int32_t pad;
+  advopt_dropout_spec drop;
+} advopt_fp8_quant_args;
+int advopt_fp8_quantize(const advopt_fp8_quant_args* args, void* stream);
+
+/* out[c] = sum over `parts` rows of partial [parts][cols], in row order, in
+ * float32, rounded once to `dtype`. */
+int advopt_col_sum(void* out, const float* partial, int64_t parts, int64_t cols, int32_t dtype, void* stream);
+
+/* D [m][n] = residual + dropout(sum_b 2^(sa[i,b] + sb[j,b] - 254) sum_{k in b} A[i,k] B[j,k] + bias):
+ * both operands K-major, float32 accumulation, one rounding to d_dtype.
+ * lda, ldb: bytes, multiples of 16, operands 16-byte aligned; ldsa, ldsb:
+ * bytes, multiples of 4, scales 4-byte aligned, every row's pitch readable.
+ * bias [n], residual [m][ldres] in d_dtype, or NULL. */
+typedef struct advopt_fp8_gemm_args {
+  const uint8_t* a;
+  int64_t lda;
+  const uint8_t* sa;
+  int64_t ldsa;
+  const uint8_t* b;
+  int64_t ldb;
+  const uint8_t* sb;
+  int64_t ldsb;
+  void* d;
+  int64_t ldd;              /* elements                                        */
+  const void* bias;
+  const void* residual;
+  int64_t ldres;            /* elements                                        */
+  int64_t m;
+  int64_t n;
+  int64_t k;
+  int32_t a_code;           /* ADVOPT_FP8_*                                    */
+  int32_t b_code;
+  int32_t a_tile;           /* 0: a scale row per row, 1: per 128 rows         */
+  int32_t b_tile;
+  int32_t d_dtype;          /* ADVOPT_DT_*                                     */
+  int32_t pad;
+  int32_t* err;             /* set to 1 if a bounded wait gave up (or NULL)    */
+  advopt_dropout_spec drop;
+} advopt_fp8_gemm_args;
+int advopt_fp8_gemm(const advopt_fp8_gemm_args* args, void* stream);
+
 /* Layout checks for bindings: sizeof of each struct. */
-size_t advopt_sizeof(int which); /* 0 adam_tensor, 1 piece, 2 adam_launch, 3 lion_tensor, 4 muon_args */
+size_t advopt_sizeof(int which); /* 0 adam_tensor, 1 piece, 2 adam_launch, 3 lion_tensor, 4 muon_args, ...,
+                                    10 dropout_spec, 11 fp8_quant_args, 12 fp8_gemm_args */
 int advopt_abi_version(void);
 /* Last error message of the calling thread ("" if none). */
 const char* advopt_last_error(void);
