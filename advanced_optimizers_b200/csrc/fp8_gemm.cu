@@ -25,6 +25,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <cstdlib>
 #include <mutex>
 
 #include "advopt.h"
@@ -37,6 +38,7 @@ namespace fp8 {
 
 constexpr int BM = 128, BK = 128;
 constexpr int THREADS = 256;
+constexpr int SMS = 148, PAIRS = SMS / 2;
 constexpr int SF_SLOTS = 4;                   // scale words of 4 x 4 blocks in flight
 constexpr int SF_SLOT_BYTES = 512 * 3;        // rows, columns 0..127, columns 128..255
 
@@ -69,26 +71,19 @@ struct Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int SF_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
-  // scale buffers in tensor memory: buffer b is written only after the MMAs
-  // that read it are known to be done, because the data stage waited for at
-  // that point was itself freed by MMAs of a later group
-  static constexpr int SF_BUFS = STAGES <= 4 ? 2 : 3;
+  static constexpr int SF_BUFS = 2;   // scale buffers in tensor memory
   static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
   static constexpr int USED = BN + SF_BUFS * SF_COLS;
   static constexpr uint32_t TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
 };
 
-// Shared-memory matrix descriptor: start, stride between 8-row groups, version 1.
-__device__ __forceinline__ uint64_t desc_of(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint64_t swizzle) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
-         ((uint64_t)1 << 46) | (swizzle << 61);
-}
-
 // Instruction descriptor of kind::mxf8f6f4 with E8M0 scales, K-major operands.
-__device__ __forceinline__ uint32_t instr_desc(int rows, int cols, int a_code, int b_code, uint32_t sf_id) {
-  return (sf_id << 4) | ((uint32_t)a_code << 7) | ((uint32_t)b_code << 10) | ((uint32_t)(cols >> 3) << 17) |
-         (1u << 23) | ((uint32_t)(rows >> 4) << 24) | (sf_id << 29);
+__device__ __forceinline__ uint32_t instr_desc(int rows, int cols, int a_code, int b_code) {
+  return ((uint32_t)a_code << 7) | ((uint32_t)b_code << 10) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) |
+         ((uint32_t)(rows >> 4) << 24);
 }
+// ... and which byte of the scale words it takes, for both operands.
+__device__ __forceinline__ constexpr uint32_t sf_id(uint32_t j) { return (j << 4) | (j << 29); }
 
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -129,14 +124,43 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Bounded wait that also gives up once another role of the CTA has.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// Bounded wait of a whole warp that also gives up once another role has; all
+// lanes get the same answer, so that they stay together afterwards.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 0; i < (1u << 22); ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u && *abort_flag) return false;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
   }
   return false;
 }
+
+// One lane of a converged warp.  The issuing warps run their loops with all
+// lanes, so that addresses, descriptors and counters stay in uniform registers,
+// and only the copies and MMAs themselves are predicated: a loop inside
+// `if (lane == 0)` took about 1000 cycles per K block, twice the MMAs' own time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// A position in a ring of N barriers: slot, and the parity of its use.
+template <int N>
+struct Ring {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// A matrix descriptor's high half; the low half is the address and counts up in 16-byte units.
+__device__ __forceinline__ uint64_t desc_at(uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; }
+constexpr uint32_t TILE_HI = (1024u >> 4) | (1u << 14) | (2u << 29);    // 1024 bytes between 8-row groups, 128-byte swizzle
+constexpr uint32_t SCALE_HI = (128u >> 4) | (1u << 14);                  // 128 bytes between 8-row groups, none
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4); }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -270,61 +294,75 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   bool have = false;   // the epilogue warps: the accumulator is ready
   if (warp == 0) {
-    if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % C::STAGES;
-        if (i >= C::STAGES && !wait_or_abort(&empty[s], (uint32_t)(i / C::STAGES - 1) & 1u, abort_v)) {
-          abort_flag = 1;
-          break;
-        }
-        unsigned char* sp = smem + s * C::STAGE_BYTES;
-        mbar_arrive_tx(&full[s], C::STAGE_BYTES);
-        tma_load_2d(sp, &map_p, (kb0 + i) * BK, (int)p0, &full[s]);
-        tma_load_2d(sp + C::A_BYTES, &map_q, (kb0 + i) * BK, (int)q0, &full[s]);
-        issued = i + 1;
+    const bool one = elect_one();
+    Ring<C::STAGES> st;
+    int issued = 0;
+    for (int i = 0; i < nkb; ++i, st.next()) {
+      if (i >= C::STAGES && !wait_warp(&empty[st.slot], st.phase ^ 1u, abort_v)) {
+        abort_flag = 1;
+        break;
       }
-      loads_issued = issued;
+      if (one) {
+        unsigned char* sp = smem + st.slot * C::STAGE_BYTES;
+        mbar_arrive_tx(&full[st.slot], C::STAGE_BYTES);
+        tma_load_2d(sp, &map_p, (kb0 + i) * BK, (int)p0, &full[st.slot]);
+        tma_load_2d(sp + C::A_BYTES, &map_q, (kb0 + i) * BK, (int)q0, &full[st.slot]);
+      }
+      __syncwarp();
+      issued = i + 1;
     }
+    if (one) loads_issued = issued;
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int i = 0; i < nkb && ok; ++i) {
-        const int grp = i >> 2, buf = grp % C::SF_BUFS, slot = grp % SF_SLOTS;
-        const uint32_t sfp = tmem + BN + buf * C::SF_COLS, sfq = sfp + 4;
-        const int s = i % C::STAGES;
-        ok = wait_or_abort(&full[s], (uint32_t)(i / C::STAGES) & 1u, abort_v);
-        if (ok && (i & 3) == 0) {
-          ok = wait_or_abort(&sf_full[slot], (uint32_t)(grp / SF_SLOTS) & 1u, abort_v);
-          if (ok) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = smem_u32(smem + C::SF_OFF + slot * SF_SLOT_BYTES);
-            copy_scales(sfp, desc_of(src, 0, 128, 0));
-            copy_scales(sfq, desc_of(src + 512, 0, 128, 0));
-            if (BN > 128) copy_scales(sfq + 4, desc_of(src + 1024, 0, 128, 0));
-            mma_commit(&sf_empty[slot]);
-          }
-        }
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t sp = smem_u32(smem + s * C::STAGE_BYTES), sq = sp + C::A_BYTES;
-        const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code, (uint32_t)(i & 3));
-#pragma unroll
-        for (int k = 0; k < BK / 32; ++k)
-          mma_scaled(tmem, desc_of(sp + k * 32, 16, 1024, 2), desc_of(sq + k * 32, 16, 1024, 2), idesc, sfp, sfq,
-                     (i > 0 || k > 0) ? 1u : 0u);
-        mma_commit(&empty[s]);
+    const bool one = elect_one();
+    const uint32_t tiles_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem + C::SF_OFF));
+    const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code);
+    Ring<C::STAGES> st;
+    Ring<SF_SLOTS> sf;
+    bool ok = true;
+    for (int i = 0, grp = 0; i < nkb && ok; i += 4, ++grp, sf.next()) {
+      const uint32_t sfp = tmem + BN + (uint32_t)(grp % C::SF_BUFS) * C::SF_COLS, sfq = sfp + 4;
+      ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
+      // this buffer's last readers, the MMAs of SF_BUFS groups ago, are done
+      if (ok && grp >= C::SF_BUFS) ok = wait_warp(&sf_empty[(grp - C::SF_BUFS) % SF_SLOTS],
+                                                      (uint32_t)((grp - C::SF_BUFS) / SF_SLOTS) & 1u, abort_v);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t src = sf_lo + sf.slot * (SF_SLOT_BYTES / 16);
+      if (one) {
+        copy_scales(sfp, desc_at(src, SCALE_HI));
+        copy_scales(sfq, desc_at(src + 32, SCALE_HI));
+        if (BN > 128) copy_scales(sfq + 4, desc_at(src + 64, SCALE_HI));
       }
-      if (!ok) abort_flag = 1;
-      // also when giving up: the commit tells when everything issued is done
-      mma_commit(&acc_full);
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i + j < nkb && ok) {
+          ok = wait_warp(&full[st.slot], st.phase, abort_v);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
+          if (ok && one) {
+#pragma unroll
+            for (int k = 0; k < BK / 32; ++k)
+              mma_scaled(tmem, desc_at(lo + 2 * k, TILE_HI), desc_at(lo + C::A_BYTES / 16 + 2 * k, TILE_HI),
+                         idesc | sf_id(j), sfp, sfq, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
+            mma_commit(&empty[st.slot]);
+          }
+          __syncwarp();
+          st.next();
+        }
+      }
+      if (one) mma_commit(&sf_empty[sf.slot]);
+      __syncwarp();
     }
+    if (!ok) abort_flag = 1;
+    // also when giving up: the commit tells when everything issued is done
+    if (one) mma_commit(&acc_full);
   } else if (warp == 2) {
     bool ok = true;
     for (int i = 0; i < nkb; i += 4) {
       const int grp = i >> 2, slot = grp % SF_SLOTS;
-      if (grp >= SF_SLOTS) ok = wait_or_abort(&sf_empty[slot], (uint32_t)(grp / SF_SLOTS - 1) & 1u, abort_v);
-      if (!__all_sync(0xffffffffu, ok)) {
+      if (grp >= SF_SLOTS) ok = wait_warp(&sf_empty[slot], (uint32_t)(grp / SF_SLOTS - 1) & 1u, abort_v);
+      if (!ok) {
         abort_flag = 1;
         break;
       }
@@ -344,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_arrive(&sf_full[slot]);
     }
   } else if (warp >= 4) {
-    have = wait_or_abort(&acc_full, 0, abort_v);
+    have = wait_warp(&acc_full, 0, abort_v);
     if (!have) abort_flag = 1;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   }
@@ -412,6 +450,352 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
+// A chunk of a long float32 sum: adds what D holds of the earlier chunks and,
+// unless it is the last, leaves the sum there.  The same thread reads and
+// writes each element.
+__device__ __forceinline__ void add_chunk(const GemmArgs& g, int64_t p, int64_t q0, bool last, bool more, float (&v)[16]) {
+  if (p >= g.p.extent || q0 >= g.q.extent) return;
+  float* at = static_cast<float*>(g.d) + p * g.ldd + q0;
+  const int w = g.q.extent - q0 < 16 ? (int)(g.q.extent - q0) : 16;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (e < w) {
+      if (more) v[e] = __fadd_rn(v[e], at[e]);
+      if (!last) at[e] = v[e];
+    }
+}
+// ---- many tiles: pairs of CTAs (cta_group::2), persistent, two accumulators ----
+// A pair computes 256 x BN tiles: each CTA stages its 128 rows of P and half
+// of Q's BN rows, so a staged byte feeds twice the multiplications of the
+// single-CTA kernel; the even CTA issues the MMAs for both.  Each CTA's tensor
+// memory holds its 128 rows of two accumulators.  At BN = 256 these and the
+// scales do not fit 512 columns: the accumulators then share 32 columns, which
+// the epilogue reads first, and the next tile's MMAs start once it has.
+//
+// float32 results of long K are summed in chunks of at most CHUNK blocks, each
+// a product of its own that the epilogue adds in float32: the tensor cores
+// truncate as they accumulate, an error that grows with K (7e-7 relative at
+// K = 8192, 1.5e-7 of a rounding sum); bf16 results round at 2^-9.
+constexpr int CHUNK = 64;
+
+template <int BN>
+struct PairCfg {
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN > 192 ? 6 : 7;
+  static constexpr int SF_OFF = STAGES * STAGE_BYTES;
+  static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
+  static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
+  static constexpr int SF_BUFS = BN > 192 ? 2 : 3;
+  static constexpr int SHARED = 2 * BN + SF_BUFS * SF_COLS > 512 ? 32 : 0;
+  static constexpr int ACC_STRIDE = BN - SHARED;
+  static constexpr int SF_COL = BN + ACC_STRIDE;
+};
+
+struct PairArgs {
+  int p_tiles, q_tiles;   // of 256 and BN
+  int chunks, chunk_blocks;
+};
+
+__device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// A load into this CTA that reports to the even CTA's barrier (no multicast).
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_scaled_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                                uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrives at this barrier of both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Tile t: bands of BAND row tiles, walked row-fastest, so that the tiles in
+// flight form a near-square patch and share both operands in L2.
+constexpr int BAND = 8;
+__device__ __forceinline__ void pair_origin(int t, const PairArgs& w, int bn, int64_t& p0, int64_t& q0) {
+  const int band = t / (BAND * w.q_tiles), r = t - band * BAND * w.q_tiles;
+  const int rows = min(BAND, w.p_tiles - band * BAND);
+  p0 = (int64_t)(band * BAND + r % rows) * (2 * BM);
+  q0 = (int64_t)(r / rows) * bn;
+}
+
+template <int BN, bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, GemmArgs g,
+                PairArgs w, DropSpec d) {
+  using C = PairCfg<BN>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full[2], acc_empty[2];
+  __shared__ uint64_t drain;
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag;
+  volatile int* abort_v = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int n_tiles = w.p_tiles * w.q_tiles;
+  const int first = (int)(blockIdx.x >> 1), stride = (int)(gridDim.x >> 1);
+  // the other CTA learns of a wait that gave up
+  auto give_up = [&]() {
+    abort_flag = 1;
+    const uint32_t other = map_to(smem_u32(&abort_flag), rank ^ 1u);
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(other), "r"(1u) : "memory");
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < SF_SLOTS; ++s) {
+      mbar_init(&sf_full[s], 2);
+      mbar_init(&sf_empty[s], 1);
+    }
+    mbar_init(&acc_full[0], 1);
+    mbar_init(&acc_full[1], 1);
+    mbar_init(&acc_empty[0], 8);
+    mbar_init(&acc_empty[1], 8);
+    mbar_init(&drain, 1);
+    abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_base;
+
+  if (warp == 0) {
+    const bool one = elect_one();
+    Ring<C::STAGES> st;
+    bool ok = true, filled = false;
+    for (int t = first; t < n_tiles && ok; t += stride) {
+      int64_t p0, q0;
+      pair_origin(t, w, BN, p0, q0);
+      p0 += rank * BM;
+      q0 += rank * (BN / 2);
+      for (int kb = 0; kb < g.kblocks; ++kb) {
+        if (filled) ok = wait_warp(&empty[st.slot], st.phase ^ 1u, abort_v);
+        if (!ok) {
+          give_up();
+          break;
+        }
+        if (one) {
+          unsigned char* sp = smem + st.slot * C::STAGE_BYTES;
+          const uint32_t bar = map_to(smem_u32(&full[st.slot]), 0);
+          if (rank == 0) mbar_arrive_tx(&full[st.slot], 2 * C::STAGE_BYTES);
+          tma_load_pair(sp, &map_p, kb * BK, (int)p0, bar);
+          tma_load_pair(sp + C::A_BYTES, &map_q, kb * BK, (int)q0, bar);
+        }
+        __syncwarp();
+        st.next();
+        if (st.slot == 0) filled = true;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool one = elect_one();
+      const uint32_t tiles_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem + C::SF_OFF));
+      const uint32_t idesc = instr_desc(2 * BM, BN, g.p.code, g.q.code);
+      Ring<C::STAGES> st;
+      Ring<SF_SLOTS> sf, freed;   // freed: the group whose MMAs must be done before a scale buffer is written again
+      Ring<C::SF_BUFS> buf;
+      uint32_t item = 0, groups = 0;
+      bool ok = true;
+      for (int t = first; t < n_tiles && ok; t += stride) {
+        for (int ch = 0; ch < w.chunks && ok; ++ch, ++item) {
+          const int kb0 = ch * w.chunk_blocks, kb1 = min(g.kblocks, kb0 + w.chunk_blocks);
+          if (C::SHARED) {
+            if (item > 0) ok = wait_warp(&acc_empty[0], (item - 1) & 1u, abort_v);
+          } else if (item > 1) {
+            ok = wait_warp(&acc_empty[item & 1u], (item / 2 - 1) & 1u, abort_v);
+          }
+          const uint32_t acc = tmem + (item & 1u) * C::ACC_STRIDE;
+          for (int kb = kb0; kb < kb1 && ok; kb += 4, ++groups) {
+            const uint32_t sfp = tmem + C::SF_COL + buf.slot * C::SF_COLS, sfq = sfp + 4;
+            ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
+            if (ok && groups >= C::SF_BUFS) {
+              ok = wait_warp(&sf_empty[freed.slot], freed.phase, abort_v);
+              freed.next();
+            }
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t src = sf_lo + sf.slot * (SF_SLOT_BYTES / 16);
+            if (one) {
+              copy_scales_pair(sfp, desc_at(src, SCALE_HI));
+              copy_scales_pair(sfq, desc_at(src + 32, SCALE_HI));
+              if (BN > 128) copy_scales_pair(sfq + 4, desc_at(src + 64, SCALE_HI));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (kb + j < kb1 && ok) {
+                ok = wait_warp(&full[st.slot], st.phase, abort_v);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
+                if (ok && one) {
+#pragma unroll
+                  for (int k = 0; k < BK / 32; ++k)
+                    mma_scaled_pair(acc, desc_at(lo + 2 * k, TILE_HI), desc_at(lo + C::A_BYTES / 16 + 2 * k, TILE_HI),
+                                    idesc | sf_id(j), sfp, sfq, (kb > kb0 || j > 0 || k > 0) ? 1u : 0u);
+                  commit_pair(&empty[st.slot]);
+                }
+                __syncwarp();
+                st.next();
+              }
+            }
+            if (one) commit_pair(&sf_empty[sf.slot]);
+            __syncwarp();
+            sf.next();
+            buf.next();
+          }
+          if (ok && one) commit_pair(&acc_full[item & 1u]);
+          __syncwarp();
+        }
+      }
+      if (!ok) give_up();
+    }
+  } else if (warp == 2) {
+    uint32_t sf = 0;
+    bool ok = true;
+    for (int t = first; t < n_tiles && ok; t += stride) {
+      int64_t p0, q0;
+      pair_origin(t, w, BN, p0, q0);
+      p0 += rank * BM;
+      for (int kg = 0; kg * 4 < g.kblocks; ++kg, ++sf) {
+        const int slot = (int)(sf % SF_SLOTS);
+        uint32_t a[4], b[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = scale_word(g.p, p0 + 32 * e + lane, kg);
+#pragma unroll
+        for (int c = 0; c < (BN + 127) / 128; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) b[c][e] = scale_word(g.q, q0 + 128 * c + 32 * e + lane, kg);
+        if (sf >= SF_SLOTS) ok = wait_warp(&sf_empty[slot], (sf / SF_SLOTS - 1) & 1u, abort_v);
+        if (!ok) {
+          if (lane == 0) give_up();
+          break;
+        }
+        unsigned char* dst = smem + C::SF_OFF + slot * SF_SLOT_BYTES + lane * 16;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int c = 0; c < (BN + 127) / 128; ++c)
+          *reinterpret_cast<uint4*>(dst + 512 * (c + 1)) = make_uint4(b[c][0], b[c][1], b[c][2], b[c][3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_at(map_to(smem_u32(&sf_full[slot]), 0));
+      }
+    }
+  } else if (warp >= 4) {
+    const uint32_t step = g.drop ? drop_step(d) : 0u;
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t empty_bar[2] = {map_to(smem_u32(&acc_empty[0]), 0), map_to(smem_u32(&acc_empty[1]), 0)};
+    uint32_t item = 0;
+    bool ok = true;
+    for (int t = first; t < n_tiles && ok; t += stride) {
+      int64_t p0, q0;
+      pair_origin(t, w, BN, p0, q0);
+      const int64_t p = p0 + rank * BM + row;
+      for (int ch = 0; ch < w.chunks; ++ch, ++item) {
+        const uint32_t odd = item & 1u;
+        ok = wait_warp(&acc_full[odd], (item >> 1) & 1u, abort_v);
+        if (!ok) {
+          if (lane == 0) give_up();
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + odd * C::ACC_STRIDE;
+#pragma unroll 1
+        for (int i = 0; i < BN / 32; ++i) {
+          // the columns shared with the other accumulator come first
+          const int c = 32 * (C::SHARED && !odd ? (i == 0 ? BN / 32 - 1 : i - 1) : i);
+          uint32_t r[32];
+          tmem_ld32(taddr + c, r);
+          if (i == (C::SHARED ? 0 : BN / 32 - 1)) {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive_at(empty_bar[C::SHARED ? 0 : odd]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[16 * h + e]);
+            if (!BF16 && w.chunks > 1) add_chunk(g, p, q0 + c + 16 * h, ch == w.chunks - 1, ch > 0, v);
+            if (BF16 || ch == w.chunks - 1) emit<BF16, 16>(g, d, step, p, q0 + c + 16 * h, v);
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  if (abort_flag) {
+    // wait (bounded) for the MMAs in flight (the thread that issued them) and for loads to land
+    if (warp == 1 && rank == 0 && elect_one()) {
+      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&drain))
+                   : "memory");
+      mbar_wait(&drain, 0, 1u << 20);
+    }
+    if (threadIdx.x == 0) {
+      if (rank == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+          // whichever phase is current: it completes when its loads have landed
+          if (!mbar_wait(&full[s], 0, 1u << 12)) mbar_wait(&full[s], 1, 1u << 12);
+        }
+      }
+      if (g.err) *reinterpret_cast<volatile int32_t*>(g.err) = 1;
+    }
+    __syncthreads();
+    cluster_sync();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // ---- host ----
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
@@ -471,6 +855,28 @@ int launch_t(const Launch& L) {
   cfg.numAttrs = S > 1 ? 1 : 0;
   e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, L.g, L.d);
   return check_cuda(e, "advopt_fp8_gemm");
+}
+
+template <int BN, bool BF16>
+int launch_pair(const Launch& L) {
+  using C = PairCfg<BN>;
+  CUtensorMap mp, mq;
+  int rc = encode_map(&mp, L.p, L.g.p.extent, L.k, L.ldp, BM);
+  if (rc == ADVOPT_OK) rc = encode_map(&mq, L.q, L.g.q.extent, L.k, L.ldq, BN / 2);
+  if (rc != ADVOPT_OK) return rc;
+  const auto kernel = pair_kernel<BN, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
+  PairArgs w;
+  w.p_tiles = (int)((L.g.p.extent + 2 * BM - 1) / (2 * BM));
+  w.q_tiles = (int)((L.g.q.extent + BN - 1) / BN);
+  if ((int64_t)w.p_tiles * w.q_tiles > (1 << 30)) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
+  w.chunks = BF16 ? 1 : (L.g.kblocks + CHUNK - 1) / CHUNK;
+  w.chunk_blocks = ((L.g.kblocks + w.chunks - 1) / w.chunks + 3) / 4 * 4;
+  w.chunks = (L.g.kblocks + w.chunk_blocks - 1) / w.chunk_blocks;
+  const int tiles = w.p_tiles * w.q_tiles;
+  kernel<<<2 * (tiles < PAIRS ? tiles : PAIRS), THREADS, C::SMEM, L.stream>>>(mp, mq, L.g, w, L.d);
+  return check_cuda(cudaGetLastError(), "advopt_fp8_gemm");
 }
 
 template <int BN, bool BF16>
@@ -545,6 +951,13 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   g.err = a->err;
   L.d = drop_spec(a->drop);
   L.stream = static_cast<cudaStream_t>(stream);
+  const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
+  if (force ? force < 3000 : (a->m > 256 && a->n > 256 && ((a->m + 255) / 256) * ((a->n + 255) / 256) >= 40)) {
+    const int bn = force ? force : 256;
+    if (a->d_dtype == ADVOPT_DT_BF16)
+      return bn == 256 ? fp8::launch_pair<256, true>(L) : bn == 192 ? fp8::launch_pair<192, true>(L) : fp8::launch_pair<128, true>(L);
+    return bn == 256 ? fp8::launch_pair<256, false>(L) : bn == 192 ? fp8::launch_pair<192, false>(L) : fp8::launch_pair<128, false>(L);
+  }
   const int64_t q = g.q.extent;
   const int bn = q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256;
   const int64_t tiles = ((g.p.extent + 127) / 128) * ((q + bn - 1) / bn);
