@@ -92,23 +92,53 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
-                                           uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
+// The four K = 32 steps of one staged block and the commit that frees the stage
+// (of both CTAs of a pair).  One asm statement with the predicate inside: all
+// lanes reach it together, so descriptors stay in uniform registers; as four
+// calls under a branch on the elected lane they took 500 cycles to issue, as
+// many as the MMAs take to run.
+#define ADVOPT_FP8_BLOCK(GROUP, COMMIT)                                                                              \
+  "{\n .reg .pred p, q, t;\n .reg .b32 al, bl;\n .reg .b64 a, b;\n"                                              \
+  " setp.ne.b32 q, %9, 0;\n setp.ne.b32 p, %6, 0;\n setp.eq.b32 t, 0, 0;\n"                                       \
+  " mov.b64 a, {%1, %8};\n mov.b64 b, {%2, %8};\n"                                                                 \
+  " @q tcgen05.mma.cta_group::" GROUP ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %3, [%4], [%5], p;\n"   \
+  " add.u32 al, %1, 2;\n add.u32 bl, %2, 2;\n mov.b64 a, {al, %8};\n mov.b64 b, {bl, %8};\n"                     \
+  " @q tcgen05.mma.cta_group::" GROUP ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %3, [%4], [%5], t;\n"   \
+  " add.u32 al, %1, 4;\n add.u32 bl, %2, 4;\n mov.b64 a, {al, %8};\n mov.b64 b, {bl, %8};\n"                     \
+  " @q tcgen05.mma.cta_group::" GROUP ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %3, [%4], [%5], t;\n"   \
+  " add.u32 al, %1, 6;\n add.u32 bl, %2, 6;\n mov.b64 a, {al, %8};\n mov.b64 b, {bl, %8};\n"                     \
+  " @q tcgen05.mma.cta_group::" GROUP ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %3, [%4], [%5], t;\n"   \
+  " @q tcgen05.commit.cta_group::" GROUP COMMIT "\n}\n"
+template <bool PAIR>
+__device__ __forceinline__ void mma_block(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate, uint64_t* freed, uint32_t hi, uint32_t one) {
+  if (PAIR)
+    asm volatile(
+        ADVOPT_FP8_BLOCK("2", ".mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%7], %10;")
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(smem_u32(freed)), "r"(hi),
+        "r"(one), "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile(
+        ADVOPT_FP8_BLOCK("1", ".mbarrier::arrive::one.shared::cluster.b64 [%7];")
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(smem_u32(freed)), "r"(hi),
+        "r"(one)
+        : "memory");
 }
+#undef ADVOPT_FP8_BLOCK
 
 // 32 rows of 16 bytes -> 4 tensor-memory columns, repeated for the four lane quarters.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc, uint32_t one) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n"
+               ::"r"(taddr), "l"(desc), "r"(one)
+               : "memory");
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t one) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n"
+      ::"r"(smem_u32(bar)), "r"(one)
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -132,6 +162,22 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
     if ((i & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag)) return false;
   }
   return false;
+}
+
+// A look at a barrier that does not wait: asked for a block ahead, its answer
+// is there when the block before has been issued (a wait that succeeds at once
+// costs the issuing warp 125 cycles, a quarter of a block's MMAs).
+__device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool wait_seen(uint32_t seen, uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, seen) || wait_warp(bar, parity, abort_flag);
 }
 
 // One lane of a converged warp.  The issuing warps run their loops with all
@@ -318,45 +364,40 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code);
     Ring<C::STAGES> st;
     Ring<SF_SLOTS> sf;
+    uint32_t seen = 0, sf_seen = 0;
     bool ok = true;
-    for (int i = 0, grp = 0; i < nkb && ok; i += 4, ++grp, sf.next()) {
+    for (int i = 0, grp = 0; i < nkb && ok; i += 4, ++grp) {
       const uint32_t sfp = tmem + BN + (uint32_t)(grp % C::SF_BUFS) * C::SF_COLS, sfq = sfp + 4;
-      ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
+      ok = wait_seen(sf_seen, &sf_full[sf.slot], sf.phase, abort_v);
       // this buffer's last readers, the MMAs of SF_BUFS groups ago, are done
       if (ok && grp >= C::SF_BUFS) ok = wait_warp(&sf_empty[(grp - C::SF_BUFS) % SF_SLOTS],
                                                       (uint32_t)((grp - C::SF_BUFS) / SF_SLOTS) & 1u, abort_v);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t src = sf_lo + sf.slot * (SF_SLOT_BYTES / 16);
-      if (one) {
-        copy_scales(sfp, desc_at(src, SCALE_HI));
-        copy_scales(sfq, desc_at(src + 32, SCALE_HI));
-        if (BN > 128) copy_scales(sfq + 4, desc_at(src + 64, SCALE_HI));
-      }
-      __syncwarp();
+      copy_scales(sfp, desc_at(src, SCALE_HI), one);
+      copy_scales(sfq, desc_at(src + 32, SCALE_HI), one);
+      if (BN > 128) copy_scales(sfq + 4, desc_at(src + 64, SCALE_HI), one);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (i + j < nkb && ok) {
-          ok = wait_warp(&full[st.slot], st.phase, abort_v);
+          ok = wait_seen(seen, &full[st.slot], st.phase, abort_v);
+          if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
-          if (ok && one) {
-#pragma unroll
-            for (int k = 0; k < BK / 32; ++k)
-              mma_scaled(tmem, desc_at(lo + 2 * k, TILE_HI), desc_at(lo + C::A_BYTES / 16 + 2 * k, TILE_HI),
-                         idesc | sf_id(j), sfp, sfq, (i > 0 || j > 0 || k > 0) ? 1u : 0u);
-            mma_commit(&empty[st.slot]);
-          }
-          __syncwarp();
+          uint64_t* freed = &empty[st.slot];
           st.next();
+          seen = mbar_test(&full[st.slot], st.phase);
+          mma_block<false>(tmem, lo, lo + C::A_BYTES / 16, idesc | sf_id(j), sfp, sfq, i + j > 0, freed, TILE_HI, one);
         }
       }
-      if (one) mma_commit(&sf_empty[sf.slot]);
-      __syncwarp();
+      mma_commit(&sf_empty[sf.slot], one);
+      sf.next();
+      sf_seen = mbar_test(&sf_full[sf.slot], sf.phase);
     }
     if (!ok) abort_flag = 1;
     // also when giving up: the commit tells when everything issued is done
-    if (one) mma_commit(&acc_full);
+    mma_commit(&acc_full, one);
   } else if (warp == 2) {
     bool ok = true;
     for (int i = 0; i < nkb; i += 4) {
@@ -512,22 +553,17 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void mma_scaled_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
-                                                uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc, uint32_t one) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n @q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n"
+               ::"r"(taddr), "l"(desc), "r"(one)
+               : "memory");
 }
 // Arrives at this barrier of both CTAs when the MMAs issued so far are done.
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+__device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t one) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n"
+      ::"r"(smem_u32(bar)), "h"((uint16_t)3), "r"(one)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -639,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       Ring<C::STAGES> st;
       Ring<SF_SLOTS> sf, freed;   // freed: the group whose MMAs must be done before a scale buffer is written again
       Ring<C::SF_BUFS> buf;
-      uint32_t item = 0, groups = 0;
+      uint32_t item = 0, groups = 0, seen = 0, sf_seen = 0, freed_seen = 0;
       bool ok = true;
       for (int t = first; t < n_tiles && ok; t += stride) {
         for (int ch = 0; ch < w.chunks && ok; ++ch, ++item) {
@@ -652,44 +688,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const uint32_t acc = tmem + (item & 1u) * C::ACC_STRIDE;
           for (int kb = kb0; kb < kb1 && ok; kb += 4, ++groups) {
             const uint32_t sfp = tmem + C::SF_COL + buf.slot * C::SF_COLS, sfq = sfp + 4;
-            ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
+            ok = wait_seen(sf_seen, &sf_full[sf.slot], sf.phase, abort_v);
             if (ok && groups >= C::SF_BUFS) {
-              ok = wait_warp(&sf_empty[freed.slot], freed.phase, abort_v);
+              ok = wait_seen(freed_seen, &sf_empty[freed.slot], freed.phase, abort_v);
               freed.next();
             }
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = sf_lo + sf.slot * (SF_SLOT_BYTES / 16);
-            if (one) {
-              copy_scales_pair(sfp, desc_at(src, SCALE_HI));
-              copy_scales_pair(sfq, desc_at(src + 32, SCALE_HI));
-              if (BN > 128) copy_scales_pair(sfq + 4, desc_at(src + 64, SCALE_HI));
-            }
-            __syncwarp();
+            copy_scales_pair(sfp, desc_at(src, SCALE_HI), one);
+            copy_scales_pair(sfq, desc_at(src + 32, SCALE_HI), one);
+            if (BN > 128) copy_scales_pair(sfq + 4, desc_at(src + 64, SCALE_HI), one);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               if (kb + j < kb1 && ok) {
-                ok = wait_warp(&full[st.slot], st.phase, abort_v);
+                ok = wait_seen(seen, &full[st.slot], st.phase, abort_v);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
-                if (ok && one) {
-#pragma unroll
-                  for (int k = 0; k < BK / 32; ++k)
-                    mma_scaled_pair(acc, desc_at(lo + 2 * k, TILE_HI), desc_at(lo + C::A_BYTES / 16 + 2 * k, TILE_HI),
-                                    idesc | sf_id(j), sfp, sfq, (kb > kb0 || j > 0 || k > 0) ? 1u : 0u);
-                  commit_pair(&empty[st.slot]);
-                }
-                __syncwarp();
+                uint64_t* done = &empty[st.slot];
                 st.next();
+                seen = mbar_test(&full[st.slot], st.phase);
+                if (j == 3) {   // the next group's scales too
+                  sf_seen = mbar_test(&sf_full[(sf.slot + 1) % SF_SLOTS], sf.phase ^ (sf.slot + 1 == SF_SLOTS ? 1u : 0u));
+                  freed_seen = mbar_test(&sf_empty[freed.slot], freed.phase);
+                }
+                mma_block<true>(acc, lo, lo + C::A_BYTES / 16, idesc | sf_id(j), sfp, sfq, kb + j > kb0, done, TILE_HI, one);
               }
             }
-            if (one) commit_pair(&sf_empty[sf.slot]);
-            __syncwarp();
+            if (kb + 4 > kb1) sf_seen = freed_seen = 0;   // a short group: not asked
+            commit_pair(&sf_empty[sf.slot], one);
             sf.next();
             buf.next();
           }
-          if (ok && one) commit_pair(&acc_full[item & 1u]);
-          __syncwarp();
+          if (ok) commit_pair(&acc_full[item & 1u], one);
         }
       }
       if (!ok) give_up();
