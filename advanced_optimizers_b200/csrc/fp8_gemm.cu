@@ -164,22 +164,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
   return false;
 }
 
-// A look at a barrier that does not wait: asked for a block ahead, its answer
-// is there when the block before has been issued (a wait that succeeds at once
-// costs the issuing warp 125 cycles, a quarter of a block's MMAs).
-__device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok;
-}
-__device__ __forceinline__ bool wait_seen(uint32_t seen, uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, seen) || wait_warp(bar, parity, abort_flag);
-}
-
 // One lane of a converged warp.  The issuing warps run their loops with all
 // lanes, so that addresses, descriptors and counters stay in uniform registers,
 // and only the copies and MMAs themselves are predicated: a loop inside
@@ -229,6 +213,28 @@ __device__ __forceinline__ uint32_t scale_word(const Side& s, int64_t r, int gro
   if (r >= s.extent) return 0x7F7F7F7Fu;
   return __ldg(reinterpret_cast<const uint32_t*>(s.scales + (r >> s.shift) * s.ld) + group);
 }
+
+// One group's scale words of a tile, four rows a lane.
+template <int BN>
+struct ScaleWords {
+  static constexpr int PARTS = 1 + (BN + 127) / 128;
+  uint32_t w[PARTS][4];
+  __device__ __forceinline__ void load(const GemmArgs& g, int64_t p0, int64_t q0, int group, int lane) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[0][e] = scale_word(g.p, p0 + 32 * e + lane, group);
+#pragma unroll
+    for (int c = 1; c < PARTS; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[c][e] = scale_word(g.q, q0 + 128 * (c - 1) + 32 * e + lane, group);
+  }
+  // row 32 e + l goes to 16-byte line l, word e: what the copy to tensor memory takes
+  __device__ __forceinline__ void store(unsigned char* slot, int lane) const {
+#pragma unroll
+    for (int c = 0; c < PARTS; ++c)
+      *reinterpret_cast<uint4*>(slot + 512 * c + 16 * lane) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+};
 
 // W accumulator values of lane p, columns q0 .. q0 + W - 1, through bias, dropout and residual into D.
 template <bool BF16, int W>
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   using C = Cfg<BN>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full;
+  __shared__ uint64_t full[C::STAGES / 2], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag, loads_issued;
   volatile int* abort_v = &abort_flag;
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      if (s % 2 == 0) mbar_init(&full[s / 2], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < SF_SLOTS; ++s) {
@@ -336,7 +342,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_base;
+  // through a warp reduction: it lands in a uniform register, where the MMAs want it
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
 
   bool have = false;   // the epilogue warps: the accumulator is ready
   if (warp == 0) {
@@ -350,9 +357,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (one) {
         unsigned char* sp = smem + st.slot * C::STAGE_BYTES;
-        mbar_arrive_tx(&full[st.slot], C::STAGE_BYTES);
-        tma_load_2d(sp, &map_p, (kb0 + i) * BK, (int)p0, &full[st.slot]);
-        tma_load_2d(sp + C::A_BYTES, &map_q, (kb0 + i) * BK, (int)q0, &full[st.slot]);
+        uint64_t* bar = &full[st.slot >> 1];
+        if ((i & 1) == 0) mbar_arrive_tx(bar, i + 1 < nkb ? 2 * C::STAGE_BYTES : C::STAGE_BYTES);
+        tma_load_2d(sp, &map_p, (kb0 + i) * BK, (int)p0, bar);
+        tma_load_2d(sp + C::A_BYTES, &map_q, (kb0 + i) * BK, (int)q0, bar);
       }
       __syncwarp();
       issued = i + 1;
@@ -362,13 +370,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool one = elect_one();
     const uint32_t tiles_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem + C::SF_OFF));
     const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code);
-    Ring<C::STAGES> st;
+    Ring<C::STAGES / 2> st;
     Ring<SF_SLOTS> sf;
-    uint32_t seen = 0, sf_seen = 0;
     bool ok = true;
     for (int i = 0, grp = 0; i < nkb && ok; i += 4, ++grp) {
       const uint32_t sfp = tmem + BN + (uint32_t)(grp % C::SF_BUFS) * C::SF_COLS, sfq = sfp + 4;
-      ok = wait_seen(sf_seen, &sf_full[sf.slot], sf.phase, abort_v);
+      ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
       // this buffer's last readers, the MMAs of SF_BUFS groups ago, are done
       if (ok && grp >= C::SF_BUFS) ok = wait_warp(&sf_empty[(grp - C::SF_BUFS) % SF_SLOTS],
                                                       (uint32_t)((grp - C::SF_BUFS) / SF_SLOTS) & 1u, abort_v);
@@ -379,48 +386,45 @@ __global__ void __launch_bounds__(THREADS, 1)
       copy_scales(sfq, desc_at(src + 32, SCALE_HI), one);
       if (BN > 128) copy_scales(sfq + 4, desc_at(src + 64, SCALE_HI), one);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; j += 2) {
         if (i + j < nkb && ok) {
-          ok = wait_seen(seen, &full[st.slot], st.phase, abort_v);
+          ok = wait_warp(&full[st.slot], st.phase, abort_v);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
-          uint64_t* freed = &empty[st.slot];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (i + j + h < nkb) {
+              const uint32_t lo = tiles_lo + (2 * st.slot + h) * (C::STAGE_BYTES / 16);
+              mma_block<false>(tmem, lo, lo + C::A_BYTES / 16, idesc | sf_id(j + h), sfp, sfq, i + j + h > 0,
+                               &empty[2 * st.slot + h], TILE_HI, one);
+            }
+          }
           st.next();
-          seen = mbar_test(&full[st.slot], st.phase);
-          mma_block<false>(tmem, lo, lo + C::A_BYTES / 16, idesc | sf_id(j), sfp, sfq, i + j > 0, freed, TILE_HI, one);
         }
       }
       mma_commit(&sf_empty[sf.slot], one);
       sf.next();
-      sf_seen = mbar_test(&sf_full[sf.slot], sf.phase);
     }
     if (!ok) abort_flag = 1;
     // also when giving up: the commit tells when everything issued is done
     mma_commit(&acc_full, one);
-  } else if (warp == 2) {
+  } else if (warp < 4) {
+    // warps 2 and 3 take the groups in turn, each loading its next one before it stores the present one
     bool ok = true;
-    for (int i = 0; i < nkb; i += 4) {
-      const int grp = i >> 2, slot = grp % SF_SLOTS;
+    ScaleWords<BN> now, then;
+    int grp = warp - 2;
+    if (4 * grp < nkb) now.load(g, p0, q0, (kb0 >> 2) + grp, lane);
+    for (; 4 * grp < nkb; grp += 2) {
+      const int slot = grp % SF_SLOTS;
+      if (4 * (grp + 2) < nkb) then.load(g, p0, q0, (kb0 >> 2) + grp + 2, lane);
       if (grp >= SF_SLOTS) ok = wait_warp(&sf_empty[slot], (uint32_t)(grp / SF_SLOTS - 1) & 1u, abort_v);
       if (!ok) {
         abort_flag = 1;
         break;
       }
-      const int kg = (kb0 >> 2) + grp;
-      unsigned char* dst = smem + C::SF_OFF + slot * SF_SLOT_BYTES + lane * 16;
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = scale_word(g.p, p0 + 32 * e + lane, kg);
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-      for (int c = 0; c < (BN + 127) / 128; ++c) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = scale_word(g.q, q0 + 128 * c + 32 * e + lane, kg);
-        *reinterpret_cast<uint4*>(dst + 512 * (c + 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      now.store(smem + C::SF_OFF + slot * SF_SLOT_BYTES, lane);
       mbar_arrive(&sf_full[slot]);
+      now = then;
     }
   } else if (warp >= 4) {
     have = wait_warp(&acc_full, 0, abort_v);
@@ -479,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // wait (bounded) for the loads and MMAs in flight before memory is given back
     if (threadIdx.x == 0) {
       for (int i = loads_issued > C::STAGES ? loads_issued - C::STAGES : 0; i < loads_issued; ++i)
-        mbar_wait(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, 1u << 20);
+        mbar_wait(&full[i % C::STAGES / 2], (uint32_t)(i / C::STAGES) & 1u, 1u << 20);
       mbar_wait(&acc_full, 0, 1u << 20);
       if (g.err) *reinterpret_cast<volatile int32_t*>(g.err) = 1;
     }
@@ -523,7 +527,7 @@ template <int BN>
 struct PairCfg {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN > 192 ? 6 : 7;
+  static constexpr int STAGES = BN > 128 ? 6 : 8;   // even: blocks are staged, and waited for, in twos
   static constexpr int SF_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
   static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
@@ -595,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   using C = PairCfg<BN>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[C::STAGES / 2], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full[2], acc_empty[2];
   __shared__ uint64_t drain;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag;
@@ -613,7 +617,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      if (s % 2 == 0) mbar_init(&full[s / 2], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < SF_SLOTS; ++s) {
@@ -638,33 +642,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   __syncthreads();
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_base;
+  // through a warp reduction: it lands in a uniform register, where the MMAs want it
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
 
   if (warp == 0) {
     const bool one = elect_one();
-    Ring<C::STAGES> st;
-    bool ok = true, filled = false;
+    Ring<C::STAGES / 2> st;
+    uint32_t filled[2] = {}, phases[2] = {};   // per slot: whether it has been filled, the parity of its next release
+    bool ok = true;
     for (int t = first; t < n_tiles && ok; t += stride) {
       int64_t p0, q0;
       pair_origin(t, w, BN, p0, q0);
       p0 += rank * BM;
       q0 += rank * (BN / 2);
-      for (int kb = 0; kb < g.kblocks; ++kb) {
-        if (filled) ok = wait_warp(&empty[st.slot], st.phase ^ 1u, abort_v);
-        if (!ok) {
-          give_up();
-          break;
+      for (int kb = 0; kb < g.kblocks && ok; kb += 2) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // an odd last block leaves the second slot of its two empty
+          const bool used = kb + h < g.kblocks;
+          if (used && ok && (filled[h] >> st.slot & 1u)) ok = wait_warp(&empty[2 * st.slot + h], phases[h] >> st.slot & 1u, abort_v);
+          if (used && ok) {
+            if (one) {
+              unsigned char* sp = smem + (2 * st.slot + h) * C::STAGE_BYTES;
+              const uint32_t bar = map_to(smem_u32(&full[st.slot]), 0);
+              if (rank == 0 && h == 0) mbar_arrive_tx(&full[st.slot], kb + 1 < g.kblocks ? 4 * C::STAGE_BYTES : 2 * C::STAGE_BYTES);
+              tma_load_pair(sp, &map_p, (kb + h) * BK, (int)p0, bar);
+              tma_load_pair(sp + C::A_BYTES, &map_q, (kb + h) * BK, (int)q0, bar);
+            }
+            __syncwarp();
+            if (filled[h] >> st.slot & 1u) phases[h] ^= 1u << st.slot;
+            filled[h] |= 1u << st.slot;
+          }
         }
-        if (one) {
-          unsigned char* sp = smem + st.slot * C::STAGE_BYTES;
-          const uint32_t bar = map_to(smem_u32(&full[st.slot]), 0);
-          if (rank == 0) mbar_arrive_tx(&full[st.slot], 2 * C::STAGE_BYTES);
-          tma_load_pair(sp, &map_p, kb * BK, (int)p0, bar);
-          tma_load_pair(sp + C::A_BYTES, &map_q, kb * BK, (int)q0, bar);
-        }
-        __syncwarp();
+        if (!ok) give_up();
         st.next();
-        if (st.slot == 0) filled = true;
       }
     }
   } else if (warp == 1) {
@@ -672,10 +683,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const bool one = elect_one();
       const uint32_t tiles_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem + C::SF_OFF));
       const uint32_t idesc = instr_desc(2 * BM, BN, g.p.code, g.q.code);
-      Ring<C::STAGES> st;
+      Ring<C::STAGES / 2> st;
       Ring<SF_SLOTS> sf, freed;   // freed: the group whose MMAs must be done before a scale buffer is written again
       Ring<C::SF_BUFS> buf;
-      uint32_t item = 0, groups = 0, seen = 0, sf_seen = 0, freed_seen = 0;
+      uint32_t item = 0, groups = 0;
       bool ok = true;
       for (int t = first; t < n_tiles && ok; t += stride) {
         for (int ch = 0; ch < w.chunks && ok; ++ch, ++item) {
@@ -688,9 +699,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const uint32_t acc = tmem + (item & 1u) * C::ACC_STRIDE;
           for (int kb = kb0; kb < kb1 && ok; kb += 4, ++groups) {
             const uint32_t sfp = tmem + C::SF_COL + buf.slot * C::SF_COLS, sfq = sfp + 4;
-            ok = wait_seen(sf_seen, &sf_full[sf.slot], sf.phase, abort_v);
+            ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
             if (ok && groups >= C::SF_BUFS) {
-              ok = wait_seen(freed_seen, &sf_empty[freed.slot], freed.phase, abort_v);
+              ok = wait_warp(&sf_empty[freed.slot], freed.phase, abort_v);
               freed.next();
             }
             if (!ok) break;
@@ -700,23 +711,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             copy_scales_pair(sfq, desc_at(src + 32, SCALE_HI), one);
             if (BN > 128) copy_scales_pair(sfq + 4, desc_at(src + 64, SCALE_HI), one);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; j += 2) {
               if (kb + j < kb1 && ok) {
-                ok = wait_seen(seen, &full[st.slot], st.phase, abort_v);
+                ok = wait_warp(&full[st.slot], st.phase, abort_v);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t lo = tiles_lo + st.slot * (C::STAGE_BYTES / 16);
-                uint64_t* done = &empty[st.slot];
-                st.next();
-                seen = mbar_test(&full[st.slot], st.phase);
-                if (j == 3) {   // the next group's scales too
-                  sf_seen = mbar_test(&sf_full[(sf.slot + 1) % SF_SLOTS], sf.phase ^ (sf.slot + 1 == SF_SLOTS ? 1u : 0u));
-                  freed_seen = mbar_test(&sf_empty[freed.slot], freed.phase);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  if (kb + j + h < kb1) {
+                    const uint32_t lo = tiles_lo + (2 * st.slot + h) * (C::STAGE_BYTES / 16);
+                    mma_block<true>(acc, lo, lo + C::A_BYTES / 16, idesc | sf_id(j + h), sfp, sfq, kb + j + h > kb0,
+                                    &empty[2 * st.slot + h], TILE_HI, one);
+                  }
                 }
-                mma_block<true>(acc, lo, lo + C::A_BYTES / 16, idesc | sf_id(j), sfp, sfq, kb + j > kb0, done, TILE_HI, one);
+                st.next();
               }
             }
-            if (kb + 4 > kb1) sf_seen = freed_seen = 0;   // a short group: not asked
             commit_pair(&sf_empty[sf.slot], one);
             sf.next();
             buf.next();
@@ -726,36 +736,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
       if (!ok) give_up();
     }
-  } else if (warp == 2) {
-    uint32_t sf = 0;
-    bool ok = true;
-    for (int t = first; t < n_tiles && ok; t += stride) {
+  } else if (warp < 4) {
+    // warps 2 and 3 take the groups in turn, each loading its next one before
+    // it stores the present one: one warp that loaded and stored in turn took
+    // 2500 cycles for a group whose MMAs take 2048
+    const int per_tile = (g.kblocks + 3) / 4;
+    const int n_groups = (n_tiles - first + stride - 1) / stride * per_tile;   // first < n_tiles: the grid is no larger
+    ScaleWords<BN> now, then;
+    auto load = [&](ScaleWords<BN>& w4, int i) {
       int64_t p0, q0;
-      pair_origin(t, w, BN, p0, q0);
-      p0 += rank * BM;
-      for (int kg = 0; kg * 4 < g.kblocks; ++kg, ++sf) {
-        const int slot = (int)(sf % SF_SLOTS);
-        uint32_t a[4], b[2][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = scale_word(g.p, p0 + 32 * e + lane, kg);
-#pragma unroll
-        for (int c = 0; c < (BN + 127) / 128; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) b[c][e] = scale_word(g.q, q0 + 128 * c + 32 * e + lane, kg);
-        if (sf >= SF_SLOTS) ok = wait_warp(&sf_empty[slot], (sf / SF_SLOTS - 1) & 1u, abort_v);
-        if (!ok) {
-          if (lane == 0) give_up();
-          break;
-        }
-        unsigned char* dst = smem + C::SF_OFF + slot * SF_SLOT_BYTES + lane * 16;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(a[0], a[1], a[2], a[3]);
-#pragma unroll
-        for (int c = 0; c < (BN + 127) / 128; ++c)
-          *reinterpret_cast<uint4*>(dst + 512 * (c + 1)) = make_uint4(b[c][0], b[c][1], b[c][2], b[c][3]);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive_at(map_to(smem_u32(&sf_full[slot]), 0));
+      pair_origin(first + i / per_tile * stride, w, BN, p0, q0);
+      w4.load(g, p0 + rank * BM, q0, i % per_tile, lane);
+    };
+    int i = warp - 2;
+    bool ok = true;
+    if (i < n_groups) load(now, i);
+    for (; i < n_groups; i += 2) {
+      const int slot = i % SF_SLOTS;
+      if (i + 2 < n_groups) load(then, i + 2);
+      if (i >= SF_SLOTS) ok = wait_warp(&sf_empty[slot], (uint32_t)(i / SF_SLOTS - 1) & 1u, abort_v);
+      if (!ok) {
+        if (lane == 0) give_up();
+        break;
       }
+      now.store(smem + C::SF_OFF + slot * SF_SLOT_BYTES, lane);
+      __syncwarp();
+      if (lane == 0) arrive_at(map_to(smem_u32(&sf_full[slot]), 0));
+      now = then;
     }
   } else if (warp >= 4) {
     const uint32_t step = g.drop ? drop_step(d) : 0u;
@@ -814,7 +821,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (rank == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
           // whichever phase is current: it completes when its loads have landed
-          if (!mbar_wait(&full[s], 0, 1u << 12)) mbar_wait(&full[s], 1, 1u << 12);
+          if (!mbar_wait(&full[s / 2], 0, 1u << 12)) mbar_wait(&full[s / 2], 1, 1u << 12);
         }
       }
       if (g.err) *reinterpret_cast<volatile int32_t*>(g.err) = 1;
