@@ -60,6 +60,7 @@ struct GemmArgs {
   int kblocks;
   int swap;           // D[q][p] instead of D[p][q]
   int vec;            // rows of D and the residual are 16-byte aligned
+  int vec_bias;
   int drop;
   int32_t* err;
 };
@@ -150,6 +151,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -206,6 +219,13 @@ __device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
   return v;
+}
+
+// Two bf16 values, the first in the low half.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // Scale word (four consecutive K blocks) of row r; rows outside get 1.
@@ -295,7 +315,89 @@ __device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint3
   }
 }
 
-// Tile blockIdx.y (columns) x blockIdx.z... of one cluster of S CTAs along x.
+// Eight consecutive values of row p through bias, dropout and residual into D.
+// `more`: D holds the sum of K's earlier chunks; `last`: this is the last one.
+template <bool BF16>
+__device__ __forceinline__ void emit8(const GemmArgs& g, const DropSpec& d, uint32_t step, int64_t p, int64_t q0, bool more,
+                                      bool last, float (&v)[8]) {
+  if (p >= g.p.extent || q0 >= g.q.extent) return;
+  const int w = g.q.extent - q0 < 8 ? (int)(g.q.extent - q0) : 8;
+  const bool vec = g.vec && w == 8;
+  float t[8];
+  if (!BF16 && more) {
+    const float* at = static_cast<const float*>(g.d) + p * g.ldd + q0;   // not through the read-only path: D is written here
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+      if (vec) {
+        const float4 f = *reinterpret_cast<const float4*>(at + h);
+        t[h] = f.x; t[h + 1] = f.y; t[h + 2] = f.z; t[h + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = h; e < h + 4; ++e) t[e] = e < w ? at[e] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(t[e], v[e]);
+  }
+  if (last) {
+    if (g.bias) {
+      load8<BF16>(g.bias, q0, w, g.vec_bias && w == 8, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], t[e]);
+    }
+    if (g.drop) {
+      const uint32_t keep = drop_keep<8>(d, step, (uint64_t)(p * g.n + q0));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (keep >> e) & 1u ? __fmul_rn(v[e], d.scale) : 0.0f;
+    }
+    if (g.residual) {
+      load8<BF16>(g.residual, p * g.ldres + q0, w, vec, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], t[e]);
+    }
+  }
+  if (BF16) {
+    if (vec) {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.d) + p * g.ldd + q0) =
+          make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < w) static_cast<uint16_t*>(g.d)[p * g.ldd + q0 + e] = (uint16_t)bf16x2(v[e], 0.0f);
+    }
+  } else {
+    store8_f32(g.d, p * g.ldd + q0, w, vec, v);
+  }
+}
+
+// A warp's 32 x 32 block, a row per lane, turned through shared memory (4 KB of
+// the warp's own) so that four lanes hold a row's 32 columns: D, the residual
+// and the bias are then touched in whole sectors, and one Philox evaluation
+// serves a lane's eight elements.  With a row per lane the epilogue took as
+// long as the MMAs of K = 4096 (16.5k cycles a tile).
+// 16-byte piece c of row r lies at c ^ (r & 7): stores and loads touch all banks.
+template <bool BF16>
+__device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d, uint32_t step, unsigned char* turn, int64_t p0,
+                                           int64_t q0, bool more, bool last, const uint32_t (&r)[32]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(turn + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+  __syncwarp();
+  const int part = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    const float4 a = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part) ^ (row & 7)) << 4));
+    const float4 b = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part + 1) ^ (row & 7)) << 4));
+    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    emit8<BF16>(g, d, step, p0 + row, q0 + 8 * part, more, last, v);
+  }
+  __syncwarp();
+}
+
+// One 128 x BN tile, split over the S CTAs of a cluster along K.
 template <int BN, int S, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, GemmArgs g,
@@ -437,13 +539,21 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16);
   if (S == 1) {
     if (warp >= 4 && have) {
-      for (int c = 0; c < BN; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(taddr + c, r);
-        float v[16];
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        if (!g.swap) {
+          // over the ring, which is drained once the accumulator is complete
+          emit_block<BF16>(g, d, step, smem + quarter * 4096, p0 + quarter * 32, q0 + c, false, true, r);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]);
-        emit<BF16, 16>(g, d, step, p0 + row, q0 + c, v);
+          for (int h = 0; h < 2; ++h) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[16 * h + e]);
+            emit<BF16, 16>(g, d, step, p0 + row, q0 + c + 16 * h, v);
+          }
+        }
       }
     }
   } else {
@@ -495,20 +605,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// A chunk of a long float32 sum: adds what D holds of the earlier chunks and,
-// unless it is the last, leaves the sum there.  The same thread reads and
-// writes each element.
-__device__ __forceinline__ void add_chunk(const GemmArgs& g, int64_t p, int64_t q0, bool last, bool more, float (&v)[16]) {
-  if (p >= g.p.extent || q0 >= g.q.extent) return;
-  float* at = static_cast<float*>(g.d) + p * g.ldd + q0;
-  const int w = g.q.extent - q0 < 16 ? (int)(g.q.extent - q0) : 16;
-#pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (e < w) {
-      if (more) v[e] = __fadd_rn(v[e], at[e]);
-      if (!last) at[e] = v[e];
-    }
-}
 // ---- many tiles: pairs of CTAs (cta_group::2), persistent, two accumulators ----
 // A pair computes 256 x BN tiles: each CTA stages its 128 rows of P and half
 // of Q's BN rows, so a staged byte feeds twice the multiplications of the
@@ -529,7 +625,8 @@ struct PairCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = BN > 128 ? 6 : 8;   // even: blocks are staged, and waited for, in twos
   static constexpr int SF_OFF = STAGES * STAGE_BYTES;
-  static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
+  static constexpr int TURN_OFF = SF_OFF + SF_SLOTS * SF_SLOT_BYTES;
+  static constexpr int SMEM = TURN_OFF + 4 * 4096 + 1024;
   static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
   static constexpr int SF_BUFS = BN > 192 ? 2 : 3;
   static constexpr int SHARED = 2 * BN + SF_BUFS * SF_COLS > 512 ? 32 : 0;
@@ -570,18 +667,6 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t one) {
       ::"r"(smem_u32(bar)), "h"((uint16_t)3), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 // Tile t: bands of BAND row tiles, walked row-fastest, so that the tiles in
 // flight form a near-square patch and share both operands in L2.
 constexpr int BAND = 8;
@@ -766,14 +851,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else if (warp >= 4) {
     const uint32_t step = g.drop ? drop_step(d) : 0u;
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const int quarter = warp & 3;
+    unsigned char* turn = smem + C::TURN_OFF + quarter * 4096;
     const uint32_t empty_bar[2] = {map_to(smem_u32(&acc_empty[0]), 0), map_to(smem_u32(&acc_empty[1]), 0)};
     uint32_t item = 0;
     bool ok = true;
     for (int t = first; t < n_tiles && ok; t += stride) {
       int64_t p0, q0;
       pair_origin(t, w, BN, p0, q0);
-      const int64_t p = p0 + rank * BM + row;
+      const int64_t p = p0 + rank * BM + quarter * 32;
       for (int ch = 0; ch < w.chunks; ++ch, ++item) {
         const uint32_t odd = item & 1u;
         ok = wait_warp(&acc_full[odd], (item >> 1) & 1u, abort_v);
@@ -794,14 +880,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             __syncwarp();
             if (lane == 0) arrive_at(empty_bar[C::SHARED ? 0 : odd]);
           }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[16 * h + e]);
-            if (!BF16 && w.chunks > 1) add_chunk(g, p, q0 + c + 16 * h, ch == w.chunks - 1, ch > 0, v);
-            if (BF16 || ch == w.chunks - 1) emit<BF16, 16>(g, d, step, p, q0 + c + 16 * h, v);
-          }
+          emit_block<BF16>(g, d, step, turn, p, q0 + c, ch > 0, ch == w.chunks - 1, r);
         }
       }
     }
@@ -986,6 +1065,7 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   const int64_t es = a->d_dtype == ADVOPT_DT_BF16 ? 2 : 4;
   g.vec = reinterpret_cast<uintptr_t>(a->d) % 16 == 0 && a->ldd * es % 16 == 0 &&
           (!a->residual || (reinterpret_cast<uintptr_t>(a->residual) % 16 == 0 && a->ldres * es % 16 == 0));
+  g.vec_bias = reinterpret_cast<uintptr_t>(a->bias) % 16 == 0;
   g.drop = a->drop.threshold > 0;
   g.err = a->err;
   L.d = drop_spec(a->drop);
