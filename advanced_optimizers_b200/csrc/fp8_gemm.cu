@@ -386,15 +386,81 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
         make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
   __syncwarp();
   const int part = lane & 3;
+  const int64_t p = p0 + (lane >> 2), q = q0 + 8 * part;
+  float v[4][8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 8 * i + (lane >> 2);
     const float4 a = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part) ^ (row & 7)) << 4));
     const float4 b = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part + 1) ^ (row & 7)) << 4));
-    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    emit8<BF16>(g, d, step, p0 + row, q0 + 8 * part, more, last, v);
+    v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+    v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
   }
   __syncwarp();
+  if (!g.vec || p0 + 32 > g.p.extent || q0 + 32 > g.q.extent) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) emit8<BF16>(g, d, step, p + 8 * i, q, more, last, v[i]);
+    return;
+  }
+  // a whole block: the four rows' loads and stores go out together
+  if (!BF16 && more) {
+    const float* at = static_cast<const float*>(g.d) + p * g.ldd + q;
+    float4 f[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i][0] = *reinterpret_cast<const float4*>(at + 8 * i * g.ldd);
+      f[i][1] = *reinterpret_cast<const float4*>(at + 8 * i * g.ldd + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float t[8] = {f[i][0].x, f[i][0].y, f[i][0].z, f[i][0].w, f[i][1].x, f[i][1].y, f[i][1].z, f[i][1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(t[e], v[i][e]);
+    }
+  }
+  if (last) {
+    float t[4][8];
+    if (g.residual) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load8<BF16>(g.residual, (p + 8 * i) * g.ldres + q, 8, true, t[i]);
+    }
+    if (g.bias) {
+      float bias[8];
+      load8<BF16>(g.bias, q, 8, g.vec_bias, bias);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(v[i][e], bias[e]);
+    }
+    if (g.drop) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t keep = drop_keep<8>(d, step, (uint64_t)((p + 8 * i) * g.n + q));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = (keep >> e) & 1u ? __fmul_rn(v[i][e], d.scale) : 0.0f;
+      }
+    }
+    if (g.residual) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(v[i][e], t[i][e]);
+    }
+  }
+  if (BF16) {
+    uint16_t* out = static_cast<uint16_t*>(g.d) + p * g.ldd + q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(out + 8 * i * g.ldd) = make_uint4(bf16x2(v[i][0], v[i][1]), bf16x2(v[i][2], v[i][3]),
+                                                                  bf16x2(v[i][4], v[i][5]), bf16x2(v[i][6], v[i][7]));
+  } else {
+    float* out = static_cast<float*>(g.d) + p * g.ldd + q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<float4*>(out + 8 * i * g.ldd) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+      *reinterpret_cast<float4*>(out + 8 * i * g.ldd + 4) = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+    }
+  }
 }
 
 // One 128 x BN tile, split over the S CTAs of a cluster along K.
