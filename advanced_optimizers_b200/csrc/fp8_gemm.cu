@@ -151,6 +151,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// 32 accumulator columns of a lane's row.  The values are there after
+// tmem_wait32, which names them so that no use moves before it.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -160,7 +162,16 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -376,15 +387,41 @@ __device__ __forceinline__ void emit8(const GemmArgs& g, const DropSpec& d, uint
 // serves a lane's eight elements.  With a row per lane the epilogue took as
 // long as the MMAs of K = 4096 (16.5k cycles a tile).
 // 16-byte piece c of row r lies at c ^ (r & 7): stores and loads touch all banks.
-template <bool BF16>
-__device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d, uint32_t step, unsigned char* turn, int64_t p0,
-                                           int64_t q0, bool more, bool last, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void turn_in(unsigned char* turn, const uint32_t (&r)[32]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int c = 0; c < 8; ++c)
     *reinterpret_cast<uint4*>(turn + lane * 128 + ((c ^ (lane & 7)) << 4)) =
         make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
   __syncwarp();
+}
+
+// A block at D's edge, or of a D whose rows are not 16-byte aligned.
+template <bool BF16>
+__device__ __noinline__ void emit_edge(const GemmArgs& g, const DropSpec& d, uint32_t step, const unsigned char* turn,
+                                       int64_t p0, int64_t q0, bool more, bool last) {
+  const int lane = threadIdx.x & 31, part = lane & 3;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    const int row = 8 * i + (lane >> 2);
+    const float4 a = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part) ^ (row & 7)) << 4));
+    const float4 b = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part + 1) ^ (row & 7)) << 4));
+    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    emit8<BF16>(g, d, step, p0 + row, q0 + 8 * part, more, last, v);
+  }
+  __syncwarp();
+}
+
+// EXTRA: there may be a bias, a dropout or a residual.  Without one the code
+// between a block's loads and its stores is short.
+template <bool BF16, bool EXTRA>
+__device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d, uint32_t step, const unsigned char* turn,
+                                           int64_t p0, int64_t q0, bool more, bool last) {
+  if (!g.vec || p0 + 32 > g.p.extent || q0 + 32 > g.q.extent) {
+    emit_edge<BF16>(g, d, step, turn, p0, q0, more, last);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
   const int part = lane & 3;
   const int64_t p = p0 + (lane >> 2), q = q0 + 8 * part;
   float v[4][8];
@@ -397,12 +434,7 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
     v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
   }
   __syncwarp();
-  if (!g.vec || p0 + 32 > g.p.extent || q0 + 32 > g.q.extent) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) emit8<BF16>(g, d, step, p + 8 * i, q, more, last, v[i]);
-    return;
-  }
-  // a whole block: the four rows' loads and stores go out together
+  // the four rows' loads and stores go out together
   if (!BF16 && more) {
     const float* at = static_cast<const float*>(g.d) + p * g.ldd + q;
     float4 f[4][2];
@@ -418,7 +450,7 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
       for (int e = 0; e < 8; ++e) v[i][e] = __fadd_rn(t[e], v[i][e]);
     }
   }
-  if (last) {
+  if (EXTRA && last) {
     float t[4][8];
     if (g.residual) {
 #pragma unroll
@@ -466,8 +498,8 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
 // One 128 x BN tile, split over the S CTAs of a cluster along K.
 template <int BN, int S, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, GemmArgs g,
-                DropSpec d) {
+    gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                const __grid_constant__ GemmArgs g, const __grid_constant__ DropSpec d) {
   using C = Cfg<BN>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -605,12 +637,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16);
   if (S == 1) {
     if (warp >= 4 && have) {
+#pragma unroll 1
       for (int c = 0; c < BN; c += 32) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
+        tmem_wait32(r);
         if (!g.swap) {
           // over the ring, which is drained once the accumulator is complete
-          emit_block<BF16>(g, d, step, smem + quarter * 4096, p0 + quarter * 32, q0 + c, false, true, r);
+          unsigned char* turn = smem + quarter * 4096;
+          turn_in(turn, r);
+          emit_block<BF16, true>(g, d, step, turn, p0 + quarter * 32, q0 + c, false, true);
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -689,12 +725,14 @@ template <int BN>
 struct PairCfg {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN > 128 ? 6 : 8;   // even: blocks are staged, and waited for, in twos
+  static constexpr int STAGES = 6;   // even: blocks are staged, and waited for, in twos
   static constexpr int SF_OFF = STAGES * STAGE_BYTES;
   static constexpr int TURN_OFF = SF_OFF + SF_SLOTS * SF_SLOT_BYTES;
-  static constexpr int SMEM = TURN_OFF + 4 * 4096 + 1024;
+  static constexpr int EPI = BN > 224 ? 4 : 8;   // epilogue warps: as many as there is shared memory to turn blocks in
+  static constexpr int SMEM = TURN_OFF + EPI * 4096 + 1024;
+  static constexpr int THREADS = 128 + 32 * EPI;
   static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
-  static constexpr int SF_BUFS = BN > 192 ? 2 : 3;
+  static constexpr int SF_BUFS = BN > 224 ? 2 : 3;
   static constexpr int SHARED = 2 * BN + SF_BUFS * SF_COLS > 512 ? 32 : 0;
   static constexpr int ACC_STRIDE = BN - SHARED;
   static constexpr int SF_COL = BN + ACC_STRIDE;
@@ -743,10 +781,10 @@ __device__ __forceinline__ void pair_origin(int t, const PairArgs& w, int bn, in
   q0 = (int64_t)(r / rows) * bn;
 }
 
-template <int BN, bool BF16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, GemmArgs g,
-                PairArgs w, DropSpec d) {
+template <int BN, bool BF16, bool EXTRA>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                const __grid_constant__ GemmArgs g, const __grid_constant__ PairArgs w, const __grid_constant__ DropSpec d) {
   using C = PairCfg<BN>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -777,8 +815,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     mbar_init(&acc_full[0], 1);
     mbar_init(&acc_full[1], 1);
-    mbar_init(&acc_empty[0], 8);
-    mbar_init(&acc_empty[1], 8);
+    mbar_init(&acc_empty[0], 2 * C::EPI);
+    mbar_init(&acc_empty[1], 2 * C::EPI);
     mbar_init(&drain, 1);
     abort_flag = 0;
     mbar_fence_init();
@@ -917,8 +955,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else if (warp >= 4) {
     const uint32_t step = g.drop ? drop_step(d) : 0u;
-    const int quarter = warp & 3;
-    unsigned char* turn = smem + C::TURN_OFF + quarter * 4096;
+    const int quarter = warp & 3, share = (warp - 4) >> 2;
+    unsigned char* turn = smem + C::TURN_OFF + (warp - 4) * 4096;
     const uint32_t empty_bar[2] = {map_to(smem_u32(&acc_empty[0]), 0), map_to(smem_u32(&acc_empty[1]), 0)};
     uint32_t item = 0;
     bool ok = true;
@@ -935,18 +973,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16) + odd * C::ACC_STRIDE;
+        // this warp's blocks: every EPI / 4-th of the tile's.  The columns shared
+        // with the other accumulator come first.
+        constexpr int BLOCKS = BN / 32, SHARE = C::EPI / 4;
+        const int mine = (BLOCKS - share + SHARE - 1) / SHARE;
+        auto column = [&](int i) {
+          const int b = share + i * SHARE;
+          return 32 * (C::SHARED && !odd ? (b == 0 ? BLOCKS - 1 : b - 1) : b);
+        };
+        auto release = [&]() {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive_at(empty_bar[C::SHARED ? 0 : odd]);
+        };
+        uint32_t r[32];
+        tmem_ld32(taddr + column(0), r);
+        tmem_wait32(r);
+        if (C::SHARED || mine == 1) release();
+        // one copy of the loop's body: unrolled, it ran into instruction cache misses
 #pragma unroll 1
-        for (int i = 0; i < BN / 32; ++i) {
-          // the columns shared with the other accumulator come first
-          const int c = 32 * (C::SHARED && !odd ? (i == 0 ? BN / 32 - 1 : i - 1) : i);
-          uint32_t r[32];
-          tmem_ld32(taddr + c, r);
-          if (i == (C::SHARED ? 0 : BN / 32 - 1)) {
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) arrive_at(empty_bar[C::SHARED ? 0 : odd]);
+        for (int i = 0; i < mine; ++i) {
+          turn_in(turn, r);
+          if (i + 1 < mine) tmem_ld32(taddr + column(i + 1), r);   // on its way while this block goes out
+          emit_block<BF16, EXTRA>(g, d, step, turn, p, q0 + column(i), ch > 0, ch == w.chunks - 1);
+          if (i + 1 < mine) {
+            tmem_wait32(r);
+            if (!C::SHARED && i + 2 == mine) release();
           }
-          emit_block<BF16>(g, d, step, turn, p, q0 + c, ch > 0, ch == w.chunks - 1, r);
         }
       }
     }
@@ -1048,7 +1101,8 @@ int launch_pair(const Launch& L) {
   int rc = encode_map(&mp, L.p, L.g.p.extent, L.k, L.ldp, BM);
   if (rc == ADVOPT_OK) rc = encode_map(&mq, L.q, L.g.q.extent, L.k, L.ldq, BN / 2);
   if (rc != ADVOPT_OK) return rc;
-  const auto kernel = pair_kernel<BN, BF16>;
+  const bool extra = L.g.bias || L.g.residual || L.g.drop;
+  const auto kernel = extra ? pair_kernel<BN, BF16, true> : pair_kernel<BN, BF16, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
   PairArgs w;
@@ -1059,7 +1113,7 @@ int launch_pair(const Launch& L) {
   w.chunk_blocks = ((L.g.kblocks + w.chunks - 1) / w.chunks + 3) / 4 * 4;
   w.chunks = (L.g.kblocks + w.chunk_blocks - 1) / w.chunk_blocks;
   const int tiles = w.p_tiles * w.q_tiles;
-  kernel<<<2 * (tiles < PAIRS ? tiles : PAIRS), THREADS, C::SMEM, L.stream>>>(mp, mq, L.g, w, L.d);
+  kernel<<<2 * (tiles < PAIRS ? tiles : PAIRS), C::THREADS, C::SMEM, L.stream>>>(mp, mq, L.g, w, L.d);
   return check_cuda(cudaGetLastError(), "advopt_fp8_gemm");
 }
 
@@ -1111,7 +1165,7 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   fp8::Launch L;
   const fp8::Side A{a->sa, a->ldsa, a->m, a->a_tile ? 7 : 0, a->a_code};
   const fp8::Side B{a->sb, a->ldsb, a->n, a->b_tile ? 7 : 0, a->b_code};
-  const bool swap = a->m <= 128 && a->n > a->m;
+  const bool swap = getenv("FP8_SWAP") ? atoi(getenv("FP8_SWAP")) : a->m <= 128 && a->n > a->m;
   fp8::GemmArgs& g = L.g;
   g.p = swap ? B : A;
   g.q = swap ? A : B;
@@ -1136,17 +1190,18 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   g.err = a->err;
   L.d = drop_spec(a->drop);
   L.stream = static_cast<cudaStream_t>(stream);
-  const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
-  if (force ? force < 3000 : (a->m > 256 && a->n > 256 && ((a->m + 255) / 256) * ((a->n + 255) / 256) >= 40)) {
-    const int bn = force ? force : 256;
-    if (a->d_dtype == ADVOPT_DT_BF16)
-      return bn == 256 ? fp8::launch_pair<256, true>(L) : bn == 192 ? fp8::launch_pair<192, true>(L) : fp8::launch_pair<128, true>(L);
-    return bn == 256 ? fp8::launch_pair<256, false>(L) : bn == 192 ? fp8::launch_pair<192, false>(L) : fp8::launch_pair<128, false>(L);
-  }
   const int64_t q = g.q.extent;
-  const int bn = q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256;
+  int bn = q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256;
   const int64_t tiles = ((g.p.extent + 127) / 128) * ((q + bn - 1) / bn);
   int split = 1;
   while (split < 8 && tiles * split * 2 <= 148 && nb >= 8 * split) split *= 2;
+  const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
+  if (force > 1000) { bn = force % 1000; split = force / 1000; }
+  if (force ? force < 1000 : (a->m > 256 && a->n > 256 && ((a->m + 255) / 256) * ((a->n + 255) / 256) >= 40)) {
+    const int bn = force ? force : 256;
+    if (a->d_dtype == ADVOPT_DT_BF16)
+      return bn == 256 ? fp8::launch_pair<256, true>(L) : bn == 224 ? fp8::launch_pair<224, true>(L) : bn == 192 ? fp8::launch_pair<192, true>(L) : fp8::launch_pair<128, true>(L);
+    return bn == 256 ? fp8::launch_pair<256, false>(L) : bn == 224 ? fp8::launch_pair<224, false>(L) : bn == 192 ? fp8::launch_pair<192, false>(L) : fp8::launch_pair<128, false>(L);
+  }
   return a->d_dtype == ADVOPT_DT_BF16 ? fp8::launch_n<true>(L, bn, split) : fp8::launch_n<false>(L, bn, split);
 }
