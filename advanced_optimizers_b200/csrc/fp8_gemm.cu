@@ -25,7 +25,6 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <cstdlib>
 #include <mutex>
 
 #include "advopt.h"
@@ -67,7 +66,7 @@ struct GemmArgs {
 
 template <int BN>
 struct Cfg {
-  static constexpr int STAGES = BN >= 256 ? 4 : 6;
+  static constexpr int STAGES = BN >= 256 || BN <= 32 ? 4 : 6;
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int SF_OFF = STAGES * STAGE_BYTES;
@@ -140,15 +139,6 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t one) {
       "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n"
       ::"r"(smem_u32(bar)), "r"(one)
       : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // 32 accumulator columns of a lane's row.  The values are there after
@@ -239,6 +229,14 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   return r;
 }
 
+__device__ __forceinline__ float4 peer_float4(uint32_t saddr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote));
+  return v;
+}
+
 // Scale word (four consecutive K blocks) of row r; rows outside get 1.
 __device__ __forceinline__ uint32_t scale_word(const Side& s, int64_t r, int group) {
   if (r >= s.extent) return 0x7F7F7F7Fu;
@@ -267,117 +265,26 @@ struct ScaleWords {
   }
 };
 
-// W accumulator values of lane p, columns q0 .. q0 + W - 1, through bias, dropout and residual into D.
+// Swapped operands: W tokens (columns) of feature p, one of D's columns per lane.
 template <bool BF16, int W>
 __device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint32_t step, int64_t p, int64_t q0,
                                      float (&v)[W]) {
   if (p >= g.p.extent || q0 >= g.q.extent) return;
   const int w = g.q.extent - q0 < W ? (int)(g.q.extent - q0) : W;
-  const uint16_t* bias_h = static_cast<const uint16_t*>(g.bias);
-  const float* bias_f = static_cast<const float*>(g.bias);
-  if (g.swap) {
-    const float b = !g.bias ? 0.0f : BF16 ? bf16_to_f(bias_h[p]) : bias_f[p];
+  const float b = !g.bias ? 0.0f
+                  : BF16  ? bf16_to_f(static_cast<const uint16_t*>(g.bias)[p])
+                          : static_cast<const float*>(g.bias)[p];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      if (j >= w) break;
-      float x = __fadd_rn(v[j], b);
-      if (g.drop) x = drop_keep1(d, step, (uint64_t)((q0 + j) * g.n + p)) ? __fmul_rn(x, d.scale) : 0.0f;
-      if (g.residual)
-        x = __fadd_rn(x, BF16 ? bf16_to_f(static_cast<const uint16_t*>(g.residual)[(q0 + j) * g.ldres + p])
-                              : static_cast<const float*>(g.residual)[(q0 + j) * g.ldres + p]);
-      if (BF16) static_cast<uint16_t*>(g.d)[(q0 + j) * g.ldd + p] = (uint16_t)f_to_bf16_rne(x);
-      else static_cast<float*>(g.d)[(q0 + j) * g.ldd + p] = x;
-    }
-    return;
-  }
-  if (g.bias) {
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (j < w) v[j] = __fadd_rn(v[j], BF16 ? bf16_to_f(bias_h[q0 + j]) : bias_f[q0 + j]);
-  }
-  if (g.drop) {
-    const uint32_t keep = drop_keep<W>(d, step, (uint64_t)(p * g.n + q0));
-#pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = (keep >> j) & 1u ? __fmul_rn(v[j], d.scale) : 0.0f;
-  }
-#pragma unroll
-  for (int c = 0; c < W; c += 8) {
-    constexpr int STEP = W < 8 ? W : 8;
-    const int left = w - c;
-    if (left <= 0) break;
-    const bool vec = STEP == 8 && g.vec && left >= 8;
-    if (g.residual) {
-      float r[8];
-      load8<BF16>(g.residual, p * g.ldres + q0 + c, left < STEP ? left : STEP, vec, r);
-#pragma unroll
-      for (int e = 0; e < STEP; ++e) v[c + e] = __fadd_rn(v[c + e], r[e]);
-    }
-    if (BF16) {
-      uint32_t u[8];
-#pragma unroll
-      for (int e = 0; e < STEP; ++e) u[e] = f_to_bf16_rne(v[c + e]);
-      store8_bf16(g.d, p * g.ldd + q0 + c, left < STEP ? left : STEP, vec, u);
-    } else {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < STEP; ++e) x[e] = v[c + e];
-      store8_f32(g.d, p * g.ldd + q0 + c, left < STEP ? left : STEP, vec, x);
-    }
-  }
-}
-
-// Eight consecutive values of row p through bias, dropout and residual into D.
-// `more`: D holds the sum of K's earlier chunks; `last`: this is the last one.
-template <bool BF16>
-__device__ __forceinline__ void emit8(const GemmArgs& g, const DropSpec& d, uint32_t step, int64_t p, int64_t q0, bool more,
-                                      bool last, float (&v)[8]) {
-  if (p >= g.p.extent || q0 >= g.q.extent) return;
-  const int w = g.q.extent - q0 < 8 ? (int)(g.q.extent - q0) : 8;
-  const bool vec = g.vec && w == 8;
-  float t[8];
-  if (!BF16 && more) {
-    const float* at = static_cast<const float*>(g.d) + p * g.ldd + q0;   // not through the read-only path: D is written here
-#pragma unroll
-    for (int h = 0; h < 8; h += 4) {
-      if (vec) {
-        const float4 f = *reinterpret_cast<const float4*>(at + h);
-        t[h] = f.x; t[h + 1] = f.y; t[h + 2] = f.z; t[h + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int e = h; e < h + 4; ++e) t[e] = e < w ? at[e] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(t[e], v[e]);
-  }
-  if (last) {
-    if (g.bias) {
-      load8<BF16>(g.bias, q0, w, g.vec_bias && w == 8, t);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], t[e]);
-    }
-    if (g.drop) {
-      const uint32_t keep = drop_keep<8>(d, step, (uint64_t)(p * g.n + q0));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (keep >> e) & 1u ? __fmul_rn(v[e], d.scale) : 0.0f;
-    }
-    if (g.residual) {
-      load8<BF16>(g.residual, p * g.ldres + q0, w, vec, t);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = __fadd_rn(v[e], t[e]);
-    }
-  }
-  if (BF16) {
-    if (vec) {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.d) + p * g.ldd + q0) =
-          make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < w) static_cast<uint16_t*>(g.d)[p * g.ldd + q0 + e] = (uint16_t)bf16x2(v[e], 0.0f);
-    }
-  } else {
-    store8_f32(g.d, p * g.ldd + q0, w, vec, v);
+  for (int j = 0; j < W; ++j) {
+    if (j >= w) break;
+    float x = v[j];
+    if (g.bias) x = __fadd_rn(x, b);
+    if (g.drop) x = drop_keep1(d, step, (uint64_t)((q0 + j) * g.n + p)) ? __fmul_rn(x, d.scale) : 0.0f;
+    if (g.residual)
+      x = __fadd_rn(x, BF16 ? bf16_to_f(static_cast<const uint16_t*>(g.residual)[(q0 + j) * g.ldres + p])
+                            : static_cast<const float*>(g.residual)[(q0 + j) * g.ldres + p]);
+    if (BF16) static_cast<uint16_t*>(g.d)[(q0 + j) * g.ldd + p] = (uint16_t)bf16x2(x, 0.0f);
+    else static_cast<float*>(g.d)[(q0 + j) * g.ldd + p] = x;
   }
 }
 
@@ -396,18 +303,59 @@ __device__ __forceinline__ void turn_in(unsigned char* turn, const uint32_t (&r)
   __syncwarp();
 }
 
-// A block at D's edge, or of a D whose rows are not 16-byte aligned.
+// A block at D's edge, or of a D whose rows are not 16-byte aligned: a column
+// per lane and a row at a time, so that what a warp touches is still contiguous
+// (with eight columns a lane, 333 x 2041 took 29 us instead of 10).
+__device__ __forceinline__ float turned(const unsigned char* turn, int r, int lane) {
+  return *reinterpret_cast<const float*>(turn + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + ((lane & 3) << 2));
+}
+template <bool BF16>
+__device__ __noinline__ void store_edge(void* d, int64_t ldd, const unsigned char* turn, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+  if (lane < cols) {
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) x[r] = turned(turn, r0 + r, lane);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r0 + r < rows) {
+          if (BF16) static_cast<uint16_t*>(d)[(r0 + r) * ldd + lane] = (uint16_t)bf16x2(x[r], 0.0f);
+          else static_cast<float*>(d)[(r0 + r) * ldd + lane] = x[r];
+        }
+    }
+  }
+  __syncwarp();
+}
 template <bool BF16>
 __device__ __noinline__ void emit_edge(const GemmArgs& g, const DropSpec& d, uint32_t step, const unsigned char* turn,
                                        int64_t p0, int64_t q0, bool more, bool last) {
-  const int lane = threadIdx.x & 31, part = lane & 3;
-#pragma unroll 1
-  for (int i = 0; i < 4; ++i) {
-    const int row = 8 * i + (lane >> 2);
-    const float4 a = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part) ^ (row & 7)) << 4));
-    const float4 b = *reinterpret_cast<const float4*>(turn + row * 128 + (((2 * part + 1) ^ (row & 7)) << 4));
-    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    emit8<BF16>(g, d, step, p0 + row, q0 + 8 * part, more, last, v);
+  const int lane = threadIdx.x & 31;
+  const int64_t q = q0 + lane;
+  const int rows = g.p.extent - p0 < 32 ? (int)(g.p.extent - p0) : 32;
+  if (q < g.q.extent) {
+    const bool drop = g.drop, add = g.residual && last;
+    const float bias = !last || !g.bias ? 0.0f
+                       : BF16           ? bf16_to_f(static_cast<const uint16_t*>(g.bias)[q])
+                                        : static_cast<const float*>(g.bias)[q];
+    const bool biased = last && g.bias;
+    const int64_t ldd = g.ldd, ldres = g.ldres;
+    void* at = BF16 ? (void*)(static_cast<uint16_t*>(g.d) + p0 * ldd + q) : (void*)(static_cast<float*>(g.d) + p0 * ldd + q);
+    const void* res = BF16 ? (const void*)(static_cast<const uint16_t*>(g.residual) + p0 * ldres + q)
+                           : (const void*)(static_cast<const float*>(g.residual) + p0 * ldres + q);
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      float x = turned(turn, r, lane);
+      const float t = !add ? 0.0f : BF16 ? bf16_to_f(static_cast<const uint16_t*>(res)[r * ldres])
+                                         : static_cast<const float*>(res)[r * ldres];
+      if (!BF16 && more) x = __fadd_rn(static_cast<const float*>(at)[r * ldd], x);
+      if (biased) x = __fadd_rn(x, bias);
+      if (drop && last) x = drop_keep1(d, step, (uint64_t)((p0 + r) * g.n + q)) ? __fmul_rn(x, d.scale) : 0.0f;
+      if (add) x = __fadd_rn(x, t);
+      if (BF16) static_cast<uint16_t*>(at)[r * ldd] = (uint16_t)bf16x2(x, 0.0f);
+      else static_cast<float*>(at)[r * ldd] = x;
+    }
   }
   __syncwarp();
 }
@@ -418,7 +366,15 @@ template <bool BF16, bool EXTRA>
 __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d, uint32_t step, const unsigned char* turn,
                                            int64_t p0, int64_t q0, bool more, bool last) {
   if (!g.vec || p0 + 32 > g.p.extent || q0 + 32 > g.q.extent) {
-    emit_edge<BF16>(g, d, step, turn, p0, q0, more, last);
+    if (p0 >= g.p.extent || q0 >= g.q.extent) {
+      __syncwarp();
+    } else if (more || (EXTRA && last && (g.bias || g.drop || g.residual))) {
+      emit_edge<BF16>(g, d, step, turn, p0, q0, more, last);
+    } else {
+      const int64_t at = p0 * g.ldd + q0, rows = g.p.extent - p0, cols = g.q.extent - q0;
+      store_edge<BF16>(BF16 ? (void*)(static_cast<uint16_t*>(g.d) + at) : (void*)(static_cast<float*>(g.d) + at), g.ldd, turn,
+                       rows < 32 ? (int)rows : 32, cols < 32 ? (int)cols : 32);
+    }
     return;
   }
   const int lane = threadIdx.x & 31;
@@ -497,7 +453,7 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
 
 // One 128 x BN tile, split over the S CTAs of a cluster along K.
 template <int BN, int S, bool BF16>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                 const __grid_constant__ GemmArgs g, const __grid_constant__ DropSpec d) {
   using C = Cfg<BN>;
@@ -659,31 +615,66 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else {
-    // the ring is drained once the accumulator is complete: [column][row] floats over it
+    // over the ring, which is drained once the accumulator is complete.  Rank r
+    // adds up columns r BN / S ..: swapped, [column][row] floats, a row (one of
+    // D's columns) per lane; else the turned 32 x 32 blocks, so that D's rows
+    // are written in whole sectors.
     float* acc = reinterpret_cast<float*>(smem);
     if (warp >= 4 && have) {
-      for (int c = 0; c < BN; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(taddr + c, r);
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c, r);
+        tmem_wait32(r);
+        if (!nkb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[(c + e) * BM + row] = nkb ? __uint_as_float(r[e]) : 0.0f;
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+        if (g.swap) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[(c + e) * BM + row] = __uint_as_float(r[e]);
+        } else {
+          turn_in(smem + (c / 32 * 4 + quarter) * 4096, r);
+        }
       }
     }
     __syncwarp();
     cluster_sync();
     if (warp >= 4 && have) {
-      constexpr int PER = BN / S, W = PER < 16 ? PER : 16;
+      if (g.swap) {
+        constexpr int PER = BN / S, W = PER < 16 ? PER : 16;
 #pragma unroll 1
-      for (int c = 0; c < PER; c += W) {
-        float v[W];
+        for (int c = 0; c < PER; c += W) {
+          float v[W];
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const uint32_t at = smem_u32(acc + (rank * PER + c + e) * BM + row);
-          v[e] = peer_float(at, 0);
+          for (int e = 0; e < W; ++e) {
+            const uint32_t at = smem_u32(acc + (rank * PER + c + e) * BM + row);
+            v[e] = peer_float(at, 0);
 #pragma unroll
-          for (int o = 1; o < S; ++o) v[e] = __fadd_rn(v[e], peer_float(at, o));
+            for (int o = 1; o < S; ++o) v[e] = __fadd_rn(v[e], peer_float(at, o));
+          }
+          emit<BF16, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
         }
-        emit<BF16, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
+      } else {
+        // the tile's 4 BN / 32 blocks, dealt out to the cluster's 4 S warps
+        constexpr int BLOCKS = 4 * BN / 32;
+#pragma unroll 1
+        for (int b = quarter * S + (int)rank; b < BLOCKS; b += 4 * S) {
+          unsigned char* turn = smem + b * 4096;
+          unsigned char* own = smem + BLOCKS * 4096 + quarter * 4096;   // this block's sum
+#pragma unroll 4
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t at = smem_u32(turn + (i * 32 + lane) * 16);
+            float4 x = peer_float4(at, 0);
+#pragma unroll
+            for (int o = 1; o < S; ++o) {
+              const float4 y = peer_float4(at, o);
+              x = make_float4(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y), __fadd_rn(x.z, y.z), __fadd_rn(x.w, y.w));
+            }
+            *reinterpret_cast<float4*>(own + (i * 32 + lane) * 16) = x;
+          }
+          __syncwarp();
+          emit_block<BF16, true>(g, d, step, own, p0 + (b & 3) * 32, q0 + b / 4 * 32, false, true);
+        }
       }
     }
     __syncwarp();
@@ -1137,6 +1128,84 @@ int launch_n(const Launch& L, int bn, int split) {
   }
 }
 
+// Which kernel, tile and split a shape gets: the least of an estimate in
+// microseconds whose constants come from timing every variant on about forty
+// shapes of 1 x 1024 .. 8192 x 14336 x 14336 on one B200 (back to back calls,
+// cold operands).  Over those shapes the variant it picks is within 5% of the
+// fastest one (geometric mean).  What it weighs:
+//   * pairs (256 x BN tiles): a K block costs the MMAs' 2 BN cycles, more below
+//     BN = 256 where the staged bytes per MMA grow (475 / 440 / 400); BN = 256
+//     waits 2800 cycles between tiles for the shared accumulator columns, so
+//     8192 x 14336 x 4096 takes 336 us at 256 and 322 at 224, and
+//     8192 x 4096 x 14336 324 and 359;
+//   * single CTAs (128 x BN): a K block costs what 16 KB + BN * 128 bytes take
+//     from L2 (290 .. 680 cycles); splitting K pays a cluster's exchange:
+//     1 x 4096 x 4096 takes 11.5 / 9.0 / 7.7 / 8.0 us split 1 / 2 / 4 / 8,
+//     256 x 4096 x 4096 at BN = 64 10.6 us unsplit, at BN = 128 11.9 split in 2;
+//   * swapped operands write D a token at a time, a feature per lane, whatever
+//     D's alignment: 333 x 2041 x 1000 takes 6.9 us swapped, 8.3 not.
+struct Variant {
+  bool pair, swap;
+  int bn, split;
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+inline Variant choose(int64_t m, int64_t n, int64_t kblocks, bool whole_rows, bool f32) {
+  Variant best{false, false, 32, 1};
+  double least = 1e300;
+  static constexpr int single_bn[4] = {32, 64, 128, 256}, pair_bn[4] = {256, 224, 192, 128};
+  static constexpr double single_block[4] = {330, 340, 440, 680}, pair_block[4] = {512, 475, 440, 400};
+  static constexpr double pair_gap[4] = {2800, 400, 400, 400}, pair_out[4] = {10000, 8500, 7500, 5500};
+  for (int swap = 0; swap < 2; ++swap) {
+    const int64_t p = swap ? n : m, q = swap ? m : n;
+    for (int lg = 0; lg < 4; ++lg) {
+      const int split = 1 << lg;
+      if (split > 1 && ceil_div(kblocks, 4) < split) break;
+      for (int i = 0; i < 4; ++i) {
+        const int bn = single_bn[i];
+        if (i > 0 && bn >= 2 * q) break;
+        const double ctas = (double)ceil_div(p, 128) * ceil_div(q, bn) * split;
+        const double waves = ceil_div((int64_t)ctas, i == 0 ? 2 * SMS : SMS);   // BN = 32: two CTAs fit an SM
+        double block = single_block[i];
+        if (i == 0) block = ctas > SMS ? 500 : ctas * 330 / SMS > 170 ? ctas * 330 / SMS : 170;
+        const int64_t blocks = 4 * ceil_div(ceil_div(kblocks, 4), split);
+        if (f32 && blocks > CHUNK && split < 8 && ceil_div(kblocks, 4) >= 2 * split) continue;   // float32 sums stay short
+        const double body = (double)(blocks < kblocks ? blocks : kblocks) * block / 1800;
+        const double out = bn / 32 * (swap ? 0.35 : whole_rows ? 0.3 : 0.8) / split;
+        const double join = split == 1 ? 0 : bn / 32 * 0.3 + (split == 2 ? 1.0 : split == 4 ? 1.2 : i == 0 ? 1.5 : 6.0);
+        const double t = 2.8 + (waves - 1) * (body + out + 1.2) + body + out + join;
+        if (t < least) {
+          least = t;
+          best = Variant{false, swap != 0, bn, split};
+        }
+      }
+    }
+  }
+  for (int i = 0; i < 4; ++i) {
+    const double waves = (double)ceil_div(ceil_div(m, 256) * ceil_div(n, pair_bn[i]), PAIRS);
+    const double tile = (double)kblocks * pair_block[i] + pair_gap[i];
+    const double t = 4.0 + (waves * (tile > 0.7 * pair_out[i] ? tile : 0.7 * pair_out[i]) + 0.8 * pair_out[i]) / 1750;
+    if (t < least) {
+      least = t;
+      best = Variant{true, false, pair_bn[i], 1};
+    }
+  }
+  return best;
+}
+
+// advopt_fp8_gemm_args.variant: BN of a pair kernel, or 1000 * split + BN of a
+// single-CTA kernel, plus 100000 with the operands swapped.
+inline bool named(int32_t code, int64_t groups, Variant* v) {
+  if (code < 0) return false;
+  const int swap = code / 100000, split = code % 100000 / 1000, bn = code % 1000;
+  *v = Variant{split == 0, swap == 1, bn, split ? split : 1};
+  if (swap > 1) return false;
+  if (v->pair) return !swap && (bn == 128 || bn == 192 || bn == 224 || bn == 256);
+  return (bn == 32 || bn == 64 || bn == 128 || bn == 256) && (split == 1 || split == 2 || split == 4 || split == 8) &&
+         split <= groups;
+}
+
 }  // namespace fp8
 }  // namespace advopt
 
@@ -1165,7 +1234,11 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   fp8::Launch L;
   const fp8::Side A{a->sa, a->ldsa, a->m, a->a_tile ? 7 : 0, a->a_code};
   const fp8::Side B{a->sb, a->ldsb, a->n, a->b_tile ? 7 : 0, a->b_code};
-  const bool swap = getenv("FP8_SWAP") ? atoi(getenv("FP8_SWAP")) : a->m <= 128 && a->n > a->m;
+  const bool bf16 = a->d_dtype == ADVOPT_DT_BF16;
+  fp8::Variant v = fp8::choose(a->m, a->n, nb, a->n * (bf16 ? 2 : 4) % 16 == 0, !bf16);
+  if (a->variant && !fp8::named(a->variant, (nb + 3) / 4, &v))
+    return set_error(ADVOPT_E_INVALID, "advopt_fp8_gemm: no such variant for this shape");
+  const bool swap = v.swap;
   fp8::GemmArgs& g = L.g;
   g.p = swap ? B : A;
   g.q = swap ? A : B;
@@ -1190,18 +1263,13 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
   g.err = a->err;
   L.d = drop_spec(a->drop);
   L.stream = static_cast<cudaStream_t>(stream);
-  const int64_t q = g.q.extent;
-  int bn = q <= 32 ? 32 : q <= 64 ? 64 : q <= 128 ? 128 : 256;
-  const int64_t tiles = ((g.p.extent + 127) / 128) * ((q + bn - 1) / bn);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 148 && nb >= 8 * split) split *= 2;
-  const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
-  if (force > 1000) { bn = force % 1000; split = force / 1000; }
-  if (force ? force < 1000 : (a->m > 256 && a->n > 256 && ((a->m + 255) / 256) * ((a->n + 255) / 256) >= 40)) {
-    const int bn = force ? force : 256;
-    if (a->d_dtype == ADVOPT_DT_BF16)
-      return bn == 256 ? fp8::launch_pair<256, true>(L) : bn == 224 ? fp8::launch_pair<224, true>(L) : bn == 192 ? fp8::launch_pair<192, true>(L) : fp8::launch_pair<128, true>(L);
-    return bn == 256 ? fp8::launch_pair<256, false>(L) : bn == 224 ? fp8::launch_pair<224, false>(L) : bn == 192 ? fp8::launch_pair<192, false>(L) : fp8::launch_pair<128, false>(L);
+  if (v.pair) {
+    switch (v.bn) {
+      case 256: return bf16 ? fp8::launch_pair<256, true>(L) : fp8::launch_pair<256, false>(L);
+      case 224: return bf16 ? fp8::launch_pair<224, true>(L) : fp8::launch_pair<224, false>(L);
+      case 192: return bf16 ? fp8::launch_pair<192, true>(L) : fp8::launch_pair<192, false>(L);
+      default: return bf16 ? fp8::launch_pair<128, true>(L) : fp8::launch_pair<128, false>(L);
+    }
   }
-  return a->d_dtype == ADVOPT_DT_BF16 ? fp8::launch_n<true>(L, bn, split) : fp8::launch_n<false>(L, bn, split);
+  return bf16 ? fp8::launch_n<true>(L, v.bn, v.split) : fp8::launch_n<false>(L, v.bn, v.split);
 }

@@ -192,7 +192,7 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.flo
     return (r, c) if layout == "both" else r if layout == "rows" else c
 
 
-def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP):
+def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP, variant=0):
     m, n = out.shape
     dev = out.device
     with on_device(dev):
@@ -201,7 +201,7 @@ def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP):
                        b.codes.data_ptr(), b.ld, b.scales.data_ptr(), b.lds, out.data_ptr(), n,
                        0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n,
                        m, n, a.k, _CODE[a.codes.dtype], _CODE[b.codes.dtype], a.square, b.square,
-                       dtype_code(out.dtype), 0, _ERR.pointer(), *drop), raw_stream(dev)),
+                       dtype_code(out.dtype), variant, _ERR.pointer(), *drop), raw_stream(dev)),
             "advopt_fp8_gemm")
     return out
 

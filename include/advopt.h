@@ -664,7 +664,10 @@ typedef struct advopt_fp8_gemm_args {
   int32_t a_tile;           /* 0: a scale row per row, 1: per 128 rows         */
   int32_t b_tile;
   int32_t d_dtype;          /* ADVOPT_DT_*                                     */
-  int32_t pad;
+  int32_t variant;          /* 0: chosen by the shape.  Else, for tests and tuning: BN (128,
+                               192, 224, 256) of a CTA pair's 256 x BN tile, or 1000 * split
+                               + BN (32, 64, 128, 256) of one CTA's 128 x BN tile, K split
+                               over 1, 2, 4 or 8 CTAs; + 100000: D^T = B A^T           */
   int32_t* err;             /* set to 1 if a bounded wait gave up (or NULL)    */
   advopt_dropout_spec drop;
 } advopt_fp8_gemm_args;

@@ -81,7 +81,7 @@ def test_quantize_c_refusals(bad):
 def gemm_args(**kw):
     from advanced_optimizers_b200 import fp8
     f = dict(a=4096, lda=256, sa=1024, ldsa=4, b=8192, ldb=256, sb=2048, ldsb=4, d=65536, ldd=128, bias=0, residual=0, ldres=128,
-             m=4, n=128, k=256, a_code=0, b_code=0, a_tile=0, b_tile=0, d_dtype=1, pad=0, err=0, seed=1, step_dev=0, site=0,
+             m=4, n=128, k=256, a_code=0, b_code=0, a_tile=0, b_tile=0, d_dtype=1, variant=0, err=0, seed=1, step_dev=0, site=0,
              step=0, threshold=0, scale=1.0)
     f.update(kw)
     return fp8._GEMM.pack(*f.values())
@@ -91,7 +91,8 @@ def gemm_args(**kw):
                                  dict(d_dtype=2), dict(a_code=2), dict(b_code=-1), dict(a=4104), dict(b=8200), dict(lda=248),
                                  dict(ldb=240), dict(sa=1026), dict(ldsa=2), dict(ldsb=0), dict(sb=2049), dict(ldd=127),
                                  dict(residual=4096, ldres=100), dict(threshold=1 << 20), dict(step_dev=1), dict(m=1 << 31),
-                                 dict(n=1 << 31, ldd=1 << 31)])
+                                 dict(n=1 << 31, ldd=1 << 31), dict(variant=160),
+                                 dict(variant=-1), dict(variant=100256), dict(variant=3128), dict(variant=8032), dict(variant=201128)])
 def test_gemm_c_refusals(bad):
     from advanced_optimizers_b200 import _lib as L
     assert L.lib().advopt_fp8_gemm(gemm_args(**bad), None) in (-1, -3)

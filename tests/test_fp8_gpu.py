@@ -162,6 +162,36 @@ def test_matmul(m, n, k, out):
     A.check_fp8_errors()
 
 
+VARIANTS = [256, 224, 192, 128] + [swap + 1000 * split + bn for swap in (0, 100000) for split in (1, 2, 4, 8)
+                                   for bn in (32, 64, 128, 256)]
+
+
+@pytest.mark.parametrize("out", [B, F])
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_matmul_every_variant(variant, out):
+    """Each kernel the rule can pick, over whole and ragged tiles, short and long K, with every part of the epilogue."""
+    from advanced_optimizers_b200 import check_fp8_errors, fp8
+    from advanced_optimizers_b200.dropout import drop_fields
+    split = variant % 100000 // 1000
+    for m, n, k in ((300, 520, 4224), (97, 261, 640), (513, 1000, 2100), (1, 7, 5000), (700, 900, 17000), (2500, 3100, 130)):
+        if split > -(-(-(-k // 128)) // 4):
+            continue
+        a, b = operands(m, n, k, E4, E5, n % 2 == 0)
+        av, bv = ref.values(a), ref.values(b)
+        close_product(fp8._gemm(a, b, torch.empty(m, n, dtype=out, device="cuda"), variant=variant), av, bv, f"{m} {n} {k}")
+        if m < 1000:
+            bias, res = data(1, n, out, 7)[0], data(m, n, out, 8)
+            key = (77, 3, 5)
+            drop = drop_fields(0.25, *key, None)
+            d = fp8._gemm(a, b, torch.empty(m, n, dtype=out, device="cuda"), bias, res, drop, variant)
+            f = ref.keep_factor((m, n), 0.25, *key)
+            want = (av @ bv.t() + bias.double()) * f + res.double()
+            mag = (av.abs() @ bv.abs().t() + bias.double().abs()) * f + res.double().abs()
+            slack = ((k + 64) * 2.0 ** -22 + 3 * 2.0 ** -23) * mag + half_step(out) * want.abs() * (1 + 2.0 ** -10)
+            assert bool(((d.double() - want).abs() <= slack).all()), (m, n, k)
+    check_fp8_errors()
+
+
 @pytest.mark.parametrize("m,n,k", [(4096, 4096, 8192), (300, 14336, 4096), (8, 4096, 14336), (2048, 2048, 2048)])
 def test_matmul_large_float32(m, n, k):
     """float32 results: the error of the whole matrix stays near float32's."""
