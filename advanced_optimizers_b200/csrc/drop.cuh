@@ -16,7 +16,9 @@ namespace advopt {
 struct DropSpec {
   PhiloxKeys keys;
   const int64_t* step_dev;
-  uint32_t site, step, threshold;
+  uint32_t site, step;
+  uint32_t cut;     // threshold << 16, what a 16-bit value in the high half of a word has to reach
+  uint32_t none;    // threshold 65536: nothing is kept
   float scale;
 };
 
@@ -26,7 +28,8 @@ inline DropSpec drop_spec(const advopt_dropout_spec& s) {
   d.step_dev = s.step_dev;
   d.site = s.site;
   d.step = s.step;
-  d.threshold = s.threshold;
+  d.none = s.threshold > 65535u;
+  d.cut = d.none ? 0xFFFFFFFFu : s.threshold << 16;
   d.scale = s.scale;
   return d;
 }
@@ -46,41 +49,49 @@ __device__ __forceinline__ uint32_t drop_word(const U4& w, uint32_t i) {
   return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
 }
 
-// keep bits (bit e: element k0 + e) of N consecutive elements, N a multiple
-// of 4 up to 16.  k0 a multiple of 8 takes N / 8 evaluations; other starts
-// evaluate each group they touch.
-template <int N>
-__device__ __forceinline__ uint32_t drop_keep(const DropSpec& d, uint32_t step, uint64_t k0) {
-  uint32_t bits = 0;
-  if (N >= 8 && (k0 & 7) == 0) {
+// v[e] of elements k0 + e becomes v[e] * scale where the element is kept, else
+// 0.  k0 a multiple of 8 takes one evaluation, other starts two.  The odd
+// elements' values are compared where they lie, in the words' high halves.
+__device__ __forceinline__ void drop8(float (&v)[8], const DropSpec& d, uint32_t step, uint64_t k0) {
+  if (d.none) {
 #pragma unroll
-    for (int g = 0; g < N / 8; ++g) {
-      const U4 w = drop_group(d, step, (k0 >> 3) + g);
-      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    return;
+  }
+  U4 w = drop_group(d, step, k0 >> 3);
+  const uint32_t off = (uint32_t)(k0 & 7);
+  if (off) {
+    // shift the two groups' 256 bits down by off 16-bit values: by 4, 2 and 1 of them
+    const U4 x = drop_group(d, step, (k0 >> 3) + 1);
+    const bool by4 = off & 4, by2 = off & 2, by1 = off & 1;
+    const uint32_t s0 = by4 ? w.z : w.x, s1 = by4 ? w.w : w.y, s2 = by4 ? x.x : w.z, s3 = by4 ? x.y : w.w,
+                   s4 = by4 ? x.z : x.x, s5 = by4 ? x.w : x.y;
+    const uint32_t t[5] = {by2 ? s1 : s0, by2 ? s2 : s1, by2 ? s3 : s2, by2 ? s4 : s3, by2 ? s5 : s4};
+    uint32_t r[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t r = (e & 1) ? q[e >> 1] >> 16 : q[e >> 1] & 0xFFFFu;
-        bits |= (r >= d.threshold ? 1u : 0u) << (8 * g + e);
-      }
-    }
-    return bits;
+    for (int i = 0; i < 4; ++i) r[i] = by1 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+    w = U4{r[0], r[1], r[2], r[3]};
   }
-  int e = 0;
-#pragma unroll 1
-  for (uint64_t grp = k0 >> 3; e < N; ++grp) {
-    const U4 w = drop_group(d, step, grp);
-#pragma unroll 1
-    for (uint32_t i = (uint32_t)((k0 + e) & 7); i < 8 && e < N; ++i, ++e) {
-      const uint32_t r = (drop_word(w, i >> 1) >> (16 * (i & 1))) & 0xFFFFu;
-      bits |= (r >= d.threshold ? 1u : 0u) << e;
-    }
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = __fmul_rn(v[2 * i], d.scale), b = __fmul_rn(v[2 * i + 1], d.scale);
+    v[2 * i] = (q[i] << 16) >= d.cut ? a : 0.0f;
+    v[2 * i + 1] = q[i] >= d.cut ? b : 0.0f;
   }
-  return bits;
 }
 
-__device__ __forceinline__ bool drop_keep1(const DropSpec& d, uint32_t step, uint64_t k) {
+__device__ __forceinline__ float drop1(float v, const DropSpec& d, uint32_t step, uint64_t k) {
   const uint32_t i = (uint32_t)(k & 7);
-  return ((drop_word(drop_group(d, step, k >> 3), i >> 1) >> (16 * (i & 1))) & 0xFFFFu) >= d.threshold;
+  const uint32_t w = drop_word(drop_group(d, step, k >> 3), i >> 1);
+  return !d.none && ((i & 1) ? w : w << 16) >= d.cut ? __fmul_rn(v, d.scale) : 0.0f;
+}
+
+// Two bf16 values, the first in the low half.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // Argument checks of a spec; nullptr when it is fine.

@@ -12,7 +12,7 @@ namespace {
 
 template <bool BF16, bool RES>
 __global__ void __launch_bounds__(256)
-    dropout_kernel(void* y, const void* x, const void* res, int64_t n, bool vec, DropSpec d) {
+    dropout_kernel(void* y, const void* x, const void* res, int64_t n, bool vec, const __grid_constant__ DropSpec d) {
   const uint32_t step = drop_step(d);
   const int64_t groups = (n + 7) >> 3;
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
@@ -23,17 +23,21 @@ __global__ void __launch_bounds__(256)
     float a[8], r[8];
     load8<BF16>(x, k0, nv, v, a);
     if (RES) load8<BF16>(res, k0, nv, v, r);
-    const uint32_t keep = d.threshold ? drop_keep<8>(d, step, (uint64_t)k0) : 0xFFu;
+    drop8(a, d, step, (uint64_t)k0);
+    if (RES) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t = (keep >> e) & 1u ? __fmul_rn(a[e], d.scale) : 0.0f;
-      a[e] = RES ? __fadd_rn(r[e], t) : t;
+      for (int e = 0; e < 8; ++e) a[e] = __fadd_rn(r[e], a[e]);
     }
     if (BF16) {
-      uint32_t u[8];
+      const uint32_t u[4] = {bf16x2(a[0], a[1]), bf16x2(a[2], a[3]), bf16x2(a[4], a[5]), bf16x2(a[6], a[7])};
+      uint16_t* out = static_cast<uint16_t*>(y) + k0;
+      if (v) {
+        *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] = f_to_bf16_rne(a[e]);
-      store8_bf16(y, k0, nv, v, u);
+        for (int e = 0; e < 8; ++e)
+          if (e < nv) out[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+      }
     } else {
       store8_f32(y, k0, nv, v, a);
     }

@@ -222,13 +222,6 @@ __device__ __forceinline__ float peer_float(uint32_t saddr, uint32_t rank) {
   return v;
 }
 
-// Two bf16 values, the first in the low half.
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 __device__ __forceinline__ float4 peer_float4(uint32_t saddr, uint32_t rank) {
   uint32_t remote;
   float4 v;
@@ -279,7 +272,7 @@ __device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint3
     if (j >= w) break;
     float x = v[j];
     if (g.bias) x = __fadd_rn(x, b);
-    if (g.drop) x = drop_keep1(d, step, (uint64_t)((q0 + j) * g.n + p)) ? __fmul_rn(x, d.scale) : 0.0f;
+    if (g.drop) x = drop1(x, d, step, (uint64_t)((q0 + j) * g.n + p));
     if (g.residual)
       x = __fadd_rn(x, BF16 ? bf16_to_f(static_cast<const uint16_t*>(g.residual)[(q0 + j) * g.ldres + p])
                             : static_cast<const float*>(g.residual)[(q0 + j) * g.ldres + p]);
@@ -351,7 +344,7 @@ __device__ __noinline__ void emit_edge(const GemmArgs& g, const DropSpec& d, uin
                                          : static_cast<const float*>(res)[r * ldres];
       if (!BF16 && more) x = __fadd_rn(static_cast<const float*>(at)[r * ldd], x);
       if (biased) x = __fadd_rn(x, bias);
-      if (drop && last) x = drop_keep1(d, step, (uint64_t)((p0 + r) * g.n + q)) ? __fmul_rn(x, d.scale) : 0.0f;
+      if (drop && last) x = drop1(x, d, step, (uint64_t)((p0 + r) * g.n + q));
       if (add) x = __fadd_rn(x, t);
       if (BF16) static_cast<uint16_t*>(at)[r * ldd] = (uint16_t)bf16x2(x, 0.0f);
       else static_cast<float*>(at)[r * ldd] = x;
@@ -422,11 +415,7 @@ __device__ __forceinline__ void emit_block(const GemmArgs& g, const DropSpec& d,
     }
     if (g.drop) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t keep = drop_keep<8>(d, step, (uint64_t)((p + 8 * i) * g.n + q));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = (keep >> e) & 1u ? __fmul_rn(v[i][e], d.scale) : 0.0f;
-      }
+      for (int i = 0; i < 4; ++i) drop8(v[i], d, step, (uint64_t)((p + 8 * i) * g.n + q));
     }
     if (g.residual) {
 #pragma unroll

@@ -17,10 +17,12 @@ namespace fp8q {
 
 constexpr int TILE = 128;
 
-// |x|'s bits, 0 for an infinity or NaN (they do not enter a block's scale).
-__device__ __forceinline__ uint32_t finite_bits(float x) {
+constexpr uint32_t INF_BITS = 0x7f800000u;
+// |x|'s bits; CAREFUL: 0 for an infinity or NaN (they do not enter a block's scale).
+template <bool CAREFUL>
+__device__ __forceinline__ uint32_t abs_bits(float x) {
   const uint32_t a = f2u(x) & 0x7fffffffu;
-  return a < 0x7f800000u ? a : 0u;
+  return CAREFUL && a >= INF_BITS ? 0u : a;
 }
 
 // Biased scale exponent (E8M0 byte) from the block maximum's bits.
@@ -41,19 +43,17 @@ __device__ __forceinline__ uint32_t cvt2(float lo, float hi) {
   return r;
 }
 
-// x * 2^-e; an infinity becomes NaN (0 * inf), a finite product is unchanged
-// (adding 0 of x's sign).
-__device__ __forceinline__ float scaled(float x, float inv) { return __fmaf_rn(x, 0.0f, __fmul_rn(x, inv)); }
-
-template <bool E5M2>
-__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float inv) {
-  return cvt2<E5M2>(scaled(a, inv), scaled(b, inv)) | (cvt2<E5M2>(scaled(c, inv), scaled(d, inv)) << 16);
+// x * 2^-e; CAREFUL: an infinity becomes NaN (0 * inf), a finite product is
+// unchanged (adding 0 of x's sign).
+template <bool CAREFUL>
+__device__ __forceinline__ float scaled(float x, float inv) {
+  return CAREFUL ? __fmaf_rn(x, 0.0f, __fmul_rn(x, inv)) : __fmul_rn(x, inv);
 }
 
-__device__ __forceinline__ void drop8(float (&v)[8], const DropSpec& d, uint32_t step, uint64_t k0) {
-  const uint32_t keep = drop_keep<8>(d, step, k0);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (keep >> e) & 1u ? __fmul_rn(v[e], d.scale) : 0.0f;
+template <bool E5M2, bool CAREFUL>
+__device__ __forceinline__ uint32_t code4(float a, float b, float c, float d, float inv) {
+  return cvt2<E5M2>(scaled<CAREFUL>(a, inv), scaled<CAREFUL>(b, inv)) |
+         (cvt2<E5M2>(scaled<CAREFUL>(c, inv), scaled<CAREFUL>(d, inv)) << 16);
 }
 
 struct QArgs {
@@ -71,9 +71,81 @@ struct QArgs {
   int vec, drop;
 };
 
+// Eight consecutive elements of a row.  bf16 ones stay packed: half the
+// registers, and their magnitudes are compared two at a time.
+struct Row8F {
+  float v[8];
+  __device__ __forceinline__ float at(int e) const { return v[e]; }
+  template <bool CAREFUL>
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t a = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = max(a, abs_bits<CAREFUL>(v[e]));
+    return a;
+  }
+};
+struct Row8H {
+  uint32_t w[4];
+  __device__ __forceinline__ float at(int e) const { return u2f((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16); }
+  template <bool CAREFUL>
+  __device__ __forceinline__ uint32_t top() const {
+    if (CAREFUL) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a = max(a, abs_bits<true>(at(e)));
+      return a;
+    }
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7FFF7FFFu, w[1] & 0x7FFF7FFFu),
+                                __vmaxu2(w[2] & 0x7FFF7FFFu, w[3] & 0x7FFF7FFFu));
+    return max(m << 16, m & 0xFFFF0000u);
+  }
+};
+template <bool BF16>
+__device__ __forceinline__ void load_row(Row8F& r, const void* x, int64_t k0, int nv, bool vec) {
+  load8<BF16>(x, k0, nv, vec, r.v);
+}
+template <bool BF16>
+__device__ __forceinline__ void load_row(Row8H& r, const void* x, int64_t k0, int nv, bool vec) {
+  const uint16_t* p = static_cast<const uint16_t*>(x) + k0;
+  if (vec) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r.w[i] = (2 * i < nv ? (uint32_t)p[2 * i] : 0u) | (2 * i + 1 < nv ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+  }
+}
+__device__ __forceinline__ void drop_row(Row8F& r, const DropSpec& d, uint32_t step, uint64_t k0) { drop8(r.v, d, step, k0); }
+__device__ __forceinline__ void drop_row(Row8H&, const DropSpec&, uint32_t, uint64_t) {}   // dropped values are float32
+
+__device__ __forceinline__ void store_codes(uint8_t* out, uint32_t w0, uint32_t w1, int nv) {
+  if (nv == 8) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < nv) out[e] = (uint8_t)((e < 4 ? w0 : w1) >> (8 * (e & 3)));
+  }
+}
+
+template <bool E5M2, bool CAREFUL, class Row>
+__device__ __forceinline__ void code_row(const Row& r, uint32_t byte, uint8_t* out, int nv) {
+  const float inv = inv_scale(byte);
+  store_codes(out, code4<E5M2, CAREFUL>(r.at(0), r.at(1), r.at(2), r.at(3), inv),
+              code4<E5M2, CAREFUL>(r.at(4), r.at(5), r.at(6), r.at(7), inv), nv);
+}
+
+// The largest over a half-warp's sixteen lanes.
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t a) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return a;
+}
+
 // ---- rows only, 1 x 128 blocks: sixteen lanes per block, eight elements a lane ----
-template <bool BF16, bool E5M2>
-__global__ void __launch_bounds__(256) rows_kernel(QArgs q, DropSpec d) {
+template <bool BF16, bool E5M2, class Row>
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ QArgs q, const __grid_constant__ DropSpec d) {
   const uint32_t step = q.drop ? drop_step(d) : 0u;
   const int l16 = threadIdx.x & 15;
   const int64_t nb = (q.cols + TILE - 1) / TILE;
@@ -86,121 +158,114 @@ __global__ void __launch_bounds__(256) rows_kernel(QArgs q, DropSpec d) {
     const int64_t r = live ? u / nb : 0, b = live ? u - r * nb : 0;
     const int64_t c0 = b * TILE + l16 * 8;
     const int nv = !live || c0 >= q.cols ? 0 : q.cols - c0 < 8 ? (int)(q.cols - c0) : 8;
-    float v[8];
-    load8<BF16>(q.x, r * q.ldx + c0, nv, q.vec && nv == 8, v);
-    if (q.drop && nv) drop8(v, d, step, (uint64_t)(r * q.cols + c0));
-    uint32_t a = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a = max(a, finite_bits(v[e]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const uint32_t sb = scale_byte<E5M2>(a);
-    const float inv = inv_scale(sb);
-    if (nv) {
-      const uint32_t w0 = code4<E5M2>(v[0], v[1], v[2], v[3], inv), w1 = code4<E5M2>(v[4], v[5], v[6], v[7], inv);
-      uint8_t* out = q.codes_r + r * q.ld_r + c0;
-      if (nv == 8) {
-        *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < nv) out[e] = (uint8_t)((e < 4 ? w0 : w1) >> (8 * (e & 3)));
-      }
+    Row v;
+    load_row<BF16>(v, q.x, r * q.ldx + c0, nv, q.vec && nv == 8);
+    if (q.drop && nv) drop_row(v, d, step, (uint64_t)(r * q.cols + c0));
+    uint32_t a = half_warp_max(v.template top<false>());
+    uint8_t* out = q.codes_r + r * q.ld_r + c0;
+    if (!__any_sync(0xffffffffu, a >= INF_BITS)) {
+      a = scale_byte<E5M2>(a);
+      if (nv) code_row<E5M2, false>(v, a, out, nv);
+    } else {
+      a = scale_byte<E5M2>(half_warp_max(v.template top<true>()));
+      if (nv) code_row<E5M2, true>(v, a, out, nv);
     }
-    if (live && l16 == 0) q.scales_r[r * q.ld_sr + b] = (uint8_t)sb;
+    if (live && l16 == 0) q.scales_r[r * q.ld_sr + b] = (uint8_t)a;
   }
 }
 
 // ---- one 128 x 128 tile per CTA: any layout, both block shapes, column sums ----
 // Thread (g, l) of 16 x 16 holds rows 8g .. 8g+7, columns 8l .. 8l+7.
-template <bool BF16, bool E5M2, bool SQUARE>
-__global__ void __launch_bounds__(256, 2) tile_kernel(QArgs q, DropSpec d) {
-  __shared__ __align__(16) uint32_t red[16][TILE];     // column maxima, then column sums
-  __shared__ __align__(16) uint8_t turned[TILE * TILE];
-  __shared__ uint32_t col_byte[TILE];
-  __shared__ uint32_t warp_max_bits[8];
-  const uint32_t step = q.drop ? drop_step(d) : 0u;
+struct TileShared {
+  uint32_t red[8][TILE];     // column maxima of a warp's 16 rows; column sums
+  uint8_t turned[TILE * TILE];
+  uint32_t col_byte[TILE];
+  uint32_t warp_top[8];
+};
+
+// Columns' maxima over a warp's 16 rows, into red[warp].
+template <bool CAREFUL>
+__device__ __forceinline__ void column_tops(const Row8F (&v)[8], TileShared& s) {
+  const int warp = threadIdx.x >> 5, l = threadIdx.x & 15;
+  uint32_t a[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    a[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[e] = max(a[e], abs_bits<CAREFUL>(v[i].v[e]));
+    a[e] = max(a[e], __shfl_xor_sync(0xffffffffu, a[e], 16));
+  }
+  if ((threadIdx.x & 16) == 0) {
+    *reinterpret_cast<uint4*>(&s.red[warp][l * 8]) = make_uint4(a[0], a[1], a[2], a[3]);
+    *reinterpret_cast<uint4*>(&s.red[warp][l * 8 + 4]) = make_uint4(a[4], a[5], a[6], a[7]);
+  }
+}
+template <bool CAREFUL>
+__device__ __forceinline__ void column_tops(const Row8H (&v)[8], TileShared& s) {
+  const int warp = threadIdx.x >> 5, l = threadIdx.x & 15;
+  uint32_t a[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t w = v[i].w[j] & 0x7FFF7FFFu;
+      if (CAREFUL) w = ((w & 0x7FFFu) >= 0x7F80u ? 0u : w & 0x7FFFu) | ((w >> 16) >= 0x7F80u ? 0u : w & 0x7FFF0000u);
+      m = __vmaxu2(m, w);
+    }
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    a[2 * j] = m << 16;
+    a[2 * j + 1] = m & 0xFFFF0000u;
+  }
+  if ((threadIdx.x & 16) == 0) {
+    *reinterpret_cast<uint4*>(&s.red[warp][l * 8]) = make_uint4(a[0], a[1], a[2], a[3]);
+    *reinterpret_cast<uint4*>(&s.red[warp][l * 8 + 4]) = make_uint4(a[4], a[5], a[6], a[7]);
+  }
+}
+
+template <bool E5M2, bool SQUARE, bool CAREFUL, class Row>
+__device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], TileShared& s, int nv) {
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const int64_t r0 = (int64_t)blockIdx.y * TILE, c0 = (int64_t)blockIdx.x * TILE;
   const int64_t c = c0 + l * 8;
-  const int nv = c >= q.cols ? 0 : q.cols - c < 8 ? (int)(q.cols - c) : 8;
-  float v[8][8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + g * 8 + i;
-    const int n = r < q.rows ? nv : 0;
-    load8<BF16>(q.x, r * q.ldx + c, n, q.vec && n == 8, v[i]);
-  }
-  if (q.drop) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t r = r0 + g * 8 + i;
-      if (r < q.rows && nv) drop8(v[i], d, step, (uint64_t)(r * q.cols + c));
-    }
-  }
   uint32_t square_byte = 0;
   if (SQUARE) {
     uint32_t a = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a = max(a, finite_bits(v[i][e]));
+    for (int i = 0; i < 8; ++i) a = max(a, v[i].template top<CAREFUL>());
     a = __reduce_max_sync(0xffffffffu, a);
-    if ((threadIdx.x & 31) == 0) warp_max_bits[threadIdx.x >> 5] = a;
+    if ((threadIdx.x & 31) == 0) s.warp_top[threadIdx.x >> 5] = a;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) a = max(a, warp_max_bits[w]);
+    for (int w = 0; w < 8; ++w) a = max(a, s.warp_top[w]);
     square_byte = scale_byte<E5M2>(a);
     if (threadIdx.x == 0) {
       if (q.codes_r) q.scales_r[blockIdx.y * q.ld_sr + blockIdx.x] = (uint8_t)square_byte;
       if (q.codes_c) q.scales_c[blockIdx.x * q.ld_sc + blockIdx.y] = (uint8_t)square_byte;
     }
   }
+  if (!SQUARE && q.codes_c) column_tops<CAREFUL>(v, s);
   if (q.codes_r) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int64_t r = r0 + g * 8 + i;
       uint32_t sb = square_byte;
       if (!SQUARE) {
-        uint32_t a = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a = max(a, finite_bits(v[i][e]));
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-        sb = scale_byte<E5M2>(a);
+        sb = scale_byte<E5M2>(half_warp_max(v[i].template top<CAREFUL>()));
         if (l == 0 && r < q.rows) q.scales_r[r * q.ld_sr + blockIdx.x] = (uint8_t)sb;
       }
-      if (r < q.rows && nv) {
-        const float inv = inv_scale(sb);
-        const uint32_t w0 = code4<E5M2>(v[i][0], v[i][1], v[i][2], v[i][3], inv);
-        const uint32_t w1 = code4<E5M2>(v[i][4], v[i][5], v[i][6], v[i][7], inv);
-        uint8_t* out = q.codes_r + r * q.ld_r + c;
-        if (nv == 8) {
-          *reinterpret_cast<uint2*>(out) = make_uint2(w0, w1);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < nv) out[e] = (uint8_t)((e < 4 ? w0 : w1) >> (8 * (e & 3)));
-        }
-      }
+      if (r < q.rows && nv) code_row<E5M2, CAREFUL>(v[i], sb, q.codes_r + r * q.ld_r + c, nv);
     }
   }
   if (q.codes_c) {
     if (!SQUARE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        uint32_t a = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = max(a, finite_bits(v[i][e]));
-        red[g][l * 8 + e] = a;
-      }
       __syncthreads();
       if (threadIdx.x < TILE) {
         uint32_t a = 0;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) a = max(a, red[w][threadIdx.x]);
+        for (int w = 0; w < 8; ++w) a = max(a, s.red[w][threadIdx.x]);
         const uint32_t sb = scale_byte<E5M2>(a);
-        col_byte[threadIdx.x] = sb;
+        s.col_byte[threadIdx.x] = sb;
         if (c0 + threadIdx.x < q.cols) q.scales_c[(c0 + threadIdx.x) * q.ld_sc + blockIdx.y] = (uint8_t)sb;
       }
       __syncthreads();
@@ -210,10 +275,10 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(QArgs q, DropSpec d) {
     // each of 16 rows) and its loads (one row's 16 chunks) touch all banks
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float inv = inv_scale(SQUARE ? square_byte : col_byte[l * 8 + e]);
-      const uint32_t w0 = code4<E5M2>(v[0][e], v[1][e], v[2][e], v[3][e], inv);
-      const uint32_t w1 = code4<E5M2>(v[4][e], v[5][e], v[6][e], v[7][e], inv);
-      *reinterpret_cast<uint2*>(turned + (l * 8 + e) * TILE + ((g ^ l) << 3)) = make_uint2(w0, w1);
+      const float inv = inv_scale(SQUARE ? square_byte : s.col_byte[l * 8 + e]);
+      const uint32_t w0 = code4<E5M2, CAREFUL>(v[0].at(e), v[1].at(e), v[2].at(e), v[3].at(e), inv);
+      const uint32_t w1 = code4<E5M2, CAREFUL>(v[4].at(e), v[5].at(e), v[6].at(e), v[7].at(e), inv);
+      *reinterpret_cast<uint2*>(s.turned + (l * 8 + e) * TILE + ((g ^ l) << 3)) = make_uint2(w0, w1);
     }
     __syncthreads();
     const int64_t nr = q.rows - r0 - l * 8;   // rows of x left from this thread's chunk on
@@ -221,48 +286,81 @@ __global__ void __launch_bounds__(256, 2) tile_kernel(QArgs q, DropSpec d) {
     for (int i = 0; i < 8; ++i) {
       const int tc = i * 16 + g;
       if (c0 + tc < q.cols && nr > 0) {
-        const uint2 w = *reinterpret_cast<const uint2*>(turned + tc * TILE + ((l ^ (tc >> 3)) << 3));
-        uint8_t* out = q.codes_c + (c0 + tc) * q.ld_c + r0 + l * 8;
-        if (nr >= 8) {
-          *reinterpret_cast<uint2*>(out) = w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < nr) out[e] = (uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
-        }
+        const uint2 w = *reinterpret_cast<const uint2*>(s.turned + tc * TILE + ((l ^ (tc >> 3)) << 3));
+        store_codes(q.codes_c + (c0 + tc) * q.ld_c + r0 + l * 8, w.x, w.y, nr < 8 ? (int)nr : 8);
       }
-    }
-  }
-  if (q.col_partial) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = __fadd_rn(s, v[i][e]);
-      red[g][l * 8 + e] = f2u(s);
-    }
-    __syncthreads();
-    if (threadIdx.x < TILE && c0 + threadIdx.x < q.cols) {
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) s = __fadd_rn(s, u2f(red[w][threadIdx.x]));
-      q.col_partial[(int64_t)blockIdx.y * q.cols + c0 + threadIdx.x] = s;
     }
   }
 }
 
-template <bool BF16, bool E5M2>
-void launch(const QArgs& q, const DropSpec& d, bool square, cudaStream_t s) {
+template <bool BF16, bool E5M2, bool SQUARE, class Row>
+__global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(const __grid_constant__ QArgs q, const __grid_constant__ DropSpec d) {
+  __shared__ __align__(16) TileShared s;
+  const uint32_t step = q.drop ? drop_step(d) : 0u;
+  const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int64_t r0 = (int64_t)blockIdx.y * TILE, c0 = (int64_t)blockIdx.x * TILE;
+  const int64_t c = c0 + l * 8;
+  const int nv = c >= q.cols ? 0 : q.cols - c < 8 ? (int)(q.cols - c) : 8;
+  Row v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + g * 8 + i;
+    const int n = r < q.rows ? nv : 0;
+    load_row<BF16>(v[i], q.x, r * q.ldx + c, n, q.vec && n == 8);
+  }
+  if (q.drop) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = r0 + g * 8 + i;
+      if (r < q.rows && nv) drop_row(v[i], d, step, (uint64_t)(r * q.cols + c));
+    }
+  }
+  if (q.col_partial) {
+    float t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[e] = __fadd_rn(t[e], v[i].at(e));
+      t[e] = __fadd_rn(t[e], __shfl_xor_sync(0xffffffffu, t[e], 16));
+    }
+    if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s.red[threadIdx.x >> 5][l * 8 + e] = f2u(t[e]);
+    }
+    __syncthreads();
+    if (threadIdx.x < TILE && c0 + threadIdx.x < q.cols) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t = __fadd_rn(t, u2f(s.red[w][threadIdx.x]));
+      q.col_partial[(int64_t)blockIdx.y * q.cols + c0 + threadIdx.x] = t;
+    }
+  }
+  // infinities and NaN are looked for once, and only a tile that has some pays for them
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, v[i].template top<false>());
+  if (!__syncthreads_or(a >= INF_BITS)) tile_body<E5M2, SQUARE, false>(q, v, s, nv);
+  else tile_body<E5M2, SQUARE, true>(q, v, s, nv);
+}
+
+template <bool BF16, bool E5M2, class Row>
+void launch_row(const QArgs& q, const DropSpec& d, bool square, cudaStream_t s) {
   const int64_t nb = (q.cols + TILE - 1) / TILE, mb = (q.rows + TILE - 1) / TILE;
   if (!square && !q.codes_c && !q.col_partial) {
     const int64_t blocks = (q.rows * nb + 15) / 16;
-    rows_kernel<BF16, E5M2><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(q, d);
+    rows_kernel<BF16, E5M2, Row><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, s>>>(q, d);
     return;
   }
   const dim3 grid((unsigned)nb, (unsigned)mb);
-  if (square) tile_kernel<BF16, E5M2, true><<<grid, 256, 0, s>>>(q, d);
-  else tile_kernel<BF16, E5M2, false><<<grid, 256, 0, s>>>(q, d);
+  if (square) tile_kernel<BF16, E5M2, true, Row><<<grid, 256, 0, s>>>(q, d);
+  else tile_kernel<BF16, E5M2, false, Row><<<grid, 256, 0, s>>>(q, d);
+}
+
+template <bool BF16, bool E5M2>
+void launch(const QArgs& q, const DropSpec& d, bool square, cudaStream_t s) {
+  if (BF16 && !q.drop) launch_row<BF16, E5M2, Row8H>(q, d, square, s);
+  else launch_row<BF16, E5M2, Row8F>(q, d, square, s);
 }
 
 // Column sums of the slabs' sums, in slab order.
