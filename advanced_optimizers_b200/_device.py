@@ -87,4 +87,4 @@ _HERE = contextlib.nullcontext()
 
 def on_device(device):
     """A context in which `device` is the current one (free when it is already)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)

@@ -25,6 +25,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "advopt.h"
@@ -1037,6 +1038,19 @@ int encode_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, i
   return ADVOPT_OK;
 }
 
+// A kernel's shared-memory limit, raised once for each device (`ready`: a bit a device).
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (ready.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 struct Launch {
   const void *p, *q;
   int64_t ldp, ldq, k;
@@ -1053,8 +1067,8 @@ int launch_t(const Launch& L) {
   if (rc == ADVOPT_OK) rc = encode_map(&mq, L.q, L.g.q.extent, L.k, L.ldq, BN);
   if (rc != ADVOPT_OK) return rc;
   const auto kernel = gemm_kernel<BN, S, BF16>;
-  // per call, not once: the attribute belongs to the current device
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem(kernel, C::SMEM, ready);
   if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
   const int64_t tiles = ((L.g.p.extent + BM - 1) / BM) * ((L.g.q.extent + BN - 1) / BN);
   if (tiles * S > 0x7fffffff) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
@@ -1083,7 +1097,8 @@ int launch_pair(const Launch& L) {
   if (rc != ADVOPT_OK) return rc;
   const bool extra = L.g.bias || L.g.residual || L.g.drop;
   const auto kernel = extra ? pair_kernel<BN, BF16, true> : pair_kernel<BN, BF16, false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static std::atomic<uint64_t> ready[2];
+  cudaError_t e = allow_smem(kernel, C::SMEM, ready[extra]);
   if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
   PairArgs w;
   w.p_tiles = (int)((L.g.p.extent + 2 * BM - 1) / (2 * BM));

@@ -41,11 +41,12 @@ def drop_fields(p, seed, site, step, device):
 
 
 def _launch(x, residual, fields):
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x)
     with on_device(x.device):
-        L.check(L.lib().advopt_dropout(y.data_ptr(), x.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                                       x.numel(), dtype_code(x.dtype), SPEC.pack(*fields), raw_stream(x.device)),
-                "advopt_dropout")
+        rc = L.lib().advopt_dropout(y.data_ptr(), x.data_ptr(), 0 if residual is None else residual.data_ptr(), x.numel(),
+                                    dtype_code(x.dtype), SPEC.pack(*fields), raw_stream(x.device))
+    if rc:
+        L.check(rc, "advopt_dropout")
     return y
 
 
@@ -53,14 +54,19 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, step_tensor, fields):
         ctx.fields = fields
-        ctx.save_for_backward(*(() if step_tensor is None else (step_tensor,)))
-        return _launch(x.contiguous(), None if residual is None else residual.contiguous(), fields)
+        if step_tensor is not None:
+            ctx.save_for_backward(step_tensor)
+        return _launch(x, residual, fields)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        _ = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
-        dx = _launch(dy.contiguous(), None, ctx.fields) if ctx.needs_input_grad[0] else None
+        step = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
+        dx = None
+        if ctx.needs_input_grad[0]:
+            g = dy.contiguous()
+            # the gradient's own gradient is the same mask again
+            dx = (_Dropout.apply(g, None, step[0] if step else None, ctx.fields) if torch.is_grad_enabled() and g.requires_grad
+                  else _launch(g, None, ctx.fields))
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None
 
 
@@ -85,6 +91,9 @@ def philox_dropout(x: torch.Tensor, p: float, *, seed: int = 42, site: int = 0, 
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("philox_dropout: the residual must have x's shape, dtype and device")
     fields = drop_fields(p, seed, site, step, x.device)
+    x = x.contiguous()
+    if residual is not None:
+        residual = residual.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return _Dropout.apply(x, residual, step if isinstance(step, torch.Tensor) else None, fields)
-    return _launch(x.contiguous(), None if residual is None else residual.contiguous(), fields)
+    return _launch(x, residual, fields)

@@ -63,13 +63,13 @@ def _round_up(n, to):
     return (n + to - 1) // to * to
 
 
-def _empty_codes(rows, k, dtype, device):
-    t = torch.empty((rows, _round_up(k, 16)), dtype=dtype, device=device)
+def _empty_codes(rows, k, dtype, like):
+    t = like.new_empty((rows, _round_up(k, 16)), dtype=dtype)
     return t if t.shape[1] == k else t[:, :k]
 
 
-def _empty_scales(rows, nb, device):
-    t = torch.empty((rows, _round_up(nb, 4)), dtype=_E8M0, device=device)
+def _empty_scales(rows, nb, like):
+    t = like.new_empty((rows, _round_up(nb, 4)), dtype=_E8M0)
     return t if t.shape[1] == nb else t[:, :nb]
 
 
@@ -84,7 +84,7 @@ class Fp8Blocks:
     Codes whose rows do not start at whole 16 bytes, and scales whose rows do
     not hold whole 4 bytes, are copied once into such a layout here."""
 
-    __slots__ = ("codes", "scales", "rows", "k", "square", "ld", "lds")
+    __slots__ = ("codes", "scales", "rows", "k", "square", "ld", "lds", "codes_ptr", "scales_ptr", "code")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype not in _CODE or scales.dtype != _E8M0:
@@ -106,20 +106,21 @@ class Fp8Blocks:
         if rows and k:
             ld = codes.stride(0) if rows > 1 else _round_up(k, 16)
             if codes.data_ptr() % 16 or ld % 16 or ld < k or (k > 1 and codes.stride(1) != 1):
-                own = _empty_codes(rows, k, codes.dtype, codes.device)
+                own = _empty_codes(rows, k, codes.dtype, codes)
                 own.view(torch.uint8).copy_(codes.view(torch.uint8))
                 codes, ld = own, _round_up(k, 16)
             lds = scales.stride(0) if scales.shape[0] > 1 else _round_up(nb, 4)
             if scales.data_ptr() % 4 or lds % 4 or lds < nb or (nb > 1 and scales.stride(1) != 1) or (
                     nb % 4 and scales.untyped_storage().nbytes() <
                     scales.storage_offset() + (scales.shape[0] - 1) * lds + _round_up(nb, 4)):
-                own = _empty_scales(scales.shape[0], nb, scales.device)
+                own = _empty_scales(scales.shape[0], nb, scales)
                 own.view(torch.uint8).copy_(scales.view(torch.uint8))
                 scales, lds = own, _round_up(nb, 4)
             self.ld, self.lds = ld, lds
         else:
             self.ld, self.lds = _round_up(k, 16), _round_up(nb, 4)
         self.codes, self.scales, self.rows, self.k, self.square = codes, scales, rows, k, square
+        self.codes_ptr, self.scales_ptr, self.code = codes.data_ptr(), scales.data_ptr(), _CODE[codes.dtype]
 
     @property
     def block(self):
@@ -130,39 +131,46 @@ class Fp8Blocks:
         return self.codes.device
 
 
-def _blocks(codes, scales, rows, k, square, ld, lds):
-    """An Fp8Blocks of tensors this module laid out itself."""
+class _Kept:
+    """Quantised blocks inside `fp8_linear`, in one buffer and without tensor
+    views of their own (two views and two allocations cost the host as much as
+    two kernel launches)."""
+
+    __slots__ = ("buffer", "rows", "k", "square", "ld", "lds", "codes_ptr", "scales_ptr", "code")
+
+    def __init__(self, rows, k, square, like):
+        self.rows, self.k, self.square, self.code = rows, k, square, 0
+        self.ld, self.lds = _round_up(k, 16), _round_up((k + 127) // 128, 4)
+        size = rows * self.ld                  # whole 16 bytes, so the scales behind are aligned
+        self.buffer = like.new_empty(size + ((rows + 127) // 128 if square else rows) * self.lds, dtype=torch.uint8)
+        self.codes_ptr = self.buffer.data_ptr()
+        self.scales_ptr = self.codes_ptr + size
+
+
+def _owned(rows, k, square, dtype, like):
+    """An Fp8Blocks of new tensors."""
     b = object.__new__(Fp8Blocks)
-    b.codes, b.scales, b.rows, b.k, b.square, b.ld, b.lds = codes, scales, rows, k, square, ld, lds
+    b.codes = _empty_codes(rows, k, dtype, like)
+    b.scales = _empty_scales((rows + 127) // 128 if square else rows, (k + 127) // 128, like)
+    b.rows, b.k, b.square, b.code = rows, k, square, _CODE[dtype]
+    b.ld, b.lds = _round_up(k, 16), _round_up((k + 127) // 128, 4)
+    b.codes_ptr, b.scales_ptr = b.codes.data_ptr(), b.scales.data_ptr()
     return b
 
 
-def _quantize(x, square, dtype, rows, cols, sums=False, drop=NO_DROP):
-    """(blocks of x or None, blocks of x^T or None, column sums of 128-row slabs or None)."""
+def _quantize(x, by_row, by_col, square, code, partial=None, drop=NO_DROP):
+    """Fills by_row (blocks of x), by_col (blocks of x^T) and partial (column sums of 128-row slabs); each may be None."""
     R, C = x.shape
-    dev = x.device
     if C > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < C:
         x = x.contiguous()
-    ldx = x.stride(0) if R > 1 else C
-    nr, nc = (R + 127) // 128, (C + 127) // 128
-    br = bc = partial = None
-    args_r = args_c = (0, 0, 0, 0)
-    if rows:
-        br = _blocks(_empty_codes(R, C, dtype, dev), _empty_scales(nr if square else R, nc, dev), R, C, square,
-                     _round_up(C, 16), _round_up(nc, 4))
-        args_r = (br.codes.data_ptr(), br.ld, br.scales.data_ptr(), br.lds)
-    if cols:
-        bc = _blocks(_empty_codes(C, R, dtype, dev), _empty_scales(nc if square else C, nr, dev), C, R, square,
-                     _round_up(R, 16), _round_up(nr, 4))
-        args_c = (bc.codes.data_ptr(), bc.ld, bc.scales.data_ptr(), bc.lds)
-    if sums:
-        partial = torch.empty((nr, C), dtype=torch.float32, device=dev)
+    dev = x.device
     with on_device(dev):
-        L.check(L.lib().advopt_fp8_quantize(
-            _QUANT.pack(x.data_ptr(), ldx, R, C, *args_r, *args_c, partial.data_ptr() if sums else 0,
-                        dtype_code(x.dtype), 1 if square else 0, _CODE[dtype], 0, *drop), raw_stream(dev)),
-            "advopt_fp8_quantize")
-    return br, bc, partial
+        rc = L.lib().advopt_fp8_quantize(_QUANT.pack(
+            x.data_ptr(), x.stride(0) if R > 1 else C, R, C,
+            *((0, 0, 0, 0) if by_row is None else (by_row.codes_ptr, by_row.ld, by_row.scales_ptr, by_row.lds)),
+            *((0, 0, 0, 0) if by_col is None else (by_col.codes_ptr, by_col.ld, by_col.scales_ptr, by_col.lds)),
+            0 if partial is None else partial.data_ptr(), dtype_code(x.dtype), square, code, 0, *drop), raw_stream(dev))
+    L.check(rc, "advopt_fp8_quantize")
 
 
 def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.float8_e4m3fn, layout: str = "rows"):
@@ -188,7 +196,10 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.flo
     if not x.is_cuda:
         raise NotImplementedError("quantize_fp8: tensors must live on a CUDA device (no CPU fallback)")
     dtype_code(x.dtype)
-    r, c, _ = _quantize(x.detach(), block[0] == 128, dtype, layout != "cols", layout != "rows")
+    (R, C), square = x.shape, block[0] == 128
+    r = _owned(R, C, square, dtype, x) if layout != "cols" else None
+    c = _owned(C, R, square, dtype, x) if layout != "rows" else None
+    _quantize(x, r, c, square, _CODE[dtype])
     return (r, c) if layout == "both" else r if layout == "rows" else c
 
 
@@ -196,13 +207,11 @@ def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP, variant=0):
     m, n = out.shape
     dev = out.device
     with on_device(dev):
-        L.check(L.lib().advopt_fp8_gemm(
-            _GEMM.pack(a.codes.data_ptr(), a.ld, a.scales.data_ptr(), a.lds,
-                       b.codes.data_ptr(), b.ld, b.scales.data_ptr(), b.lds, out.data_ptr(), n,
-                       0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n,
-                       m, n, a.k, _CODE[a.codes.dtype], _CODE[b.codes.dtype], a.square, b.square,
-                       dtype_code(out.dtype), variant, _ERR.pointer(), *drop), raw_stream(dev)),
-            "advopt_fp8_gemm")
+        rc = L.lib().advopt_fp8_gemm(_GEMM.pack(
+            a.codes_ptr, a.ld, a.scales_ptr, a.lds, b.codes_ptr, b.ld, b.scales_ptr, b.lds, out.data_ptr(), n,
+            0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n, m, n, a.k,
+            a.code, b.code, a.square, b.square, dtype_code(out.dtype), variant, _ERR.pointer(), *drop), raw_stream(dev))
+    L.check(rc, "advopt_fp8_gemm")
     return out
 
 
@@ -218,46 +227,52 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     dtype_code(out_dtype)
     if a.k == 0:
         return torch.zeros((a.rows, b.rows), dtype=out_dtype, device=a.device)
-    return _gemm(a, b, torch.empty((a.rows, b.rows), dtype=out_dtype, device=a.codes.device))
+    return _gemm(a, b, a.codes.new_empty((a.rows, b.rows), dtype=out_dtype))
 
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, w_rows, w_cols, step_tensor, drop):
         need_x, need_w = ctx.needs_input_grad[:2]
-        e4m3 = torch.float8_e4m3fn
-        xr, xc, _ = _quantize(x, False, e4m3, True, need_w)
+        T, K = x.shape
+        N = weight.shape[0]
+        xr = _Kept(T, K, False, x)
+        xc = _Kept(K, T, False, x) if need_w else None
+        _quantize(x, xr, xc, False, 0)
         if w_rows is None:
-            w_rows, w_cols, _ = _quantize(weight, True, e4m3, True, need_x)
-        y = torch.empty((x.shape[0], weight.shape[0]), dtype=x.dtype, device=x.device)
-        _gemm(xr, w_rows, y, bias, residual, drop)
+            w_rows = _Kept(N, K, True, weight)
+            w_cols = _Kept(K, N, True, weight) if need_x else None
+            _quantize(weight, w_rows, w_cols, True, 0)
         ctx.drop, ctx.w_dtype, ctx.x_dtype = drop, weight.dtype, x.dtype
-        ctx.xc, ctx.wc = xc if need_w else None, w_cols if need_x else None
-        ctx.save_for_backward(*(() if step_tensor is None else (step_tensor,)))
-        return y
+        ctx.xc, ctx.wc = xc, w_cols if need_x else None
+        if step_tensor is not None:
+            ctx.save_for_backward(step_tensor)
+        return _gemm(xr, w_rows, x.new_empty((T, N)), bias, residual, drop)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         _ = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        dev = dy.device
+        dx = dw = db = partial = None
         T, N = dy.shape
         if need_x or need_w or need_b:
             # g = mask * dy / q once, for every gradient that reads it
-            gr, gc, sums = _quantize(dy, False, torch.float8_e4m3fn, need_x or not need_w, need_w, need_b, ctx.drop)
-            if need_x:
-                dx = torch.empty((T, ctx.wc.rows), dtype=ctx.x_dtype, device=dev)
-                _gemm(gr, ctx.wc, dx)
-            if need_w:
-                dw = torch.empty((N, ctx.xc.rows), dtype=ctx.w_dtype, device=dev)
-                _gemm(gc, ctx.xc, dw)
+            gr = _Kept(T, N, False, dy) if need_x or not need_w else None
+            gc = _Kept(N, T, False, dy) if need_w else None
             if need_b:
-                db = torch.empty((N,), dtype=dy.dtype, device=dev)
-                with on_device(dev):
-                    L.check(L.lib().advopt_col_sum(db.data_ptr(), sums.data_ptr(), sums.shape[0], N,
-                                                   dtype_code(db.dtype), raw_stream(dev)), "advopt_col_sum")
+                partial = dy.new_empty(((T + 127) // 128, N), dtype=torch.float32)
+            _quantize(dy, gr, gc, False, 0, partial, ctx.drop)
+            if need_x:
+                dx = _gemm(gr, ctx.wc, dy.new_empty((T, ctx.wc.rows), dtype=ctx.x_dtype))
+            if need_w:
+                dw = _gemm(gc, ctx.xc, dy.new_empty((N, ctx.xc.rows), dtype=ctx.w_dtype))
+            if need_b:
+                db = dy.new_empty((N,))
+                with on_device(dy.device):
+                    rc = L.lib().advopt_col_sum(db.data_ptr(), partial.data_ptr(), partial.shape[0], N, dtype_code(db.dtype),
+                                                raw_stream(dy.device))
+                L.check(rc, "advopt_col_sum")
         return dx, dw, db, (dy if need_r else None), None, None, None, None
 
 
@@ -285,9 +300,10 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     that do not change between calls (accumulation, evaluation)."""
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp8_linear: x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
-    for t in (x, weight, bias, residual):
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise NotImplementedError("fp8_linear: tensors must live on one CUDA device (no CPU fallback)")
+    dev = x.device
+    if not x.is_cuda or weight.device != dev or (bias is not None and bias.device != dev) or (
+            residual is not None and residual.device != dev):
+        raise NotImplementedError("fp8_linear: tensors must live on one CUDA device (no CPU fallback)")
     dtype_code(x.dtype), dtype_code(weight.dtype)
     N, K = weight.shape
     if bias is not None and (bias.shape != (N,) or bias.dtype != x.dtype):
@@ -296,7 +312,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         raise ValueError("fp8_linear: the residual must have the result's shape and dtype")
     if N == 0 or K == 0:
         raise ValueError("fp8_linear: the weight is empty")
-    drop = drop_fields(dropout_p, seed, site, step, x.device)
+    drop = NO_DROP if dropout_p == 0 else drop_fields(dropout_p, seed, site, step, dev)
     w_rows = w_cols = None
     if weight_blocks is not None:
         w_rows, w_cols = weight_blocks
@@ -306,7 +322,11 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if x.numel() == 0:   # no tokens: no products, and gradients of zeros
         y = x.new_zeros((*x.shape[:-1], N)) if residual is None else residual.clone()
         return y + 0.0 * (x.sum() + weight.sum(dtype=x.dtype) + (0.0 if bias is None else bias.sum()))
-    y = _Fp8Linear.apply(x.reshape(-1, K), weight, None if bias is None else bias.contiguous(),
-                         None if residual is None else residual.reshape(-1, N).contiguous(), w_rows, w_cols,
+    flat = x.dim() == 2
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if residual is not None:
+        residual = (residual if flat else residual.reshape(-1, N)).contiguous()
+    y = _Fp8Linear.apply(x if flat else x.reshape(-1, K), weight, bias, residual, w_rows, w_cols,
                          step if isinstance(step, torch.Tensor) else None, drop)
-    return y.view(*x.shape[:-1], N)
+    return y if flat else y.view(*x.shape[:-1], N)

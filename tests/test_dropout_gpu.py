@@ -139,3 +139,12 @@ def test_empty():
     x = torch.zeros(0, 5, device="cuda", requires_grad=True)
     y = A.philox_dropout(x, 0.5)
     assert tuple(y.shape) == (0, 5) and tuple(torch.autograd.grad(y.sum(), x)[0].shape) == (0, 5)
+
+
+def test_gradient_of_the_gradient():
+    import advanced_optimizers_b200 as A
+    x = torch.randn(300, device="cuda", requires_grad=True)
+    dy = torch.randn(300, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(A.philox_dropout(x, 0.5, **KEY), x, dy, create_graph=True)
+    gg, = torch.autograd.grad(g, dy, torch.ones_like(g))
+    assert torch.equal(gg, (2.0 * (ref.keep_factor((300,), 0.5, **KEY) > 0)).float())
