@@ -1103,7 +1103,10 @@ int launch_pair(const Launch& L) {
   PairArgs w;
   w.p_tiles = (int)((L.g.p.extent + 2 * BM - 1) / (2 * BM));
   w.q_tiles = (int)((L.g.q.extent + BN - 1) / BN);
-  if ((int64_t)w.p_tiles * w.q_tiles > (1 << 30)) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
+  // the kernel counts a pair's tiles and scale groups in 32 bits
+  if ((int64_t)w.p_tiles * w.q_tiles > (1 << 30) ||
+      ((int64_t)w.p_tiles * w.q_tiles / PAIRS + 1) * ((L.g.kblocks + 3) / 4) > (1 << 30))
+    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
   w.chunks = BF16 ? 1 : (L.g.kblocks + CHUNK - 1) / CHUNK;
   w.chunk_blocks = ((L.g.kblocks + w.chunks - 1) / w.chunks + 3) / 4 * 4;
   w.chunks = (L.g.kblocks + w.chunk_blocks - 1) / w.chunk_blocks;

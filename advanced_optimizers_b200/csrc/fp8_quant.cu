@@ -249,9 +249,9 @@ __device__ __forceinline__ uint32_t scatter_max(const uint32_t (&a)[8]) {
 
 // FULL: the tile lies inside the matrix.
 template <bool E5M2, bool SQUARE, bool CAREFUL, bool FULL, class Row>
-__device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], TileShared& s, int nv) {
+__device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], TileShared& s, int64_t tr, int64_t tc, int nv) {
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t r0 = (int64_t)blockIdx.y * TILE, c0 = (int64_t)blockIdx.x * TILE;
+  const int64_t r0 = tr * TILE, c0 = tc * TILE;
   const int64_t c = c0 + l * 8;
   uint32_t square_byte = 0;
   if (SQUARE) {
@@ -265,8 +265,8 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
     for (int w = 0; w < 8; ++w) a = max(a, s.warp_top[w]);
     square_byte = scale_byte<E5M2>(a);
     if (threadIdx.x == 0) {
-      if (q.codes_r) q.scales_r[blockIdx.y * q.ld_sr + blockIdx.x] = (uint8_t)square_byte;
-      if (q.codes_c) q.scales_c[blockIdx.x * q.ld_sc + blockIdx.y] = (uint8_t)square_byte;
+      if (q.codes_r) q.scales_r[tr * q.ld_sr + tc] = (uint8_t)square_byte;
+      if (q.codes_c) q.scales_c[tc * q.ld_sc + tr] = (uint8_t)square_byte;
     }
   }
   if (!SQUARE && q.codes_c) column_tops<CAREFUL>(v, s);
@@ -277,7 +277,7 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] = v[i].template top<CAREFUL>();
       row_byte = scale_byte<E5M2>(scatter_max(a));
-      if (l < 8 && (FULL || r0 + g * 8 + l < q.rows)) q.scales_r[(r0 + g * 8 + l) * q.ld_sr + blockIdx.x] = (uint8_t)row_byte;
+      if (l < 8 && (FULL || r0 + g * 8 + l < q.rows)) q.scales_r[(r0 + g * 8 + l) * q.ld_sr + tc] = (uint8_t)row_byte;
     }
     uint8_t* out = q.codes_r + (r0 + g * 8) * q.ld_r + c;
     const int left = FULL ? 8 : q.rows - r0 - g * 8 < 8 ? (int)(q.rows - r0 - g * 8) : 8;
@@ -297,7 +297,7 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
         for (int w = 0; w < 8; ++w) a = max(a, s.red[w][threadIdx.x]);
         const uint32_t sb = scale_byte<E5M2>(a);
         s.col_byte[threadIdx.x] = sb;
-        if (c0 + threadIdx.x < q.cols) q.scales_c[(c0 + threadIdx.x) * q.ld_sc + blockIdx.y] = (uint8_t)sb;
+        if (c0 + threadIdx.x < q.cols) q.scales_c[(c0 + threadIdx.x) * q.ld_sc + tr] = (uint8_t)sb;
       }
       __syncthreads();
     }
@@ -317,9 +317,9 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
     uint8_t* out = q.codes_c + (c0 + g) * q.ld_c + r0 + l * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int tc = i * 16 + g;
-      if (FULL || (c0 + tc < q.cols && nr > 0)) {
-        const uint2 w = *reinterpret_cast<const uint2*>(s.turned + tc * TILE + ((l ^ (tc >> 3)) << 3));
+      const int col = i * 16 + g;
+      if (FULL || (c0 + col < q.cols && nr > 0)) {
+        const uint2 w = *reinterpret_cast<const uint2*>(s.turned + col * TILE + ((l ^ (col >> 3)) << 3));
         store_codes(out, w.x, w.y, FULL ? 8 : nr);
       }
       out += 16 * q.ld_c;
@@ -332,7 +332,9 @@ __global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(co
   __shared__ __align__(16) TileShared s;
   const uint32_t step = q.drop ? drop_step(d) : 0u;
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t r0 = (int64_t)blockIdx.y * TILE, c0 = (int64_t)blockIdx.x * TILE;
+  const uint32_t across = (uint32_t)((q.cols + TILE - 1) / TILE);
+  const int64_t tr = blockIdx.x / across, tc = blockIdx.x - (uint32_t)tr * across;
+  const int64_t r0 = tr * TILE, c0 = tc * TILE;
   const int64_t c = c0 + l * 8;
   const int nv = c >= q.cols ? 0 : q.cols - c < 8 ? (int)(q.cols - c) : 8;
   const bool full = q.vec && r0 + TILE <= q.rows && c0 + TILE <= q.cols;
@@ -373,16 +375,16 @@ __global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(co
       float t = 0.0f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) t = __fadd_rn(t, u2f(s.red[w][threadIdx.x]));
-      q.col_partial[(int64_t)blockIdx.y * q.cols + c0 + threadIdx.x] = t;
+      q.col_partial[tr * q.cols + c0 + threadIdx.x] = t;
     }
   }
   // infinities and NaN are looked for once, and only a tile that has some pays for them
   uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) a = max(a, v[i].template top<false>());
-  if (__syncthreads_or(a >= INF_BITS)) tile_body<E5M2, SQUARE, true, false>(q, v, s, nv);
-  else if (full) tile_body<E5M2, SQUARE, false, true>(q, v, s, nv);
-  else tile_body<E5M2, SQUARE, false, false>(q, v, s, nv);
+  if (__syncthreads_or(a >= INF_BITS)) tile_body<E5M2, SQUARE, true, false>(q, v, s, tr, tc, nv);
+  else if (full) tile_body<E5M2, SQUARE, false, true>(q, v, s, tr, tc, nv);
+  else tile_body<E5M2, SQUARE, false, false>(q, v, s, tr, tc, nv);
 }
 
 template <bool BF16, bool E5M2, class Row>
@@ -396,7 +398,7 @@ void launch_row(const QArgs& q, const DropSpec& d, bool square, cudaStream_t s) 
       return;
     }
   }
-  const dim3 grid((unsigned)nb, (unsigned)mb);
+  const unsigned grid = (unsigned)(nb * mb);
   if (square) tile_kernel<BF16, E5M2, true, Row><<<grid, 256, 0, s>>>(q, d);
   else tile_kernel<BF16, E5M2, false, Row><<<grid, 256, 0, s>>>(q, d);
 }
@@ -438,7 +440,8 @@ extern "C" int advopt_fp8_quantize(const advopt_fp8_quant_args* a, void* stream)
   if ((a->codes_r && (a->ld_r < a->cols || a->ld_r % 16 || reinterpret_cast<uintptr_t>(a->codes_r) % 16 || a->ld_sr < nb)) ||
       (a->codes_c && (a->ld_c < a->rows || a->ld_c % 16 || reinterpret_cast<uintptr_t>(a->codes_c) % 16 || a->ld_sc < mb)))
     return set_error(ADVOPT_E_INVALID, "advopt_fp8_quantize: codes must be 16-byte aligned with pitches that hold a row");
-  if (nb > 0x7fffffff || mb > 65535) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_quantize: at most 8388480 rows");
+  if (nb > 0x7fffffff || mb > 0x7fffffff / nb)
+    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_quantize: at most 2^31 - 1 tiles of 128 x 128");
   const int64_t es = a->x_dtype == ADVOPT_DT_BF16 ? 2 : 4;
   fp8q::QArgs q;
   q.x = a->x;

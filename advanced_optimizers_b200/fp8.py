@@ -230,24 +230,30 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     return _gemm(a, b, a.codes.new_empty((a.rows, b.rows), dtype=out_dtype))
 
 
+def _linear(x, weight, bias, residual, w_rows, w_cols, drop, need_x, need_w):
+    """(y, blocks of x^T, blocks of the weight's transpose), the latter two as far as the gradients need them."""
+    T, K = x.shape
+    N = weight.shape[0]
+    xr = _Kept(T, K, False, x)
+    xc = _Kept(K, T, False, x) if need_w else None
+    _quantize(x, xr, xc, False, 0)
+    if w_rows is None:
+        w_rows = _Kept(N, K, True, weight)
+        w_cols = _Kept(K, N, True, weight) if need_x else None
+        _quantize(weight, w_rows, w_cols, True, 0)
+    return _gemm(xr, w_rows, x.new_empty((T, N)), bias, residual, drop), xc, w_cols
+
+
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, w_rows, w_cols, step_tensor, drop):
         need_x, need_w = ctx.needs_input_grad[:2]
-        T, K = x.shape
-        N = weight.shape[0]
-        xr = _Kept(T, K, False, x)
-        xc = _Kept(K, T, False, x) if need_w else None
-        _quantize(x, xr, xc, False, 0)
-        if w_rows is None:
-            w_rows = _Kept(N, K, True, weight)
-            w_cols = _Kept(K, N, True, weight) if need_x else None
-            _quantize(weight, w_rows, w_cols, True, 0)
+        y, ctx.xc, w_cols = _linear(x, weight, bias, residual, w_rows, w_cols, drop, need_x, need_w)
+        ctx.wc = w_cols if need_x else None
         ctx.drop, ctx.w_dtype, ctx.x_dtype = drop, weight.dtype, x.dtype
-        ctx.xc, ctx.wc = xc, w_cols if need_x else None
         if step_tensor is not None:
             ctx.save_for_backward(step_tensor)
-        return _gemm(xr, w_rows, x.new_empty((T, N)), bias, residual, drop)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -327,6 +333,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         bias = bias.contiguous()
     if residual is not None:
         residual = (residual if flat else residual.reshape(-1, N)).contiguous()
-    y = _Fp8Linear.apply(x if flat else x.reshape(-1, K), weight, bias, residual, w_rows, w_cols,
-                         step if isinstance(step, torch.Tensor) else None, drop)
+    x2 = x if flat else x.reshape(-1, K)
+    if torch.is_grad_enabled():
+        y = _Fp8Linear.apply(x2, weight, bias, residual, w_rows, w_cols, step if isinstance(step, torch.Tensor) else None, drop)
+    else:   # no transposed codes, whatever the parameters' requires_grad
+        y = _linear(x2, weight, bias, residual, w_rows, w_cols, drop, False, False)[0]
     return y if flat else y.view(*x.shape[:-1], N)

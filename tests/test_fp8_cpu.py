@@ -70,7 +70,7 @@ def quant_args(**kw):
                                  dict(codes_r=0), dict(scales_r=0), dict(ld_r=248), dict(ld_r=240), dict(codes_r=8200), dict(ld_sr=1),
                                  dict(codes_c=8192, ld_c=16, scales_c=0), dict(codes_c=8192, ld_c=8, scales_c=4096, ld_sc=1),
                                  dict(codes_c=8192, ld_c=16, scales_c=4096, ld_sc=0), dict(threshold=65537), dict(step_dev=4),
-                                 dict(rows=8388481)])
+                                 dict(rows=1 << 38)])
 def test_quantize_c_refusals(bad):
     from advanced_optimizers_b200 import _lib as L
     assert L.lib().advopt_fp8_quantize(quant_args(**bad), None) in (-1, -3)

@@ -274,7 +274,7 @@ def linear_reference(x, w, bias, residual, dy, p, key, out_dtype):
     return f, xq, wq, g32.double(), g, gt, xt
 
 
-@pytest.mark.parametrize("xd,wd", [(B, B), (F, F), (B, F)])
+@pytest.mark.parametrize("xd,wd", [(B, B), (F, F), (B, F), (F, B)])
 @pytest.mark.parametrize("T,N,K,p,bias,residual", [
     (1, 128, 64, 0.0, False, False), (1, 300, 500, 0.25, True, True), (9, 257, 130, 0.5, True, False),
     (128, 128, 128, 0.1, False, True), (200, 385, 513, 0.1, True, True), (300, 96, 1000, 0.0, True, True),
