@@ -10,6 +10,8 @@
 namespace advopt {
 namespace {
 
+__host__ __device__ constexpr int groups_a_trip(bool bf16, bool res) { return bf16 && !res ? 4 : 2; }
+
 template <bool BF16>
 struct Raw {
   uint4 w[BF16 ? 1 : 2];   // eight elements as they lie in memory
@@ -58,7 +60,7 @@ __device__ __forceinline__ void store_group(void* y, int64_t k0, int nv, bool ve
 template <bool BF16, bool RES>
 __global__ void __launch_bounds__(256)
     dropout_kernel(void* y, const void* x, const void* res, int64_t n, bool vec, const __grid_constant__ DropSpec d) {
-  constexpr int U = BF16 && !RES ? 4 : 2;
+  constexpr int U = groups_a_trip(BF16, RES);
   const uint32_t step = drop_step(d);
   const int64_t stride = (int64_t)gridDim.x * blockDim.x;
   int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -102,8 +104,9 @@ __global__ void __launch_bounds__(256)
 
 template <bool BF16>
 void launch(void* y, const void* x, const void* res, int64_t n, const DropSpec& d, cudaStream_t s) {
-  const int64_t groups = (n + 7) >> 3;
-  const int64_t blocks = (groups + 255) / 256;
+  const int64_t groups = (n + 7) >> 3, trip = 256 * groups_a_trip(BF16, res != nullptr);
+  // whole trips for every thread where that still gives each SM two CTAs, else one group a thread
+  const int64_t blocks = groups >= 2 * 148 * trip ? (groups + trip - 1) / trip : (groups + 255) / 256;
   const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
   const bool vec = ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(res)) & 15) == 0;
   if (res) dropout_kernel<BF16, true><<<grid, 256, 0, s>>>(y, x, res, n, vec, d);
