@@ -18,7 +18,7 @@
 //   * warp 1 (one lane): copies scale words to tensor memory (tcgen05.cp) and
 //     issues the MMAs;
 //   * warp 2: gathers the scale words of four blocks at a time;
-//   * warps 4..7: the epilogue.
+//   * then all eight warps: the epilogue.
 // Every wait is bounded and gives up when another role has; the CTA then
 // waits (bounded) for its copies and MMAs in flight, frees its tensor memory
 // and reports through *err.
@@ -491,7 +491,6 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
   // through a warp reduction: it lands in a uniform register, where the MMAs want it
   const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
 
-  bool have = false;   // the epilogue warps: the accumulator is ready
   if (warp == 0) {
     const bool one = elect_one();
     Ring<C::STAGES> st;
@@ -572,25 +571,26 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
       mbar_arrive(&sf_full[slot]);
       now = then;
     }
-  } else if (warp >= 4) {
-    have = wait_warp(&acc_full, 0, abort_v);
-    if (!have) abort_flag = 1;
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   }
+  // the ring's warps are done: all eight share the epilogue
+  __syncwarp();
+  const bool have = wait_warp(&acc_full, 0, abort_v);
+  if (!have) abort_flag = 1;
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
   const uint32_t step = g.drop ? drop_step(d) : 0u;
-  const int quarter = warp & 3, row = quarter * 32 + lane;
+  const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
   const uint32_t taddr = tmem + ((uint32_t)(quarter * 32) << 16);
   if (S == 1) {
-    if (warp >= 4 && have) {
+    if (have) {
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = 32 * half; c < BN; c += 64) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_wait32(r);
         if (!g.swap) {
           // over the ring, which is drained once the accumulator is complete
-          unsigned char* turn = smem + quarter * 4096;
+          unsigned char* turn = smem + warp * 4096;
           turn_in(turn, r);
           emit_block<BF16, true>(g, d, step, turn, p0 + quarter * 32, q0 + c, false, true);
         } else {
@@ -610,9 +610,9 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     // D's columns) per lane; else the turned 32 x 32 blocks, so that D's rows
     // are written in whole sectors.
     float* acc = reinterpret_cast<float*>(smem);
-    if (warp >= 4 && have) {
+    if (have) {
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = 32 * half; c < BN; c += 64) {
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_wait32(r);
@@ -629,11 +629,11 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     }
     __syncwarp();
     cluster_sync();
-    if (warp >= 4 && have) {
+    if (have) {
       if (g.swap) {
-        constexpr int PER = BN / S, W = PER < 16 ? PER : 16;
+        constexpr int PER = BN / S, W = PER < 16 ? PER / 2 : 8;
 #pragma unroll 1
-        for (int c = 0; c < PER; c += W) {
+        for (int c = W * half; c < PER; c += 2 * W) {
           float v[W];
 #pragma unroll
           for (int e = 0; e < W; ++e) {
@@ -645,12 +645,12 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
           emit<BF16, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
         }
       } else {
-        // the tile's 4 BN / 32 blocks, dealt out to the cluster's 4 S warps
+        // the tile's 4 BN / 32 blocks, dealt out to the cluster's 8 S warps
         constexpr int BLOCKS = 4 * BN / 32;
 #pragma unroll 1
-        for (int b = quarter * S + (int)rank; b < BLOCKS; b += 4 * S) {
+        for (int b = warp * S + (int)rank; b < BLOCKS; b += 8 * S) {
           unsigned char* turn = smem + b * 4096;
-          unsigned char* own = smem + BLOCKS * 4096 + quarter * 4096;   // this block's sum
+          unsigned char* own = smem + (BLOCKS + warp) * 4096;   // this block's sum
 #pragma unroll 4
           for (int i = 0; i < 8; ++i) {
             const uint32_t at = smem_u32(turn + (i * 32 + lane) * 16);
