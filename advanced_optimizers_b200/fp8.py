@@ -9,6 +9,7 @@ its gradients, optional bias, residual and dropout.
 """
 from __future__ import annotations
 
+import functools
 import struct
 
 import torch
@@ -123,28 +124,16 @@ class Fp8Blocks:
         self.codes_ptr, self.scales_ptr, self.code = codes.data_ptr(), scales.data_ptr(), _CODE[codes.dtype]
 
     @property
+    def operand(self):
+        return self.codes_ptr, self.ld, self.scales_ptr, self.lds
+
+    @property
     def block(self):
         return (128, 128) if self.square else (1, 128)
 
     @property
     def device(self):
         return self.codes.device
-
-
-class _Kept:
-    """Quantised blocks inside `fp8_linear`, in one buffer and without tensor
-    views of their own (two views and two allocations cost the host as much as
-    two kernel launches)."""
-
-    __slots__ = ("buffer", "rows", "k", "square", "ld", "lds", "codes_ptr", "scales_ptr", "code")
-
-    def __init__(self, rows, k, square, like):
-        self.rows, self.k, self.square, self.code = rows, k, square, 0
-        self.ld, self.lds = _round_up(k, 16), _round_up((k + 127) // 128, 4)
-        size = rows * self.ld                  # whole 16 bytes, so the scales behind are aligned
-        self.buffer = like.new_empty(size + ((rows + 127) // 128 if square else rows) * self.lds, dtype=torch.uint8)
-        self.codes_ptr = self.buffer.data_ptr()
-        self.scales_ptr = self.codes_ptr + size
 
 
 def _owned(rows, k, square, dtype, like):
@@ -158,19 +147,33 @@ def _owned(rows, k, square, dtype, like):
     return b
 
 
-def _quantize(x, by_row, by_col, square, code, partial=None, drop=NO_DROP):
-    """Fills by_row (blocks of x), by_col (blocks of x^T) and partial (column sums of 128-row slabs); each may be None."""
+def _quantize(x, by_row, by_col, square, code, partial=0, drop=NO_DROP):
+    """Fills by_row (blocks of x), by_col (blocks of x^T), each (codes pointer, pitch, scales pointer, pitch) or
+    _NONE, and partial (column sums of 128-row slabs, a pointer or 0).  x's device is the current one."""
     R, C = x.shape
-    if C > 1 and x.stride(1) != 1 or R > 1 and x.stride(0) < C:
+    rs, cs = x.stride()
+    if C > 1 and cs != 1 or R > 1 and rs < C:
         x = x.contiguous()
-    dev = x.device
-    with on_device(dev):
-        rc = L.lib().advopt_fp8_quantize(_QUANT.pack(
-            x.data_ptr(), x.stride(0) if R > 1 else C, R, C,
-            *((0, 0, 0, 0) if by_row is None else (by_row.codes_ptr, by_row.ld, by_row.scales_ptr, by_row.lds)),
-            *((0, 0, 0, 0) if by_col is None else (by_col.codes_ptr, by_col.ld, by_col.scales_ptr, by_col.lds)),
-            0 if partial is None else partial.data_ptr(), dtype_code(x.dtype), square, code, 0, *drop), raw_stream(dev))
-    L.check(rc, "advopt_fp8_quantize")
+        rs = C
+    rc = L.lib().advopt_fp8_quantize(_QUANT.pack(x.data_ptr(), rs if R > 1 else C, R, C, *by_row, *by_col, partial,
+                                                 dtype_code(x.dtype), square, code, 0, *drop), raw_stream(x.device))
+    if rc:
+        L.check(rc, "advopt_fp8_quantize")
+
+
+_NONE = (0, 0, 0, 0)
+
+
+@functools.lru_cache(maxsize=4096)
+def _layout(rows, k, square):
+    """(codes' pitch, scales' offset, scales' pitch, bytes) of blocks kept in a buffer of their own."""
+    ld, lds = _round_up(k, 16), _round_up((k + 127) // 128, 4)
+    size = rows * ld                          # whole 16 bytes, so the scales behind are aligned
+    return ld, size, lds, _round_up(size + ((rows + 127) // 128 if square else rows) * lds, 16)
+
+
+def _at(base, layout):
+    return base, layout[0], base + layout[1], layout[2]
 
 
 def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.float8_e4m3fn, layout: str = "rows"):
@@ -199,20 +202,26 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.flo
     (R, C), square = x.shape, block[0] == 128
     r = _owned(R, C, square, dtype, x) if layout != "cols" else None
     c = _owned(C, R, square, dtype, x) if layout != "rows" else None
-    _quantize(x, r, c, square, _CODE[dtype])
+    with on_device(x.device):
+        _quantize(x, _NONE if r is None else r.operand, _NONE if c is None else c.operand, square, _CODE[dtype])
     return (r, c) if layout == "both" else r if layout == "rows" else c
 
 
-def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP, variant=0):
+def _product(a, b, k, a_code, b_code, a_square, b_square, out, bias=None, residual=None, drop=NO_DROP, variant=0):
+    """out = epilogue(A B^T) of two operands (codes pointer, pitch, scales pointer, pitch).  out's device is the current one."""
     m, n = out.shape
-    dev = out.device
-    with on_device(dev):
-        rc = L.lib().advopt_fp8_gemm(_GEMM.pack(
-            a.codes_ptr, a.ld, a.scales_ptr, a.lds, b.codes_ptr, b.ld, b.scales_ptr, b.lds, out.data_ptr(), n,
-            0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n, m, n, a.k,
-            a.code, b.code, a.square, b.square, dtype_code(out.dtype), variant, _ERR.pointer(), *drop), raw_stream(dev))
-    L.check(rc, "advopt_fp8_gemm")
+    rc = L.lib().advopt_fp8_gemm(_GEMM.pack(
+        *a, *b, out.data_ptr(), n, 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n,
+        m, n, k, a_code, b_code, a_square, b_square, dtype_code(out.dtype), variant, _ERR.pointer(), *drop),
+        raw_stream(out.device))
+    if rc:
+        L.check(rc, "advopt_fp8_gemm")
     return out
+
+
+def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP, variant=0):
+    with on_device(out.device):
+        return _product(a.operand, b.operand, a.k, a.code, b.code, a.square, b.square, out, bias, residual, drop, variant)
 
 
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -230,27 +239,45 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     return _gemm(a, b, a.codes.new_empty((a.rows, b.rows), dtype=out_dtype))
 
 
-def _linear(x, weight, bias, residual, w_rows, w_cols, drop, need_x, need_w):
-    """(y, blocks of x^T, blocks of the weight's transpose), the latter two as far as the gradients need them."""
+def _linear(x, weight, bias, residual, blocks, drop, need_x, need_w):
+    """(y, what the gradients need: a buffer and the operands x^T and weight^T in it).
+
+    The blocks of one pass lie in two buffers, one that ends with it and one
+    that is kept: an allocation for each, and tensor views of them, cost the
+    host as much as the kernel launches."""
     T, K = x.shape
     N = weight.shape[0]
-    xr = _Kept(T, K, False, x)
-    xc = _Kept(K, T, False, x) if need_w else None
-    _quantize(x, xr, xc, False, 0)
-    if w_rows is None:
-        w_rows = _Kept(N, K, True, weight)
-        w_cols = _Kept(K, N, True, weight) if need_x else None
-        _quantize(weight, w_rows, w_cols, True, 0)
-    return _gemm(xr, w_rows, x.new_empty((T, N)), bias, residual, drop), xc, w_cols
+    with on_device(x.device):
+        lx, lw = _layout(T, K, False), _layout(N, K, True)
+        own_w = blocks is None
+        passing = x.new_empty(lx[3] + (lw[3] if own_w else 0), dtype=torch.uint8)
+        at = passing.data_ptr()
+        xr, kept, xc, wc = _at(at, lx), None, _NONE, _NONE
+        size = (lxc := _layout(K, T, False))[3] if need_w else 0
+        if size or (need_x and own_w):
+            kept = x.new_empty(size + (_layout(K, N, True)[3] if need_x and own_w else 0), dtype=torch.uint8)
+            if need_w:
+                xc = _at(kept.data_ptr(), lxc)
+        _quantize(x, xr, xc, False, 0)
+        if own_w:
+            wr = _at(at + lx[3], lw)
+            if need_x:
+                wc = _at(kept.data_ptr() + size, _layout(K, N, True))
+            _quantize(weight, wr, wc, True, 0)
+            codes = 0, 0
+        else:
+            wr, wc = blocks[0].operand, blocks[1].operand
+            codes = blocks[0].code, blocks[1].code
+        y = _product(xr, wr, K, 0, codes[0], False, True, x.new_empty((T, N)), bias, residual, drop)
+    return y, (kept, xc, wc, blocks, codes[1], K)
 
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, w_rows, w_cols, step_tensor, drop):
+    def forward(ctx, x, weight, bias, residual, blocks, step_tensor, drop):
         need_x, need_w = ctx.needs_input_grad[:2]
-        y, ctx.xc, w_cols = _linear(x, weight, bias, residual, w_rows, w_cols, drop, need_x, need_w)
-        ctx.wc = w_cols if need_x else None
-        ctx.drop, ctx.w_dtype, ctx.x_dtype = drop, weight.dtype, x.dtype
+        y, ctx.kept = _linear(x, weight, bias, residual, blocks, drop, need_x, need_w)
+        ctx.drop, ctx.w_dtype = drop, weight.dtype
         if step_tensor is not None:
             ctx.save_for_backward(step_tensor)
         return y
@@ -260,26 +287,31 @@ class _Fp8Linear(torch.autograd.Function):
     def backward(ctx, dy):
         _ = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = partial = None
-        T, N = dy.shape
+        dx = dw = db = None
         if need_x or need_w or need_b:
-            # g = mask * dy / q once, for every gradient that reads it
-            gr = _Kept(T, N, False, dy) if need_x or not need_w else None
-            gc = _Kept(N, T, False, dy) if need_w else None
-            if need_b:
-                partial = dy.new_empty(((T + 127) // 128, N), dtype=torch.float32)
-            _quantize(dy, gr, gc, False, 0, partial, ctx.drop)
-            if need_x:
-                dx = _gemm(gr, ctx.wc, dy.new_empty((T, ctx.wc.rows), dtype=ctx.x_dtype))
-            if need_w:
-                dw = _gemm(gc, ctx.xc, dy.new_empty((N, ctx.xc.rows), dtype=ctx.w_dtype))
-            if need_b:
-                db = dy.new_empty((N,))
-                with on_device(dy.device):
-                    rc = L.lib().advopt_col_sum(db.data_ptr(), partial.data_ptr(), partial.shape[0], N, dtype_code(db.dtype),
-                                                raw_stream(dy.device))
-                L.check(rc, "advopt_col_sum")
-        return dx, dw, db, (dy if need_r else None), None, None, None, None
+            T, N = dy.shape
+            _, xc, wc, _, w_code, K = ctx.kept
+            with on_device(dy.device):
+                # g = mask * dy / q once, for every gradient that reads it
+                by_row = need_x or not need_w
+                lr, lc = _layout(T, N, False) if by_row else _ZERO, _layout(N, T, False) if need_w else _ZERO
+                slabs = (T + 127) // 128
+                passing = dy.new_empty(lr[3] + lc[3] + (4 * slabs * N if need_b else 0), dtype=torch.uint8)
+                at = passing.data_ptr()
+                gr, gc, partial = _at(at, lr), _at(at + lr[3], lc), at + lr[3] + lc[3]
+                _quantize(dy, gr if by_row else _NONE, gc if need_w else _NONE, False, 0, partial if need_b else 0, ctx.drop)
+                if need_x:
+                    dx = _product(gr, wc, N, 0, w_code, False, True, dy.new_empty((T, K)))
+                if need_w:
+                    dw = _product(gc, xc, T, 0, 0, False, False, dy.new_empty((N, K), dtype=ctx.w_dtype))
+                if need_b:
+                    db = dy.new_empty((N,))
+                    L.check(L.lib().advopt_col_sum(db.data_ptr(), partial, slabs, N, dtype_code(db.dtype),
+                                                   raw_stream(dy.device)), "advopt_col_sum")
+        return dx, dw, db, (dy if need_r else None), None, None, None
+
+
+_ZERO = (0, 0, 0, 0)
 
 
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
@@ -319,11 +351,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if N == 0 or K == 0:
         raise ValueError("fp8_linear: the weight is empty")
     drop = NO_DROP if dropout_p == 0 else drop_fields(dropout_p, seed, site, step, dev)
-    w_rows = w_cols = None
     if weight_blocks is not None:
-        w_rows, w_cols = weight_blocks
-        if not (w_rows.square and w_cols.square and (w_rows.rows, w_rows.k) == (N, K) == (w_cols.k, w_cols.rows)
-                and w_rows.device == x.device == w_cols.device):
+        r, c = weight_blocks
+        if not (r.square and c.square and (r.rows, r.k) == (N, K) == (c.k, c.rows) and r.device == dev == c.device):
             raise ValueError("fp8_linear: weight_blocks is quantize_fp8(weight, (128, 128), layout='both')")
     if x.numel() == 0:   # no tokens: no products, and gradients of zeros
         y = x.new_zeros((*x.shape[:-1], N)) if residual is None else residual.clone()
@@ -335,7 +365,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         residual = (residual if flat else residual.reshape(-1, N)).contiguous()
     x2 = x if flat else x.reshape(-1, K)
     if torch.is_grad_enabled():
-        y = _Fp8Linear.apply(x2, weight, bias, residual, w_rows, w_cols, step if isinstance(step, torch.Tensor) else None, drop)
+        y = _Fp8Linear.apply(x2, weight, bias, residual, weight_blocks, step if isinstance(step, torch.Tensor) else None, drop)
     else:   # no transposed codes, whatever the parameters' requires_grad
-        y = _linear(x2, weight, bias, residual, w_rows, w_cols, drop, False, False)[0]
+        y = _linear(x2, weight, bias, residual, weight_blocks, drop, False, False)[0]
     return y if flat else y.view(*x.shape[:-1], N)
