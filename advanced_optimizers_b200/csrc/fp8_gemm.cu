@@ -207,6 +207,15 @@ constexpr uint32_t TILE_HI = (1024u >> 4) | (1u << 14) | (2u << 29);    // 1024 
 constexpr uint32_t SCALE_HI = (128u >> 4) | (1u << 14);                  // 128 bytes between 8-row groups, none
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4); }
 
+// The product is launched while the kernel before it in the stream may still
+// run (programmatic dependent launch): barriers and tensor memory are set up
+// meanwhile, and nothing is read or written before that kernel's results are
+// there.  The kernel after it may start its own set-up as early.
+__device__ __forceinline__ void after_earlier_kernels() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -488,6 +497,7 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  after_earlier_kernels();
   // through a warp reduction: it lands in a uniform register, where the MMAs want it
   const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
 
@@ -721,6 +731,7 @@ struct PairCfg {
 
 struct PairArgs {
   int p_tiles, q_tiles;   // of 256 and BN
+  int band;
   int chunks, chunk_blocks;
 };
 
@@ -752,13 +763,16 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar, uint32_t one) {
       ::"r"(smem_u32(bar)), "h"((uint16_t)3), "r"(one)
       : "memory");
 }
-// Tile t: bands of BAND row tiles, walked row-fastest, so that the tiles in
-// flight form a near-square patch and share both operands in L2.
-constexpr int BAND = 8;
+// Tile t: bands of `band` row tiles, walked row-fastest, so that the tiles in
+// flight share both operands in L2.  Every band reads all of the column operand
+// again, so bands are as tall as the operands of 74 tiles in flight stay within
+// 40 MB of L2: 8192 x 14336 x 4096 takes 400 / 390 / 384 us in bands of 8 / 16 /
+// 32 (under the power cap), 8192 x 4096 x 14336, where 8 hold 62 MB already,
+// 392 / 412 / 435.
 __device__ __forceinline__ void pair_origin(int t, const PairArgs& w, int bn, int64_t& p0, int64_t& q0) {
-  const int band = t / (BAND * w.q_tiles), r = t - band * BAND * w.q_tiles;
-  const int rows = min(BAND, w.p_tiles - band * BAND);
-  p0 = (int64_t)(band * BAND + r % rows) * (2 * BM);
+  const int band = t / (w.band * w.q_tiles), r = t - band * w.band * w.q_tiles;
+  const int rows = min(w.band, w.p_tiles - band * w.band);
+  p0 = (int64_t)(band * w.band + r % rows) * (2 * BM);
   q0 = (int64_t)(r / rows) * bn;
 }
 
@@ -812,6 +826,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   __syncthreads();
   cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  after_earlier_kernels();
   // through a warp reduction: it lands in a uniform register, where the MMAs want it
   const uint32_t tmem = __reduce_max_sync(0xffffffffu, tmem_base);
 
@@ -1077,13 +1092,15 @@ int launch_t(const Launch& L) {
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = L.stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = S;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = S;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = S > 1 ? 1 : 0;
+  cfg.numAttrs = S > 1 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, L.g, L.d);
   return check_cuda(e, "advopt_fp8_gemm");
 }
@@ -1107,12 +1124,24 @@ int launch_pair(const Launch& L) {
   if ((int64_t)w.p_tiles * w.q_tiles > (1 << 30) ||
       ((int64_t)w.p_tiles * w.q_tiles / PAIRS + 1) * ((L.g.kblocks + 3) / 4) > (1 << 30))
     return set_error(ADVOPT_E_UNSUPPORTED, "advopt_fp8_gemm: too many output tiles");
+  w.band = 8;
+  while (w.band < 32 && (2.0 * w.band * 2 * BM + (double)PAIRS / (2 * w.band) * BN) * (double)L.k <= 40e6) w.band *= 2;
   w.chunks = BF16 ? 1 : (L.g.kblocks + CHUNK - 1) / CHUNK;
   w.chunk_blocks = ((L.g.kblocks + w.chunks - 1) / w.chunks + 3) / 4 * 4;
   w.chunks = (L.g.kblocks + w.chunk_blocks - 1) / w.chunk_blocks;
   const int tiles = w.p_tiles * w.q_tiles;
-  kernel<<<2 * (tiles < PAIRS ? tiles : PAIRS), C::THREADS, C::SMEM, L.stream>>>(mp, mq, L.g, w, L.d);
-  return check_cuda(cudaGetLastError(), "advopt_fp8_gemm");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < PAIRS ? tiles : PAIRS)));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = L.stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, mp, mq, L.g, w, L.d);
+  return check_cuda(e, "advopt_fp8_gemm");
 }
 
 template <int BN, bool BF16>
@@ -1146,11 +1175,11 @@ int launch_n(const Launch& L, int bn, int split) {
 //     8192 x 14336 x 4096 takes 336 us at 256 and 322 at 224, and
 //     8192 x 4096 x 14336 324 and 359;
 //   * single CTAs (128 x BN): a K block costs what 16 KB + BN * 128 bytes take
-//     from L2 (290 .. 680 cycles); splitting K pays a cluster's exchange:
-//     1 x 4096 x 4096 takes 11.5 / 9.0 / 7.7 / 8.0 us split 1 / 2 / 4 / 8,
-//     256 x 4096 x 4096 at BN = 64 10.6 us unsplit, at BN = 128 11.9 split in 2;
+//     from L2 (170 .. 680 cycles); splitting K pays a cluster's exchange:
+//     1 x 4096 x 4096 takes 10.9 / 8.5 / 7.4 / 6.9 us split 1 / 2 / 4 / 8,
+//     256 x 4096 x 4096 at BN = 64 10.5 us unsplit, at BN = 128 11.0 split in 2;
 //   * swapped operands write D a token at a time, a feature per lane, whatever
-//     D's alignment: 333 x 2041 x 1000 takes 6.9 us swapped, 8.3 not.
+//     D's alignment: 333 x 2041 x 1000 takes 5.3 us swapped, 6.1 not.
 struct Variant {
   bool pair, swap;
   int bn, split;
@@ -1175,12 +1204,13 @@ inline Variant choose(int64_t m, int64_t n, int64_t kblocks, bool whole_rows, bo
         const double ctas = (double)ceil_div(p, 128) * ceil_div(q, bn) * split;
         const double waves = ceil_div((int64_t)ctas, i == 0 ? 2 * SMS : SMS);   // BN = 32: two CTAs fit an SM
         double block = single_block[i];
-        if (i == 0) block = ctas > SMS ? 500 : ctas * 330 / SMS > 170 ? ctas * 330 / SMS : 170;
+        if (i == 0) block = ctas > SMS ? 400 : ctas * 330 / SMS > 170 ? ctas * 330 / SMS : 170;
+        if (i == 0 && q > 32) block *= 1.4;   // the other operand is read again for each 32 columns
         const int64_t blocks = 4 * ceil_div(ceil_div(kblocks, 4), split);
         if (f32 && blocks > CHUNK && split < 8 && ceil_div(kblocks, 4) >= 2 * split) continue;   // float32 sums stay short
         const double body = (double)(blocks < kblocks ? blocks : kblocks) * block / 1800;
         const double out = bn / 32 * (swap ? 0.35 : whole_rows ? 0.3 : 0.8) / split;
-        const double join = split == 1 ? 0 : bn / 32 * 0.3 + (split == 2 ? 1.0 : split == 4 ? 1.2 : i == 0 ? 1.5 : 6.0);
+        const double join = split == 1 ? 0 : bn / 32 * 0.3 + (split == 2 ? (i ? 1.0 : 0.7) : split == 4 ? 1.2 : i ? 6.0 : 1.3);
         const double t = 2.8 + (waves - 1) * (body + out + 1.2) + body + out + join;
         if (t < least) {
           least = t;

@@ -146,6 +146,8 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t a) {
 // rows a lane and shares the work of finding their scales.
 template <bool BF16, bool E5M2, class Row>
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ QArgs q, const __grid_constant__ DropSpec d) {
+  // a product behind this kernel may set itself up meanwhile; it waits for the codes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t step = q.drop ? drop_step(d) : 0u;
   const int l16 = threadIdx.x & 15;
   const int64_t nb = (q.cols + TILE - 1) / TILE;
@@ -330,6 +332,8 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
 template <bool BF16, bool E5M2, bool SQUARE, class Row>
 __global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(const __grid_constant__ QArgs q, const __grid_constant__ DropSpec d) {
   __shared__ __align__(16) TileShared s;
+  // a product behind this kernel may set itself up meanwhile; it waits for the codes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t step = q.drop ? drop_step(d) : 0u;
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const uint32_t across = (uint32_t)((q.cols + TILE - 1) / TILE);

@@ -66,12 +66,12 @@ def _round_up(n, to):
 
 def _empty_codes(rows, k, dtype, like):
     t = like.new_empty((rows, _round_up(k, 16)), dtype=dtype)
-    return t if t.shape[1] == k else t[:, :k]
+    return t if k % 16 == 0 else t.narrow(1, 0, k)
 
 
 def _empty_scales(rows, nb, like):
     t = like.new_empty((rows, _round_up(nb, 4)), dtype=_E8M0)
-    return t if t.shape[1] == nb else t[:, :nb]
+    return t if nb % 4 == 0 else t.narrow(1, 0, nb)
 
 
 class Fp8Blocks:
