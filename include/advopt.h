@@ -544,7 +544,7 @@ int advopt_muon_stage(const advopt_muon_args* args, int32_t stage, void* stream)
  *     {c0, c1, c2, c3, k0, k1}, out receives n x 4 words (device pointers).
  *   advopt_noise_fill: the n 16-bit values a kernel draws for elements
  *     0 .. n-1 of tensor `tensor_id` at `step` from noise stream `stream_id`
- *     (0 = v, 1 = m, 2 = param); counter = (k >> 3, stream_id << 24,
+ *     (0 = v, 1 = m, 2 = param, 4 = dropout); counter = (k >> 3, stream_id << 24,
  *     tensor_id, step), key = seed, element k takes half (k & 1) of word
  *     (k & 7) >> 1. */
 int advopt_philox4x32_10(const uint32_t* counters_keys, uint32_t* out, int64_t n, void* stream);
