@@ -435,3 +435,82 @@ def test_training_run_with_an_optimizer():
         for p, q in zip((w1, w2, b2), before):
             assert not torch.equal(p.detach(), q)
     A.check_fp8_errors()
+
+
+def test_products_on_two_streams_at_once():
+    import advanced_optimizers_b200 as A
+    cases = [operands(m, n, k, E4, E4, True, i) for i, (m, n, k) in enumerate(((8, 4096, 4096), (700, 2048, 2048), (33, 500, 8192)))]
+    want = [A.fp8_matmul(a, b, F) for a, b in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] += [A.fp8_matmul(a, b, F) for a, b in cases]
+    torch.cuda.synchronize()
+    for results in got:
+        for i, d in enumerate(results):
+            assert torch.equal(d, want[i % 3])
+    A.check_fp8_errors()
+
+
+def test_products_captured_and_replayed_on_new_data():
+    """A captured chain quantise -> product -> product, as the first call that would need the error word, and replays on other data."""
+    import advanced_optimizers_b200 as A
+    from advanced_optimizers_b200 import fp8
+    x = data(40, 512, B)
+    w1, w2 = (A.quantize_fp8(data(n, k, F, n) * 0.05, (128, 128)) for n, k in ((768, 512), (300, 768)))
+
+    def chain():
+        return A.fp8_matmul(A.quantize_fp8(A.fp8_matmul(A.quantize_fp8(x), w1)), w2, F)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        chain()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    word, fp8._ERR.word = fp8._ERR.word, None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain()
+    fp8._ERR.word = word
+    for seed in (5, 6, 7):
+        x.copy_(data(40, 512, B, seed))
+        graph.replay()
+        assert torch.equal(out, chain())
+
+
+def test_a_matrix_times_itself():
+    import advanced_optimizers_b200 as A
+    x = data(260, 384, F).requires_grad_()
+    y = A.fp8_linear(x, x)
+    dy = data(260, 260, F, 1)
+    g, = torch.autograd.grad(y, x, dy)
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    ga, gb = torch.autograd.grad(A.fp8_linear(a, b), (a, b), dy)
+    assert torch.equal(g, ga + gb)
+
+
+def test_refusals_on_the_device():
+    import advanced_optimizers_b200 as A
+    x = torch.zeros(4, 256, device="cuda")
+    q = A.quantize_fp8(x)
+    with pytest.raises(NotImplementedError):
+        A.quantize_fp8(x.half())
+    with pytest.raises(NotImplementedError):
+        A.fp8_matmul(q, q, torch.float16)
+    with pytest.raises(ValueError, match="quantised along"):
+        A.fp8_matmul(q, A.quantize_fp8(x[:, :128]))
+    with pytest.raises(ValueError, match="need scales"):
+        A.Fp8Blocks(q.codes, q.scales[:, :1])
+    with pytest.raises(ValueError, match="weight_blocks"):
+        A.fp8_linear(x, torch.zeros(8, 256, device="cuda"), weight_blocks=A.quantize_fp8(x, (128, 128), layout="both"))
+    with pytest.raises(ValueError, match="bias"):
+        A.fp8_linear(x, torch.zeros(8, 256, device="cuda"), torch.zeros(7, device="cuda"))
+    with pytest.raises(ValueError, match="residual"):
+        A.fp8_linear(x, torch.zeros(8, 256, device="cuda"), residual=torch.zeros(4, 9, device="cuda"))
+    with pytest.raises(NotImplementedError):
+        A.fp8_linear(x.half(), torch.zeros(8, 256, device="cuda"))
