@@ -114,6 +114,53 @@ __device__ __forceinline__ void load_row(Row8H& r, const void* x, int64_t k0, in
       r.w[i] = (2 * i < nv ? (uint32_t)p[2 * i] : 0u) | (2 * i + 1 < nv ? (uint32_t)p[2 * i + 1] << 16 : 0u);
   }
 }
+// Eight bf16 elements of each of eight rows whose starts are not 16-byte
+// aligned (`at`: the lane's first element's address; all lanes take part): a
+// lane loads the aligned 16 bytes its elements begin in, takes the next 16
+// from the lane behind (the last lane loads them too, where it needs them) and
+// shifts: 8192 x 4097 takes 36 us, element by element 50.  float32 rows, whose
+// elements are loads of 4 bytes, gain nothing by it (54 us either way).  Every
+// aligned 16 bytes that are read hold an element of the row, so
+// the reads stay in the matrix's memory to within those 16 bytes.
+__device__ __forceinline__ void shifted(const uint4& a, const uint4& b, uint32_t halves, uint32_t (&w)[4]) {
+  const bool by4 = halves & 4, by2 = halves & 2, by1 = halves & 1;
+  const uint32_t s0 = by4 ? a.z : a.x, s1 = by4 ? a.w : a.y, s2 = by4 ? b.x : a.z, s3 = by4 ? b.y : a.w, s4 = by4 ? b.z : b.x,
+                 s5 = by4 ? b.w : b.y;
+  const uint32_t t[5] = {by2 ? s1 : s0, by2 ? s2 : s1, by2 ? s3 : s2, by2 ? s4 : s3, by2 ? s5 : s4};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = by1 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+}
+__device__ __forceinline__ uint4 from_lane_behind(const uint4& a) {
+  return make_uint4(__shfl_down_sync(0xffffffffu, a.x, 1, 16), __shfl_down_sync(0xffffffffu, a.y, 1, 16),
+                    __shfl_down_sync(0xffffffffu, a.z, 1, 16), __shfl_down_sync(0xffffffffu, a.w, 1, 16));
+}
+// `at`: the lane's first element's address; all lanes of the warp take part.
+__device__ __forceinline__ void load_rows_unaligned(Row8H (&v)[8], const unsigned char* at, int64_t pitch) {
+  const bool last = (threadIdx.x & 15) == 15;
+  uint4 a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned char* p = at + i * pitch;
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+    const uint4* q = reinterpret_cast<const uint4*>(p - off);
+    a[i] = __ldg(q);
+    if (last && off) b[i] = __ldg(q + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint4 n = from_lane_behind(a[i]);
+    if (!last) b[i] = n;
+    shifted(a[i], b[i], ((uint32_t)reinterpret_cast<uintptr_t>(at + i * pitch) & 15u) >> 1, v[i].w);
+  }
+}
+__device__ __forceinline__ void load_rows_unaligned(Row8F (&v)[8], const unsigned char* at, int64_t pitch) {
+  Row8H h[8];
+  load_rows_unaligned(h, at, pitch);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i].v[e] = h[i].at(e);
+}
 __device__ __forceinline__ void drop_row(Row8F& r, const DropSpec& d, uint32_t step, uint64_t k0) { drop8(r.v, d, step, k0); }
 __device__ __forceinline__ void drop_row(Row8H&, const DropSpec&, uint32_t, uint64_t) {}   // dropped values are float32
 
@@ -341,10 +388,12 @@ __global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(co
   const int64_t r0 = tr * TILE, c0 = tc * TILE;
   const int64_t c = c0 + l * 8;
   const int nv = c >= q.cols ? 0 : q.cols - c < 8 ? (int)(q.cols - c) : 8;
-  const bool full = q.vec && r0 + TILE <= q.rows && c0 + TILE <= q.cols;
+  const bool full = r0 + TILE <= q.rows && c0 + TILE <= q.cols;
   Row v[8];
   int64_t at = (r0 + g * 8) * q.ldx + c;
-  if (full) {
+  if (BF16 && full && !q.vec) {
+    load_rows_unaligned(v, static_cast<const unsigned char*>(q.x) + at * 2, q.ldx * 2);
+  } else if (full && q.vec) {
 #pragma unroll
     for (int i = 0; i < 8; ++i, at += q.ldx) load_row<BF16>(v[i], q.x, at, 8, true);
   } else {

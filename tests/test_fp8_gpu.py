@@ -58,7 +58,7 @@ def data(rows, cols, dtype, seed=0):
 @pytest.mark.parametrize("block", [1, 128])
 @pytest.mark.parametrize("dtype", [B, F])
 @pytest.mark.parametrize("code", [E4, E5])
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (7, 130), (128, 128), (129, 257), (300, 1000), (2, 4096), (1000, 64)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (7, 130), (128, 128), (129, 257), (257, 387), (300, 1000), (2, 4096), (1000, 64)])
 def test_quantize(rows, cols, code, dtype, block, layout):
     import advanced_optimizers_b200 as A
     x = data(rows, cols, dtype)
@@ -99,11 +99,11 @@ def test_quantize_special_values(dtype, code, block):
 
 
 @pytest.mark.parametrize("dtype", [B, F])
-@pytest.mark.parametrize("first,cols", [(0, 200), (3, 200), (8, 256), (1, 1)])
+@pytest.mark.parametrize("first,cols", [(0, 200), (3, 200), (8, 256), (1, 1), (2, 300), (5, 261), (7, 384)])
 def test_quantize_strided_rows(first, cols, dtype):
     """A slice of columns, aligned or not, and a transposed matrix; nothing outside is touched."""
     import advanced_optimizers_b200 as A
-    wide = data(150, 520, dtype)
+    wide = data(300, 521, dtype)
     x = wide[:, first:first + cols]
     for t in (x, x.t(), x[::2], x[:, ::2]):
         r, c = A.quantize_fp8(t, layout="both")
