@@ -53,14 +53,14 @@ def _launch(x, residual, fields):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, step_tensor, fields):
-        ctx.fields = fields
-        if step_tensor is not None:
+        ctx.fields, ctx.stepped = fields, step_tensor is not None
+        if ctx.stepped:
             ctx.save_for_backward(step_tensor)
         return _launch(x, residual, fields)
 
     @staticmethod
     def backward(ctx, dy):
-        step = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
+        step = ctx.saved_tensors if ctx.stepped else ()   # raises if the step tensor was written since the forward pass
         dx = None
         if ctx.needs_input_grad[0]:
             g = dy.contiguous()

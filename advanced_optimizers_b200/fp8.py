@@ -168,7 +168,7 @@ def _quantize(x, by_row, by_col, square, code, partial=0, drop=NO_DROP):
         L.check(rc, "advopt_fp8_quantize")
 
 
-_NONE = (0, 0, 0, 0)
+_NONE = _ZERO = (0, 0, 0, 0)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -246,8 +246,15 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     return _gemm(a, b, a.codes.new_empty((a.rows, b.rows), dtype=out_dtype))
 
 
+def _kept_at(base, T, N, K, need_x, need_w, own_w):
+    """The operands x^T and weight^T in the buffer kept for the gradients, and its size."""
+    lx = _layout(K, T, False) if need_w else _ZERO
+    lw = _layout(K, N, True) if need_x and own_w else _ZERO
+    return _at(base, lx), _at(base + lx[3], lw), lx[3] + lw[3]
+
+
 def _linear(x, weight, bias, residual, blocks, drop, need_x, need_w):
-    """(y, what the gradients need: a buffer and the operands x^T and weight^T in it).
+    """(y, the buffer of x^T's and the weight^T's blocks that the gradients need, or None).
 
     The blocks of one pass lie in two buffers, one that ends with it and one
     that is kept: an allocation for each, and tensor views of them, cost the
@@ -255,70 +262,69 @@ def _linear(x, weight, bias, residual, blocks, drop, need_x, need_w):
     T, K = x.shape
     N = weight.shape[0]
     with on_device(x.device):
-        lx, lw = _layout(T, K, False), _layout(N, K, True)
         own_w = blocks is None
-        passing = x.new_empty(lx[3] + (lw[3] if own_w else 0), dtype=torch.uint8)
-        at = passing.data_ptr()
-        xr, kept, xc, wc = _at(at, lx), None, _NONE, _NONE
-        size = (lxc := _layout(K, T, False))[3] if need_w else 0
-        if size or (need_x and own_w):
-            kept = x.new_empty(size + (_layout(K, N, True)[3] if need_x and own_w else 0), dtype=torch.uint8)
-            if need_w:
-                xc = _at(kept.data_ptr(), lxc)
-        _quantize(x, xr, xc, False, 0)
+        lx, lw = _layout(T, K, False), _layout(N, K, True) if own_w else _ZERO
+        passing = x.new_empty(lx[3] + lw[3], dtype=torch.uint8)
+        xr, wr = _at(passing.data_ptr(), lx), _at(passing.data_ptr() + lx[3], lw)
+        size = _kept_at(0, T, N, K, need_x, need_w, own_w)[2]
+        kept = x.new_empty(size, dtype=torch.uint8) if size else None
+        xc, wc, _ = _kept_at(kept.data_ptr() if size else 0, T, N, K, need_x, need_w, own_w)
+        _quantize(x, xr, xc if need_w else _NONE, False, 0)
         if own_w:
-            wr = _at(at + lx[3], lw)
-            if need_x:
-                wc = _at(kept.data_ptr() + size, _layout(K, N, True))
-            _quantize(weight, wr, wc, True, 0)
-            codes = 0, 0
+            _quantize(weight, wr, wc if need_x else _NONE, True, 0)
         else:
-            wr, wc = blocks[0].operand, blocks[1].operand
-            codes = blocks[0].code, blocks[1].code
-        y = _product(xr, wr, K, 0, codes[0], False, True, x.new_empty((T, N)), bias, residual, drop)
-    return y, (kept, xc, wc, blocks, codes[1], K)
+            wr = blocks[0].operand
+        y = _product(xr, wr, K, 0, 0 if own_w else blocks[0].code, False, True, x.new_empty((T, N)), bias, residual, drop)
+    return y, kept
+
+
+def _linear_backward(ctx, dy):
+    saved = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        T, N = dy.shape
+        K, blocks = ctx.K, ctx.blocks
+        # by offset from where the buffer is now: a hook on saved tensors may have moved it
+        xc, wc, size = _kept_at(saved[0].data_ptr() if ctx.keeps else 0, T, N, K, need_x, need_w, blocks is None)
+        with on_device(dy.device):
+            # g = mask * dy / q once, for every gradient that reads it
+            by_row = need_x or not need_w
+            lr, lc = _layout(T, N, False) if by_row else _ZERO, _layout(N, T, False) if need_w else _ZERO
+            slabs = (T + 127) // 128
+            passing = dy.new_empty(lr[3] + lc[3] + (4 * slabs * N if need_b else 0), dtype=torch.uint8)
+            at = passing.data_ptr()
+            gr, gc, partial = _at(at, lr), _at(at + lr[3], lc), at + lr[3] + lc[3]
+            _quantize(dy, gr if by_row else _NONE, gc if need_w else _NONE, False, 0, partial if need_b else 0, ctx.drop)
+            if need_x:
+                w_code = 0
+                if blocks is not None:
+                    wc, w_code = blocks[1].operand, blocks[1].code
+                dx = _product(gr, wc, N, 0, w_code, False, True, dy.new_empty((T, K)))
+            if need_w:
+                dw = _product(gc, xc, T, 0, 0, False, False, dy.new_empty((N, K), dtype=ctx.w_dtype))
+            if need_b:
+                db = dy.new_empty((N,))
+                L.check(L.lib().advopt_col_sum(db.data_ptr(), partial, slabs, N, dtype_code(db.dtype),
+                                               raw_stream(dy.device)), "advopt_col_sum")
+    return dx, dw, db, (dy if need_r else None), None, None, None
+
+
+_linear_backward_once = torch.autograd.function.once_differentiable(_linear_backward)
 
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, blocks, step_tensor, drop):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        y, ctx.kept = _linear(x, weight, bias, residual, blocks, drop, need_x, need_w)
-        ctx.drop, ctx.w_dtype = drop, weight.dtype
-        if step_tensor is not None:
-            ctx.save_for_backward(step_tensor)
+        y, kept = _linear(x, weight, bias, residual, blocks, drop, *ctx.needs_input_grad[:2])
+        ctx.drop, ctx.w_dtype, ctx.K, ctx.blocks, ctx.keeps = drop, weight.dtype, x.shape[1], blocks, kept is not None
+        ctx.save_for_backward(*[t for t in (kept, step_tensor) if t is not None])
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        _ = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            T, N = dy.shape
-            _, xc, wc, _, w_code, K = ctx.kept
-            with on_device(dy.device):
-                # g = mask * dy / q once, for every gradient that reads it
-                by_row = need_x or not need_w
-                lr, lc = _layout(T, N, False) if by_row else _ZERO, _layout(N, T, False) if need_w else _ZERO
-                slabs = (T + 127) // 128
-                passing = dy.new_empty(lr[3] + lc[3] + (4 * slabs * N if need_b else 0), dtype=torch.uint8)
-                at = passing.data_ptr()
-                gr, gc, partial = _at(at, lr), _at(at + lr[3], lc), at + lr[3] + lc[3]
-                _quantize(dy, gr if by_row else _NONE, gc if need_w else _NONE, False, 0, partial if need_b else 0, ctx.drop)
-                if need_x:
-                    dx = _product(gr, wc, N, 0, w_code, False, True, dy.new_empty((T, K)))
-                if need_w:
-                    dw = _product(gc, xc, T, 0, 0, False, False, dy.new_empty((N, K), dtype=ctx.w_dtype))
-                if need_b:
-                    db = dy.new_empty((N,))
-                    L.check(L.lib().advopt_col_sum(db.data_ptr(), partial, slabs, N, dtype_code(db.dtype),
-                                                   raw_stream(dy.device)), "advopt_col_sum")
-        return dx, dw, db, (dy if need_r else None), None, None, None
-
-
-_ZERO = (0, 0, 0, 0)
+        # a second derivative is refused, without the wrapper's cost where none can be asked for
+        return _linear_backward_once(ctx, dy) if torch.is_grad_enabled() else _linear_backward(ctx, dy)
 
 
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,

@@ -514,3 +514,34 @@ def test_refusals_on_the_device():
         A.fp8_linear(x, torch.zeros(8, 256, device="cuda"), residual=torch.zeros(4, 9, device="cuda"))
     with pytest.raises(NotImplementedError):
         A.fp8_linear(x.half(), torch.zeros(8, 256, device="cuda"))
+
+
+def test_second_derivatives_are_refused():
+    import advanced_optimizers_b200 as A
+    x, w = data(40, 128, F).requires_grad_(), data(50, 128, F, 1).requires_grad_()
+    dy = data(40, 50, F, 2).requires_grad_()
+    y = A.fp8_linear(x, w)
+    want = torch.autograd.grad(A.fp8_linear(x, w), (x, w), dy.detach())
+    got = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+    assert all(torch.equal(a.detach(), b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(got[0].sum(), dy)
+
+
+def test_kept_blocks_are_saved_tensors():
+    """They go with the graph's other saved tensors: through hooks that move them, and released by the backward pass."""
+    import advanced_optimizers_b200 as A
+    x, w, dy = data(40, 256, B).requires_grad_(), data(130, 256, B, 1).requires_grad_(), data(40, 130, B, 2)
+    want = torch.autograd.grad(A.fp8_linear(x, w), (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = A.fp8_linear(x, w)
+    filler = torch.randint(0, 255, (1 << 20,), device="cuda", dtype=torch.uint8)   # over what was moved away
+    got = torch.autograd.grad(y, (x, w), dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and filler.numel()
+    y = A.fp8_linear(x, w)
+    torch.autograd.grad(y, (x, w), dy)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, (x, w), dy)
+    y = A.fp8_linear(x, w)
+    torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), want))
