@@ -49,29 +49,34 @@ __device__ __forceinline__ uint32_t drop_word(const U4& w, uint32_t i) {
   return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
 }
 
+// The 16-bit values of elements k0 .. k0 + 7, two per word.  k0 a multiple of 8
+// takes one evaluation, other starts two.
+__device__ __forceinline__ U4 drop_values(const DropSpec& d, uint32_t step, uint64_t k0) {
+  const U4 w = drop_group(d, step, k0 >> 3);
+  const uint32_t off = (uint32_t)(k0 & 7);
+  if (off == 0) return w;
+  // shift the two groups' 256 bits down by off 16-bit values: by 4, 2 and 1 of them
+  const U4 x = drop_group(d, step, (k0 >> 3) + 1);
+  const bool by4 = off & 4, by2 = off & 2, by1 = off & 1;
+  const uint32_t s0 = by4 ? w.z : w.x, s1 = by4 ? w.w : w.y, s2 = by4 ? x.x : w.z, s3 = by4 ? x.y : w.w,
+                 s4 = by4 ? x.z : x.x, s5 = by4 ? x.w : x.y;
+  const uint32_t t[5] = {by2 ? s1 : s0, by2 ? s2 : s1, by2 ? s3 : s2, by2 ? s4 : s3, by2 ? s5 : s4};
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = by1 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+  return U4{r[0], r[1], r[2], r[3]};
+}
+
 // v[e] of elements k0 + e becomes v[e] * scale where the element is kept, else
-// 0.  k0 a multiple of 8 takes one evaluation, other starts two.  The odd
-// elements' values are compared where they lie, in the words' high halves.
+// 0.  The odd elements' values are compared where they lie, in the words' high
+// halves.
 __device__ __forceinline__ void drop8(float (&v)[8], const DropSpec& d, uint32_t step, uint64_t k0) {
   if (d.none) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
     return;
   }
-  U4 w = drop_group(d, step, k0 >> 3);
-  const uint32_t off = (uint32_t)(k0 & 7);
-  if (off) {
-    // shift the two groups' 256 bits down by off 16-bit values: by 4, 2 and 1 of them
-    const U4 x = drop_group(d, step, (k0 >> 3) + 1);
-    const bool by4 = off & 4, by2 = off & 2, by1 = off & 1;
-    const uint32_t s0 = by4 ? w.z : w.x, s1 = by4 ? w.w : w.y, s2 = by4 ? x.x : w.z, s3 = by4 ? x.y : w.w,
-                   s4 = by4 ? x.z : x.x, s5 = by4 ? x.w : x.y;
-    const uint32_t t[5] = {by2 ? s1 : s0, by2 ? s2 : s1, by2 ? s3 : s2, by2 ? s4 : s3, by2 ? s5 : s4};
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = by1 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
-    w = U4{r[0], r[1], r[2], r[3]};
-  }
+  const U4 w = drop_values(d, step, k0);
   const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -79,6 +84,20 @@ __device__ __forceinline__ void drop8(float (&v)[8], const DropSpec& d, uint32_t
     v[2 * i] = (q[i] << 16) >= d.cut ? a : 0.0f;
     v[2 * i + 1] = q[i] >= d.cut ? b : 0.0f;
   }
+}
+
+// The same on packed bf16 pairs, without the scale: dropped halves become 0.
+__device__ __forceinline__ void drop_packed(uint32_t (&v)[4], const DropSpec& d, uint32_t step, uint64_t k0) {
+  if (d.none) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = 0u;
+    return;
+  }
+  const U4 w = drop_values(d, step, k0);
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] &= ((q[i] << 16) >= d.cut ? 0x0000FFFFu : 0u) | (q[i] >= d.cut ? 0xFFFF0000u : 0u);
 }
 
 __device__ __forceinline__ float drop1(float v, const DropSpec& d, uint32_t step, uint64_t k) {
