@@ -95,40 +95,43 @@ class Fp8Blocks:
     __slots__ = ("codes", "scales", "rows", "k", "square", "ld", "lds", "codes_ptr", "scales_ptr", "code")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        if codes.dtype not in _CODE or scales.dtype != _E8M0:
+        code = _CODE.get(codes.dtype)
+        if code is None or scales.dtype is not _E8M0:
             raise NotImplementedError("Fp8Blocks: codes are float8_e4m3fn or float8_e5m2, scales float8_e8m0fnu "
                                       f"(got {codes.dtype}, {scales.dtype})")
         if not codes.is_cuda or scales.device != codes.device:
             raise NotImplementedError("Fp8Blocks: codes and scales must live on one CUDA device (no CPU fallback)")
-        if codes.dim() != 2 or scales.dim() != 2:
+        shape, of_scales = codes.shape, scales.shape
+        if len(shape) != 2 or len(of_scales) != 2:
             raise ValueError("Fp8Blocks: codes and scales are matrices")
-        rows, k = codes.shape
-        nb = (k + 127) // 128
-        if tuple(scales.shape) == (rows, nb):
-            square = False
-        elif tuple(scales.shape) == ((rows + 127) // 128, nb):
-            square = True
-        else:
+        rows, k = shape
+        srows, nb = of_scales
+        square = srows != rows
+        if nb != (k + 127) // 128 or square and srows != (rows + 127) // 128:
+            nb = (k + 127) // 128
             raise ValueError(f"Fp8Blocks: codes {rows} x {k} need scales {rows} x {nb} or {(rows + 127) // 128} x {nb}, "
-                             f"got {tuple(scales.shape)}")
+                             f"got {tuple(of_scales)}")
+        codes_ptr, scales_ptr = codes.data_ptr(), scales.data_ptr()
         if rows and k:
-            ld = codes.stride(0) if rows > 1 else _round_up(k, 16)
-            if codes.data_ptr() % 16 or ld % 16 or ld < k or (k > 1 and codes.stride(1) != 1):
+            (ld, one), (lds, sone) = codes.stride(), scales.stride()
+            if rows == 1:
+                ld = _round_up(k, 16)
+            if codes_ptr % 16 or ld % 16 or ld < k or (one != 1 and k > 1):
                 own = _empty_codes(rows, k, codes.dtype, codes)
                 own.view(torch.uint8).copy_(codes.view(torch.uint8))
-                codes, ld = own, _pitch(k)
-            lds = scales.stride(0) if scales.shape[0] > 1 else _round_up(nb, 4)
-            if scales.data_ptr() % 4 or lds % 4 or lds < nb or (nb > 1 and scales.stride(1) != 1) or (
+                codes, ld, codes_ptr = own, _pitch(k), own.data_ptr()
+            if srows == 1:
+                lds = _round_up(nb, 4)
+            if scales_ptr % 4 or lds % 4 or lds < nb or (sone != 1 and nb > 1) or (
                     nb % 4 and scales.untyped_storage().nbytes() <
-                    scales.storage_offset() + (scales.shape[0] - 1) * lds + _round_up(nb, 4)):
-                own = _empty_scales(scales.shape[0], nb, scales)
+                    scales.storage_offset() + (srows - 1) * lds + _round_up(nb, 4)):
+                own = _empty_scales(srows, nb, scales)
                 own.view(torch.uint8).copy_(scales.view(torch.uint8))
-                scales, lds = own, _round_up(nb, 4)
-            self.ld, self.lds = ld, lds
+                scales, lds, scales_ptr = own, _round_up(nb, 4), own.data_ptr()
         else:
-            self.ld, self.lds = _pitch(k), _round_up(nb, 4)
-        self.codes, self.scales, self.rows, self.k, self.square = codes, scales, rows, k, square
-        self.codes_ptr, self.scales_ptr, self.code = codes.data_ptr(), scales.data_ptr(), _CODE[codes.dtype]
+            ld, lds = _pitch(k), _round_up(nb, 4)
+        self.codes, self.scales, self.rows, self.k, self.square, self.code = codes, scales, rows, k, square, code
+        self.ld, self.lds, self.codes_ptr, self.scales_ptr = ld, lds, codes_ptr, scales_ptr
 
     @property
     def operand(self):
@@ -236,14 +239,15 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     scales stand for, summed in float32 and rounded once to `out_dtype`
     (bfloat16 or float32).  The operands may differ in code type and block
     shape.  Its gradients are products of the same kind (see `fp8_linear`)."""
+    codes = a.codes
     if a.k != b.k:
         raise ValueError(f"fp8_matmul: the operands are quantised along {a.k} and {b.k} elements")
-    if a.codes.device != b.codes.device:
+    if codes.device != b.codes.device:
         raise ValueError(f"fp8_matmul: operands on {a.device} and {b.device}")
     dtype_code(out_dtype)
     if a.k == 0:
         return torch.zeros((a.rows, b.rows), dtype=out_dtype, device=a.device)
-    return _gemm(a, b, a.codes.new_empty((a.rows, b.rows), dtype=out_dtype))
+    return _gemm(a, b, codes.new_empty((a.rows, b.rows), dtype=out_dtype))
 
 
 def _kept_at(base, T, N, K, need_x, need_w, own_w):

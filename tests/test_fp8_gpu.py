@@ -545,3 +545,18 @@ def test_kept_blocks_are_saved_tensors():
     y = A.fp8_linear(x, w)
     torch.autograd.grad(y, (x, w), dy, retain_graph=True)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, w), dy), want))
+
+
+@pytest.mark.parametrize("variant", [0, 1256, 101256])
+def test_matmul_past_32_bits(variant):
+    """A result of more than 2^32 elements: its last rows are those of a small product."""
+    from advanced_optimizers_b200 import check_fp8_errors, fp8
+    m, n, k = 66000, 66048, 160
+    a, b = operands(m, n, k, E4, E4, False)
+    d = fp8._gemm(a, b, torch.empty(m, n, dtype=B, device="cuda"), variant=variant)
+    check_fp8_errors()
+    tail = fp8.Fp8Blocks(a.codes[-300:], a.scales[-300:])
+    want = fp8._gemm(tail, b, torch.empty(300, n, dtype=B, device="cuda"), variant=variant)
+    assert torch.equal(d[-300:], want)
+    close_product(want[-200:, -200:], ref.values(tail)[-200:], ref.values(b)[-200:])
+    close_product(d[:200, :200], ref.values(a)[:200], ref.values(b)[:200])
