@@ -560,3 +560,19 @@ def test_matmul_past_32_bits(variant):
     assert torch.equal(d[-300:], want)
     close_product(want[-200:, -200:], ref.values(tail)[-200:], ref.values(b)[-200:])
     close_product(d[:200, :200], ref.values(a)[:200], ref.values(b)[:200])
+
+
+def test_a_wait_that_gave_up_is_reported_once():
+    """The word a kernel's bounded wait would set (here set by the host): the next call and check_fp8_errors raise, then calls work again."""
+    import advanced_optimizers_b200 as A
+    from advanced_optimizers_b200 import _lib, fp8
+    a, b = operands(8, 128, 256, E4, E4, True)
+    want = A.fp8_matmul(a, b)
+    fp8._ERR.view[0] = 1
+    with pytest.raises(_lib.AdvOptError, match="bounded wait"):
+        A.fp8_matmul(a, b)
+    fp8._ERR.view[0] = 1
+    with pytest.raises(_lib.AdvOptError, match="bounded wait"):
+        A.check_fp8_errors()
+    A.check_fp8_errors()
+    assert torch.equal(A.fp8_matmul(a, b), want)
