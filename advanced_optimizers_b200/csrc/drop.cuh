@@ -86,7 +86,18 @@ __device__ __forceinline__ void drop8(float (&v)[8], const DropSpec& d, uint32_t
   }
 }
 
-// The same on packed bf16 pairs, without the scale: dropped halves become 0.
+// Which of elements k0 .. k0 + 7 are kept, a bit each.
+__device__ __forceinline__ uint32_t drop_bits8(const DropSpec& d, uint32_t step, uint64_t k0) {
+  if (d.none) return 0u;
+  const U4 w = drop_values(d, step, k0);
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits |= ((q[i] << 16) >= d.cut ? 1u << (2 * i) : 0u) | (q[i] >= d.cut ? 2u << (2 * i) : 0u);
+  return bits;
+}
+
+// The same as drop8 on packed bf16 pairs, without the scale: dropped halves become 0.
 __device__ __forceinline__ void drop_packed(uint32_t (&v)[4], const DropSpec& d, uint32_t step, uint64_t k0) {
   if (d.none) {
 #pragma unroll
