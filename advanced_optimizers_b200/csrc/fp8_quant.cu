@@ -101,8 +101,8 @@ struct Row8H {
 // bf16 with a dropout: the dropped halves are 0 and the values' common factor
 // is applied as they are used, so the elements stay packed (8192 x 4096, both
 // layouts: 47 us, as float32 52, without a dropout 26; the Philox rounds are
-// most of the rest).  The largest
-// product is the product with the largest element, since rounding is monotonic.
+// most of the rest).  The largest product is the product with the largest
+// element, since rounding is monotonic.
 struct Row8D : Row8H {
   float f;
   __device__ __forceinline__ float at(int e) const { return __fmul_rn(Row8H::at(e), f); }

@@ -72,8 +72,7 @@ def _pitch(k):
 
 def _empty_codes(rows, k, dtype, like):
     ld = _pitch(k)
-    t = like.new_empty((rows, ld), dtype=dtype)
-    return t if k == ld else t.narrow(1, 0, k)
+    return like.new_empty((rows, k), dtype=dtype) if k == ld else like.new_empty_strided((rows, k), (ld, 1), dtype=dtype)
 
 
 def _empty_scales(rows, nb, like):

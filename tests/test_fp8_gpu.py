@@ -576,3 +576,33 @@ def test_a_wait_that_gave_up_is_reported_once():
         A.check_fp8_errors()
     A.check_fp8_errors()
     assert torch.equal(A.fp8_matmul(a, b), want)
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("T,N", [(256, 384), (150, 261)])
+def test_linear_infinities_in_dropped_places(T, N, dtype):
+    """What is dropped does not reach a gradient, whatever stands there; a kept infinity reaches its row of dx and of dweight alone."""
+    import advanced_optimizers_b200 as A
+    x, w = data(T, 256, dtype).requires_grad_(), (data(N, 256, dtype, 1) * 0.1).requires_grad_()
+    b = torch.zeros(N, device="cuda", dtype=dtype, requires_grad=True)
+    key = (123, 4, 5)
+    f = ref.keep_factor((T, N), 0.5, *key)
+    dy = torch.where(f > 0, data(T, N, dtype, 2).float(), torch.zeros((), device="cuda")).to(dtype)
+    run = lambda g: torch.autograd.grad(A.fp8_linear(x, w, b, dropout_p=0.5, seed=key[0], site=key[1], step=key[2]), (x, w, b), g)  # noqa: E731
+    want = run(dy)
+    bad = dy.clone()
+    at = (f == 0).nonzero()
+    bad[at[::3, 0], at[::3, 1]] = float("inf")
+    bad[at[1::3, 0], at[1::3, 1]] = float("nan")
+    for got, w0 in zip(run(bad), want):
+        assert bool(torch.isfinite(got).all()) and torch.equal(got, w0)
+    i, j = (f > 0).nonzero()[1000].tolist()
+    bad[i, j] = float("-inf")
+    dx, dw, db = run(bad)
+    rows = torch.zeros(T, dtype=torch.bool, device="cuda")
+    rows[i] = True
+    assert torch.equal(torch.isnan(dx).all(1), rows) and torch.equal(torch.isnan(dx).any(1), rows)
+    cols = torch.zeros(N, dtype=torch.bool, device="cuda")
+    cols[j] = True
+    assert torch.equal(torch.isnan(dw).all(1), cols) and torch.equal(torch.isnan(dw).any(1), cols)
+    assert torch.equal(~torch.isfinite(db), cols)
