@@ -40,6 +40,15 @@ def drop_fields(p, seed, site, step, device):
     return seed, step_ptr, site, step, threshold, scale
 
 
+def with_saved_step(fields, step, device):
+    """`fields` with the step where the unpacked saved tensor `step` holds it: a hook on saved tensors gives another
+    tensor than the caller's, which may have been advanced or freed since the forward pass."""
+    if step.dtype != torch.int64 or step.numel() != 1 or step.device != device:
+        raise RuntimeError(f"a hook on saved tensors gave {step.dtype} {tuple(step.shape)} on {step.device} for the step, "
+                           f"one int64 value on {device} was saved")
+    return fields[0], step.data_ptr(), *fields[2:]
+
+
 def _launch(x, residual, fields):
     y = torch.empty_like(x)
     with on_device(x.device):
@@ -60,13 +69,16 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        step = ctx.saved_tensors if ctx.stepped else ()   # raises if the step tensor was written since the forward pass
-        dx = None
+        dx = step = None
+        fields = ctx.fields
+        if ctx.stepped:
+            step, = ctx.saved_tensors   # raises if the step tensor was written since the forward pass
+            fields = with_saved_step(fields, step, dy.device)
         if ctx.needs_input_grad[0]:
             g = dy.contiguous()
             # the gradient's own gradient is the same mask again
-            dx = (_Dropout.apply(g, None, step[0] if step else None, ctx.fields) if torch.is_grad_enabled() and g.requires_grad
-                  else _launch(g, None, ctx.fields))
+            dx = (_Dropout.apply(g, None, step, fields) if torch.is_grad_enabled() and g.requires_grad
+                  else _launch(g, None, fields))
         return dx, (dy if ctx.needs_input_grad[1] else None), None, None
 
 
@@ -81,7 +93,11 @@ def philox_dropout(x: torch.Tensor, p: float, *, seed: int = 42, site: int = 0, 
     one model apart, `step` the training steps: an int, or a one-element int64
     tensor on x's device, which is read when the kernel runs, so that each
     replay of a captured graph draws another mask.  It may be advanced only
-    after the backward pass, which reads it again.
+    after the backward pass, which reads it again: a write between the two
+    raises.  Hooks on saved tensors that keep a copy (`save_on_cpu`) keep the
+    forward pass's value with it.  A checkpointed region runs its forward pass
+    again and reads the step as it is then; pass it as an argument of
+    `checkpoint`, which raises if it was written, not through a closure.
 
     x and residual (of x's shape and dtype): float32 or bfloat16 on one CUDA
     device; other strides than contiguous ones are copied first."""

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib as L
 from ._device import dtype_code, on_device, raw_stream
-from .dropout import NO_DROP, drop_fields
+from .dropout import NO_DROP, drop_fields, with_saved_step
 
 _CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _E8M0 = torch.float8_e8m0fnu
@@ -288,6 +288,7 @@ def _linear_backward(ctx, dy):
     if need_x or need_w or need_b:
         T, N = dy.shape
         K, blocks = ctx.K, ctx.blocks
+        drop = with_saved_step(ctx.drop, saved[-1], dy.device) if ctx.stepped else ctx.drop
         # by offset from where the buffer is now: a hook on saved tensors may have moved it
         xc, wc, size = _kept_at(saved[0].data_ptr() if ctx.keeps else 0, T, N, K, need_x, need_w, blocks is None)
         with on_device(dy.device):
@@ -298,7 +299,7 @@ def _linear_backward(ctx, dy):
             passing = dy.new_empty(lr[3] + lc[3] + (4 * slabs * N if need_b else 0), dtype=torch.uint8)
             at = passing.data_ptr()
             gr, gc, partial = _at(at, lr), _at(at + lr[3], lc), at + lr[3] + lc[3]
-            _quantize(dy, gr if by_row else _NONE, gc if need_w else _NONE, False, 0, partial if need_b else 0, ctx.drop)
+            _quantize(dy, gr if by_row else _NONE, gc if need_w else _NONE, False, 0, partial if need_b else 0, drop)
             if need_x:
                 w_code = 0
                 if blocks is not None:
@@ -321,6 +322,7 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, blocks, step_tensor, drop):
         y, kept = _linear(x, weight, bias, residual, blocks, drop, *ctx.needs_input_grad[:2])
         ctx.drop, ctx.w_dtype, ctx.K, ctx.blocks, ctx.keeps = drop, weight.dtype, x.shape[1], blocks, kept is not None
+        ctx.stepped = step_tensor is not None
         ctx.save_for_backward(*[t for t in (kept, step_tensor) if t is not None])
         return y
 

@@ -1,0 +1,95 @@
+"""Autograd rules of the dropout and fp8 operators that need no GPU: the kernel
+launches are replaced by readers of the addresses that they are given."""
+import ctypes
+import gc
+
+import pytest
+import torch
+from torch.autograd.graph import saved_tensors_hooks
+from torch.utils.checkpoint import checkpoint
+
+
+@pytest.fixture
+def steps_read(monkeypatch):
+    """`_Dropout` on CPU tensors: a launch multiplies by the step at the address of its fields, and notes it."""
+    from advanced_optimizers_b200 import dropout
+    seen = []
+
+    def launch(x, residual, fields):
+        step = ctypes.c_int64.from_address(fields[1]).value if fields[1] else fields[3]
+        seen.append(step)
+        return x * step if residual is None else residual + x * step
+
+    monkeypatch.setattr(dropout, "_launch", launch)
+    return seen
+
+
+def apply(x, step):
+    from advanced_optimizers_b200.dropout import _Dropout, drop_fields
+    return _Dropout.apply(x, None, step, drop_fields(0.5, 1, 0, step, x.device))
+
+
+copying = lambda: saved_tensors_hooks(lambda t: t.clone(), lambda t: t)  # noqa: E731
+
+
+def test_step_of_a_copied_saved_tensor_is_the_forward_pass_s(steps_read):
+    """A hook that keeps a copy keeps the step's value too, whatever the caller does to the tensor in between."""
+    x, step = torch.ones(4, requires_grad=True), torch.tensor([7])
+    with copying():
+        y = apply(x, step)
+    step.add_(1)
+    g, = torch.autograd.grad(y.sum(), x)
+    assert steps_read == [7, 7] and torch.equal(g, torch.full((4,), 7.0))
+
+
+def test_step_of_a_copied_saved_tensor_outlives_the_caller_s(steps_read):
+    x, step = torch.ones(4, requires_grad=True), torch.tensor([7])
+    kept = step                       # the test's own reference, so that the overwritten memory stays the test's
+    with copying():
+        y = apply(x, step)
+    del step
+    gc.collect()
+    kept.data.fill_(99)               # what the address holds once it is someone else's
+    torch.autograd.grad(y.sum(), x)
+    assert steps_read == [7, 7]
+
+
+def test_step_of_the_second_derivative_is_the_saved_one(steps_read):
+    x, dy, step = torch.ones(4, requires_grad=True), torch.ones(4, requires_grad=True), torch.tensor([7])
+    with copying():
+        y = apply(x, step)
+        step.add_(1)
+        g, = torch.autograd.grad(y, x, dy, create_graph=True)
+    torch.autograd.grad(g.sum(), dy)
+    assert steps_read == [7, 7, 7]
+
+
+def test_step_written_between_the_passes_is_refused(steps_read):
+    x, step = torch.ones(4, requires_grad=True), torch.tensor([7])
+    y = apply(x, step)
+    step.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    step = torch.tensor([7])
+    y = checkpoint(apply, x, step, use_reentrant=False)
+    step.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    assert 8 not in steps_read
+
+
+def test_step_under_checkpointing(steps_read):
+    x, step = torch.ones(4, requires_grad=True), torch.tensor([7])
+    g, = torch.autograd.grad(checkpoint(apply, x, step, use_reentrant=False).sum(), x)
+    assert torch.equal(g, torch.full((4,), 7.0)) and set(steps_read) == {7}
+
+
+@pytest.mark.parametrize("unpacked", [torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int64),
+                                      torch.zeros(1, dtype=torch.int64, device="meta")])
+def test_a_hook_that_gives_another_kind_of_step_is_refused(steps_read, unpacked):
+    x, step = torch.ones(4, requires_grad=True), torch.tensor([7])
+    with saved_tensors_hooks(lambda t: t, lambda t: unpacked):
+        y = apply(x, step)
+    with pytest.raises(RuntimeError, match="for the step"):
+        torch.autograd.grad(y.sum(), x)
+    assert steps_read == [7]

@@ -1,0 +1,64 @@
+"""Autograd rules of the dropout and fp8 operators on the device: saved-tensor
+hooks, checkpointing and forward-mode derivatives.  Results are compared for
+equality with those of the same call without them."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+pytestmark = pytest.mark.gpu
+
+B, F = torch.bfloat16, torch.float32
+
+
+def inputs(T=70, N=200, K=256, dtype=B):
+    g = torch.Generator(device="cuda").manual_seed(T + N + K)
+    x = torch.randn(T, K, generator=g, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn(N, K, generator=g, device="cuda") * 0.05).to(dtype).requires_grad_()
+    b = torch.randn(N, generator=g, device="cuda").to(dtype).requires_grad_()
+    dy = torch.randn(T, N, generator=g, device="cuda").to(dtype)
+    return x, w, b, dy
+
+
+def linear(x, w, b, step):
+    import advanced_optimizers_b200 as A
+    return A.fp8_linear(x, w, b, dropout_p=0.4, seed=9, site=4, step=step)
+
+
+def dropout(x, step):
+    import advanced_optimizers_b200 as A
+    return A.philox_dropout(x, 0.4, seed=9, site=4, step=step)
+
+
+@pytest.mark.parametrize("how", ["advanced", "freed"])
+def test_device_step_on_saved_tensors_kept_elsewhere(how):
+    """The backward pass draws the forward pass's mask from the kept copy of the step, though the caller's was advanced or freed."""
+    x, w, b, dy = inputs()
+    want_l = torch.autograd.grad(linear(x, w, b, 7), (x, w, b), dy)
+    want_d, = torch.autograd.grad(dropout(w, 7), w, w.detach())
+    with torch.autograd.graph.save_on_cpu():
+        step = torch.full((1,), 7, dtype=torch.int64, device="cuda")
+        y, d = linear(x, w, b, step), dropout(w, step)
+    step.fill_(8)                     # freed memory is anyone's
+    if how == "freed":
+        del step
+        others = [torch.full((1,), 8, dtype=torch.int64, device="cuda") for _ in range(64)]
+        assert len(others) == 64
+    for got, want in zip(torch.autograd.grad(y, (x, w, b), dy), want_l):
+        assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(d, w, w.detach())[0], want_d)
+
+
+def test_device_step_under_checkpointing():
+    x, w, b, dy = inputs()
+    want_l = torch.autograd.grad(linear(x, w, b, 7), (x, w, b), dy)
+    want_d, = torch.autograd.grad(dropout(w, 7), w, w.detach())
+    step = torch.full((1,), 7, dtype=torch.int64, device="cuda")
+    for got, want in zip(torch.autograd.grad(checkpoint(linear, x, w, b, step, use_reentrant=False), (x, w, b), dy), want_l):
+        assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(checkpoint(dropout, w, step, use_reentrant=False), w, w.detach())[0], want_d)
+    y, d = checkpoint(linear, x, w, b, step, use_reentrant=False), checkpoint(dropout, w, step, use_reentrant=False)
+    step.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, (x, w, b), dy)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(d, w, w.detach())
