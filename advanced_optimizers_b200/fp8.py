@@ -291,6 +291,11 @@ def _linear_backward(ctx, dy):
         drop = with_saved_step(ctx.drop, saved[-1], dy.device) if ctx.stepped else ctx.drop
         # by offset from where the buffer is now: a hook on saved tensors may have moved it
         xc, wc, size = _kept_at(saved[0].data_ptr() if ctx.keeps else 0, T, N, K, need_x, need_w, blocks is None)
+        if ctx.keeps:
+            kept = saved[0]
+            if kept.dtype is not torch.uint8 or kept.device != dy.device or kept.numel() != size or not kept.is_contiguous():
+                raise RuntimeError(f"a hook on saved tensors gave {kept.dtype} {tuple(kept.shape)} on {kept.device} for the kept "
+                                   f"blocks, {size} bytes on {dy.device} were saved")
         with on_device(dy.device):
             # g = mask * dy / q once, for every gradient that reads it
             by_row = need_x or not need_w

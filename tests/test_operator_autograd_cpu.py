@@ -2,6 +2,7 @@
 launches are replaced by readers of the addresses that they are given."""
 import ctypes
 import gc
+import types
 
 import pytest
 import torch
@@ -93,3 +94,17 @@ def test_a_hook_that_gives_another_kind_of_step_is_refused(steps_read, unpacked)
     with pytest.raises(RuntimeError, match="for the step"):
         torch.autograd.grad(y.sum(), x)
     assert steps_read == [7]
+
+
+@pytest.mark.parametrize("kept", [dict(size=-1), dict(size=1), dict(dtype=torch.int8), dict(device="meta"), dict(stride=2)])
+def test_a_hook_that_gives_other_kept_blocks_is_refused(kept):
+    """Before any launch: the kernels would read what is not there."""
+    from advanced_optimizers_b200 import fp8
+    T, N, K = 5, 40, 256
+    size = fp8._kept_at(0, T, N, K, True, True, True)[2] + kept.get("size", 0)
+    t = torch.zeros(size * kept.get("stride", 1), dtype=kept.get("dtype", torch.uint8),
+                    device=kept.get("device", "cpu"))[::kept.get("stride", 1)]
+    ctx = types.SimpleNamespace(saved_tensors=(t,), needs_input_grad=(True, True, False, False), K=K, blocks=None, keeps=True,
+                                stepped=False, drop=fp8.NO_DROP, w_dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="for the kept blocks"):
+        fp8._linear_backward(ctx, torch.zeros(T, N))
