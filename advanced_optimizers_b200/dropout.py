@@ -37,6 +37,8 @@ def drop_fields(p, seed, site, step, device):
         raise ValueError("step must fit 32 unsigned bits")
     threshold = round(p * 65536)
     scale = 65536 / (65536 - threshold) if threshold < 65536 else 0.0
+    if threshold in (0, 65536):
+        step_ptr = 0   # all or nothing is kept at every step: none is read, and it may be written at any time
     return seed, step_ptr, site, step, threshold, scale
 
 
@@ -111,5 +113,5 @@ def philox_dropout(x: torch.Tensor, p: float, *, seed: int = 42, site: int = 0, 
     if residual is not None:
         residual = residual.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, step if isinstance(step, torch.Tensor) else None, fields)
+        return _Dropout.apply(x, residual, step if fields[1] else None, fields)
     return _launch(x, residual, fields)

@@ -388,7 +388,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
         residual = (residual if flat else residual.reshape(-1, N)).contiguous()
     x2 = x if flat else x.reshape(-1, K)
     if torch.is_grad_enabled():
-        y = _Fp8Linear.apply(x2, weight, bias, residual, weight_blocks, step if isinstance(step, torch.Tensor) else None, drop)
+        y = _Fp8Linear.apply(x2, weight, bias, residual, weight_blocks, step if drop[1] else None, drop)
     else:   # no transposed codes, whatever the parameters' requires_grad
         y = _linear(x2, weight, bias, residual, weight_blocks, drop, False, False)[0]
     return y if flat else y.view(*x.shape[:-1], N)

@@ -108,3 +108,12 @@ def test_a_hook_that_gives_other_kept_blocks_is_refused(kept):
                                 stepped=False, drop=fp8.NO_DROP, w_dtype=torch.float32)
     with pytest.raises(RuntimeError, match="for the kept blocks"):
         fp8._linear_backward(ctx, torch.zeros(T, N))
+
+
+@pytest.mark.parametrize("p,reads", [(0.0, False), (1e-6, False), (0.5, True), (1.0, False)])
+def test_a_mask_that_is_the_same_at_every_step_reads_none(p, reads):
+    from advanced_optimizers_b200.dropout import drop_fields
+    step = torch.tensor([7])
+    assert drop_fields(p, 1, 0, step, step.device)[1] == (step.data_ptr() if reads else 0)
+    with pytest.raises(ValueError, match="step tensor"):
+        drop_fields(p, 1, 0, torch.zeros(2, dtype=torch.int64), step.device)

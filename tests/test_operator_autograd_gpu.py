@@ -62,3 +62,17 @@ def test_device_step_under_checkpointing():
         torch.autograd.grad(y, (x, w, b), dy)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(d, w, w.detach())
+
+
+@pytest.mark.parametrize("p", [0.0, 1e-6, 1.0])
+def test_a_step_that_no_mask_depends_on_may_be_advanced(p):
+    import advanced_optimizers_b200 as A
+    x, w, b, dy = inputs()
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    lin = lambda s: A.fp8_linear(x, w, b, dropout_p=p, step=s)  # noqa: E731
+    drop = lambda s: A.philox_dropout(w, p, step=s)  # noqa: E731
+    y, d = lin(step), drop(step)
+    step.add_(1)
+    for got, want in zip(torch.autograd.grad(y, (x, w, b), dy), torch.autograd.grad(lin(0), (x, w, b), dy)):
+        assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(d, w, w.detach())[0], torch.autograd.grad(drop(0), w, w.detach())[0])
