@@ -7,6 +7,7 @@ import contextlib
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 
 def require_cuda_tensor(t: torch.Tensor, what: str):
@@ -24,6 +25,13 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return 1
     raise NotImplementedError(f"parameter dtype {dt} is not supported (float32 and bfloat16 are)")
+
+
+def refuse_tangents(what: str, *tensors):
+    """Raises for dual tensors: kernels that are launched outside an autograd
+    function would lose their tangents without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
 
 
 def stream_handle(device) -> int:

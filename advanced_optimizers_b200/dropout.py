@@ -12,7 +12,7 @@ import struct
 import torch
 
 from . import _lib as L
-from ._device import dtype_code, on_device, raw_stream
+from ._device import dtype_code, on_device, raw_stream, refuse_tangents
 
 # advopt_dropout_spec: seed, step_dev, site, step, threshold, scale
 SPEC = struct.Struct("<QQIIIf")
@@ -102,13 +102,15 @@ def philox_dropout(x: torch.Tensor, p: float, *, seed: int = 42, site: int = 0, 
     `checkpoint`, which raises if it was written, not through a closure.
 
     x and residual (of x's shape and dtype): float32 or bfloat16 on one CUDA
-    device; other strides than contiguous ones are copied first."""
+    device; other strides than contiguous ones are copied first.  Forward-mode
+    derivatives are refused."""
     if not x.is_cuda:
         raise NotImplementedError("philox_dropout: tensors must live on a CUDA device (no CPU fallback)")
     dtype_code(x.dtype)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("philox_dropout: the residual must have x's shape, dtype and device")
     fields = drop_fields(p, seed, site, step, x.device)
+    refuse_tangents("philox_dropout", x, residual)
     x = x.contiguous()
     if residual is not None:
         residual = residual.contiguous()

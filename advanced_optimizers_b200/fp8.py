@@ -15,7 +15,7 @@ import struct
 import torch
 
 from . import _lib as L
-from ._device import dtype_code, on_device, raw_stream
+from ._device import dtype_code, on_device, raw_stream, refuse_tangents
 from .dropout import NO_DROP, drop_fields, with_saved_step
 
 _CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
@@ -191,7 +191,8 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), dtype: torch.dtype = torch.flo
     For each block the scale is the least power of two that brings the largest
     finite magnitude into the type's range (1 for a block of zeros, never below
     2^-127), and a code is the nearest value of the type, ties to even.
-    Infinities and NaN become NaN codes and do not enter a scale.
+    Infinities and NaN become NaN codes and do not enter a scale.  Codes carry
+    no derivative, in either mode; `fp8_linear` is the differentiable layer.
 
     layout  "rows": Fp8Blocks of x, quantised along its columns' index
             "cols": Fp8Blocks of x^T [C][R], quantised along the rows' index
@@ -358,7 +359,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     x, bias and residual share a dtype (float32 or bfloat16), the weight may
     have the other one; dweight has the weight's.  `weight_blocks` takes
     quantize_fp8(weight, (128, 128), layout="both") made before, for weights
-    that do not change between calls (accumulation, evaluation)."""
+    that do not change between calls (accumulation, evaluation).  Second and
+    forward-mode derivatives are refused."""
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"fp8_linear: x [..., K] and weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
     dev = x.device
@@ -381,6 +383,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     if x.numel() == 0:   # no tokens: no products, and gradients of zeros
         y = x.new_zeros((*x.shape[:-1], N)) if residual is None else residual.clone()
         return y + 0.0 * (x.sum() + weight.sum(dtype=x.dtype) + (0.0 if bias is None else bias.sum()))
+    refuse_tangents("fp8_linear", x, weight, bias, residual)
     flat = x.dim() == 2
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()

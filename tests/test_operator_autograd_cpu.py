@@ -117,3 +117,24 @@ def test_a_mask_that_is_the_same_at_every_step_reads_none(p, reads):
     assert drop_fields(p, 1, 0, step, step.device)[1] == (step.data_ptr() if reads else 0)
     with pytest.raises(ValueError, match="step tensor"):
         drop_fields(p, 1, 0, torch.zeros(2, dtype=torch.int64), step.device)
+
+
+def test_tangents_are_found():
+    """At the level they belong to, with gradients off, and through the functional transform."""
+    from torch.autograd import forward_ad
+    from advanced_optimizers_b200._device import refuse_tangents
+    x = torch.ones(3)
+    refuse_tangents("op", x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        refuse_tangents("op", x, None)
+        for guard in (torch.enable_grad, torch.no_grad):
+            with guard(), pytest.raises(NotImplementedError, match="op: forward-mode"):
+                refuse_tangents("op", None, x, dual)
+
+    def seen(t):
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            refuse_tangents("op", t)
+        return t
+
+    torch.func.jvp(seen, (x,), (x,))

@@ -76,3 +76,23 @@ def test_a_step_that_no_mask_depends_on_may_be_advanced(p):
     for got, want in zip(torch.autograd.grad(y, (x, w, b), dy), torch.autograd.grad(lin(0), (x, w, b), dy)):
         assert torch.equal(got, want)
     assert torch.equal(torch.autograd.grad(d, w, w.detach())[0], torch.autograd.grad(drop(0), w, w.detach())[0])
+
+
+def test_forward_mode_is_refused():
+    """It was lost without a word where the call does not go through an autograd function."""
+    import advanced_optimizers_b200 as A
+    from torch.autograd import forward_ad
+    x, w, b, _ = (t.detach() for t in inputs())
+    r = torch.zeros(70, 200, device="cuda", dtype=B)
+    for guard in (torch.enable_grad, torch.no_grad):
+        with guard(), forward_ad.dual_level():
+            dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+            for call in (lambda: A.philox_dropout(dual(x), 0.3), lambda: A.philox_dropout(x, 0.3, residual=dual(x)),
+                         lambda: A.fp8_linear(dual(x), w, b, residual=r), lambda: A.fp8_linear(x, dual(w), b, residual=r),
+                         lambda: A.fp8_linear(x, w, dual(b), residual=r), lambda: A.fp8_linear(x, w, b, residual=dual(r))):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+            assert tuple(A.philox_dropout(x, 0.3).shape) == tuple(x.shape)
+            assert tuple(A.fp8_linear(x, w, b, residual=r).shape) == (70, 200)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: A.philox_dropout(t, 0.3), (x,), (x,))
