@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import functools
 import struct
+import threading
 
 import torch
 
@@ -29,18 +30,23 @@ _GEMM = struct.Struct("<QqQqQqQqQqQQqqqqiiiiiiQQQIIIf")
 class _ErrorWord:
     """The word that a kernel's bounded wait sets when it gives up: pinned host
     memory that the kernels write directly, so that every call can look at it
-    without waiting for the GPU."""
+    without waiting for the GPU.  One for the process: whichever thread's call
+    comes next reports it, for whichever device."""
 
     def __init__(self):
-        self.word = None
+        self.word = self.view = None
+        self.lock = threading.Lock()
 
     def pointer(self) -> int:
         if self.word is None:
             if torch.cuda.is_current_stream_capturing():
                 return 0   # no allocation of pinned memory during a capture
-            self.word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            self.view = self.word.numpy()
-        elif self.view[0]:
+            with self.lock:
+                if self.word is None:
+                    word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                    self.view = word.numpy()   # before the word, which other threads find without the lock
+                    self.word = word
+        if self.view[0]:
             self.raise_()
         return self.word.data_ptr()
 
@@ -53,8 +59,10 @@ _ERR = _ErrorWord()
 
 
 def check_fp8_errors():
-    """Waits for the GPU and raises if an fp8 product's bounded wait gave up
-    (a guard that is not expected to fire; otherwise the next call raises)."""
+    """Waits for the GPU and raises if an fp8 product's bounded wait gave up (a
+    guard that is not expected to fire; otherwise the process's next product
+    raises, on whichever thread or device).  Products captured before the
+    process's first eager one have no word to report to."""
     torch.cuda.synchronize()
     if _ERR.word is not None and _ERR.view[0]:
         _ERR.raise_()
