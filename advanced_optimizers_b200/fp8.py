@@ -386,7 +386,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     drop = NO_DROP if dropout_p == 0 else drop_fields(dropout_p, seed, site, step, dev)
     if weight_blocks is not None:
         r, c = weight_blocks
-        if not (r.square and c.square and (r.rows, r.k) == (N, K) == (c.k, c.rows) and r.device == dev == c.device):
+        # of a single row, 1 x 128 and 128 x 128 blocks are the same
+        if not ((r.square or r.rows == 1) and (c.square or c.rows == 1) and (r.rows, r.k) == (N, K) == (c.k, c.rows) and
+                r.device == dev == c.device):
             raise ValueError("fp8_linear: weight_blocks is quantize_fp8(weight, (128, 128), layout='both')")
     if x.numel() == 0:   # no tokens: no products, and gradients of zeros
         y = x.new_zeros((*x.shape[:-1], N)) if residual is None else residual.clone()

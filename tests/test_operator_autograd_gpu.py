@@ -96,3 +96,22 @@ def test_forward_mode_is_refused():
             assert tuple(A.fp8_linear(x, w, b, residual=r).shape) == (70, 200)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: A.philox_dropout(t, 0.3), (x,), (x,))
+
+
+@pytest.mark.parametrize("N,K", [(1, 300), (200, 1), (1, 1), (200, 300)])
+def test_weight_blocks_made_from_their_tensors(N, K):
+    """Also of a single row or column, whose scales do not tell the two block shapes apart."""
+    import advanced_optimizers_b200 as A
+    x, w, b, dy = inputs(70, N, K)
+    blocks = A.quantize_fp8(w, (128, 128), layout="both")
+    again = [A.Fp8Blocks(q.codes, q.scales) for q in blocks]
+    y, want = A.fp8_linear(x, w, b, weight_blocks=blocks), A.fp8_linear(x, w, b)
+    z = A.fp8_linear(x, w, b, weight_blocks=again)
+    assert torch.equal(y, want) and torch.equal(z, want)
+    grads = [torch.autograd.grad(t, (x, w, b), dy) for t in (want, y, z)]
+    for got in grads[1:]:
+        assert all(torch.equal(g, h) for g, h in zip(got, grads[0]))
+    rows = A.quantize_fp8(w, (1, 128), layout="both")
+    if N > 1 and K > 1:
+        with pytest.raises(ValueError, match="weight_blocks"):
+            A.fp8_linear(x, w, b, weight_blocks=rows)
