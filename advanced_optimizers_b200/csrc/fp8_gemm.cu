@@ -33,6 +33,7 @@
 #include "capi_internal.h"
 #include "common.cuh"
 #include "drop.cuh"
+#include "fp8_ring.cuh"
 
 namespace advopt {
 namespace fp8 {
@@ -872,6 +873,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   __shared__ uint64_t full[C::STAGES / 2], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full[2], acc_empty[2];
   __shared__ uint64_t drain;
   __shared__ uint32_t tmem_base;
+  __shared__ __align__(8) uint32_t loads[2][2];   // loads: the even CTA's, what each CTA's Fills ended with
   __shared__ int abort_flag;
   volatile int* abort_v = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -919,7 +921,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
   if (warp == 0) {
     const bool one = elect_one();
     Ring<C::STAGES / 2> st;
-    uint32_t filled[2] = {}, phases[2] = {};   // per slot: whether it has been filled, the parity of its next release
+    Fills fills[2];   // of the slots' first and second blocks
     bool ok = true;
     for (int t = first; t < n_tiles && ok; t += stride) {
       int64_t p0, q0;
@@ -931,7 +933,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
         for (int h = 0; h < 2; ++h) {
           // an odd last block leaves the second slot of its two empty
           const bool used = kb + h < g.kblocks;
-          if (used && ok && (filled[h] >> st.slot & 1u)) ok = wait_warp(&empty[2 * st.slot + h], phases[h] >> st.slot & 1u, abort_v);
+          if (used && ok && fills[h].any(st.slot)) ok = wait_warp(&empty[2 * st.slot + h], fills[h].latest(st.slot), abort_v);
           if (used && ok) {
             if (one) {
               unsigned char* sp = smem + (2 * st.slot + h) * C::STAGE_BYTES;
@@ -941,8 +943,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
               tma_load_pair(sp + C::A_BYTES, &map_q, (kb + h) * BK, (int)q0, bar);
             }
             __syncwarp();
-            if (filled[h] >> st.slot & 1u) phases[h] ^= 1u << st.slot;
-            filled[h] |= 1u << st.slot;
+            fills[h].next(st.slot);
           }
         }
         if (!ok) give_up();
@@ -952,7 +953,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     // the even CTA's commits arrive here too: its last ones have come before
     // this CTA's shared memory goes to another
     for (int s = 0; s < C::STAGES && ok; ++s)
-      if (filled[s & 1] >> (s >> 1) & 1u) ok = wait_warp(&empty[s], phases[s & 1] >> (s >> 1) & 1u, abort_v);
+      if (fills[s & 1].any(s >> 1)) ok = wait_warp(&empty[s], fills[s & 1].latest(s >> 1), abort_v);
+    // both CTAs' loads report to the even one's barriers, where they are awaited should a wait have given up
+    if (one)
+      asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(map_to(smem_u32(loads[rank]), 0)), "r"(fills[0].begun),
+                   "r"(fills[0].parity)
+                   : "memory");
   } else if (warp == 1) {
     if (rank == 0) {
       const bool one = elect_one();
@@ -1105,10 +1111,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     }
     if (threadIdx.x == 0) {
       if (rank == 0) {
-        for (int s = 0; s < C::STAGES; ++s) {
-          // whichever phase is current: it completes when its loads have landed
-          if (!mbar_wait(&full[s / 2], 0, 1u << 12)) mbar_wait(&full[s / 2], 1, 1u << 12);
-        }
+        // One CTA may have got a fill further than the other.  Its phase, or that of the fill which the other
+        // has no part in, does not end then: the wait's limit is what gives the loads the time to land.
+        for (int r = 0; r < 2; ++r)
+          await_fills(Fills{loads[r][0], loads[r][1]}, C::STAGES / 2,
+                      [&](int slot, uint32_t parity) { mbar_wait(&full[slot], parity, 1u << 20); });
       }
       if (g.err) *reinterpret_cast<volatile int32_t*>(g.err) = 1;
     }
