@@ -585,7 +585,10 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     // the commits' last arrivals have come before this CTA's shared memory goes
     // to another: each slot's latest use
     for (int i = nkb > C::STAGES ? nkb - C::STAGES : 0; i < nkb && issued == nkb; ++i)
-      if (!wait_warp(&empty[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, abort_v)) break;
+      if (!wait_warp(&empty[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, abort_v)) {
+        abort_flag = 1;
+        break;
+      }
   } else if (warp == 1) {
     const bool one = elect_one();
     const uint32_t tiles_lo = desc_lo(smem_u32(smem)), sf_lo = desc_lo(smem_u32(smem + C::SF_OFF));
@@ -954,6 +957,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     // this CTA's shared memory goes to another
     for (int s = 0; s < C::STAGES && ok; ++s)
       if (fills[s & 1].any(s >> 1)) ok = wait_warp(&empty[s], fills[s & 1].latest(s >> 1), abort_v);
+    if (!ok) give_up();
     // both CTAs' loads report to the even one's barriers, where they are awaited should a wait have given up
     if (one)
       asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(map_to(smem_u32(loads[rank]), 0)), "r"(fills[0].begun),
@@ -1047,6 +1051,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<BN>::THREADS
     }
     for (int j = n_groups > SF_SLOTS ? n_groups - SF_SLOTS : 0; j < n_groups && ok; ++j)
       ok = wait_warp(&sf_empty[j % SF_SLOTS], (uint32_t)(j / SF_SLOTS) & 1u, abort_v);
+    if (!ok && lane == 0) give_up();
   } else if (warp >= 4) {
     const uint32_t step = g.drop ? drop_step(d) : 0u;
     const int quarter = warp & 3, share = (warp - 4) >> 2;
