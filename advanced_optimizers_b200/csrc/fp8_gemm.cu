@@ -649,6 +649,11 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
       mbar_arrive(&sf_full[slot]);
       now = then;
     }
+    // these commits' last arrivals too
+    const int n_groups = (nkb + 3) / 4;
+    for (int j = n_groups > SF_SLOTS ? n_groups - SF_SLOTS : 0; j < n_groups && ok; ++j)
+      ok = wait_warp(&sf_empty[j % SF_SLOTS], (uint32_t)(j / SF_SLOTS) & 1u, abort_v);
+    if (!ok) abort_flag = 1;
   } else {
     // warps 4..7 have no part in the main loop: meanwhile they bring the
     // residual near and draw the masks of the blocks this CTA will write
