@@ -625,7 +625,9 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
           st.next();
         }
       }
-      mma_commit(&sf_empty[sf.slot], one);
+      // the last groups' buffers are not written again: an arrival that no one waits for could come after this
+      // CTA's shared memory went to another (waiting for them cost 1 x 4096 x 4096 0.25 us of 6.9)
+      mma_commit(&sf_empty[sf.slot], one && i + 4 * C::SF_BUFS < nkb);
       sf.next();
     }
     if (!ok) abort_flag = 1;
@@ -649,11 +651,6 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
       mbar_arrive(&sf_full[slot]);
       now = then;
     }
-    // these commits' last arrivals too
-    const int n_groups = (nkb + 3) / 4;
-    for (int j = n_groups > SF_SLOTS ? n_groups - SF_SLOTS : 0; j < n_groups && ok; ++j)
-      ok = wait_warp(&sf_empty[j % SF_SLOTS], (uint32_t)(j / SF_SLOTS) & 1u, abort_v);
-    if (!ok) abort_flag = 1;
   } else {
     // warps 4..7 have no part in the main loop: meanwhile they bring the
     // residual near and draw the masks of the blocks this CTA will write
