@@ -43,6 +43,18 @@ constexpr int THREADS = 256;
 constexpr int SMS = 148, PAIRS = SMS / 2;
 constexpr int SF_SLOTS = 4;                   // scale words of 4 x 4 blocks in flight
 constexpr int SF_SLOT_BYTES = 512 * 3;        // rows, columns 0..127, columns 128..255
+// float32 results of long K are summed in chunks of at most CHUNK blocks, each a
+// product of its own, which are added in float32 and in order: the tensor cores
+// truncate as they accumulate, an error that grows with K.  A chunk of 64 blocks
+// is low by 5e-7 of the result in the Frobenius norm (normal values; 7e-7 with
+// columns ten times as large; a product that rounds: 1.5e-7), and so is a sum of
+// chunks; uncut, 128 blocks are off by 1.2e-6 and 980 by 1.8e-5.  bf16 results
+// round at 2^-9 and do without.
+// The pairs' epilogue adds its chunks to D.  Single CTAs split K over a cluster
+// and keep a CTA's chunks in accumulators of their own, long_accs of them; a
+// longer sum takes a launch for each as many, which adds to D.
+constexpr int CHUNK = 64;
+constexpr int long_accs(int bn) { return bn <= 64 ? 7 : bn <= 128 ? 3 : 1; }
 
 // One operand as the kernel sees it.
 struct Side {
@@ -64,10 +76,13 @@ struct GemmArgs {
   int vec;            // rows of D and the residual are 16-byte aligned
   int vec_bias;
   int drop;
+  int more;           // LONG: D holds the sum of the blocks before these
   int32_t* err;
 };
 
-template <int BN>
+// LONG: float32 sums of more than CHUNK blocks a CTA, in as many accumulators as
+// tensor memory has room for.
+template <int BN, bool LONG>
 struct Cfg {
   static constexpr int STAGES = BN >= 256 || BN <= 32 ? 4 : 6;
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
@@ -76,8 +91,11 @@ struct Cfg {
   static constexpr int SMEM = SF_OFF + SF_SLOTS * SF_SLOT_BYTES + 1024;
   static constexpr int SF_BUFS = 2;   // scale buffers in tensor memory
   static constexpr int SF_COLS = 4 + (BN > 128 ? 8 : 4);
-  static constexpr int USED = BN + SF_BUFS * SF_COLS;
+  static constexpr int ACCS = LONG ? long_accs(BN) : 1;
+  static constexpr int SF_COL = ACCS * BN;
+  static constexpr int USED = SF_COL + SF_BUFS * SF_COLS;
   static constexpr uint32_t TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+  static_assert(USED <= (BN <= 32 ? 256 : 512), "two CTAs share an SM's tensor memory at BN = 32");
 };
 
 // Instruction descriptor of kind::mxf8f6f4 with E8M0 scales, K-major operands.
@@ -165,6 +183,15 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                :
                : "memory");
   asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// r += 32 columns of another accumulator, in float32.
+__device__ __forceinline__ void add_columns(uint32_t taddr, uint32_t (&r)[32]) {
+  uint32_t t[32];
+  tmem_ld32(taddr, t);
+  tmem_wait32(t);
+#pragma unroll
+  for (int e = 0; e < 32; ++e) r[e] = f2u(__fadd_rn(u2f(r[e]), u2f(t[e])));
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -271,7 +298,7 @@ struct ScaleWords {
 };
 
 // Swapped operands: W tokens (columns) of feature p, one of D's columns per lane.
-template <bool BF16, int W>
+template <bool BF16, bool LONG, int W>
 __device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint32_t step, int64_t p, int64_t q0,
                                      float (&v)[W]) {
   if (p >= g.p.extent || q0 >= g.q.extent) return;
@@ -283,6 +310,7 @@ __device__ __forceinline__ void emit(const GemmArgs& g, const DropSpec& d, uint3
   for (int j = 0; j < W; ++j) {
     if (j >= w) break;
     float x = v[j];
+    if (LONG && g.more) x = __fadd_rn(static_cast<const float*>(g.d)[(q0 + j) * g.ldd + p], x);
     if (g.bias) x = __fadd_rn(x, b);
     if (g.drop) x = drop1(x, d, step, (uint64_t)((q0 + j) * g.n + p));
     if (g.residual)
@@ -512,11 +540,13 @@ __device__ __forceinline__ void prefetch_rows(const void* base, int64_t ld, int 
 }
 
 // One 128 x BN tile, split over the S CTAs of a cluster along K.
-template <int BN, int S, bool BF16>
+// LONG is a kernel of its own: its branches and its tensor memory cost the
+// others 0.1 to 0.2 us.
+template <int BN, int S, bool BF16, bool LONG>
 __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                 const __grid_constant__ GemmArgs g, const __grid_constant__ DropSpec d) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, LONG>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[C::STAGES / 2], empty[C::STAGES], sf_full[SF_SLOTS], sf_empty[SF_SLOTS], acc_full;
@@ -534,6 +564,9 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
   const int kb0 = 4 * (int)((int64_t)groups * rank / S);
   const int kb1 = min(g.kblocks, 4 * (int)((int64_t)groups * (rank + 1) / S));
   const int nkb = kb1 > kb0 ? kb1 - kb0 : 0;
+  // LONG: accumulators, and blocks in each (whole groups of four)
+  const int accs = LONG ? (nkb + CHUNK - 1) / CHUNK : 1;
+  const int chunk = LONG && nkb ? ((nkb + accs - 1) / accs + 3) / 4 * 4 : 4;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -595,9 +628,15 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
     const uint32_t idesc = instr_desc(BM, BN, g.p.code, g.q.code);
     Ring<C::STAGES / 2> st;
     Ring<SF_SLOTS> sf;
+    uint32_t acc = tmem;
+    int next = 0;   // LONG: the block that the next accumulator starts with
     bool ok = true;
     for (int i = 0, grp = 0; i < nkb && ok; i += 4, ++grp) {
-      const uint32_t sfp = tmem + BN + (uint32_t)(grp % C::SF_BUFS) * C::SF_COLS, sfq = sfp + 4;
+      const uint32_t sfp = tmem + C::SF_COL + (uint32_t)(grp % C::SF_BUFS) * C::SF_COLS, sfq = sfp + 4;
+      if (LONG && i == next) {
+        next += chunk;
+        acc += i ? BN : 0;
+      }
       ok = wait_warp(&sf_full[sf.slot], sf.phase, abort_v);
       // this buffer's last readers, the MMAs of SF_BUFS groups ago, are done
       if (ok && grp >= C::SF_BUFS) ok = wait_warp(&sf_empty[(grp - C::SF_BUFS) % SF_SLOTS],
@@ -618,7 +657,8 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
           for (int h = 0; h < 2; ++h) {
             if (i + j + h < nkb) {
               const uint32_t lo = tiles_lo + (2 * st.slot + h) * (C::STAGE_BYTES / 16);
-              mma_block<false>(tmem, lo, lo + C::A_BYTES / 16, idesc | sf_id(j + h), sfp, sfq, i + j + h > 0,
+              mma_block<false>(acc, lo, lo + C::A_BYTES / 16, idesc | sf_id(j + h), sfp, sfq,
+                               LONG ? i + j + h + chunk > next : i + j + h > 0,
                                &empty[2 * st.slot + h], TILE_HI, one);
             }
           }
@@ -688,19 +728,22 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_wait32(r);
+        if (LONG)
+#pragma unroll 1
+          for (int i = chunk; i < nkb; i += chunk) add_columns(taddr + i / chunk * BN + c, r);
         if (!g.swap) {
           // over the ring, which is drained once the accumulator is complete
           unsigned char* turn = smem + warp * 4096;
           turn_in(turn, r);
-          if (extra) emit_block<BF16, true>(g, d, step, turn, p0 + quarter * 32, q0 + c, false, true, masks[quarter][c / 32]);
-          else emit_block<BF16, false>(g, d, step, turn, p0 + quarter * 32, q0 + c, false, true);
+          if (extra) emit_block<BF16, true>(g, d, step, turn, p0 + quarter * 32, q0 + c, LONG && g.more, true, masks[quarter][c / 32]);
+          else emit_block<BF16, false>(g, d, step, turn, p0 + quarter * 32, q0 + c, LONG && g.more, true);
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float v[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[16 * h + e]);
-            emit<BF16, 16>(g, d, step, p0 + row, q0 + c + 16 * h, v);
+            emit<BF16, LONG, 16>(g, d, step, p0 + row, q0 + c + 16 * h, v);
           }
         }
       }
@@ -717,6 +760,9 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
         uint32_t r[32];
         tmem_ld32(taddr + c, r);
         tmem_wait32(r);
+        if (LONG)
+#pragma unroll 1
+          for (int i = chunk; i < nkb; i += chunk) add_columns(taddr + i / chunk * BN + c, r);
         if (!nkb)
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
@@ -743,7 +789,7 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
 #pragma unroll
             for (int o = 1; o < S; ++o) v[e] = __fadd_rn(v[e], peer_float(at, o));
           }
-          emit<BF16, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
+          emit<BF16, LONG, W>(g, d, step, p0 + row, q0 + rank * PER + c, v);
         }
       } else {
         // the tile's 4 BN / 32 blocks, dealt out to the cluster's 8 S warps
@@ -764,8 +810,8 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
             *reinterpret_cast<float4*>(own + (i * 32 + lane) * 16) = x;
           }
           __syncwarp();
-          if (extra) emit_block<BF16, true>(g, d, step, own, p0 + (b & 3) * 32, q0 + b / 4 * 32, false, true, masks[b & 3][b / 4]);
-          else emit_block<BF16, false>(g, d, step, own, p0 + (b & 3) * 32, q0 + b / 4 * 32, false, true);
+          if (extra) emit_block<BF16, true>(g, d, step, own, p0 + (b & 3) * 32, q0 + b / 4 * 32, LONG && g.more, true, masks[b & 3][b / 4]);
+          else emit_block<BF16, false>(g, d, step, own, p0 + (b & 3) * 32, q0 + b / 4 * 32, LONG && g.more, true);
         }
       }
     }
@@ -797,13 +843,6 @@ __global__ void __launch_bounds__(THREADS, BN <= 32 ? 2 : 1)
 // memory holds its 128 rows of two accumulators.  At BN = 256 these and the
 // scales do not fit 512 columns: the accumulators then share 32 columns, which
 // the epilogue reads first, and the next tile's MMAs start once it has.
-//
-// float32 results of long K are summed in chunks of at most CHUNK blocks, each
-// a product of its own that the epilogue adds in float32: the tensor cores
-// truncate as they accumulate, an error that grows with K (7e-7 relative at
-// K = 8192, 1.5e-7 of a rounding sum); bf16 results round at 2^-9.
-constexpr int CHUNK = 64;
-
 template <int BN>
 struct PairCfg {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN / 2 * BK;
@@ -1180,14 +1219,14 @@ struct Launch {
   cudaStream_t stream;
 };
 
-template <int BN, int S, bool BF16>
+template <int BN, int S, bool BF16, bool LONG>
 int launch_t(const Launch& L) {
-  using C = Cfg<BN>;
+  using C = Cfg<BN, LONG>;
   CUtensorMap mp, mq;
   int rc = encode_map(&mp, L.p, L.g.p.extent, L.k, L.ldp, BM);
   if (rc == ADVOPT_OK) rc = encode_map(&mq, L.q, L.g.q.extent, L.k, L.ldq, BN);
   if (rc != ADVOPT_OK) return rc;
-  const auto kernel = gemm_kernel<BN, S, BF16>;
+  const auto kernel = gemm_kernel<BN, S, BF16, LONG>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(kernel, C::SMEM, ready);
   if (e != cudaSuccess) return check_cuda(e, "advopt_fp8_gemm: smem attribute");
@@ -1250,23 +1289,23 @@ int launch_pair(const Launch& L) {
   return check_cuda(e, "advopt_fp8_gemm");
 }
 
-template <int BN, bool BF16>
+template <int BN, bool BF16, bool LONG>
 int launch_s(const Launch& L, int split) {
   switch (split) {
-    case 8: return launch_t<BN, 8, BF16>(L);
-    case 4: return launch_t<BN, 4, BF16>(L);
-    case 2: return launch_t<BN, 2, BF16>(L);
-    default: return launch_t<BN, 1, BF16>(L);
+    case 8: return launch_t<BN, 8, BF16, LONG>(L);
+    case 4: return launch_t<BN, 4, BF16, LONG>(L);
+    case 2: return launch_t<BN, 2, BF16, LONG>(L);
+    default: return launch_t<BN, 1, BF16, LONG>(L);
   }
 }
 
-template <bool BF16>
+template <bool BF16, bool LONG>
 int launch_n(const Launch& L, int bn, int split) {
   switch (bn) {
-    case 32: return launch_s<32, BF16>(L, split);
-    case 64: return launch_s<64, BF16>(L, split);
-    case 128: return launch_s<128, BF16>(L, split);
-    default: return launch_s<256, BF16>(L, split);
+    case 32: return launch_s<32, BF16, LONG>(L, split);
+    case 64: return launch_s<64, BF16, LONG>(L, split);
+    case 128: return launch_s<128, BF16, LONG>(L, split);
+    default: return launch_s<256, BF16, LONG>(L, split);
   }
 }
 
@@ -1284,6 +1323,11 @@ int launch_n(const Launch& L, int bn, int split) {
 //     from L2 (170 .. 680 cycles); splitting K pays a cluster's exchange:
 //     1 x 4096 x 4096 takes 10.9 / 8.5 / 7.4 / 6.9 us split 1 / 2 / 4 / 8,
 //     256 x 4096 x 4096 at BN = 64 10.5 us unsplit, at BN = 128 11.0 split in 2;
+//   * a float32 sum that takes a CTA's accumulators several times over takes
+//     another launch each time, 6.5 us of a single wave: 256 x 256 x 262144 split
+//     in 8 takes 58 us at BN = 64 in one launch, 72 at BN = 128 in two; and more of
+//     several: 1024 x 1024 x 131072 at BN = 256 takes 211 us split in 8 (two waves,
+//     two launches), 148 split in 4 (one wave, four launches), 375 in pairs;
 //   * swapped operands write D a token at a time, a feature per lane, whatever
 //     D's alignment: 333 x 2041 x 1000 takes 5.3 us swapped, 6.1 not.
 struct Variant {
@@ -1312,12 +1356,14 @@ inline Variant choose(int64_t m, int64_t n, int64_t kblocks, bool whole_rows, bo
         double block = single_block[i];
         if (i == 0) block = ctas > SMS ? 400 : ctas * 330 / SMS > 170 ? ctas * 330 / SMS : 170;
         if (i == 0 && q > 32) block *= 1.4;   // the other operand is read again for each 32 columns
-        const int64_t blocks = 4 * ceil_div(ceil_div(kblocks, 4), split);
-        if (f32 && blocks > CHUNK && split < 8 && ceil_div(kblocks, 4) >= 2 * split) continue;   // float32 sums stay short
+        const int64_t groups = ceil_div(kblocks, 4), sums = split * (CHUNK / 4);
+        const int64_t parts = f32 ? ceil_div(groups, sums * long_accs(bn)) : 1;
+        if (f32 && groups > sums && split < 8 && kblocks <= 8 * CHUNK && groups >= 2 * split) continue;   // one sum a CTA
+        const int64_t blocks = 4 * ceil_div(groups, split);
         const double body = (double)(blocks < kblocks ? blocks : kblocks) * block / 1800;
         const double out = bn / 32 * (swap ? 0.35 : whole_rows ? 0.3 : 0.8) / split;
         const double join = split == 1 ? 0 : bn / 32 * 0.3 + (split == 2 ? (i ? 1.0 : 0.7) : split == 4 ? 1.2 : i ? 6.0 : 1.3);
-        const double t = 2.8 + (waves - 1) * (body + out + 1.2) + body + out + join;
+        const double t = 2.8 + (waves - 1) * (body + out + 1.2) + body + out + join + (parts - 1) * (waves > 1 ? 30.0 : 6.5);
         if (t < least) {
           least = t;
           best = Variant{false, swap != 0, bn, split};
@@ -1403,6 +1449,7 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
           (!a->residual || (reinterpret_cast<uintptr_t>(a->residual) % 16 == 0 && a->ldres * es % 16 == 0));
   g.vec_bias = reinterpret_cast<uintptr_t>(a->bias) % 16 == 0;
   g.drop = a->drop.threshold > 0;
+  g.more = 0;
   g.err = a->err;
   L.d = drop_spec(a->drop);
   L.stream = static_cast<cudaStream_t>(stream);
@@ -1414,5 +1461,28 @@ extern "C" int advopt_fp8_gemm(const advopt_fp8_gemm_args* a, void* stream) {
       default: return bf16 ? fp8::launch_pair<128, true>(L) : fp8::launch_pair<128, false>(L);
     }
   }
-  return bf16 ? fp8::launch_n<true>(L, v.bn, v.split) : fp8::launch_n<false>(L, v.bn, v.split);
+  // launches, of whole scale words of K
+  const int64_t groups = (nb + 3) / 4, sums = v.split * (fp8::CHUNK / 4);
+  const bool longer = !bf16 && groups > sums;
+  const int64_t parts = longer ? fp8::ceil_div(groups, sums * fp8::long_accs(v.bn)) : 1;
+  const fp8::Launch whole = L;
+  for (int64_t i = 0; i < parts; ++i) {
+    const int64_t g0 = groups * i / parts, g1 = groups * (i + 1) / parts, k0 = g0 * 512;
+    const bool last = i + 1 == parts;
+    L.p = static_cast<const uint8_t*>(whole.p) + k0;
+    L.q = static_cast<const uint8_t*>(whole.q) + k0;
+    L.k = (last ? a->k : g1 * 512) - k0;
+    g.p.scales = whole.g.p.scales + g0 * 4;
+    g.q.scales = whole.g.q.scales + g0 * 4;
+    g.kblocks = (int)((last ? nb : g1 * 4) - g0 * 4);
+    g.more = i > 0;
+    g.bias = last ? whole.g.bias : nullptr;
+    g.residual = last ? whole.g.residual : nullptr;
+    g.drop = last ? whole.g.drop : 0;
+    const int rc = bf16     ? fp8::launch_n<true, false>(L, v.bn, v.split)
+                   : longer ? fp8::launch_n<false, true>(L, v.bn, v.split)
+                            : fp8::launch_n<false, false>(L, v.bn, v.split);
+    if (rc != ADVOPT_OK) return rc;
+  }
+  return ADVOPT_OK;
 }

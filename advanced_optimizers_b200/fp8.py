@@ -244,9 +244,15 @@ def _gemm(a, b, out, bias=None, residual=None, drop=NO_DROP, variant=0):
 
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a @ b^T [a.rows][b.rows]: products of the values that the codes and
-    scales stand for, summed in float32 and rounded once to `out_dtype`
-    (bfloat16 or float32).  The operands may differ in code type and block
-    shape.  Its gradients are products of the same kind (see `fp8_linear`)."""
+    scales stand for, summed in the tensor cores' float32 accumulators and
+    rounded once to `out_dtype` (bfloat16 or float32).  These accumulators
+    truncate: a sum of up to 8192 elements is low by up to 5e-7 to 7e-7 of the
+    result (Frobenius norm, K = 8192; a float32 product that rounds is off by
+    1.5e-7).  Longer float32 results are float32 sums of such sums, so that the
+    error does not grow with the length; longer bfloat16 ones are one such sum
+    (2e-5 at 10^6 elements, where half a step of bfloat16 is 4e-3).  The operands
+    may differ in code type and block shape.  Its gradients are products of the
+    same kind (see `fp8_linear`)."""
     codes = a.codes
     if a.k != b.k:
         raise ValueError(f"fp8_matmul: the operands are quantised along {a.k} and {b.k} elements")

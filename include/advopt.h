@@ -638,7 +638,9 @@ int advopt_fp8_quantize(const advopt_fp8_quant_args* args, void* stream);
 int advopt_col_sum(void* out, const float* partial, int64_t parts, int64_t cols, int32_t dtype, void* stream);
 
 /* D [m][n] = residual + dropout(sum_b 2^(sa[i,b] + sb[j,b] - 254) sum_{k in b} A[i,k] B[j,k] + bias):
- * both operands K-major, float32 accumulation, one rounding to d_dtype.
+ * both operands K-major, one rounding to d_dtype.  The products are summed in
+ * the tensor cores' float32 accumulators, which truncate; a float32 D is the
+ * float32 sum, in order, of such sums of at most 8192 elements (a CTA's).
  * lda, ldb: bytes, multiples of 16, operands 16-byte aligned; ldsa, ldsb:
  * bytes, multiples of 4, scales 4-byte aligned, every row's pitch readable.
  * bias [n], residual [m][ldres] in d_dtype, or NULL. */
