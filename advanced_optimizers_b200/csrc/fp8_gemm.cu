@@ -117,7 +117,7 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 // (of both CTAs of a pair).  One asm statement with the predicate inside: all
 // lanes reach it together, so descriptors stay in uniform registers.  As four
 // calls under a branch on the elected lane, 8192 x 14336 x 4096 took 424 us
-// instead of 381.
+// instead of 375.
 #define ADVOPT_FP8_BLOCK(GROUP, COMMIT)                                                                              \
   "{\n .reg .pred p, q, t;\n .reg .b32 al, bl;\n .reg .b64 a, b;\n"                                              \
   " setp.ne.b32 q, %9, 0;\n setp.ne.b32 p, %6, 0;\n setp.eq.b32 t, 0, 0;\n"                                       \

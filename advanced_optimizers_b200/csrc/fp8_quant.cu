@@ -420,6 +420,10 @@ __device__ __forceinline__ void tile_body(const QArgs& q, const Row (&v)[8], Til
   }
 }
 
+// Packed bf16 rows take 80 registers and three CTAs an SM, which spills up to 84
+// bytes a thread; with two CTAs of 128 registers nothing spills and 8192 x 4096
+// in both layouts takes 30.0 us instead of 25.8 (2048 x 2048, 256 tiles: 4.5,
+// 4.8).  float32 rows have room for two: 35.8 us, 0.86 of HBM.
 template <bool BF16, bool E5M2, bool SQUARE, class Row>
 __global__ void __launch_bounds__(256, sizeof(Row) == 16 ? 3 : 2) tile_kernel(const __grid_constant__ QArgs q, const __grid_constant__ DropSpec d) {
   __shared__ __align__(16) TileShared s;

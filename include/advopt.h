@@ -590,7 +590,7 @@ typedef struct advopt_dropout_spec {
 } advopt_dropout_spec;
 
 /* x, y, residual (may be NULL): n contiguous elements of `dtype` (ADVOPT_DT_*);
- * y may be x or residual. */
+ * y may be x or residual, and else overlaps neither. */
 int advopt_dropout(void* y, const void* x, const void* residual, int64_t n, int32_t dtype,
                    const advopt_dropout_spec* spec, void* stream);
 
@@ -643,7 +643,7 @@ int advopt_col_sum(void* out, const float* partial, int64_t parts, int64_t cols,
  * float32 sum, in order, of such sums of at most 8192 elements (a CTA's).
  * lda, ldb: bytes, multiples of 16, operands 16-byte aligned; ldsa, ldsb:
  * bytes, multiples of 4, scales 4-byte aligned, every row's pitch readable.
- * bias [n], residual [m][ldres] in d_dtype, or NULL. */
+ * bias [n], residual [m][ldres] in d_dtype, or NULL.  D overlaps no input. */
 typedef struct advopt_fp8_gemm_args {
   const uint8_t* a;
   int64_t lda;
