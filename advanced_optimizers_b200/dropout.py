@@ -64,7 +64,7 @@ def _launch(x, residual, fields):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, step_tensor, fields):
-        ctx.fields, ctx.stepped = fields, step_tensor is not None
+        ctx.fields, ctx.stepped = fields, step_tensor is not None and ctx.needs_input_grad[0]   # the residual's needs no mask
         if ctx.stepped:
             ctx.save_for_backward(step_tensor)
         return _launch(x, residual, fields)

@@ -342,8 +342,8 @@ class _Fp8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, blocks, step_tensor, drop):
         y, kept = _linear(x, weight, bias, residual, blocks, drop, *ctx.needs_input_grad[:2])
         ctx.drop, ctx.w_dtype, ctx.K, ctx.blocks, ctx.keeps = drop, weight.dtype, x.shape[1], blocks, kept is not None
-        ctx.stepped = step_tensor is not None
-        ctx.save_for_backward(*[t for t in (kept, step_tensor) if t is not None])
+        ctx.stepped = step_tensor is not None and any(ctx.needs_input_grad[:3])   # the residual's gradient needs no mask
+        ctx.save_for_backward(*[t for t in (kept, step_tensor if ctx.stepped else None) if t is not None])
         return y
 
     @staticmethod

@@ -138,3 +138,12 @@ def test_tangents_are_found():
         return t
 
     torch.func.jvp(seen, (x,), (x,))
+
+
+def test_a_residual_s_gradient_does_not_read_the_step(steps_read):
+    from advanced_optimizers_b200.dropout import _Dropout, drop_fields
+    x, r, step = torch.ones(4), torch.zeros(4, requires_grad=True), torch.tensor([7])
+    y = _Dropout.apply(x, r, step, drop_fields(0.5, 1, 0, step, x.device))
+    step.add_(1)
+    g, = torch.autograd.grad(y.sum(), r)
+    assert torch.equal(g, torch.ones(4)) and steps_read == [7]

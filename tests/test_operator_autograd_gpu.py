@@ -115,3 +115,15 @@ def test_weight_blocks_made_from_their_tensors(N, K):
     if N > 1 and K > 1:
         with pytest.raises(ValueError, match="weight_blocks"):
             A.fp8_linear(x, w, b, weight_blocks=rows)
+
+
+def test_a_residual_s_gradient_does_not_read_the_step():
+    import advanced_optimizers_b200 as A
+    x, w, b, dy = (t.detach() for t in inputs())
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    r, q = (torch.zeros(s, device="cuda", dtype=B, requires_grad=True) for s in ((70, 200), (70, 256)))
+    y = A.fp8_linear(x, w, b, residual=r, dropout_p=0.4, step=step)
+    d = A.philox_dropout(x, 0.4, residual=q, step=step)
+    step.add_(1)
+    assert torch.equal(torch.autograd.grad(y, r, dy)[0], dy)
+    assert torch.equal(torch.autograd.grad(d, q, x)[0], x)
