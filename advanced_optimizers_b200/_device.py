@@ -4,10 +4,13 @@ for device memory and streams."""
 from __future__ import annotations
 
 import contextlib
+import threading
 
 import numpy as np
 import torch
 from torch.autograd import forward_ad
+
+from . import _lib as L
 
 
 def require_cuda_tensor(t: torch.Tensor, what: str):
@@ -96,3 +99,55 @@ _HERE = contextlib.nullcontext()
 def on_device(device):
     """A context in which `device` is the current one (free when it is already)."""
     return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+class ErrorWord:
+    """The word that a kernel sets when something is wrong that only the device
+    sees (a bounded wait that gave up, an index outside its table): pinned host
+    memory that the kernels write directly, so that every call can look at it
+    without waiting for the GPU.  One for the process: whichever thread's call
+    comes next reports it, for whichever device."""
+
+    def __init__(self, message="an earlier kernel reported an error"):
+        self.message = message
+        self.word = self.view = None
+        self.lock = threading.Lock()
+
+    def pointer(self) -> int:
+        if self.word is None:
+            if torch.cuda.is_current_stream_capturing():
+                return 0   # no allocation of pinned memory during a capture
+            with self.lock:
+                if self.word is None:
+                    word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                    self.view = word.numpy()   # before the word, which other threads find without the lock
+                    self.word = word
+        if self.view[0]:
+            self.raise_()
+        return self.word.data_ptr()
+
+    def raise_(self):
+        self.view[0] = 0
+        raise L.AdvOptError(self.message)
+
+    def check(self):
+        """Waits for the GPU and raises what it reported."""
+        torch.cuda.synchronize()
+        if self.word is not None and self.view[0]:
+            self.raise_()
+
+
+def saved(t, what, dtype, shape, device):
+    """A saved tensor as the backward pass gets it, contiguous: a hook on saved tensors may have given another one."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        raise RuntimeError(f"a hook on saved tensors gave {t.dtype} {tuple(t.shape)} on {t.device} for the {what}, "
+                           f"{dtype} {tuple(shape)} on {device} was saved")
+    return t.contiguous()
+
+
+def rows_of(t):
+    """(t, pitch) of a matrix whose rows the kernels may read as they lie; a copy where their elements are not consecutive or rows overlap."""
+    R, C = t.shape
+    if (C > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < C):
+        t = t.contiguous()
+    return t, t.stride(0) if R > 1 else C

@@ -15,7 +15,7 @@ import numpy as np
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libadvopt.so")
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 # ---- constants mirrored from include/advopt.h ----
 DT_F32, DT_BF16 = 0, 1
@@ -162,6 +162,14 @@ class MuonArgs(ctypes.Structure):
 DROPOUT_SPEC_BYTES = 32
 FP8_QUANT_ARGS_BYTES = 152
 FP8_GEMM_ARGS_BYTES = 192
+# likewise (embeddings.py, norms.py, losses.py)
+EMBEDDING_ARGS_BYTES = 80
+EMBEDDING_GRAD_ARGS_BYTES = 80
+LAYER_NORM_ARGS_BYTES = 80
+LAYER_NORM_GRAD_ARGS_BYTES = 104
+TOKEN_LOGPROBS_ARGS_BYTES = 104
+POLICY_LOSS_ARGS_BYTES = 176
+PREFERENCE_LOSS_ARGS_BYTES = 112
 
 _LIB = None
 _LOCK = threading.Lock()
@@ -220,6 +228,20 @@ def lib():
             "advopt_fp8_quantize": ([P, P], ctypes.c_int),
             "advopt_col_sum": ([P, P, ctypes.c_int64, ctypes.c_int64, I32, P], ctypes.c_int),
             "advopt_fp8_gemm": ([P, P], ctypes.c_int),
+            "advopt_embedding": ([P, P], ctypes.c_int),
+            "advopt_embedding_grad_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+            "advopt_embedding_grad": ([P, P], ctypes.c_int),
+            "advopt_layer_norm": ([P, P], ctypes.c_int),
+            "advopt_layer_norm_grad_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+            "advopt_layer_norm_grad": ([P, P], ctypes.c_int),
+            "advopt_token_logprobs": ([P, P], ctypes.c_int),
+            "advopt_token_logprobs_grad": ([P, P, P, P], ctypes.c_int),
+            "advopt_policy_loss_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+            "advopt_policy_loss": ([P, P], ctypes.c_int),
+            "advopt_policy_loss_grad": ([P, P, P, P, ctypes.c_int64, ctypes.c_int64, I32, P], ctypes.c_int),
+            "advopt_preference_loss_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+            "advopt_preference_loss": ([P, P], ctypes.c_int),
+            "advopt_preference_loss_grad": ([P, P, P, P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, I32, P], ctypes.c_int),
             "advopt_spectral_step": ([ctypes.POINTER(AdamLaunch), P, P, I32, P, I32, P], ctypes.c_int),
         }
         for name, (args, res) in sig.items():
@@ -233,7 +255,10 @@ def lib():
                             (4, ctypes.sizeof(MuonArgs)), (5, ctypes.sizeof(KourkoutasArgs)),
                             (6, PRODIGY_DEV_BYTES), (7, ctypes.sizeof(ProdigyScalarArgs)),
                             (8, ctypes.sizeof(ProdigyDArgs)), (9, SPECTRAL_TENSOR_DT.itemsize),
-                            (10, DROPOUT_SPEC_BYTES), (11, FP8_QUANT_ARGS_BYTES), (12, FP8_GEMM_ARGS_BYTES)):
+                            (10, DROPOUT_SPEC_BYTES), (11, FP8_QUANT_ARGS_BYTES), (12, FP8_GEMM_ARGS_BYTES),
+                            (13, EMBEDDING_ARGS_BYTES), (14, EMBEDDING_GRAD_ARGS_BYTES), (15, LAYER_NORM_ARGS_BYTES),
+                            (16, LAYER_NORM_GRAD_ARGS_BYTES), (17, TOKEN_LOGPROBS_ARGS_BYTES),
+                            (18, POLICY_LOSS_ARGS_BYTES), (19, PREFERENCE_LOSS_ARGS_BYTES)):
             got = L.advopt_sizeof(which)
             if got != size:
                 raise AdvOptError(f"struct layout mismatch (#{which}: C {got} bytes, Python {size})")
@@ -256,7 +281,11 @@ def exported_symbols():
             "advopt_prodigy_scalars", "advopt_prodigy_update_d", "advopt_lr_sketch", "advopt_lr_gemm",
             "advopt_lr_qr_work", "advopt_lr_qr", "advopt_ipc_get_handle", "advopt_ipc_open", "advopt_ipc_close",
             "advopt_enable_peer", "advopt_copy_async", "advopt_spectral_step", "advopt_dropout",
-            "advopt_fp8_quantize", "advopt_col_sum", "advopt_fp8_gemm"]
+            "advopt_fp8_quantize", "advopt_col_sum", "advopt_fp8_gemm", "advopt_embedding", "advopt_embedding_grad_work",
+            "advopt_embedding_grad", "advopt_layer_norm", "advopt_layer_norm_grad_work", "advopt_layer_norm_grad",
+            "advopt_token_logprobs", "advopt_token_logprobs_grad", "advopt_policy_loss_work", "advopt_policy_loss",
+            "advopt_policy_loss_grad", "advopt_preference_loss_work", "advopt_preference_loss",
+            "advopt_preference_loss_grad"]
 
 
 _OCC_CACHE = {}

@@ -39,6 +39,13 @@ extern "C" size_t advopt_sizeof(int which) {
     case 10: return sizeof(advopt_dropout_spec);
     case 11: return sizeof(advopt_fp8_quant_args);
     case 12: return sizeof(advopt_fp8_gemm_args);
+    case 13: return sizeof(advopt_embedding_args);
+    case 14: return sizeof(advopt_embedding_grad_args);
+    case 15: return sizeof(advopt_layer_norm_args);
+    case 16: return sizeof(advopt_layer_norm_grad_args);
+    case 17: return sizeof(advopt_token_logprobs_args);
+    case 18: return sizeof(advopt_policy_loss_args);
+    case 19: return sizeof(advopt_preference_loss_args);
     default: return 0;
   }
 }

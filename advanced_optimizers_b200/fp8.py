@@ -11,14 +11,14 @@ from __future__ import annotations
 
 import functools
 import struct
-import threading
 
 import torch
 
 from . import _lib as L
-from ._device import dtype_code, on_device, raw_stream, refuse_tangents
+from ._device import ErrorWord, dtype_code, on_device, raw_stream, refuse_tangents
 from .dropout import NO_DROP, drop_fields, with_saved_step
 
+_ErrorWord = ErrorWord
 _CODE = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _E8M0 = torch.float8_e8m0fnu
 
@@ -27,35 +27,7 @@ _QUANT = struct.Struct("<QqqqQqQqQqQqQiiiiQQIIIf")
 _GEMM = struct.Struct("<QqQqQqQqQqQQqqqqiiiiiiQQQIIIf")
 
 
-class _ErrorWord:
-    """The word that a kernel's bounded wait sets when it gives up: pinned host
-    memory that the kernels write directly, so that every call can look at it
-    without waiting for the GPU.  One for the process: whichever thread's call
-    comes next reports it, for whichever device."""
-
-    def __init__(self):
-        self.word = self.view = None
-        self.lock = threading.Lock()
-
-    def pointer(self) -> int:
-        if self.word is None:
-            if torch.cuda.is_current_stream_capturing():
-                return 0   # no allocation of pinned memory during a capture
-            with self.lock:
-                if self.word is None:
-                    word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-                    self.view = word.numpy()   # before the word, which other threads find without the lock
-                    self.word = word
-        if self.view[0]:
-            self.raise_()
-        return self.word.data_ptr()
-
-    def raise_(self):
-        self.view[0] = 0
-        raise L.AdvOptError("an earlier fp8 product gave up waiting for its copies (bounded wait); its result is not valid")
-
-
-_ERR = _ErrorWord()
+_ERR = ErrorWord("an earlier fp8 product gave up waiting for its copies (bounded wait); its result is not valid")
 
 
 def check_fp8_errors():
@@ -63,9 +35,7 @@ def check_fp8_errors():
     guard that is not expected to fire; otherwise the process's next product
     raises, on whichever thread or device).  Products captured before the
     process's first eager one have no word to report to."""
-    torch.cuda.synchronize()
-    if _ERR.word is not None and _ERR.view[0]:
-        _ERR.raise_()
+    _ERR.check()
 
 
 def _round_up(n, to):

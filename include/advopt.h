@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define ADVOPT_ABI_VERSION 6
+#define ADVOPT_ABI_VERSION 7
 
 /* ---- error codes ---- */
 #define ADVOPT_OK 0
@@ -675,9 +675,207 @@ typedef struct advopt_fp8_gemm_args {
 } advopt_fp8_gemm_args;
 int advopt_fp8_gemm(const advopt_fp8_gemm_args* args, void* stream);
 
+/* ---- Token embedding ----
+ * y [tokens][width] = scale * weight[ids[t]], one rounding.  An id outside
+ * [0, vocab) gives a row of NaN and sets *err (or NULL) to 1. */
+typedef struct advopt_embedding_args {
+  void* y;                  /* contiguous                                      */
+  const void* weight;       /* [vocab][ldw]                                    */
+  const void* ids;          /* contiguous, int32 or int64                      */
+  int32_t* err;
+  int64_t ldw;              /* elements                                        */
+  int64_t tokens;           /* below 2^31, as vocab                            */
+  int64_t vocab;
+  int64_t width;
+  int32_t dtype;            /* ADVOPT_DT_*: y and weight                       */
+  int32_t id_bytes;         /* 4 or 8                                          */
+  float scale;
+  int32_t pad;
+} advopt_embedding_args;
+int advopt_embedding(const advopt_embedding_args* args, void* stream);
+
+/* dweight [vocab][width] = scale * sum of dy's rows whose token is the row's id,
+ * in float32 in an order that the ids alone decide, one rounding; every row is
+ * written.  Ids outside [0, vocab), and `padding` (-1: none), contribute
+ * nothing.  `work`: advopt_embedding_grad_work(tokens, width) bytes, 16-byte
+ * aligned. */
+typedef struct advopt_embedding_grad_args {
+  void* dweight;            /* contiguous, as dy                               */
+  const void* dy;
+  const void* ids;
+  void* work;
+  int64_t tokens;
+  int64_t vocab;
+  int64_t width;
+  int64_t padding;
+  int32_t dtype;
+  int32_t id_bytes;
+  float scale;
+  int32_t pad;
+} advopt_embedding_grad_args;
+int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width);
+int advopt_embedding_grad(const advopt_embedding_grad_args* args, void* stream);
+
+/* ---- Layer norm ----
+ * y = (x - mean) * rstd * weight + bias over the rows of x [rows][cols] in
+ * float32, one rounding; rstd = 1 / sqrt(mean of (x - mean)^2 + eps).  weight
+ * and bias [cols] in w_dtype, or NULL (ones, zeros).  stats (or NULL) receives
+ * {mean, rstd} of each row. */
+typedef struct advopt_layer_norm_args {
+  void* y;                  /* contiguous                                      */
+  const void* x;            /* [rows][ldx]                                     */
+  const void* weight;
+  const void* bias;
+  float* stats;             /* [rows][2]                                       */
+  int64_t ldx;              /* elements                                        */
+  int64_t rows;
+  int64_t cols;
+  float eps;
+  int32_t x_dtype;          /* ADVOPT_DT_*: x and y                            */
+  int32_t w_dtype;
+  int32_t pad;
+} advopt_layer_norm_args;
+int advopt_layer_norm(const advopt_layer_norm_args* args, void* stream);
+
+/* With g = dy * weight and h = (x - mean) * rstd: dx = rstd * (g - mean of g -
+ * h * mean of g h), dweight = sum over the rows of dy h, dbias = sum of dy, in
+ * float32, one rounding each.  dx, or dweight and dbias, may be NULL.  `work`:
+ * advopt_layer_norm_grad_work(rows, cols) bytes, 16-byte aligned, where
+ * dweight or dbias is wanted. */
+typedef struct advopt_layer_norm_grad_args {
+  void* dx;                 /* contiguous                                      */
+  void* dweight;            /* [cols] in w_dtype                               */
+  void* dbias;
+  const void* dy;           /* [rows][lddy]                                    */
+  const void* x;            /* [rows][ldx]                                     */
+  const void* weight;
+  const float* stats;
+  void* work;
+  int64_t lddy;
+  int64_t ldx;
+  int64_t rows;
+  int64_t cols;
+  int32_t x_dtype;          /* x, dy and dx                                    */
+  int32_t w_dtype;
+} advopt_layer_norm_grad_args;
+int64_t advopt_layer_norm_grad_work(int64_t rows, int64_t cols);
+int advopt_layer_norm_grad(const advopt_layer_norm_grad_args* args, void* stream);
+
+/* ---- Log-probabilities of tokens ----
+ * logprobs[r] = z_k - log sum_j exp(z_j) with z = logits row r / temperature
+ * and k = tokens[r].  Row r = (a, b) with b < inner starts at a * ld_outer +
+ * b * ld_inner.  A token `ignore` gives 0; any other outside [0, vocab) NaN,
+ * and sets *err (or NULL) to 1.  stats (or NULL) receives {largest logit,
+ * sum of exp((logit - largest) / temperature)}. */
+typedef struct advopt_token_logprobs_args {
+  float* logprobs;          /* [rows]                                          */
+  float* stats;             /* [rows][2]                                       */
+  const void* logits;
+  const void* tokens;       /* contiguous, int32 or int64                      */
+  int32_t* err;
+  int64_t inner;
+  int64_t ld_outer;         /* elements                                        */
+  int64_t ld_inner;
+  int64_t rows;
+  int64_t vocab;            /* below 2^31                                      */
+  int64_t ignore;
+  int32_t dtype;            /* ADVOPT_DT_*: logits                             */
+  int32_t token_bytes;      /* 4 or 8                                          */
+  float temperature;        /* positive                                        */
+  int32_t pad;
+} advopt_token_logprobs_args;
+int advopt_token_logprobs(const advopt_token_logprobs_args* args, void* stream);
+
+/* dlogits [rows][vocab] (contiguous, in the logits' dtype) = dlogprobs[r] /
+ * temperature * ((j == k) - p_j); rows with dlogprobs[r] == 0 and rows whose
+ * token is `ignore` are zeros and are not read.  Of args: logits, tokens,
+ * stats (as the forward call left them) and the sizes. */
+int advopt_token_logprobs_grad(void* dlogits, const float* dlogprobs, const advopt_token_logprobs_args* args, void* stream);
+
+/* ---- Clipped policy loss with a KL term ----
+ * For each token with mask (NULL: all): d = logprob - old; with A the
+ * advantage, clipped iff A > 0 and d > log1p(clip_high) or A < 0 and d <
+ * log1p(-clip_low) (both as given, in float64); gain = clipped ? (1 +
+ * clip_high or 1 - clip_low) A : e^d A; q = ref - logprob, kl = e^q - q - 1 (0
+ * without ref).  loss = mean of kl_weight kl - gain over the tokens (by_rows =
+ * 0), or over the rows with a token of the means over their tokens (1).
+ * stats receives {mean kl over the tokens, share of clipped tokens}; with no
+ * token these and the loss are 0.  Values where the mask is 0 are not looked at.
+ * slope (or NULL, [rows][cols] contiguous float32) and scale ([rows] float32)
+ * receive what advopt_policy_loss_grad needs.  `work`:
+ * advopt_policy_loss_work(rows, cols) bytes, 16-byte aligned. */
+typedef struct advopt_policy_loss_args {
+  float* loss;              /* one value                                       */
+  float* stats;             /* [2]                                             */
+  float* slope;
+  float* scale;
+  const void* logprobs;     /* [rows][ld_...], elements of dtype               */
+  const void* old;
+  const void* ref;          /* or NULL                                         */
+  const void* advantages;   /* [rows][ld_adv], or [rows] with ld_adv < 0       */
+  const uint8_t* mask;      /* [rows][ld_mask], or NULL                        */
+  void* work;
+  int64_t ld_logprobs;
+  int64_t ld_old;
+  int64_t ld_ref;
+  int64_t ld_adv;
+  int64_t ld_mask;
+  int64_t rows;
+  int64_t cols;
+  double log_high;          /* log1p(clip_high)                                */
+  double log_low;           /* log1p(-clip_low)                                */
+  float clip_low;
+  float clip_high;
+  float kl_weight;
+  int32_t by_rows;
+  int32_t dtype;
+  int32_t pad;
+} advopt_policy_loss_args;
+int64_t advopt_policy_loss_work(int64_t rows, int64_t cols);
+int advopt_policy_loss(const advopt_policy_loss_args* args, void* stream);
+/* dlogprobs [rows][cols] (contiguous, dtype) = *dloss * scale[row] * slope. */
+int advopt_policy_loss_grad(void* dlogprobs, const float* dloss, const float* slope, const float* scale, int64_t rows,
+                            int64_t cols, int32_t dtype, void* stream);
+
+/* ---- Preference loss of paired rows ----
+ * Rows 0 .. pairs-1 are the chosen ones, row pairs + i the rejected one of
+ * pair i.  s_r = sum over the row's tokens with mask (NULL: all) of logprob -
+ * ref (ref NULL: 0), divided by their number (at least 1) if `average`;
+ * h = beta (s_chosen - s_rejected); loss = mean over the pairs of
+ * -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h); rewards[r] =
+ * beta s_r.  slope [2 pairs] (or NULL) receives d loss / d logprob of a row's
+ * tokens.  `work`: advopt_preference_loss_work(pairs, cols) bytes,
+ * 16-byte aligned. */
+typedef struct advopt_preference_loss_args {
+  float* loss;              /* one value                                       */
+  float* rewards;           /* [2 pairs]                                       */
+  float* slope;
+  const void* logprobs;     /* [2 pairs][ld_...], elements of dtype            */
+  const void* ref;
+  const uint8_t* mask;
+  void* work;
+  int64_t ld_logprobs;
+  int64_t ld_ref;
+  int64_t ld_mask;
+  int64_t pairs;
+  int64_t cols;
+  float beta;
+  float smoothing;
+  int32_t average;
+  int32_t dtype;
+} advopt_preference_loss_args;
+int64_t advopt_preference_loss_work(int64_t pairs, int64_t cols);
+int advopt_preference_loss(const advopt_preference_loss_args* args, void* stream);
+/* dlogprobs [2 pairs][cols] (contiguous, dtype) = mask ? *dloss * slope[row] : 0. */
+int advopt_preference_loss_grad(void* dlogprobs, const float* dloss, const float* slope, const uint8_t* mask, int64_t ld_mask,
+                                int64_t pairs, int64_t cols, int32_t dtype, void* stream);
+
 /* Layout checks for bindings: sizeof of each struct. */
 size_t advopt_sizeof(int which); /* 0 adam_tensor, 1 piece, 2 adam_launch, 3 lion_tensor, 4 muon_args, ...,
-                                    10 dropout_spec, 11 fp8_quant_args, 12 fp8_gemm_args */
+                                    10 dropout_spec, 11 fp8_quant_args, 12 fp8_gemm_args,
+                                    13 embedding_args, 14 embedding_grad_args, 15 layer_norm_args,
+                                    16 layer_norm_grad_args, 17 token_logprobs_args, 18 policy_loss_args,
+                                    19 preference_loss_args */
 int advopt_abi_version(void);
 /* Last error message of the calling thread ("" if none). */
 const char* advopt_last_error(void);
