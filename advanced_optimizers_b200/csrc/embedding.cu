@@ -6,11 +6,11 @@
 // Gradient: bound by HBM too (dy read once, every row of dW written once, of
 // which most are zeros).  The tokens are put in order of their ids first (a
 // stable radix sort, so that the order of a row's sum follows from the ids
-// alone); then each warp sums 32 tokens of that order for 256 columns in
-// registers and writes the rows that begin and end among them.  A row that
-// reaches over several such chunks leaves a float32 partial sum in each, and
-// a third launch adds these up in order.  No atomics: results repeat bit for
-// bit.
+// alone); then each warp takes 32 tokens of that order for 256 columns and
+// sums and writes, from registers, the rows that begin among them.  A row
+// that fills a whole such chunk, and so may be of any length, leaves a float32
+// partial sum in each of its chunks, and a third launch adds these up in
+// order.  No atomics: results repeat bit for bit.
 #include <cooperative_groups.h>
 
 #include "advopt.h"
@@ -98,18 +98,18 @@ constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int BITS = 9, BINS = 1 << BITS;
 constexpr int SORT_SMEM = (SORT_WARPS * BINS + 2 * BINS + SORT_WARPS) * 4;
+constexpr int FILL_THREADS = 512, FILL = 4;   // 16-byte stores of a thread that writes zeros
 constexpr uint32_t CHUNK = 32;         // tokens of one warp, so that a lane holds one token's id
 
-// One cluster sorts while the other ones write the zeros: the sort reads and
-// writes a few hundred KB that stay in L2, and takes less time than the
-// zeros of a large table.
+// One cluster sorts, beside the kernel that writes the zeros: the sort reads and
+// writes a few hundred KB that stay in L2, and takes less time than the zeros
+// of a large table.
 //
-// A pass of the sort: every warp counts the digits of its contiguous share,
+// A pass: every warp counts the digits of its contiguous share,
 // the counts are summed over the digits, CTAs and warps before it, and the
 // warp walks its share again, in order, and places each token behind those of
 // its digit that came before.
-template <int UNUSED>
-__device__ void sort_cluster(const Grad& g, uint32_t* sm) {
+__device__ __forceinline__ void sort_cluster(const Grad& g, uint32_t* sm) {
   cg::cluster_group cluster = cg::this_cluster();
   uint32_t* hist = sm;                                  // [SORT_WARPS][BINS]
   uint32_t* total = sm + SORT_WARPS * BINS;             // [BINS] of this CTA
@@ -191,154 +191,267 @@ __device__ void sort_cluster(const Grad& g, uint32_t* sm) {
   }
 }
 
-template <bool BF16>
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(SORT_THREADS) order_kernel(const __grid_constant__ Grad g) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the zeros do not wait for the order
   extern __shared__ uint32_t sm[];
-  if (blockIdx.x < CLUSTER) {
-    sort_cluster<0>(g, sm);
-    return;
-  }
-  // zeros: dw is 16-byte aligned
-  const int64_t bytes = (int64_t)g.vocab * g.width * (BF16 ? 2 : 4);
-  uint4* p = static_cast<uint4*>(g.dw);
-  const int64_t n = bytes >> 4, stride = (int64_t)(gridDim.x - CLUSTER) * SORT_THREADS;
-  const int64_t i0 = (int64_t)(blockIdx.x - CLUSTER) * SORT_THREADS + threadIdx.x;
-  for (int64_t i = i0; i < n; i += stride) p[i] = make_uint4(0, 0, 0, 0);
-  const int tail = (int)(bytes & 15) / (BF16 ? 2 : 4);
-  if (i0 < tail) {
-    if (BF16) reinterpret_cast<uint16_t*>(p + n)[i0] = 0;
-    else reinterpret_cast<float*>(p + n)[i0] = 0.0f;
-  }
+  sort_cluster(g, sm);
 }
 
+// Zeros for all of dw (16-byte aligned), beside the sort on the other SMs.  In
+// the order of the CTAs the stores reach HBM at 7.4 TB/s, a grid's width apart
+// at 6.0.  The grid ends behind the sort, since its last CTA waits for it.
 template <bool BF16>
-__device__ __forceinline__ void write_row(const Grad& g, uint32_t row, int64_t c, int nv, bool vec, const float (&acc)[8]) {
-  float v[8];
+__global__ void __launch_bounds__(FILL_THREADS) zero_kernel(void* dw, int64_t bytes) {
+  uint4* p = static_cast<uint4*>(dw);
+  const int64_t n = bytes >> 4;
+  int64_t i = (int64_t)blockIdx.x * (FILL_THREADS * FILL) + threadIdx.x;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(acc[e], g.scale);
-  Oct<BF16> o;
-  o.set(v);
-  o.put(g.dw, (int64_t)row * g.width + c, nv, vec);
+  for (int k = 0; k < FILL; ++k, i += FILL_THREADS)
+    if (i < n) p[i] = make_uint4(0, 0, 0, 0);
+  if (blockIdx.x != gridDim.x - 1) return;
+  const int tail = (int)(bytes & 15) / (BF16 ? 2 : 4);
+  if (threadIdx.x < tail) {
+    if (BF16) reinterpret_cast<uint16_t*>(p + n)[threadIdx.x] = 0;
+    else reinterpret_cast<float*>(p + n)[threadIdx.x] = 0.0f;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// A warp: CHUNK tokens in order x 256 columns, eight a lane.
+// 16 bytes of a row: the columns of a lane.
 template <bool BF16>
-__global__ void __launch_bounds__(256) sums_kernel(const __grid_constant__ Grad g, uint32_t slabs, int vec) {
+struct Cols {
+  static constexpr int E = BF16 ? 8 : 4;
+  uint32_t w[4];
+  __device__ __forceinline__ float at(int e) const { return BF16 ? u2f((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16) : u2f(w[e & 3]); }
+  __device__ __forceinline__ void get(const void* base, int64_t k, int nv, bool vec) {
+    if (vec && nv == E) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + k * (BF16 ? 2 : 4)));
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    } else if (BF16) {
+      const uint16_t* p = static_cast<const uint16_t*>(base) + k;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = (2 * i < nv ? (uint32_t)__ldg(p + 2 * i) : 0u) | (2 * i + 1 < nv ? (uint32_t)__ldg(p + 2 * i + 1) << 16 : 0u);
+    } else {
+      const uint32_t* p = static_cast<const uint32_t*>(base) + k;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = i < nv ? __ldg(p + i) : 0u;
+    }
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ void write_row(const Grad& g, uint32_t row, int64_t c, int nv, bool vec, const float (&acc)[Cols<BF16>::E]) {
+  constexpr int E = Cols<BF16>::E;
+  const int64_t k = (int64_t)row * g.width + c;
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = __fmul_rn(acc[e], g.scale);
+  if constexpr (BF16) {
+    uint16_t* p = static_cast<uint16_t*>(g.dw) + k;
+    if (vec && nv == E) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2(v[0], v[1]), bf16x2(v[2], v[3]), bf16x2(v[4], v[5]), bf16x2(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < nv) p[e] = (uint16_t)f_to_bf16_rne(v[e]);
+    }
+  } else {
+    float* p = static_cast<float*>(g.dw) + k;
+    if (vec && nv == E) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < nv) p[e] = v[e];
+    }
+  }
+}
+
+// Whether a row that crosses from one chunk to the next is a long one, which
+// fills one of them: `first` is the first key of the one, `end` the last of the
+// other (g.vocab where that is not whole).
+__device__ __forceinline__ bool is_long(uint32_t row, uint32_t first, uint32_t end) { return first == row || end == row; }
+
+template <int E>
+__device__ __forceinline__ void write_part(float* part, int nv, bool vec, const float (&acc)[E]) {
+  if (vec && nv == E) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(part + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < nv) part[e] = acc[e];
+  }
+}
+
+constexpr int SUM_WARPS = 4;
+
+// A warp: the rows that begin among CHUNK tokens in order, for 16 bytes a lane.  A row that goes on into the next chunk, but fills neither, is
+// followed there; of one that does, each chunk's warp sums its own tokens.
+template <bool BF16>
+__global__ void __launch_bounds__(SUM_WARPS * 32, 7) sums_kernel(const __grid_constant__ Grad g, uint32_t slabs, int vec) {
   const int lane = threadIdx.x & 31;
-  const int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t u = (int64_t)blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
   const uint32_t chunk = (uint32_t)(u / slabs);
-  const uint32_t first = chunk * CHUNK;
   if ((int64_t)chunk * CHUNK >= g.tokens) return;
-  const int64_t c = (int64_t)(u - (int64_t)chunk * slabs) * 256 + lane * 8;
-  const int nv = c >= g.width ? 0 : g.width - c < 8 ? (int)(g.width - c) : 8;
+  const uint32_t first = chunk * CHUNK;
+  constexpr int E = Cols<BF16>::E;
+  const int64_t c = ((u - (int64_t)chunk * slabs) * 32 + lane) * E;
+  const int nv = c >= g.width ? 0 : g.width - c < E ? (int)(g.width - c) : E;
   const uint32_t* keys = g.keys[(g.passes + 1) & 1];
   const uint32_t* at = g.at[(g.passes + 1) & 1];
-  const uint32_t key = first + lane < g.tokens ? keys[first + lane] : g.vocab;
-  const uint32_t pos = first + lane < g.tokens ? at[first + lane] : 0u;
+  const uint32_t mine = first + lane, next = mine + CHUNK;
+  const uint32_t key = mine < g.tokens ? keys[mine] : g.vocab, pos = mine < g.tokens ? at[mine] : 0u;
+  const uint32_t more = next < g.tokens ? keys[next] : g.vocab, more_pos = next < g.tokens ? at[next] : 0u;
   const uint32_t n = __popc(__ballot_sync(0xffffffffu, key < g.vocab));   // those that contribute come first
   if (n == 0) return;
-  const uint32_t ahead = first ? keys[first - 1] : g.vocab;
-  const uint32_t behind = first + CHUNK < g.tokens ? keys[first + CHUNK] : g.vocab;
-  float acc[8] = {};
-  uint32_t cur = __shfl_sync(0xffffffffu, key, 0);
-  bool open_ahead = cur == ahead;
+  const uint32_t head = __shfl_sync(0xffffffffu, key, 0), tail = __shfl_sync(0xffffffffu, key, 31);
+  // the row that comes from the chunk before: long, or summed there
+  const bool comes = first && keys[first - 1] == head;
+  const bool long_ahead = comes && is_long(head, keys[first - CHUNK], tail);
+  uint32_t begin = 0;
+  if (comes && !long_ahead) begin = __popc(__ballot_sync(0xffffffffu, key == head));
+  // the row that goes on into the next one
+  const bool goes = n == CHUNK && __shfl_sync(0xffffffffu, more, 0) == tail;
+  const bool long_behind = goes && is_long(tail, head, __shfl_sync(0xffffffffu, more, 31));
+  uint32_t end = n;
+  if (goes && !long_behind && begin < n) end += __popc(__ballot_sync(0xffffffffu, more == tail));
+  if (begin >= n) return;
+  float acc[E] = {};
+  uint32_t cur = __shfl_sync(0xffffffffu, key, begin);
+  bool partial = long_ahead;
   float* part = g.part + (int64_t)chunk * 2 * g.width + c;
-  constexpr int U = 8;
-  for (uint32_t i0 = 0; i0 < n; i0 += U) {
-    Oct<BF16> v[U];
+  constexpr int U = 8;   // tokens whose values are on their way
+  for (uint32_t i0 = begin; i0 < end; i0 += U) {
+    Cols<BF16> v[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const uint32_t p = __shfl_sync(0xffffffffu, pos, i0 + i);
-      if (i0 + i < n) v[i].get(g.dy, (int64_t)p * g.width + c, nv, vec);
-      else v[i].zero();
+      const uint32_t j = i0 + i;
+      const uint32_t p0 = __shfl_sync(0xffffffffu, pos, j & 31), p1 = __shfl_sync(0xffffffffu, more_pos, j & 31);
+      if (j < end) v[i].get(g.dy, (int64_t)(j < CHUNK ? p0 : p1) * g.width + c, nv, vec);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const uint32_t k = __shfl_sync(0xffffffffu, key, i0 + i);
-      if (i0 + i >= n) break;
+      const uint32_t j = i0 + i;
+      const uint32_t k0 = __shfl_sync(0xffffffffu, key, j & 31);
+      if (j >= end) break;
+      const uint32_t k = j < CHUNK ? k0 : tail;
       if (k != cur) {
-        if (open_ahead) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < nv) part[e] = acc[e];
-          open_ahead = false;
-        } else if (nv) {
-          write_row<BF16>(g, cur, c, nv, vec, acc);
-        }
+        if (partial) write_part(part, nv, vec, acc);
+        else if (nv) write_row<BF16>(g, cur, c, nv, vec, acc);
+        partial = false;
         cur = k;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+        for (int e = 0; e < E; ++e) acc[e] = 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = __fadd_rn(acc[e], v[i].at(e));
+      for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], v[i].at(e));
     }
   }
-  if (open_ahead || (n == CHUNK && cur == behind)) {
-    if (!open_ahead) part += g.width;
+  // a long row's sum of this chunk: the second place where the row begins here
+  if (partial) write_part(part, nv, vec, acc);
+  else if (long_behind) write_part(part + g.width, nv, vec, acc);
+  else if (nv) write_row<BF16>(g, cur, c, nv, vec, acc);
+}
+
+// The long rows: a CTA takes those that begin in JOIN chunks, for 128 columns,
+// a warp each; of rows of more than FAR parts every warp adds a share, and the
+// shares are added in order.
+constexpr int JOIN = 8;
+constexpr uint32_t FAR = 64;
+
+__device__ __forceinline__ void add_parts(float (&s)[4], const Grad& g, uint32_t chunk, uint32_t begin, uint32_t end, int64_t c, int nv, bool vec) {
+  // part 0 is in its chunk's second place, the others in their first
+  const auto at = [&](uint32_t p) { return g.part + ((int64_t)(chunk + p) * 2 + (p == 0)) * g.width + c; };
+  if (vec && nv == 4) {
+#pragma unroll 8
+    for (uint32_t p = begin; p < end; ++p) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(at(p)));
+      s[0] = __fadd_rn(s[0], q.x);
+      s[1] = __fadd_rn(s[1], q.y);
+      s[2] = __fadd_rn(s[2], q.z);
+      s[3] = __fadd_rn(s[3], q.w);
+    }
+  } else {
+#pragma unroll 4
+    for (uint32_t p = begin; p < end; ++p) {
+      const float* q = at(p);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < nv) part[e] = acc[e];
-  } else if (nv) {
-    write_row<BF16>(g, cur, c, nv, vec, acc);
+      for (int e = 0; e < 4; ++e)
+        if (e < nv) s[e] = __fadd_rn(s[e], __ldg(q + e));
+    }
   }
 }
 
-// The rows that reach over chunks: a CTA looks at 32 chunks for those that
-// begin in them, for 128 columns.  The partial sums of a row are split over
-// the warps in order, and the warps' sums are added in order.
-constexpr int JOIN_WARPS = 16;
+template <bool BF16>
+__device__ __forceinline__ void write_sum(const Grad& g, uint32_t row, int64_t c, float sum) {
+  sum = __fmul_rn(sum, g.scale);
+  const int64_t k = (int64_t)row * g.width + c;
+  if (BF16) static_cast<uint16_t*>(g.dw)[k] = (uint16_t)f_to_bf16_rne(sum);
+  else static_cast<float*>(g.dw)[k] = sum;
+}
 
 template <bool BF16>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ Grad g, uint32_t slabs) {
-  __shared__ float red[JOIN_WARPS][128];
+__global__ void __launch_bounds__(JOIN * 32) join_kernel(const __grid_constant__ Grad g, uint32_t slabs) {
+  __shared__ float red[JOIN][128];
+  __shared__ uint32_t far_row[JOIN], far_parts[JOIN];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t slab = blockIdx.x % slabs, group = blockIdx.x / slabs;
+  const uint32_t slab = blockIdx.x % slabs, chunk0 = blockIdx.x / slabs * JOIN, chunk = chunk0 + warp;
   const uint32_t* keys = g.keys[(g.passes + 1) & 1];
   const uint32_t T = g.tokens;
-  const uint64_t last = ((uint64_t)group * 32 + lane + 1) * CHUNK - 1;   // the last token of this lane's chunk
-  uint32_t key = g.vocab;
-  bool begins = false;
+  const uint64_t last = ((uint64_t)chunk + 1) * CHUNK - 1;   // the last token of the warp's chunk
+  uint32_t row = g.vocab, parts = 0;
   if (last + 1 < T) {
-    key = keys[last];
-    begins = key < g.vocab && keys[last + 1] == key && (last < CHUNK || keys[last - CHUNK] != key);
+    row = keys[last];
+    const uint32_t head = keys[last + 1 - CHUNK];
+    const bool begins = row < g.vocab && keys[last + 1] == row && (last < CHUNK || keys[last - CHUNK] != row) &&
+                        is_long(row, head, last + CHUNK < T ? keys[last + CHUNK] : g.vocab);
+    if (begins) {
+      // the first token behind the row's, between lo and hi: each lane looks at one of 32 places between
+      uint32_t lo = (uint32_t)last + 2, hi = T;
+      while (lo < hi) {
+        const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, at < hi && keys[at] == row));
+        if (n == 0) break;
+        const uint32_t reach = lo + n * step;
+        lo += (n - 1) * step + 1;
+        if (reach < hi) hi = reach;
+      }
+      parts = (lo - 1) / CHUNK - chunk + 1;   // this chunk's and the following ones'
+    }
   }
-  uint32_t todo = __ballot_sync(0xffffffffu, begins);
+  const bool far = parts > FAR;
+  if (lane == 0) {
+    far_row[warp] = row;
+    far_parts[warp] = far ? parts : 0u;
+  }
   const int64_t c = (int64_t)slab * 128 + lane * 4;
   const int nv = c >= g.width ? 0 : g.width - c < 4 ? (int)(g.width - c) : 4;
-  while (todo) {
-    const int b = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const uint32_t row = __shfl_sync(0xffffffffu, key, b);
-    const uint32_t chunk = group * 32 + b;
-    // the first token behind the row's
-    uint32_t lo = (chunk + 1) * CHUNK, hi = T;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (keys[mid] > row) hi = mid;
-      else lo = mid + 1;
-    }
-    const uint32_t parts = (lo - 1) / CHUNK - chunk + 1;   // this chunk's and the following ones'
-    const uint32_t each = (parts + JOIN_WARPS - 1) / JOIN_WARPS;
-    const uint32_t p0 = warp * each < parts ? warp * each : parts, p1 = p0 + each < parts ? p0 + each : parts;
+  const bool vec = (g.width & 3) == 0;   // the partial sums are 16-byte aligned
+  if (parts && !far) {
     float s[4] = {};
-    for (uint32_t p = p0; p < p1; ++p) {
-      // part 0 is what the chunk ends in, the others what they begin in
-      const float* from = g.part + ((int64_t)(chunk + p) * 2 + (p == 0)) * g.width + c;
+    add_parts(s, g, chunk, 0, parts, c, nv, vec);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < nv) s[e] = __fadd_rn(s[e], from[e]);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (e < nv) write_sum<BF16>(g, row, c + e, s[e]);
+  }
+  if (!__syncthreads_or(far)) return;
+  for (int b = 0; b < JOIN; ++b) {
+    const uint32_t all = far_parts[b];
+    if (all == 0) continue;
+    const uint32_t each = (all + JOIN - 1) / JOIN, p0 = warp * each < all ? warp * each : all, p1 = p0 + each < all ? p0 + each : all;
+    float s[4] = {};
+    add_parts(s, g, chunk0 + b, p0, p1, c, nv, vec);
 #pragma unroll
     for (int e = 0; e < 4; ++e) red[warp][lane * 4 + e] = s[e];
     __syncthreads();
-    if (threadIdx.x < 128 && (int64_t)slab * 128 + threadIdx.x < g.width) {
+    const int64_t mine = (int64_t)slab * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && mine < g.width) {
       float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < JOIN_WARPS; ++w) sum = __fadd_rn(sum, red[w][threadIdx.x]);
-      sum = __fmul_rn(sum, g.scale);
-      const int64_t k = (int64_t)row * g.width + (int64_t)slab * 128 + threadIdx.x;
-      if (BF16) static_cast<uint16_t*>(g.dw)[k] = (uint16_t)f_to_bf16_rne(sum);
-      else static_cast<float*>(g.dw)[k] = sum;
+      for (int w = 0; w < JOIN; ++w) sum = __fadd_rn(sum, red[w][threadIdx.x]);
+      write_sum<BF16>(g, far_row[b], mine, sum);
     }
     __syncthreads();
   }
@@ -373,20 +486,34 @@ int grad(const advopt_embedding_grad_args& a, cudaStream_t s) {
   g.scale = a.scale;
   g.passes = 1;
   while (a.vocab >> (g.passes * BITS)) ++g.passes;   // the keys are 0 .. vocab
-  const int64_t trip = SORT_THREADS * 16 * 4, zeros = ceil_div(a.vocab * a.width * (BF16 ? 2 : 4), trip);
-  const int64_t most = 2 * 148 - CLUSTER;
-  const int64_t fill = ceil_div(zeros < most ? zeros : most, CLUSTER) * CLUSTER;
-  cudaError_t e = cudaFuncSetAttribute(order_kernel<BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM);
-  if (e != cudaSuccess) return check_cuda(e, "advopt_embedding_grad");
-  order_kernel<BF16><<<(unsigned)(CLUSTER + fill), SORT_THREADS, SORT_SMEM, s>>>(g);
+  const int64_t bytes = a.vocab * a.width * (BF16 ? 2 : 4), zeros = ceil_div(bytes, FILL_THREADS * FILL * 16);
+  const char* where = "advopt_embedding_grad";
+  if (a.tokens == 0) {
+    zero_kernel<BF16><<<(unsigned)zeros, FILL_THREADS, 0, s>>>(a.dweight, bytes);
+    return check_cuda(cudaGetLastError(), where);
+  }
+  cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM);
+  if (e != cudaSuccess) return check_cuda(e, where);
+  order_kernel<<<CLUSTER, SORT_THREADS, SORT_SMEM, s>>>(g);
   e = cudaGetLastError();
-  if (e != cudaSuccess || a.tokens == 0) return check_cuda(e, "advopt_embedding_grad");
-  const int64_t chunks = ceil_div(a.tokens, CHUNK), slabs = ceil_div(a.width, 256);
-  const int vec = aligned16(a.dy) && aligned16(a.dweight) && a.width * (BF16 ? 2 : 4) % 16 == 0 && a.width % 8 == 0;
-  sums_kernel<BF16><<<(unsigned)ceil_div(chunks * slabs, 8), 256, 0, s>>>(g, (uint32_t)slabs, vec);
+  if (e != cudaSuccess) return check_cuda(e, where);
+  cudaLaunchAttribute beside;
+  beside.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  beside.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)zeros);
+  config.blockDim = dim3(FILL_THREADS);
+  config.stream = s;
+  config.attrs = &beside;
+  config.numAttrs = 1;
+  e = cudaLaunchKernelEx(&config, zero_kernel<BF16>, a.dweight, bytes);
+  if (e != cudaSuccess) return check_cuda(e, where);
+  const int64_t chunks = ceil_div(a.tokens, CHUNK), slabs = ceil_div(a.width, 32 * Cols<BF16>::E);
+  const int vec = aligned16(a.dy) && aligned16(a.dweight) && a.width % Cols<BF16>::E == 0;
+  sums_kernel<BF16><<<(unsigned)ceil_div(chunks * slabs, SUM_WARPS), SUM_WARPS * 32, 0, s>>>(g, (uint32_t)slabs, vec);
   if (chunks > 1) {
     const int64_t wide = ceil_div(a.width, 128);
-    join_kernel<BF16><<<(unsigned)(ceil_div(chunks, 32) * wide), JOIN_WARPS * 32, 0, s>>>(g, (uint32_t)wide);
+    join_kernel<BF16><<<(unsigned)(ceil_div(chunks, JOIN) * wide), JOIN * 32, 0, s>>>(g, (uint32_t)wide);
   }
   return check_cuda(cudaGetLastError(), "advopt_embedding_grad");
 }
@@ -433,8 +560,8 @@ extern "C" int advopt_embedding_grad(const advopt_embedding_grad_args* a, void* 
   if (!a->dweight || !aligned16(a->dweight) || (a->tokens && (!a->dy || !a->ids || !a->work || !aligned16(a->work))))
     return set_error(ADVOPT_E_INVALID, "advopt_embedding_grad: null or unaligned pointer");
   const int64_t chunks = ceil_div(a->tokens, emb::CHUNK);
-  if (chunks * ceil_div(a->width, 256) / 8 >= emb::LIMIT - 1 || ceil_div(chunks, 32) * ceil_div(a->width, 128) >= emb::LIMIT)
-    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_embedding_grad: too many tokens for this width");
+  if (a->vocab > ((int64_t)1 << 43) / a->width || chunks * ceil_div(a->width, 128) / emb::SUM_WARPS >= emb::LIMIT - 1)
+    return set_error(ADVOPT_E_UNSUPPORTED, "advopt_embedding_grad: too many tokens or rows for this width");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->dtype == ADVOPT_DT_BF16 ? emb::grad<true>(*a, s) : emb::grad<false>(*a, s);
 }
