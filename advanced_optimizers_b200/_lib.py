@@ -229,7 +229,7 @@ def lib():
             "advopt_col_sum": ([P, P, ctypes.c_int64, ctypes.c_int64, I32, P], ctypes.c_int),
             "advopt_fp8_gemm": ([P, P], ctypes.c_int),
             "advopt_embedding": ([P, P], ctypes.c_int),
-            "advopt_embedding_grad_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
+            "advopt_embedding_grad_work": ([ctypes.c_int64, ctypes.c_int64, I32], ctypes.c_int64),
             "advopt_embedding_grad": ([P, P], ctypes.c_int),
             "advopt_layer_norm": ([P, P], ctypes.c_int),
             "advopt_layer_norm_grad_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),

@@ -97,9 +97,9 @@ constexpr int CLUSTER = 8;             // CTAs that sort
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int BITS = 9, BINS = 1 << BITS;
+constexpr int AHEAD = 8;               // tokens of a lane whose loads are on their way
 constexpr int SORT_SMEM = (SORT_WARPS * BINS + 2 * BINS + SORT_WARPS) * 4;
 constexpr int FILL_THREADS = 512, FILL = 4;   // 16-byte stores of a thread that writes zeros
-constexpr uint32_t CHUNK = 32;         // tokens of one warp, so that a lane holds one token's id
 
 // One cluster sorts, beside the kernel that writes the zeros: the sort reads and
 // writes a few hundred KB that stay in L2, and takes less time than the zeros
@@ -109,6 +109,19 @@ constexpr uint32_t CHUNK = 32;         // tokens of one warp, so that a lane hol
 // the counts are summed over the digits, CTAs and warps before it, and the
 // warp walks its share again, in order, and places each token behind those of
 // its digit that came before.
+// The lanes of `live` with this lane's digit, bit by bit (65536 tokens of a
+// vocabulary of 50257: 36 us for the sort, with __match_any_sync 42).
+__device__ __forceinline__ uint32_t peers_of(uint32_t d, uint32_t live) {
+  uint32_t peers = live;
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const bool bit = (d >> b) & 1u;
+    const uint32_t v = __ballot_sync(0xffffffffu, bit);
+    peers &= bit ? v : ~v;
+  }
+  return peers;
+}
+
 __device__ __forceinline__ void sort_cluster(const Grad& g, uint32_t* sm) {
   cg::cluster_group cluster = cg::this_cluster();
   uint32_t* hist = sm;                                  // [SORT_WARPS][BINS]
@@ -132,15 +145,23 @@ __device__ __forceinline__ void sort_cluster(const Grad& g, uint32_t* sm) {
     const int shift = pass * BITS;
     for (int i = lane; i < BINS; i += 32) mine[i] = 0;
     __syncwarp();
-    for (uint32_t i = begin + lane; i - lane < end; i += 32) {
-      const uint32_t live = __ballot_sync(0xffffffffu, i < end);
-      if (i < end) {
-        const uint32_t key = pass ? from[i] : key_of(g.ids, g.wide, i, g.vocab, g.padding);
-        const uint32_t d = (key >> shift) & (BINS - 1);
-        const uint32_t peers = __match_any_sync(live, d);
-        if (lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    for (uint32_t i0 = begin; i0 < end; i0 += 32 * AHEAD) {
+      uint32_t key[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t i = i0 + k * 32 + lane;
+        key[k] = 0;
+        if (i < end) key[k] = pass ? from[i] : key_of(g.ids, g.wide, i, g.vocab, g.padding);
       }
-      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t i = i0 + k * 32 + lane;
+        const uint32_t live = __ballot_sync(0xffffffffu, i < end);
+        if (live == 0) break;
+        const uint32_t d = (key[k] >> shift) & (BINS - 1), peers = peers_of(d, live);
+        if (i < end && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (tid < BINS) {
@@ -173,19 +194,32 @@ __device__ __forceinline__ void sort_cluster(const Grad& g, uint32_t* sm) {
       base[tid] = upto - all + before;
     }
     __syncthreads();
-    for (uint32_t i = begin + lane; i - lane < end; i += 32) {
-      const uint32_t live = __ballot_sync(0xffffffffu, i < end);
-      if (i < end) {
-        const uint32_t key = pass ? from[i] : key_of(g.ids, g.wide, i, g.vocab, g.padding);
-        const uint32_t d = (key >> shift) & (BINS - 1);
-        const uint32_t peers = __match_any_sync(live, d);
-        const uint32_t place = base[d] + mine[d] + __popc(peers & ((1u << lane) - 1u));
-        to[place] = key;
-        to_at[place] = pass ? from_at[i] : i;
-        __syncwarp(live);
-        if (lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+    for (uint32_t i0 = begin; i0 < end; i0 += 32 * AHEAD) {
+      uint32_t key[AHEAD], from_place[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t i = i0 + k * 32 + lane;
+        key[k] = from_place[k] = 0;
+        if (i < end) {
+          key[k] = pass ? from[i] : key_of(g.ids, g.wide, i, g.vocab, g.padding);
+          from_place[k] = pass ? from_at[i] : i;
+        }
       }
-      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint32_t i = i0 + k * 32 + lane;
+        const uint32_t live = __ballot_sync(0xffffffffu, i < end);
+        if (live == 0) break;
+        const uint32_t d = (key[k] >> shift) & (BINS - 1), peers = peers_of(d, live);
+        if (i < end) {
+          const uint32_t place = base[d] + mine[d] + __popc(peers & ((1u << lane) - 1u));
+          to[place] = key[k];
+          to_at[place] = from_place[k];
+        }
+        __syncwarp();
+        if (i < end && lane == __ffs(peers) - 1) mine[d] += __popc(peers);
+        __syncwarp();
+      }
     }
     cluster.sync();   // the pass's tokens are in place for all CTAs, and `total` has been read
   }
@@ -289,7 +323,7 @@ constexpr int SUM_WARPS = 4;
 
 // A warp: the rows that begin among CHUNK tokens in order, for 16 bytes a lane.  A row that goes on into the next chunk, but fills neither, is
 // followed there; of one that does, each chunk's warp sums its own tokens.
-template <bool BF16>
+template <bool BF16, uint32_t CHUNK>
 __global__ void __launch_bounds__(SUM_WARPS * 32, 7) sums_kernel(const __grid_constant__ Grad g, uint32_t slabs, int vec) {
   const int lane = threadIdx.x & 31;
   const int64_t u = (int64_t)blockIdx.x * SUM_WARPS + (threadIdx.x >> 5);
@@ -302,11 +336,12 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 7) sums_kernel(const __grid_co
   const uint32_t* keys = g.keys[(g.passes + 1) & 1];
   const uint32_t* at = g.at[(g.passes + 1) & 1];
   const uint32_t mine = first + lane, next = mine + CHUNK;
-  const uint32_t key = mine < g.tokens ? keys[mine] : g.vocab, pos = mine < g.tokens ? at[mine] : 0u;
-  const uint32_t more = next < g.tokens ? keys[next] : g.vocab, more_pos = next < g.tokens ? at[next] : 0u;
+  const bool here = lane < CHUNK && mine < g.tokens, behind = lane < CHUNK && next < g.tokens;
+  const uint32_t key = here ? keys[mine] : g.vocab, pos = here ? at[mine] : 0u;
+  const uint32_t more = behind ? keys[next] : g.vocab, more_pos = behind ? at[next] : 0u;
   const uint32_t n = __popc(__ballot_sync(0xffffffffu, key < g.vocab));   // those that contribute come first
   if (n == 0) return;
-  const uint32_t head = __shfl_sync(0xffffffffu, key, 0), tail = __shfl_sync(0xffffffffu, key, 31);
+  const uint32_t head = __shfl_sync(0xffffffffu, key, 0), tail = __shfl_sync(0xffffffffu, key, CHUNK - 1);
   // the row that comes from the chunk before: long, or summed there
   const bool comes = first && keys[first - 1] == head;
   const bool long_ahead = comes && is_long(head, keys[first - CHUNK], tail);
@@ -314,7 +349,7 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 7) sums_kernel(const __grid_co
   if (comes && !long_ahead) begin = __popc(__ballot_sync(0xffffffffu, key == head));
   // the row that goes on into the next one
   const bool goes = n == CHUNK && __shfl_sync(0xffffffffu, more, 0) == tail;
-  const bool long_behind = goes && is_long(tail, head, __shfl_sync(0xffffffffu, more, 31));
+  const bool long_behind = goes && is_long(tail, head, __shfl_sync(0xffffffffu, more, CHUNK - 1));
   uint32_t end = n;
   if (goes && !long_behind && begin < n) end += __popc(__ballot_sync(0xffffffffu, more == tail));
   if (begin >= n) return;
@@ -328,13 +363,13 @@ __global__ void __launch_bounds__(SUM_WARPS * 32, 7) sums_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t j = i0 + i;
-      const uint32_t p0 = __shfl_sync(0xffffffffu, pos, j & 31), p1 = __shfl_sync(0xffffffffu, more_pos, j & 31);
+      const uint32_t p0 = __shfl_sync(0xffffffffu, pos, j & (CHUNK - 1)), p1 = __shfl_sync(0xffffffffu, more_pos, j & (CHUNK - 1));
       if (j < end) v[i].get(g.dy, (int64_t)(j < CHUNK ? p0 : p1) * g.width + c, nv, vec);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t j = i0 + i;
-      const uint32_t k0 = __shfl_sync(0xffffffffu, key, j & 31);
+      const uint32_t k0 = __shfl_sync(0xffffffffu, key, j & (CHUNK - 1));
       if (j >= end) break;
       const uint32_t k = j < CHUNK ? k0 : tail;
       if (k != cur) {
@@ -392,7 +427,7 @@ __device__ __forceinline__ void write_sum(const Grad& g, uint32_t row, int64_t c
   else static_cast<float*>(g.dw)[k] = sum;
 }
 
-template <bool BF16>
+template <bool BF16, uint32_t CHUNK>
 __global__ void __launch_bounds__(JOIN * 32) join_kernel(const __grid_constant__ Grad g, uint32_t slabs) {
   __shared__ float red[JOIN][128];
   __shared__ uint32_t far_row[JOIN], far_parts[JOIN];
@@ -460,15 +495,34 @@ __global__ void __launch_bounds__(JOIN * 32) join_kernel(const __grid_constant__
 struct Work {
   int64_t list, part, bytes;   // bytes of one of the four lists, where the partial sums begin, all
 };
-inline Work work_of(int64_t tokens, int64_t width) {
+// Chunks of 32 tokens, a lane's worth each, unless their warps are too few to
+// hide each other's loads (16 an SM): a quarter of the tokens then takes a
+// warp a quarter of the time (2048 x 2048 bf16: 7.5 + 5.9 us for the sums and
+// the join, with 32 tokens 15.1 + 3.9; 8192 x 4096: 25 + 17, with 32 25 + 7).
+inline int64_t chunk_of(int64_t tokens, int64_t width, int size) {
+  return ceil_div(tokens, 32) * ceil_div(width * size, 512) <= 148 * 16 ? 8 : 32;
+}
+inline Work work_of(int64_t tokens, int64_t width, int64_t chunk) {
   const int64_t list = (tokens * 4 + 15) / 16 * 16;
-  return {list, 4 * list, 4 * list + ceil_div(tokens, CHUNK) * 2 * width * 4};
+  return {list, 4 * list, 4 * list + ceil_div(tokens, chunk) * 2 * width * 4};
+}
+
+template <bool BF16, uint32_t CHUNK>
+void sums(const advopt_embedding_grad_args& a, const Grad& g, cudaStream_t s) {
+  const int64_t chunks = ceil_div(a.tokens, CHUNK), slabs = ceil_div(a.width, 32 * Cols<BF16>::E);
+  const int vec = aligned16(a.dy) && aligned16(a.dweight) && a.width % Cols<BF16>::E == 0;
+  sums_kernel<BF16, CHUNK><<<(unsigned)ceil_div(chunks * slabs, SUM_WARPS), SUM_WARPS * 32, 0, s>>>(g, (uint32_t)slabs, vec);
+  if (chunks > 1) {
+    const int64_t wide = ceil_div(a.width, 128);
+    join_kernel<BF16, CHUNK><<<(unsigned)(ceil_div(chunks, JOIN) * wide), JOIN * 32, 0, s>>>(g, (uint32_t)wide);
+  }
 }
 
 template <bool BF16>
 int grad(const advopt_embedding_grad_args& a, cudaStream_t s) {
   Grad g;
-  const Work w = work_of(a.tokens, a.width);
+  const int64_t chunk = chunk_of(a.tokens, a.width, BF16 ? 2 : 4);
+  const Work w = work_of(a.tokens, a.width, chunk);
   unsigned char* at = static_cast<unsigned char*>(a.work);
   g.dw = a.dweight;
   g.dy = a.dy;
@@ -508,14 +562,9 @@ int grad(const advopt_embedding_grad_args& a, cudaStream_t s) {
   config.numAttrs = 1;
   e = cudaLaunchKernelEx(&config, zero_kernel<BF16>, a.dweight, bytes);
   if (e != cudaSuccess) return check_cuda(e, where);
-  const int64_t chunks = ceil_div(a.tokens, CHUNK), slabs = ceil_div(a.width, 32 * Cols<BF16>::E);
-  const int vec = aligned16(a.dy) && aligned16(a.dweight) && a.width % Cols<BF16>::E == 0;
-  sums_kernel<BF16><<<(unsigned)ceil_div(chunks * slabs, SUM_WARPS), SUM_WARPS * 32, 0, s>>>(g, (uint32_t)slabs, vec);
-  if (chunks > 1) {
-    const int64_t wide = ceil_div(a.width, 128);
-    join_kernel<BF16><<<(unsigned)(ceil_div(chunks, JOIN) * wide), JOIN * 32, 0, s>>>(g, (uint32_t)wide);
-  }
-  return check_cuda(cudaGetLastError(), "advopt_embedding_grad");
+  if (chunk == 8) sums<BF16, 8>(a, g, s);
+  else sums<BF16, 32>(a, g, s);
+  return check_cuda(cudaGetLastError(), where);
 }
 
 template <bool BF16>
@@ -546,8 +595,8 @@ extern "C" int advopt_embedding(const advopt_embedding_args* a, void* stream) {
   return check_cuda(cudaGetLastError(), "advopt_embedding");
 }
 
-extern "C" int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width) {
-  return tokens <= 0 || width <= 0 ? 0 : emb::work_of(tokens, width).bytes;
+extern "C" int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width, int32_t dtype) {
+  return tokens <= 0 || width <= 0 ? 0 : emb::work_of(tokens, width, emb::chunk_of(tokens, width, bytes_of(dtype))).bytes;
 }
 
 extern "C" int advopt_embedding_grad(const advopt_embedding_grad_args* a, void* stream) {
@@ -559,7 +608,7 @@ extern "C" int advopt_embedding_grad(const advopt_embedding_grad_args* a, void* 
   if (a->vocab == 0 || a->width == 0) return ADVOPT_OK;
   if (!a->dweight || !aligned16(a->dweight) || (a->tokens && (!a->dy || !a->ids || !a->work || !aligned16(a->work))))
     return set_error(ADVOPT_E_INVALID, "advopt_embedding_grad: null or unaligned pointer");
-  const int64_t chunks = ceil_div(a->tokens, emb::CHUNK);
+  const int64_t chunks = ceil_div(a->tokens, 8);
   if (a->vocab > ((int64_t)1 << 43) / a->width || chunks * ceil_div(a->width, 128) / emb::SUM_WARPS >= emb::LIMIT - 1)
     return set_error(ADVOPT_E_UNSUPPORTED, "advopt_embedding_grad: too many tokens or rows for this width");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -33,8 +33,8 @@ def index_bytes(what, t):
 
 
 @functools.lru_cache(maxsize=1024)
-def _work_bytes(tokens, width):
-    return L.lib().advopt_embedding_grad_work(tokens, width)
+def _work_bytes(tokens, width, dtype):
+    return L.lib().advopt_embedding_grad_work(tokens, width, dtype)
 
 
 def _gather(ids, weight, scale):
@@ -58,7 +58,7 @@ def _backward(ctx, dy):
         dy = dy.clone()
     dw = dy.new_empty((V, C))
     T = ids.numel()
-    work = dy.new_empty(_work_bytes(T, C), dtype=torch.uint8)
+    work = dy.new_empty(_work_bytes(T, C, dtype_code(dy.dtype)), dtype=torch.uint8)
     with on_device(dy.device):
         rc = L.lib().advopt_embedding_grad(_GRAD.pack(
             dw.data_ptr(), dy.data_ptr(), ids.data_ptr(), work.data_ptr(), T, V, C, ctx.padding, dtype_code(dy.dtype), ids.element_size(),

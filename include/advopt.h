@@ -697,7 +697,7 @@ int advopt_embedding(const advopt_embedding_args* args, void* stream);
 /* dweight [vocab][width] = scale * sum of dy's rows whose token is the row's id,
  * in float32 in an order that the ids alone decide, one rounding; every row is
  * written.  Ids outside [0, vocab), and `padding` (-1: none), contribute
- * nothing.  `work`: advopt_embedding_grad_work(tokens, width) bytes, 16-byte
+ * nothing.  `work`: advopt_embedding_grad_work(tokens, width, dtype) bytes, 16-byte
  * aligned. */
 typedef struct advopt_embedding_grad_args {
   void* dweight;            /* contiguous, as dy                               */
@@ -713,7 +713,7 @@ typedef struct advopt_embedding_grad_args {
   float scale;
   int32_t pad;
 } advopt_embedding_grad_args;
-int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width);
+int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width, int32_t dtype);
 int advopt_embedding_grad(const advopt_embedding_grad_args* args, void* stream);
 
 /* ---- Layer norm ----
