@@ -145,9 +145,16 @@ def saved(t, what, dtype, shape, device):
     return t.contiguous()
 
 
+def empty_as(t):
+    """A new contiguous tensor of t's shape and dtype (`empty_like`, the cheapest of torch's calls, keeps other orders of dimensions too)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def rows_of(t):
     """(t, pitch) of a matrix whose rows the kernels may read as they lie; a copy where their elements are not consecutive or rows overlap."""
-    R, C = t.shape
-    if (C > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < C):
-        t = t.contiguous()
-    return t, t.stride(0) if R > 1 else C
+    if t.is_contiguous():
+        return t, t.shape[1]
+    (R, C), (pitch, one) = t.shape, t.stride()
+    if (C > 1 and one != 1) or (R > 1 and pitch < C):
+        return t.contiguous(), C
+    return t, pitch if R > 1 else C

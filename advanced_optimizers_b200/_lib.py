@@ -168,7 +168,7 @@ EMBEDDING_GRAD_ARGS_BYTES = 80
 LAYER_NORM_ARGS_BYTES = 80
 LAYER_NORM_GRAD_ARGS_BYTES = 104
 TOKEN_LOGPROBS_ARGS_BYTES = 104
-POLICY_LOSS_ARGS_BYTES = 176
+POLICY_LOSS_ARGS_BYTES = 184
 PREFERENCE_LOSS_ARGS_BYTES = 112
 
 _LIB = None

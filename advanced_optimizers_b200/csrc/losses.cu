@@ -125,8 +125,8 @@ __device__ __forceinline__ void policy_finish(const advopt_policy_loss_args& a, 
     const double tokens = t[3] > 0.0 ? t[3] : 1.0;
     share = 1.0 / (a.by_rows ? (t[4] > 0.0 ? t[4] : 1.0) : tokens);
     *a.loss = (float)(t[0] * share);
-    a.stats[0] = (float)(t[1] / tokens);
-    a.stats[1] = (float)(t[2] / tokens);
+    *a.kl = (float)(t[1] / tokens);
+    *a.clipped = (float)(t[2] / tokens);
   }
   __syncthreads();
   const float s = (float)share;
@@ -273,7 +273,7 @@ extern "C" int64_t advopt_policy_loss_work(int64_t rows, int64_t cols) {
 }
 
 extern "C" int advopt_policy_loss(const advopt_policy_loss_args* a, void* stream) {
-  if (!a || !loss::sizes_ok(a->rows, a->cols) || !a->loss || !a->stats || !(a->clip_low >= 0.0f && a->clip_low <= 1.0f) || !(a->clip_high >= 0.0f) ||
+  if (!a || !loss::sizes_ok(a->rows, a->cols) || !a->loss || !a->kl || !a->clipped || !(a->clip_low >= 0.0f && a->clip_low <= 1.0f) || !(a->clip_high >= 0.0f) ||
       !(a->kl_weight - a->kl_weight == 0.0f))
     return set_error(ADVOPT_E_INVALID, "advopt_policy_loss: bad arguments");
   if (!known_dtype(a->dtype)) return set_error(ADVOPT_E_UNSUPPORTED, "advopt_policy_loss: float32 and bfloat16 are supported");

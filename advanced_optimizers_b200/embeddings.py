@@ -37,35 +37,34 @@ def _work_bytes(tokens, width, dtype):
     return L.lib().advopt_embedding_grad_work(tokens, width, dtype)
 
 
-def _gather(ids, weight, scale):
+def _gather(ids, weight, scale, dtype):
     w, ld = rows_of(weight)
     V, C = weight.shape
-    y = weight.new_empty((*ids.shape, C))
+    y = weight.new_empty(*ids.shape, C)
     with on_device(weight.device):
         rc = L.lib().advopt_embedding(_FORWARD.pack(
-            y.data_ptr(), w.data_ptr(), ids.data_ptr(), INDEX_ERRORS.pointer(), ld, ids.numel(), V, C, dtype_code(weight.dtype),
-            ids.element_size(), scale, 0), raw_stream(weight.device))
+            y.data_ptr(), w.data_ptr(), ids.data_ptr(), INDEX_ERRORS.pointer(), ld, ids.numel(), V, C, dtype, ids.element_size(), scale, 0),
+            raw_stream(weight.device))
     if rc:
         L.check(rc, "advopt_embedding")
     return y
 
 
 def _backward(ctx, dy):
-    ids = saved(ctx.saved_tensors[0], "ids", ctx.id_dtype, ctx.id_shape, dy.device)
-    V, C = ctx.table
+    id_dtype, id_shape, V, C, scale, padding, dtype = ctx.call
+    dev = dy.device
+    ids = saved(ctx.saved_tensors[0], "ids", id_dtype, id_shape, dev)
     dy = dy.contiguous()
-    if dy.data_ptr() % dy.element_size():   # never of torch's own making
-        dy = dy.clone()
-    dw = dy.new_empty((V, C))
     T = ids.numel()
-    work = dy.new_empty(_work_bytes(T, C, dtype_code(dy.dtype)), dtype=torch.uint8)
-    with on_device(dy.device):
+    dw = dy.new_empty(V, C)
+    work = dy.new_empty(_work_bytes(T, C, dtype), dtype=torch.uint8)
+    with on_device(dev):
         rc = L.lib().advopt_embedding_grad(_GRAD.pack(
-            dw.data_ptr(), dy.data_ptr(), ids.data_ptr(), work.data_ptr(), T, V, C, ctx.padding, dtype_code(dy.dtype), ids.element_size(),
-            ctx.scale, 0), raw_stream(dy.device))
+            dw.data_ptr(), dy.data_ptr(), ids.data_ptr(), work.data_ptr(), T, V, C, padding, dtype, ids.element_size(), scale, 0),
+            raw_stream(dev))
     if rc:
         L.check(rc, "advopt_embedding_grad")
-    return None, dw, None, None
+    return dw, None
 
 
 _backward_once = once_differentiable(_backward)
@@ -73,10 +72,11 @@ _backward_once = once_differentiable(_backward)
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, scale, padding):
-        ctx.id_dtype, ctx.id_shape, ctx.table, ctx.scale, ctx.padding = ids.dtype, ids.shape, weight.shape, scale, padding
+    def forward(ctx, weight, call):   # a tuple: torch looks at every argument of its own
+        ids, scale, padding, dtype = call
+        ctx.call = ids.dtype, ids.shape, *weight.shape, scale, padding, dtype
         ctx.save_for_backward(ids)
-        return _gather(ids, weight, scale)
+        return _gather(ids, weight, scale, dtype)
 
     @staticmethod
     def backward(ctx, dy):
@@ -103,7 +103,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
     index_bytes("embedding: ids", ids)
     if not weight.is_cuda or ids.device != weight.device:
         raise NotImplementedError("embedding: ids and weight must live on one CUDA device (no CPU fallback)")
-    dtype_code(weight.dtype)
+    dtype = dtype_code(weight.dtype)
     V, C = weight.shape
     scale = float(scale)
     if not math.isfinite(scale):
@@ -119,5 +119,5 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
     if not ids.is_contiguous():
         ids = ids.contiguous()
     if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(ids, weight, scale, padding)
-    return _gather(ids, weight, scale)
+        return _Embedding.apply(weight, (ids, scale, padding, dtype))
+    return _gather(ids, weight, scale, dtype)

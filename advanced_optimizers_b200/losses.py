@@ -11,17 +11,21 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._device import dtype_code, on_device, raw_stream, refuse_tangents, rows_of, saved
+from ._device import dtype_code, empty_as, on_device, raw_stream, refuse_tangents, rows_of, saved
 from .embeddings import INDEX_ERRORS, index_bytes
 
 # advopt_token_logprobs_args, advopt_policy_loss_args, advopt_preference_loss_args
 _LOGPROBS = struct.Struct("<QQQQQqqqqqqiifi")
-_POLICY = struct.Struct("<QQQQQQQQQQqqqqqqqddfffiii")
+_POLICY = struct.Struct("<QQQQQQQQQQQqqqqqqqddfffiii")
 _PREFERENCE = struct.Struct("<QQQQQQQqqqqqffii")
 
 
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
+
+
+def _round_up(n, to):
+    return (n + to - 1) // to * to
 
 
 # ---- log-probabilities ----
@@ -46,7 +50,7 @@ def _logprobs_args(out, stats, logits, tokens, temperature, ignore, err):
 
 def _token_logprobs(logits, tokens, temperature, ignore, keep):
     out = logits.new_empty(tokens.shape, dtype=torch.float32)
-    stats = logits.new_empty((tokens.numel(), 2), dtype=torch.float32) if keep else None
+    stats = logits.new_empty(tokens.numel(), 2, dtype=torch.float32) if keep else None
     with on_device(logits.device):
         x, args = _logprobs_args(out, stats, logits, tokens, temperature, ignore, INDEX_ERRORS.pointer())
         rc = L.lib().advopt_token_logprobs(args, raw_stream(logits.device))
@@ -57,18 +61,20 @@ def _token_logprobs(logits, tokens, temperature, ignore, keep):
 
 def _logprobs_backward(ctx, dlp):
     logits, tokens, stats = ctx.saved_tensors
-    if logits.dtype is not ctx.x_dtype or logits.shape != ctx.x_shape or logits.device != dlp.device:
-        saved(logits, "logits", ctx.x_dtype, ctx.x_shape, dlp.device)   # raises
-    tokens = saved(tokens, "tokens", ctx.t_dtype, dlp.shape, dlp.device)
-    stats = saved(stats, "rows' statistics", torch.float32, (tokens.numel(), 2), dlp.device)
+    x_dtype, x_shape, t_dtype, temperature, ignore = ctx.call
+    dev = dlp.device
+    if logits.dtype is not x_dtype or logits.shape != x_shape or logits.device != dev:
+        saved(logits, "logits", x_dtype, x_shape, dev)   # raises
+    tokens = saved(tokens, "tokens", t_dtype, dlp.shape, dev)
+    stats = saved(stats, "rows' statistics", torch.float32, (tokens.numel(), 2), dev)
     dlp = dlp.contiguous()
-    dx = torch.empty(ctx.x_shape, dtype=ctx.x_dtype, device=dlp.device)
-    with on_device(dlp.device):
-        x, args = _logprobs_args(None, stats, logits, tokens, ctx.temperature, ctx.ignore, 0)
-        rc = L.lib().advopt_token_logprobs_grad(dx.data_ptr(), dlp.data_ptr(), args, raw_stream(dlp.device))
+    dx = empty_as(logits)
+    with on_device(dev):
+        x, args = _logprobs_args(None, stats, logits, tokens, temperature, ignore, 0)
+        rc = L.lib().advopt_token_logprobs_grad(dx.data_ptr(), dlp.data_ptr(), args, raw_stream(dev))
     if rc:
         L.check(rc, "advopt_token_logprobs_grad")
-    return dx, None, None, None
+    return dx, None
 
 
 _logprobs_backward_once = once_differentiable(_logprobs_backward)
@@ -76,9 +82,10 @@ _logprobs_backward_once = once_differentiable(_logprobs_backward)
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, temperature, ignore):
+    def forward(ctx, logits, call):   # a tuple: torch looks at every argument of its own
+        tokens, temperature, ignore = call
         out, stats = _token_logprobs(logits, tokens, temperature, ignore, True)
-        ctx.x_dtype, ctx.x_shape, ctx.t_dtype, ctx.temperature, ctx.ignore = logits.dtype, logits.shape, tokens.dtype, temperature, ignore
+        ctx.call = logits.dtype, logits.shape, tokens.dtype, temperature, ignore
         ctx.save_for_backward(logits, tokens, stats)
         return out
 
@@ -119,34 +126,45 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogprobs.apply(logits, tokens, temperature, int(ignore_index))
+        return _TokenLogprobs.apply(logits, (tokens, temperature, int(ignore_index)))
     return _token_logprobs(logits, tokens, temperature, int(ignore_index), False)[0]
 
 
 # ---- losses ----
-def _check_rows(what, logprobs, constants, mask):
+def _check_rows(what, logprobs, mask, **constants):
     """logprobs [rows, tokens] and what is compared with it: one shape, dtype and CUDA device, gradients to logprobs alone."""
-    if logprobs.dim() != 2:
-        raise ValueError(f"{what}: log-probabilities are [sequences, tokens], got {tuple(logprobs.shape)}")
-    if not logprobs.is_cuda or any(t is not None and t.device != logprobs.device for t in (*constants.values(), mask)):
-        raise NotImplementedError(f"{what}: tensors must live on one CUDA device (no CPU fallback)")
-    dtype_code(logprobs.dtype)
+    shape, dtype, dev = logprobs.shape, logprobs.dtype, logprobs.device
+    if len(shape) != 2:
+        raise ValueError(f"{what}: log-probabilities are [sequences, tokens], got {tuple(shape)}")
+    grad = torch.is_grad_enabled()
     for name, t in constants.items():
         if t is None:
             continue
-        if t.dtype != logprobs.dtype:
-            raise ValueError(f"{what}: {name} must have the log-probabilities' dtype {logprobs.dtype}, got {t.dtype}")
-        if t.shape != logprobs.shape and name != "advantages":
-            raise ValueError(f"{what}: {name} must have the log-probabilities' shape {tuple(logprobs.shape)}, got {tuple(t.shape)}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if t.device != dev:
+            break
+        if t.dtype is not dtype:
+            raise ValueError(f"{what}: {name} must have the log-probabilities' dtype {dtype}, got {t.dtype}")
+        if name != "advantages" and t.shape != shape:
+            raise ValueError(f"{what}: {name} must have the log-probabilities' shape {tuple(shape)}, got {tuple(t.shape)}")
+        if grad and t.requires_grad:
             raise ValueError(f"{what}: {name} is a constant of the loss: detach it")
-    if mask is not None and (mask.dtype != torch.bool or mask.shape != logprobs.shape):
-        raise ValueError(f"{what}: the mask is bool of the log-probabilities' shape {tuple(logprobs.shape)}, got {mask.dtype} {tuple(mask.shape)}")
+    else:
+        if logprobs.is_cuda and (mask is None or mask.device == dev):
+            dev = None
+    if dev is not None:
+        raise NotImplementedError(f"{what}: tensors must live on one CUDA device (no CPU fallback)")
+    if mask is not None and (mask.dtype is not torch.bool or mask.shape != shape):
+        raise ValueError(f"{what}: the mask is bool of the log-probabilities' shape {tuple(shape)}, got {mask.dtype} {tuple(mask.shape)}")
     refuse_tangents(what, logprobs, *constants.values())
+    return dtype_code(dtype)
 
 
 def _rows(t):
     return (None, 0) if t is None else rows_of(t)
+
+
+def _floats(like, n):
+    return like.new_empty(n) if like.dtype is torch.float32 else like.new_empty(n, dtype=torch.float32)
 
 
 class PolicyLoss(NamedTuple):
@@ -156,42 +174,47 @@ class PolicyLoss(NamedTuple):
 
 
 @functools.lru_cache(maxsize=1024)
-def _policy_work(rows, cols):
-    return L.lib().advopt_policy_loss_work(rows, cols)
+def _policy_layout(rows, cols, keep):
+    """Floats of the kept buffer {slope [rows][cols], scale [rows], work}, where its parts begin (bytes), and its size (floats)."""
+    slope = _round_up(rows * cols, 4) if keep else 0
+    scale = slope + _round_up(rows, 4)
+    return 4 * slope, 4 * scale, scale + L.lib().advopt_policy_loss_work(rows, cols) // 4
 
 
-def _policy(logprobs, old, advantages, mask, ref, clip, kl_weight, by_rows, keep):
+def _policy(logprobs, old, advantages, mask, ref, clip, kl_weight, by_rows, dtype, keep):
+    """(loss, kl, clip fraction, kept buffer): one buffer, since an allocation costs the host as much as a launch."""
     R, C = logprobs.shape
     p, ld_p = rows_of(logprobs)
     old, ld_old = rows_of(old)
     ref, ld_ref = _rows(ref)
     mask, ld_mask = _rows(mask)
     advantages, ld_adv = (advantages.contiguous(), -1) if advantages.dim() == 1 else rows_of(advantages)
-    new = lambda *shape, dtype=torch.float32: p.new_empty(shape, dtype=dtype)  # noqa: E731
-    loss, stats, scale = new(), new(2), new(R)
-    slope = new(R, C) if keep else None
-    work = new(_policy_work(R, C), dtype=torch.uint8)
+    loss, kl, clipped = _floats(p, ()), _floats(p, ()), _floats(p, ())
+    scale, work, size = _policy_layout(R, C, keep)
+    kept = _floats(p, size)
+    at = kept.data_ptr()
     with on_device(p.device):
         rc = L.lib().advopt_policy_loss(_POLICY.pack(
-            loss.data_ptr(), stats.data_ptr(), _ptr(slope), scale.data_ptr(), p.data_ptr(), old.data_ptr(), _ptr(ref), advantages.data_ptr(),
-            _ptr(mask), work.data_ptr(), ld_p, ld_old, ld_ref, ld_adv, ld_mask, R, C, math.log1p(clip[1]),
-            math.log1p(-clip[0]) if clip[0] < 1 else -math.inf, *clip, kl_weight, by_rows, dtype_code(p.dtype), 0), raw_stream(p.device))
+            loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), at if keep else 0, at + scale, p.data_ptr(), old.data_ptr(), _ptr(ref),
+            advantages.data_ptr(), _ptr(mask), at + work, ld_p, ld_old, ld_ref, ld_adv, ld_mask, R, C, math.log1p(clip[1]),
+            math.log1p(-clip[0]) if clip[0] < 1 else -math.inf, *clip, kl_weight, by_rows, dtype, 0), raw_stream(p.device))
     if rc:
         L.check(rc, "advopt_policy_loss")
-    return loss, stats, slope, scale
+    return loss, kl, clipped, kept
 
 
-def _policy_backward(ctx, dloss, _):
-    slope, scale = ctx.saved_tensors
-    (R, C), dev = ctx.x_shape, dloss.device
-    slope, scale = saved(slope, "slopes", torch.float32, (R, C), dev), saved(scale, "rows' weights", torch.float32, (R,), dev)
-    dx = torch.empty((R, C), dtype=ctx.x_dtype, device=dev)
+def _policy_backward(ctx, dloss):
+    R, C, x_dtype, dtype = ctx.call
+    dev = dloss.device
+    scale, _, size = _policy_layout(R, C, True)
+    kept = saved(ctx.saved_tensors[0], "slopes", torch.float32, (size,), dev)
+    dx = kept.new_empty(R, C) if dtype == 0 else kept.new_empty(R, C, dtype=x_dtype)
+    at = kept.data_ptr()
     with on_device(dev):
-        rc = L.lib().advopt_policy_loss_grad(dx.data_ptr(), dloss.data_ptr(), slope.data_ptr(), scale.data_ptr(), R, C,
-                                             dtype_code(ctx.x_dtype), raw_stream(dev))
+        rc = L.lib().advopt_policy_loss_grad(dx.data_ptr(), dloss.data_ptr(), at, at + scale, R, C, dtype, raw_stream(dev))
     if rc:
         L.check(rc, "advopt_policy_loss_grad")
-    return dx, *[None] * 7
+    return dx, None
 
 
 _policy_backward_once = once_differentiable(_policy_backward)
@@ -199,18 +222,15 @@ _policy_backward_once = once_differentiable(_policy_backward)
 
 class _Policy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logprobs, old, advantages, mask, ref, clip, kl_weight, by_rows):
-        loss, stats, slope, scale = _policy(logprobs, old, advantages, mask, ref, clip, kl_weight, by_rows, True)
-        ctx.x_shape, ctx.x_dtype = logprobs.shape, logprobs.dtype
-        ctx.save_for_backward(slope, scale)
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
+    def forward(ctx, logprobs, made):   # a tuple: torch looks at every argument of its own
+        loss, kept, ctx.call = made
+        ctx.save_for_backward(kept)
+        return loss
 
     @staticmethod
-    def backward(ctx, dloss, dstats):
+    def backward(ctx, dloss):
         # a second derivative is refused, without the wrapper's cost where none can be asked for
-        return _policy_backward_once(ctx, dloss, dstats) if torch.is_grad_enabled() else _policy_backward(ctx, dloss, dstats)
+        return _policy_backward_once(ctx, dloss) if torch.is_grad_enabled() else _policy_backward(ctx, dloss)
 
 
 def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, mask: torch.Tensor | None = None, *,
@@ -234,8 +254,9 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
     advantages must not require one), is 0 at masked and, but for the KL term,
     at clipped tokens, and repeats bit for bit.  Second and forward-mode
     derivatives are refused."""
-    _check_rows("policy_loss", logprobs, dict(old_logprobs=old_logprobs, ref_logprobs=ref_logprobs, advantages=advantages), mask)
-    if advantages.shape != logprobs.shape and advantages.shape != logprobs.shape[:1]:
+    dtype = _check_rows("policy_loss", logprobs, mask, old_logprobs=old_logprobs, ref_logprobs=ref_logprobs, advantages=advantages)
+    R, C = logprobs.shape
+    if advantages.shape != (R,) and advantages.shape != (R, C):
         raise ValueError(f"policy_loss: advantages are [sequences] or [sequences, tokens], got {tuple(advantages.shape)}")
     clip = tuple(map(float, clip))
     kl_weight = float(kl_weight)
@@ -247,12 +268,12 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
         raise ValueError("policy_loss: a KL term needs ref_logprobs")
     if average not in ("tokens", "sequences"):
         raise ValueError(f"policy_loss: average is 'tokens' or 'sequences', got {average!r}")
-    args = logprobs, old_logprobs, advantages, mask, ref_logprobs, clip, kl_weight, average == "sequences"
-    if torch.is_grad_enabled() and logprobs.requires_grad:
-        loss, stats = _Policy.apply(*args)
-    else:
-        loss, stats, _, _ = _policy(*args, False)
-    return PolicyLoss(loss, stats[0], stats[1])
+    keep = logprobs.requires_grad and torch.is_grad_enabled()
+    loss, kl, clipped, kept = _policy(logprobs, old_logprobs, advantages, mask, ref_logprobs, clip, kl_weight,
+                                      average == "sequences", dtype, keep)
+    if keep:
+        loss = _Policy.apply(logprobs, (loss, kept, (R, C, logprobs.dtype, dtype)))
+    return PolicyLoss(loss, kl, clipped)
 
 
 class PreferenceLoss(NamedTuple):
@@ -262,46 +283,49 @@ class PreferenceLoss(NamedTuple):
 
 
 @functools.lru_cache(maxsize=1024)
-def _preference_work(pairs, cols):
-    return L.lib().advopt_preference_loss_work(pairs, cols)
+def _preference_layout(rows, cols):
+    """Of the buffer {slope [rows], work}: where work begins (bytes), and its size (floats)."""
+    work = _round_up(rows, 4)
+    return 4 * work, work + L.lib().advopt_preference_loss_work(rows // 2, cols) // 4
 
 
-def _preference(logprobs, ref, mask, beta, smoothing, average, keep):
-    """(loss, rewards, slope, mask as it was read)."""
+def _preference(logprobs, ref, mask, beta, smoothing, average, dtype):
+    """(loss, rewards, kept buffer)"""
     R, C = logprobs.shape
     p, ld_p = rows_of(logprobs)
     ref, ld_ref = _rows(ref)
     mask, ld_mask = _rows(mask)
-    new = lambda *shape, dtype=torch.float32: p.new_empty(shape, dtype=dtype)  # noqa: E731
-    loss, rewards = new(), new(R)
-    slope = new(R) if keep else None
-    work = new(_preference_work(R // 2, C), dtype=torch.uint8)
+    loss, rewards = _floats(p, ()), _floats(p, R)
+    work, size = _preference_layout(R, C)
+    kept = _floats(p, size)
+    at = kept.data_ptr()
     with on_device(p.device):
         rc = L.lib().advopt_preference_loss(_PREFERENCE.pack(
-            loss.data_ptr(), rewards.data_ptr(), _ptr(slope), p.data_ptr(), _ptr(ref), _ptr(mask), work.data_ptr(), ld_p, ld_ref, ld_mask,
-            R // 2, C, beta, smoothing, average, dtype_code(p.dtype)), raw_stream(p.device))
+            loss.data_ptr(), rewards.data_ptr(), at, p.data_ptr(), _ptr(ref), _ptr(mask), at + work, ld_p, ld_ref, ld_mask, R // 2, C, beta,
+            smoothing, average, dtype), raw_stream(p.device))
     if rc:
         L.check(rc, "advopt_preference_loss")
-    return loss, rewards, slope
+    return loss, rewards, kept
 
 
-def _preference_backward(ctx, dloss, _):
-    slope, *rest = ctx.saved_tensors
-    (R, C), dev = ctx.x_shape, dloss.device
-    slope = saved(slope, "rows' slopes", torch.float32, (R,), dev)
+def _preference_backward(ctx, dloss):
+    R, C, x_dtype, dtype = ctx.call
+    dev = dloss.device
+    kept, *rest = ctx.saved_tensors
+    kept = saved(kept, "rows' slopes", torch.float32, (_preference_layout(R, C)[1],), dev)
     mask, ld_mask = None, 0
     if rest:
         mask = rest[0]
-        if mask.dtype is not torch.bool or mask.shape != ctx.x_shape or mask.device != dev:
-            saved(mask, "mask", torch.bool, ctx.x_shape, dev)   # raises
+        if mask.dtype is not torch.bool or mask.shape != (R, C) or mask.device != dev:
+            saved(mask, "mask", torch.bool, (R, C), dev)   # raises
         mask, ld_mask = rows_of(mask)
-    dx = torch.empty((R, C), dtype=ctx.x_dtype, device=dev)
+    dx = kept.new_empty(R, C) if dtype == 0 else kept.new_empty(R, C, dtype=x_dtype)
     with on_device(dev):
-        rc = L.lib().advopt_preference_loss_grad(dx.data_ptr(), dloss.data_ptr(), slope.data_ptr(), _ptr(mask), ld_mask, R // 2, C,
-                                                 dtype_code(ctx.x_dtype), raw_stream(dev))
+        rc = L.lib().advopt_preference_loss_grad(dx.data_ptr(), dloss.data_ptr(), kept.data_ptr(), _ptr(mask), ld_mask, R // 2, C, dtype,
+                                                 raw_stream(dev))
     if rc:
         L.check(rc, "advopt_preference_loss_grad")
-    return dx, *[None] * 5
+    return dx, None
 
 
 _preference_backward_once = once_differentiable(_preference_backward)
@@ -309,18 +333,18 @@ _preference_backward_once = once_differentiable(_preference_backward)
 
 class _Preference(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logprobs, ref, mask, beta, smoothing, average):
-        loss, rewards, slope = _preference(logprobs, ref, mask, beta, smoothing, average, True)
-        ctx.x_shape, ctx.x_dtype = logprobs.shape, logprobs.dtype
-        ctx.save_for_backward(slope, *([] if mask is None else [mask]))
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
+    def forward(ctx, logprobs, made):   # a tuple: torch looks at every argument of its own
+        loss, kept, mask, ctx.call = made
+        if mask is None:
+            ctx.save_for_backward(kept)
+        else:
+            ctx.save_for_backward(kept, mask)
+        return loss
 
     @staticmethod
-    def backward(ctx, dloss, drewards):
+    def backward(ctx, dloss):
         # a second derivative is refused, without the wrapper's cost where none can be asked for
-        return _preference_backward_once(ctx, dloss, drewards) if torch.is_grad_enabled() else _preference_backward(ctx, dloss, drewards)
+        return _preference_backward_once(ctx, dloss) if torch.is_grad_enabled() else _preference_backward(ctx, dloss)
 
 
 def preference_loss(logprobs: torch.Tensor, ref_logprobs: torch.Tensor | None = None, mask: torch.Tensor | None = None, *, beta: float = 0.1,
@@ -340,8 +364,8 @@ def preference_loss(logprobs: torch.Tensor, ref_logprobs: torch.Tensor | None = 
     a row's sum is float32 and float64, the loss and the rewards beta s are
     float32.  The gradient goes to `logprobs` alone, in their dtype, and
     repeats bit for bit.  Second and forward-mode derivatives are refused."""
-    _check_rows("preference_loss", logprobs, dict(ref_logprobs=ref_logprobs), mask)
-    R = logprobs.shape[0]
+    dtype = _check_rows("preference_loss", logprobs, mask, ref_logprobs=ref_logprobs)
+    R, C = logprobs.shape
     if R == 0 or R % 2:
         raise ValueError(f"preference_loss: an even number of rows, the chosen and then the rejected sequences, got {R}")
     beta, label_smoothing = float(beta), float(label_smoothing)
@@ -349,9 +373,8 @@ def preference_loss(logprobs: torch.Tensor, ref_logprobs: torch.Tensor | None = 
         raise ValueError(f"preference_loss: beta must be finite, got {beta}")
     if not 0 <= label_smoothing <= 1:
         raise ValueError(f"preference_loss: label_smoothing is between 0 and 1, got {label_smoothing}")
-    args = logprobs, ref_logprobs, mask, beta, label_smoothing, bool(average)
-    if torch.is_grad_enabled() and logprobs.requires_grad:
-        loss, rewards = _Preference.apply(*args)
-    else:
-        loss, rewards, _ = _preference(*args, False)
+    keep = logprobs.requires_grad and torch.is_grad_enabled()
+    loss, rewards, kept = _preference(logprobs, ref_logprobs, mask, beta, label_smoothing, bool(average), dtype)
+    if keep:
+        loss = _Preference.apply(logprobs, (loss, kept, mask, (R, C, logprobs.dtype, dtype)))
     return PreferenceLoss(loss, rewards[: R // 2], rewards[R // 2 :])

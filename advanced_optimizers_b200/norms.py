@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._device import dtype_code, on_device, raw_stream, refuse_tangents, rows_of, saved
+from ._device import dtype_code, empty_as, on_device, raw_stream, refuse_tangents, rows_of, saved
 
 # advopt_layer_norm_args, advopt_layer_norm_grad_args
 _FORWARD = struct.Struct("<QQQQQqqqfiii")
@@ -29,8 +29,8 @@ def _forward(x, weight, bias, eps, keep):
     """(y, {mean, rstd} of the rows if `keep`) of a matrix x."""
     R, C = x.shape
     x, ld = rows_of(x)
-    y = x.new_empty((R, C))
-    stats = x.new_empty((R, 2), dtype=torch.float32) if keep else None
+    y = empty_as(x)
+    stats = x.new_empty(R, 2, dtype=torch.float32) if keep else None
     affine = weight if weight is not None else bias
     with on_device(x.device):
         rc = L.lib().advopt_layer_norm(_FORWARD.pack(
@@ -44,21 +44,22 @@ def _forward(x, weight, bias, eps, keep):
 def _backward(ctx, dy):
     x, stats, *rest = ctx.saved_tensors
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dev, w_dtype = dy.device, ctx.w_dtype
     R, C = dy.shape
-    if x.dtype is not dy.dtype or x.shape != dy.shape or x.device != dy.device:
-        saved(x, "input", dy.dtype, dy.shape, dy.device)   # raises
+    if x.dtype is not dy.dtype or x.shape != dy.shape or x.device != dev:
+        saved(x, "input", dy.dtype, dy.shape, dev)   # raises
     x, ldx = rows_of(x)
     dy, lddy = rows_of(dy)
-    stats = saved(stats, "rows' statistics", torch.float32, (R, 2), dy.device)
-    weight = saved(rest[0], "weight", ctx.w_dtype, (C,), dy.device) if rest else None
-    dx = dy.new_empty((R, C)) if need_x else None
-    dw = dy.new_empty((C,), dtype=ctx.w_dtype) if need_w else None
-    db = dy.new_empty((C,), dtype=ctx.w_dtype) if need_b else None
+    stats = saved(stats, "rows' statistics", torch.float32, (R, 2), dev)
+    weight = saved(rest[0], "weight", w_dtype, (C,), dev) if rest else None
+    dx = empty_as(dy) if need_x else None
+    dw = dy.new_empty(C, dtype=w_dtype) if need_w else None
+    db = dy.new_empty(C, dtype=w_dtype) if need_b else None
     work = dy.new_empty(_work_bytes(R, C), dtype=torch.uint8) if need_w or need_b else None
-    with on_device(dy.device):
+    with on_device(dev):
         rc = L.lib().advopt_layer_norm_grad(_GRAD.pack(
             _ptr(dx), _ptr(dw), _ptr(db), dy.data_ptr(), x.data_ptr(), _ptr(weight), stats.data_ptr(), _ptr(work), lddy, ldx, R, C,
-            dtype_code(dy.dtype), dtype_code(ctx.w_dtype)), raw_stream(dy.device))
+            dtype_code(dy.dtype), dtype_code(w_dtype)), raw_stream(dev))
     if rc:
         L.check(rc, "advopt_layer_norm_grad")
     return dx, dw, db, None
@@ -97,13 +98,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if x.dim() < 1:
         raise ValueError("layer_norm: x has at least one dimension")
     C = x.shape[-1]
-    if not x.is_cuda or any(t is not None and t.device != x.device for t in (weight, bias)):
+    dev = x.device
+    if not x.is_cuda or (weight is not None and weight.device != dev) or (bias is not None and bias.device != dev):
         raise NotImplementedError("layer_norm: tensors must live on one CUDA device (no CPU fallback)")
     dtype_code(x.dtype)
     for t in (weight, bias):
         if t is not None:
             dtype_code(t.dtype)
-            if t.shape != (C,):
+            if t.dim() != 1 or t.shape[0] != C:
                 raise ValueError(f"layer_norm: weight and bias are [{C}], got {tuple(t.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"layer_norm: weight and bias share a dtype, got {weight.dtype} and {bias.dtype}")
@@ -119,7 +121,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         bias = bias.contiguous()
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, C)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (
+            bias is not None and bias.requires_grad)):
         y = _LayerNorm.apply(x2, weight, bias, eps)
     else:
         y = _forward(x2, weight, bias, eps, False)[0]

@@ -799,14 +799,16 @@ int advopt_token_logprobs_grad(void* dlogits, const float* dlogprobs, const advo
  * clip_high or 1 - clip_low) A : e^d A; q = ref - logprob, kl = e^q - q - 1 (0
  * without ref).  loss = mean of kl_weight kl - gain over the tokens (by_rows =
  * 0), or over the rows with a token of the means over their tokens (1).
- * stats receives {mean kl over the tokens, share of clipped tokens}; with no
- * token these and the loss are 0.  Values where the mask is 0 are not looked at.
+ * kl receives the mean kl over the tokens, clipped the share of clipped tokens;
+ * with no token these and the loss are 0.  Values where the mask is 0 are not
+ * looked at.
  * slope (or NULL, [rows][cols] contiguous float32) and scale ([rows] float32)
  * receive what advopt_policy_loss_grad needs.  `work`:
  * advopt_policy_loss_work(rows, cols) bytes, 16-byte aligned. */
 typedef struct advopt_policy_loss_args {
-  float* loss;              /* one value                                       */
-  float* stats;             /* [2]                                             */
+  float* loss;              /* one value, as kl and clipped                    */
+  float* kl;
+  float* clipped;
   float* slope;
   float* scale;
   const void* logprobs;     /* [rows][ld_...], elements of dtype               */

@@ -45,7 +45,7 @@ OK = {
                                    x_dtype=1, w_dtype=0),
     "advopt_token_logprobs": dict(out=4096, stats=0, logits=4096, tokens=4096, err=0, inner=4, ld_outer=0, ld_inner=8, rows=4, vocab=8, ignore=-100,
                                   dtype=1, token_bytes=8, temperature=1.0, pad=0),
-    "advopt_policy_loss": dict(loss=4096, stats=4096, slope=0, scale=4096, logprobs=4096, old=4096, ref=0, advantages=4096, mask=0, work=4096, ld_logprobs=8,
+    "advopt_policy_loss": dict(loss=4096, kl=4096, clipped=4096, slope=0, scale=4096, logprobs=4096, old=4096, ref=0, advantages=4096, mask=0, work=4096, ld_logprobs=8,
                                ld_old=8, ld_ref=0, ld_adv=-1, ld_mask=0, rows=4, cols=8, log_high=0.2, log_low=-0.2, clip_low=0.2, clip_high=0.2,
                                kl_weight=0.0, by_rows=0, dtype=0, pad=0),
     "advopt_preference_loss": dict(loss=4096, rewards=4096, slope=0, logprobs=4096, ref=0, mask=0, work=4096, ld_logprobs=8, ld_ref=0, ld_mask=0, pairs=2,
@@ -70,7 +70,7 @@ BAD = [
     ("advopt_token_logprobs", dict(inner=0)), ("advopt_token_logprobs", dict(token_bytes=3)), ("advopt_token_logprobs", dict(temperature=0.0)),
     ("advopt_token_logprobs", dict(temperature=NAN)), ("advopt_token_logprobs", dict(temperature=float("inf"))), ("advopt_token_logprobs", dict(dtype=9)),
     ("advopt_token_logprobs", dict(out=0)), ("advopt_token_logprobs", dict(logits=0)), ("advopt_token_logprobs", dict(stats=4100)),
-    ("advopt_policy_loss", dict(rows=-1)), ("advopt_policy_loss", dict(rows=BIG)), ("advopt_policy_loss", dict(loss=0)), ("advopt_policy_loss", dict(stats=0)),
+    ("advopt_policy_loss", dict(rows=-1)), ("advopt_policy_loss", dict(rows=BIG)), ("advopt_policy_loss", dict(loss=0)), ("advopt_policy_loss", dict(kl=0)), ("advopt_policy_loss", dict(clipped=0)),
     ("advopt_policy_loss", dict(scale=0)), ("advopt_policy_loss", dict(work=0)), ("advopt_policy_loss", dict(work=4104)),
     ("advopt_policy_loss", dict(ld_old=7)), ("advopt_policy_loss", dict(ld_adv=7)), ("advopt_policy_loss", dict(mask=4096, ld_mask=7)),
     ("advopt_policy_loss", dict(ref=4096, ld_ref=7)), ("advopt_policy_loss", dict(clip_low=1.5)), ("advopt_policy_loss", dict(clip_high=NAN)),
