@@ -21,38 +21,120 @@ namespace ln {
 
 constexpr int WARPS = 8;      // rows at a time of a CTA whose warps take a row each
 
-// Sums of N values over the warp or the CTA; every thread gets them.  `red` has
-// room for two rounds, so that one barrier a round is enough.
+// Sums of N values (1, 2 or 4) over the warp: lane l gets value l / (32 / N).
+// Two values are halved with one exchange, so that N cost little more than one.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  float a = v[0];
+  int o = 16;
+  if constexpr (N == 2) {
+    a = __fadd_rn(lane & 16 ? v[1] : v[0], __shfl_xor_sync(0xffffffffu, lane & 16 ? v[0] : v[1], 16));
+    o = 8;
+  }
+  if constexpr (N == 4) {
+    float h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      h[i] = __fadd_rn(lane & 16 ? v[2 + i] : v[i], __shfl_xor_sync(0xffffffffu, lane & 16 ? v[i] : v[2 + i], 16));
+    a = __fadd_rn(lane & 8 ? h[1] : h[0], __shfl_xor_sync(0xffffffffu, lane & 8 ? h[0] : h[1], 8));
+    o = 4;
+  }
+#pragma unroll
+  for (; o > 0; o >>= 1) a = __fadd_rn(a, __shfl_xor_sync(0xffffffffu, a, o));
+  return a;
+}
+
+// Sums of N values over the warp or the CTA (up to 16 warps); every thread gets
+// them.  `red` has room for two rounds, so that one barrier a round is enough;
+// what it holds for warps that are not there is 0 (clear_sums).
 template <bool WARP, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[32 * N], int& round) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float4 (*red)[4 * N], int& round) {
+  const float a = warp_sums<N>(v);
+  if constexpr (WARP) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if constexpr (!WARP) {
-    const int warps = blockDim.x >> 5;
-    float* r = red[round & 1];
-    ++round;
-    if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) r[(threadIdx.x >> 5) * N + i] = v[i];
-    }
+    for (int i = 0; i < N; ++i) v[i] = N == 1 ? a : __shfl_sync(0xffffffffu, a, i * (32 / N));
+  } else {
+    float4* r = red[round];
+    round ^= 1;
+    const int lane = threadIdx.x & 31;
+    if (lane % (32 / N) == 0) reinterpret_cast<float*>(r + lane / (32 / N) * 4)[threadIdx.x >> 5] = a;
     __syncthreads();
+    const bool many = blockDim.x > 256;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = 0.0f;
-    for (int w = 0; w < warps; ++w) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], r[w * N + i]);
+    for (int i = 0; i < N; ++i) {
+      const float4 q = r[i * 4], p = r[i * 4 + 1];
+      v[i] = __fadd_rn(__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w)), __fadd_rn(__fadd_rn(p.x, p.y), __fadd_rn(p.z, p.w)));
     }
+    if (many) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float4 q = r[i * 4 + 2], p = r[i * 4 + 3];
+        v[i] = __fadd_rn(v[i], __fadd_rn(__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w)), __fadd_rn(__fadd_rn(p.x, p.y), __fadd_rn(p.z, p.w))));
+      }
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void clear_sums(float4 (*red)[4 * N]) {
+  if (threadIdx.x < 2 * 4 * N) red[threadIdx.x / (4 * N)][threadIdx.x % (4 * N)] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __syncthreads();
+}
+
+// A thread's columns: NV vectors of 16 bytes of x, `width` threads' apart.
+template <bool BF16, int NV>
+__device__ __forceinline__ void columns(int cols, int width, int lane, int (&c)[NV], int (&nv)[NV]) {
+  constexpr int E = BF16 ? 8 : 4;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    c[v] = (v * width + lane) * E;
+    nv[v] = c[v] >= cols ? 0 : cols - c[v] < E ? cols - c[v] : E;
   }
 }
 
-template <int NV>
-__device__ __forceinline__ void columns(int64_t cols, int width, int lane, int64_t (&c)[NV], int (&nv)[NV]) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    c[v] = ((int64_t)v * width + lane) * 8;
-    nv[v] = c[v] >= cols ? 0 : cols - c[v] < 8 ? (int)(cols - c[v]) : 8;
+// E elements: those of x's 16 bytes, or the weights that belong to them.
+template <bool BF16, int E>
+struct Vals {
+  static constexpr int W = BF16 ? E / 2 : E;
+  uint32_t w[W];
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (BF16) return u2f((e & 1) ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
+    else return u2f(w[e]);
   }
-}
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(at(2 * i), at(2 * i + 1)); }
+  __device__ __forceinline__ void set(const float (&v)[E]) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (BF16) w[i] = bf16x2(v[2 * i], v[2 * i + 1]);
+      else w[i] = f2u(v[i]);
+    }
+  }
+  // `absent` where there are no weights; zeros behind the row's end
+  __device__ __forceinline__ void weights(const void* p, float absent, int c, int nv, bool vec) {
+    if (!p) {
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = absent;
+      set(v);
+      return;
+    }
+    if (vec && nv == E) {
+      const uint2* q = reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p) + (int64_t)c * (BF16 ? 2 : 4));
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) {
+        const uint2 u = __ldg(q + i);
+        w[2 * i] = u.x;
+        w[2 * i + 1] = u.y;
+      }
+      return;
+    }
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      v[e] = e >= nv ? 0.0f : BF16 ? bf16_to_f(__ldg(static_cast<const uint16_t*>(p) + c + e)) : __ldg(static_cast<const float*>(p) + c + e);
+    set(v);
+  }
+};
 
 // Eight weights, or `absent` where there are none.
 template <bool BW>
@@ -66,90 +148,84 @@ __device__ __forceinline__ void weights(Oct<BW>& w, const void* p, float absent,
 }
 
 // ---- rows on their way through shared memory ----
-// A thread copies the 16-byte granules that it will read itself, several rows
-// ahead, so that only its own copies have to be waited for.  Rows that do not
-// start on a 16-byte boundary (A false) are copied from the boundary before:
-// every granule holds an element of the row, and a thread's eight elements
-// then reach into the granule behind its own, which is the next lane's (the
-// last lane copies it too).
+// A thread copies the 16 bytes that it will read itself, several rows ahead, so
+// that only its own copies have to be waited for.  Rows that do not start on a
+// 16-byte boundary (A false) are copied from the boundary before: each 16
+// bytes hold an element of the row, and a thread's elements then reach into
+// the ones behind its own, which are the next lane's (the last lane copies
+// them too).
 template <bool BF16, int NV, bool A, int S>
 struct Rows {
-  static constexpr int G = BF16 ? 1 : 2;            // granules of eight elements
-  static constexpr int SIZE = BF16 ? 2 : 4;
-  uint4* slots;                                     // [S][NV][G][threads], then [S][NV][warps]
-  const unsigned char* base;
-  int64_t pitch;                                    // bytes
-  int64_t bytes;                                    // of a row
-  uint32_t first[NV];                               // this thread's first granules
+  static constexpr int E = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
+  using X = Vals<BF16, E>;
+  // Shared memory, 16 bytes each: [S][NV][threads], then [S][NV][warps].
+  uint4* own;                                       // this thread's, of stage 0
+  uint4* last;                                      // this warp's
+  const unsigned char* ahead;                       // the next row to be copied
+  const unsigned char* now;                         // and to be read (A false)
+  int64_t stride;                                   // bytes from a row to the one that follows here
+  uint32_t bytes;                                   // of a row
+  uint32_t at[NV];                                  // this thread's vectors, in bytes
+  int to, from;                                     // stages
 
   // 16-byte slots of a CTA
-  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * (G * threads + (A ? 0 : threads / 32)); }
-  __device__ __forceinline__ uint4* own(int s, int v, int g) const { return slots + ((s * NV + v) * G + g) * blockDim.x + threadIdx.x; }
-  __device__ __forceinline__ uint4* last(int s, int v) const {
-    return slots + S * NV * G * blockDim.x + (s * NV + v) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  }
-  __device__ __forceinline__ static void copy(uint4* to, const unsigned char* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
-  }
-  __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t cols, const int64_t (&c)[NV]) {
-    slots = smem;
-    base = static_cast<const unsigned char*>(p);
-    pitch = ld * SIZE;
-    bytes = cols * SIZE;
+  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * (threads + (A ? 0 : threads / 32)); }
+  __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t row, int64_t step, int cols, const int (&c)[NV]) {
+    own = smem + threadIdx.x;
+    last = smem + S * NV * blockDim.x + (threadIdx.x >> 5);
+    ahead = now = static_cast<const unsigned char*>(p) + row * ld * SIZE;
+    stride = step * ld * SIZE;
+    bytes = (uint32_t)cols * SIZE;
+    to = from = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) first[v] = (uint32_t)(c[v] / 8 * G);
+    for (int v = 0; v < NV; ++v) at[v] = (uint32_t)c[v] * SIZE;
   }
-  __device__ __forceinline__ uint32_t off(int64_t r) const { return A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(base + r * pitch) & 15u; }
-  __device__ __forceinline__ void issue(int64_t r, int s) const {
-    const uint32_t o = off(r);
-    const unsigned char* p = base + r * pitch - o;
-    const int64_t end = bytes + o;
+  __device__ __forceinline__ static void copy(uint4* slot, const unsigned char* p) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot)), "l"(p) : "memory");
+  }
+  // The next row, if it is there.
+  __device__ __forceinline__ void issue(bool there) {
+    if (there) {
+      const uint32_t o = A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(ahead) & 15u, end = bytes + o;
+      const unsigned char* p = ahead - o;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (at[v] < end) copy(own + (to * NV + v) * (int)blockDim.x, p + at[v]);
+        if (!A && (threadIdx.x & 31) == 31 && at[v] + 16 < end) copy(last + (to * NV + v) * (int)(blockDim.x >> 5), p + at[v] + 16);
+      }
+    }
+    ahead += stride;
+    to = to == S - 1 ? 0 : to + 1;
+  }
+  // The next row's elements, zeros behind its end in a vector that it ends in.  All lanes take part; the copies have been waited for.
+  __device__ __forceinline__ void get(X (&x)[NV], const int (&nv)[NV]) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      const uint4* slot = own + (from * NV + v) * (int)blockDim.x;
+      const uint4 q = *slot;
+      if (A) {
+        x[v].w[0] = q.x; x[v].w[1] = q.y; x[v].w[2] = q.z; x[v].w[3] = q.w;   // behind the row's end: anything
+      } else {
+        const uint4 n = (threadIdx.x & 31) == 31 ? last[(from * NV + v) * (int)(blockDim.x >> 5)] : slot[1];
+        const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(now) & 15u;
+        const bool by8 = o & 8, by4 = o & 4, by2 = o & 2;
+        const uint32_t s[6] = {by8 ? q.z : q.x, by8 ? q.w : q.y, by8 ? n.x : q.z, by8 ? n.y : q.w, by8 ? n.z : n.x, by8 ? n.w : n.y};
+        uint32_t t[5];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const int64_t at = (int64_t)(first[v] + g) * 16;
-        if (at < end) copy(own(s, v, g), p + at);
-      }
-      if (!A && (threadIdx.x & 31) == 31) {
-        const int64_t at = (int64_t)(first[v] + G) * 16;
-        if (at < end) copy(last(s, v), p + at);
-      }
-    }
-  }
-  // Row r's elements, zeros behind its end.  All lanes take part; the copies have been waited for.
-  __device__ __forceinline__ void get(Oct<BF16>& x, int64_t r, int s, int v, int nv) const {
-    uint4 q[G + 1];
+        for (int i = 0; i < 5; ++i) t[i] = by4 ? s[i + 1] : s[i];
 #pragma unroll
-    for (int g = 0; g < G; ++g) q[g] = *own(s, v, g);
-    if (A) {
+        for (int i = 0; i < 4; ++i) x[v].w[i] = BF16 && by2 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+        if (nv[v] < E) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        x.w[4 * g] = q[g].x; x.w[4 * g + 1] = q[g].y; x.w[4 * g + 2] = q[g].z; x.w[4 * g + 3] = q[g].w;
-      }
-    } else {
-      q[G] = (threadIdx.x & 31) == 31 ? *last(s, v) : *(own(s, v, 0) + 1);
-      const uint32_t o = off(r);
-      const bool by8 = o & 8, by4 = o & 4, by2 = o & 2;
-      uint32_t t[4 * G + 4];
-#pragma unroll
-      for (int g = 0; g <= G; ++g) {
-        t[4 * g] = q[g].x; t[4 * g + 1] = q[g].y; t[4 * g + 2] = q[g].z; t[4 * g + 3] = q[g].w;
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * G + 2; ++i) t[i] = by8 ? t[i + 2] : t[i];
-#pragma unroll
-      for (int i = 0; i < 4 * G + 1; ++i) t[i] = by4 ? t[i + 1] : t[i];
-#pragma unroll
-      for (int i = 0; i < 4 * G; ++i) x.w[i] = BF16 && by2 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
-    }
-    if (nv < 8) {
-#pragma unroll
-      for (int i = 0; i < Oct<BF16>::kWords; ++i) {
-        if (BF16) x.w[i] &= (2 * i < nv ? 0xFFFFu : 0u) | (2 * i + 1 < nv ? 0xFFFF0000u : 0u);
-        else x.w[i] = i < nv ? x.w[i] : 0u;
+          for (int i = 0; i < 4; ++i) {
+            if (BF16) x[v].w[i] &= (2 * i < nv[v] ? 0xFFFFu : 0u) | (2 * i + 1 < nv[v] ? 0xFFFF0000u : 0u);
+            else x[v].w[i] = i < nv[v] ? x[v].w[i] : 0u;
+          }
+        }
       }
     }
+    now += stride;
+    from = from == S - 1 ? 0 : from + 1;
   }
 };
 template <int N>
@@ -158,148 +234,166 @@ __device__ __forceinline__ void wait_copies() {
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// Eight elements at column c of an output row.  Where rows do not start on
-// 16-byte boundaries (A false), a lane stores the granule that its elements
-// begin in, with the lane before's last ones, and by itself only elements whose
-// granule no lane has whole.  All lanes take part.
+// A thread's 16 bytes at column c of an output row.  Where rows do not start on
+// 16-byte boundaries (A false), a lane stores the aligned 16 bytes that its
+// elements begin in, with the lane before's last ones, and by itself only
+// elements whose 16 bytes no lane has whole.  All lanes take part.
 template <bool BF16, bool A>
-__device__ __forceinline__ void put_row(const Oct<BF16>& x, void* row, int64_t c, int nv, int64_t cols) {
+__device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsigned char* row, int c, int nv, int cols) {
+  constexpr int SIZE = BF16 ? 2 : 4, E = 16 / SIZE;
+  unsigned char* p = row + c * SIZE;
   if (A) {
-    if (nv) x.store(row, c);
+    if (nv) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
     return;
   }
-  constexpr int SIZE = BF16 ? 2 : 4, PER = 16 / SIZE, W = Oct<BF16>::kWords;
-  unsigned char* p = static_cast<unsigned char*>(row) + c * SIZE;
-  const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+  if (o == 0 && nv == E) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
   const int k = (int)o / SIZE, lane = threadIdx.x & 31;
-  // words: the previous lane's last four, then this lane's
-  uint32_t t[4 + W];
+  const bool whole = lane > 0 && nv == E, next = lane < 31 && c + 2 * E <= cols;
+  if (o) {
+    uint32_t t[8];   // the previous lane's words, then this lane's
 #pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = __shfl_up_sync(0xffffffffu, x.w[W - 4 + i], 1);
-#pragma unroll
-  for (int i = 0; i < W; ++i) t[4 + i] = x.w[i];
-  const bool whole = lane > 0 && nv == 8, next = lane < 31 && c + 16 <= cols;
-  if (nv == 8) {
-    // the granules from p - o on: words of t from byte 16 - o on
-    const uint32_t back = (16u - o) & 15u;
-    uint32_t u[W + 2];
-    const bool by16 = o == 0, by8 = back & 8, by4 = back & 4, by2 = back & 2;
-#pragma unroll
-    for (int i = 0; i < W + 2; ++i) u[i] = by8 ? t[i + 2 < 4 + W ? i + 2 : 3 + W] : t[i];
-#pragma unroll
-    for (int i = 0; i < W + 1; ++i) u[i] = by4 ? u[i + 1] : u[i];
-    uint32_t g[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      g[i] = BF16 && by2 ? __funnelshift_r(u[i], u[i + 1], 16) : u[i];
-      if (by16) g[i] = x.w[i];
+    for (int i = 0; i < 4; ++i) {
+      t[i] = __shfl_up_sync(0xffffffffu, x.w[i], 1);
+      t[4 + i] = x.w[i];
     }
-    uint4* to = reinterpret_cast<uint4*>(p - o);
-    if (whole || by16) to[0] = make_uint4(g[0], g[1], g[2], g[3]);
-    if constexpr (!BF16) to[1] = make_uint4(g[W - 4], g[W - 3], g[W - 2], g[W - 1]);
-    if (by16) return;
-  }
-  // one by one: those of the first granule where it is not whole, those behind the last one where the next lane does not store them
+    const uint32_t back = 16u - o;
+    const bool by8 = back & 8, by4 = back & 4, by2 = back & 2;
+    uint32_t u[6], g[5];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool early = nv == 8 ? e < PER - k && !whole : e < 8 - k;
-    const bool late = e >= 8 - k && !next;
-    if (e < nv && (early || late)) {
-      if (BF16) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(x.w[(e >> 1) & (W - 1)] >> (16 * (e & 1)));
-      else reinterpret_cast<uint32_t*>(p)[e] = x.w[e & (W - 1)];
+    for (int i = 0; i < 6; ++i) u[i] = by8 ? t[i + 2] : t[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) g[i] = by4 ? u[i + 1] : u[i];
+    if (BF16 && by2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) g[i] = __funnelshift_r(g[i], g[i + 1], 16);
     }
+    if (whole) *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
   }
+  if (o ? whole && next : nv == E) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (e < nv && (e < E - k ? !whole || !o : !next)) {
+      if (BF16) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(x.w[(e >> 1) & 3] >> (16 * (e & 1)));
+      else reinterpret_cast<uint32_t*>(p)[e] = x.w[e & 3];
+    }
 }
 
 constexpr int FWD_STAGES = 4, GRAD_STAGES = 3;
+__host__ __device__ constexpr int grad_rows(bool bf16, bool warp) { return bf16 && !warp ? 2 : 1; }
 
-template <bool BX, bool BW, int NV, bool WARP, bool A>
-__global__ void __launch_bounds__(WARP ? WARPS * 32 : 512) forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
+template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
+__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 512 ? 2 : MAX_THREADS == 256 ? 4 : 1)
+    forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
+  constexpr bool WARP = MAX_THREADS == 32;
   extern __shared__ uint4 smem[];
-  __shared__ float red[2][32];
-  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  int64_t c[NV];
-  int nv[NV];
-  columns<NV>(a.cols, width, lane, c, nv);
-  constexpr int S = FWD_STAGES;
-  Rows<BX, NV, A, S> rows;
-  rows.init(smem, a.x, a.ldx, a.cols, c);
+  __shared__ float4 red[2][4];
+  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
+  int c[NV], nv[NV];
+  columns<BX, NV>(cols, width, lane, c, nv);
+  constexpr int S = FWD_STAGES, E = BX ? 8 : 4, P = E / 2;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : 1);
   int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  Rows<BX, NV, A, S> rows;
+  rows.init(smem, a.x, a.ldx, r, step, cols, c);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
-    if (r + s * step < a.rows) rows.issue(r + s * step, s);
+    rows.issue(r + s * step < a.rows);
     commit_copies();
   }
-  Oct<BW> w[NV], b[NV];
+  if (!WARP) clear_sums<1>(red);
+  Vals<BW, E> w[NV], b[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    weights(w[v], a.weight, 1.0f, c[v], nv[v], wvec);
-    weights(b[v], a.bias, 0.0f, c[v], nv[v], wvec);
+    w[v].weights(a.weight, 1.0f, c[v], nv[v], wvec);
+    b[v].weights(a.bias, 0.0f, c[v], nv[v], wvec);
   }
-  const float inv = __fdiv_rn(1.0f, (float)a.cols);
-  int round = 0, stage = 0;
-  for (; r < a.rows; r += step) {
+  const float inv = __fdiv_rn(1.0f, (float)cols);
+  unsigned char* to = static_cast<unsigned char*>(a.y) + r * cols * (BX ? 2 : 4);
+  int round = 0;
+  for (; r < a.rows; r += step, to += step * cols * (BX ? 2 : 4)) {
     wait_copies<S - 2>();
     if (!A) __syncwarp();   // the next lane's copies are read too
-    Oct<BX> x[NV];
+    float2 x[NV][P];
+    {
+      Vals<BX, E> raw[NV];
+      rows.get(raw, nv);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) rows.get(x[v], r, stage, v, nv[v]);
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < P; ++i) x[v][i] = raw[v].pair(i);
+    }
     if (!A) __syncwarp();
-    // into the stage that was read a row ago
-    const int free = stage == 0 ? S - 1 : stage - 1;
-    if (r + (S - 1) * step < a.rows) rows.issue(r + (S - 1) * step, free);
+    rows.issue(r + (S - 1) * step < a.rows);   // into the stage that was read a row ago
     commit_copies();
-    stage = stage == S - 1 ? 0 : stage + 1;
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
+      if (nv[v]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = add2(s, x[v].pair(i));   // zeros behind the row's end
+        for (int i = 0; i < P; ++i) s = add2(s, x[v][i]);
+      }
     float t[1] = {__fadd_rn(s.x, s.y)};
     row_sum<WARP, 1>(t, red, round);
     const float mean = __fmul_rn(t[0], inv);
     s = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+      if (nv[v] == E) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 d = add2(x[v].pair(i), splat2(-mean));
-        if (nv[v] == 8) {
+        for (int i = 0; i < P; ++i) {
+          const float2 d = add2(x[v][i], splat2(-mean));
           s = fma2(d, d, s);
-        } else {
+        }
+      } else if (!A) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float2 d = add2(x[v][i], splat2(-mean));
           if (2 * i < nv[v]) s.x = __fmaf_rn(d.x, d.x, s.x);
           if (2 * i + 1 < nv[v]) s.y = __fmaf_rn(d.y, d.y, s.y);
         }
       }
+    }
     t[0] = __fadd_rn(s.x, s.y);
     row_sum<WARP, 1>(t, red, round);
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(t[0], inv, a.eps)));
+    const float2 rstd2 = splat2(rstd), shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
     if (a.stats && lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
-    unsigned char* to = static_cast<unsigned char*>(a.y) + r * a.cols * (BX ? 2 : 4);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float y[8];
+      float y[E];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 h = mul2(add2(x[v].pair(i), splat2(-mean)), splat2(rstd));
-        h = fma2(h, w[v].pair(i), b[v].pair(i));
-        y[2 * i] = h.x;
-        y[2 * i + 1] = h.y;
+      for (int i = 0; i < P; ++i) {
+        const float2 h = fma2(x[v][i], rstd2, shift2), q = fma2(h, w[v].pair(i), b[v].pair(i));
+        y[2 * i] = q.x;
+        y[2 * i + 1] = q.y;
       }
-      Oct<BX> o;
+      Vals<BX, E> o;
       o.set(y);
-      put_row<BX, A>(o, to, c[v], nv[v], a.cols);
+      put_row<BX, A>(o, to, c[v], nv[v], cols);
     }
   }
+}
+
+// Sums over a CTA of 1024 threads.
+template <int N>
+__device__ __forceinline__ void wide_sum(float (&v)[N], float (*red)[32]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = warp_sum(v[i]);
+    if ((threadIdx.x & 31) == 0) red[i][threadIdx.x >> 5] = v[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(red[i][threadIdx.x & 31]);
+  __syncthreads();
 }
 
 // Rows that no CTA's registers hold: read three times.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int vec, int wvec) {
-  __shared__ float red[2][32];
+  __shared__ float red[1][32];
   const float inv = __fdiv_rn(1.0f, (float)a.cols);
-  int round = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     float t[1] = {0.0f};
     for (int64_t c = threadIdx.x * 8; c < a.cols; c += 8192) {
@@ -308,7 +402,7 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[0] = __fadd_rn(t[0], x.at(e));
     }
-    row_sum<false, 1>(t, red, round);
+    wide_sum<1>(t, red);
     const float mean = __fmul_rn(t[0], inv);
     t[0] = 0.0f;
     for (int64_t c = threadIdx.x * 8; c < a.cols; c += 8192) {
@@ -321,7 +415,7 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
         if (e < nv) t[0] = __fmaf_rn(d, d, t[0]);
       }
     }
-    row_sum<false, 1>(t, red, round);
+    wide_sum<1>(t, red);
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(t[0], inv, a.eps)));
     if (a.stats && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
     for (int64_t c = threadIdx.x * 8; c < a.cols; c += 8192) {
@@ -341,97 +435,132 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 }
 
 // ---- the gradients ----
-template <bool BX, bool BW, int NV, bool WARP, bool A>
-__global__ void __launch_bounds__(WARP ? WARPS * 32 : 512) grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
+// RI rows of a CTA (adjacent ones) share a round of sums.
+template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
+__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 256 ? 2 : 1)
+    grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
+  constexpr bool WARP = MAX_THREADS == 32;
+  constexpr int S = GRAD_STAGES, E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, WARP);
   extern __shared__ uint4 smem[];
-  __shared__ float red[2][64];
-  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  int64_t c[NV];
-  int nv[NV];
-  columns<NV>(a.cols, width, lane, c, nv);
+  __shared__ float4 red[2][8 * RI];
+  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
+  int c[NV], nv[NV];
+  columns<BX, NV>(cols, width, lane, c, nv);
   const bool sums = a.work != nullptr;
-  constexpr int S = GRAD_STAGES;
   using R = Rows<BX, NV, A, S>;
-  R xs, dys;
-  xs.init(smem, a.x, a.ldx, a.cols, c);
-  dys.init(smem + R::slots_of(blockDim.x), a.dy, a.lddy, a.cols, c);
-  const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : 1);
-  int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+  const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : RI);
+  int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x * RI;
+  R xs[RI], dys[RI];
+#pragma unroll
+  for (int q = 0; q < RI; ++q) {
+    xs[q].init(smem + 2 * q * R::slots_of(blockDim.x), a.x, a.ldx, r + q, step, cols, c);
+    dys[q].init(smem + (2 * q + 1) * R::slots_of(blockDim.x), a.dy, a.lddy, r + q, step, cols, c);
+  }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
-    if (r + s * step < a.rows) {
-      xs.issue(r + s * step, s);
-      dys.issue(r + s * step, s);
+#pragma unroll
+    for (int q = 0; q < RI; ++q) {
+      const bool there = r + s * step + q < a.rows;
+      xs[q].issue(there);
+      dys[q].issue(there);
     }
     commit_copies();
   }
-  Oct<BW> w[NV];
+  if (!WARP) clear_sums<2 * RI>(red);
+  Vals<BW, E> w[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) weights(w[v], a.weight, 1.0f, c[v], nv[v], wvec);
-  float2 dw[NV][4], db[NV][4];
+  for (int v = 0; v < NV; ++v) w[v].weights(a.weight, 1.0f, c[v], nv[v], wvec);
+  float2 dw[NV][P], db[NV][P];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dw[v][i] = db[v][i] = make_float2(0.0f, 0.0f);
-  const float inv = __fdiv_rn(1.0f, (float)a.cols);
-  int round = 0, stage = 0;
-  for (; r < a.rows; r += step) {
-    const float2 st = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * r));
+    for (int i = 0; i < P; ++i) dw[v][i] = db[v][i] = make_float2(0.0f, 0.0f);
+  const float inv = __fdiv_rn(1.0f, (float)cols);
+  const int64_t row_bytes = (int64_t)cols * (BX ? 2 : 4);
+  unsigned char* to = static_cast<unsigned char*>(a.dx) + r * row_bytes;
+  int round = 0;
+  for (; r < a.rows; r += step, to += step * row_bytes) {
+    float2 st[RI];
+    bool here[RI];
+#pragma unroll
+    for (int q = 0; q < RI; ++q) {
+      here[q] = q == 0 || r + q < a.rows;
+      if (here[q]) st[q] = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + q)));
+    }
     wait_copies<S - 2>();
     if (!A) __syncwarp();   // the next lane's copies are read too
-    Oct<BX> x[NV], dy[NV];
+    Vals<BX, E> x[RI][NV], dy[RI][NV];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      xs.get(x[v], r, stage, v, nv[v]);
-      dys.get(dy[v], r, stage, v, nv[v]);
+    for (int q = 0; q < RI; ++q) {
+      xs[q].get(x[q], nv);
+      dys[q].get(dy[q], nv);
     }
     if (!A) __syncwarp();
-    // into the stage that was read a row ago
-    const int free = stage == 0 ? S - 1 : stage - 1;
-    if (r + (S - 1) * step < a.rows) {
-      xs.issue(r + (S - 1) * step, free);
-      dys.issue(r + (S - 1) * step, free);
+    // into the stage that was read a round ago
+#pragma unroll
+    for (int q = 0; q < RI; ++q) {
+      const bool there = r + (S - 1) * step + q < a.rows;
+      xs[q].issue(there);
+      dys[q].issue(there);
     }
     commit_copies();
-    stage = stage == S - 1 ? 0 : stage + 1;
-    const float mean = st.x, rstd = st.y;
-    float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+    float t[2 * RI];
+    float2 rstd2[RI];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
+    for (int q = 0; q < RI; ++q) {
+      float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
+      const float mean = st[q].x, rstd = st[q].y;
+      rstd2[q] = splat2(rstd);
+      const float2 shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
+      if (here[q]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 h = mul2(add2(x[v].pair(i), splat2(-mean)), splat2(rstd)), d = dy[v].pair(i);
-        const float2 g = mul2(d, w[v].pair(i));
-        s1 = add2(s1, g);   // dy is 0 behind the row's end; h, of a mean that may be infinite, is left out there
-        if (nv[v] == 8) {
-          s2 = fma2(g, h, s2);
-          dw[v][i] = fma2(d, h, dw[v][i]);
-        } else {
-          if (2 * i < nv[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
-          if (2 * i + 1 < nv[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
+        for (int v = 0; v < NV; ++v) {
+          if (nv[v] == E) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
+              s1 = add2(s1, g);
+              s2 = fma2(g, h, s2);
+              dw[v][i] = fma2(d, h, dw[v][i]);
+              db[v][i] = add2(db[v][i], d);
+            }
+          } else if (!A) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+              const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
+              s1 = add2(s1, g);   // dy is 0 behind the row's end; h, of a mean that may be infinite, is left out there
+              if (2 * i < nv[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
+              if (2 * i + 1 < nv[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
+              db[v][i] = add2(db[v][i], d);
+            }
+          }
         }
-        db[v][i] = add2(db[v][i], d);
       }
+      t[2 * q] = __fadd_rn(s1.x, s1.y);
+      t[2 * q + 1] = __fadd_rn(s2.x, s2.y);
     }
     if (!a.dx) continue;
-    float t[2] = {__fadd_rn(s1.x, s1.y), __fadd_rn(s2.x, s2.y)};
-    row_sum<WARP, 2>(t, red, round);
-    const float m1 = __fmul_rn(t[0], inv), m2 = __fmul_rn(t[1], inv);
-    unsigned char* to = static_cast<unsigned char*>(a.dx) + r * a.cols * (BX ? 2 : 4);
+    row_sum<WARP, 2 * RI>(t, red, round);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      float o[8];
+    for (int q = 0; q < RI; ++q) {
+      if (!here[q]) continue;
+      // dx = rstd g - rstd m2 h - rstd m1, with h = x rstd - mean rstd
+      const float mean = st[q].x, rstd = st[q].y, m1 = __fmul_rn(t[2 * q], inv), m2 = __fmul_rn(t[2 * q + 1], inv);
+      const float slope = -__fmul_rn(__fmul_rn(rstd, rstd), m2);
+      const float2 slope2 = splat2(slope), rest2 = splat2(-__fmaf_rn(rstd, m1, __fmul_rn(slope, mean)));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 h = mul2(add2(x[v].pair(i), splat2(-mean)), splat2(rstd)), d = dy[v].pair(i);
-        const float2 g = mul2(d, w[v].pair(i));
-        const float2 q = mul2(fma2(h, splat2(-m2), add2(g, splat2(-m1))), splat2(rstd));
-        o[2 * i] = q.x;
-        o[2 * i + 1] = q.y;
+      for (int v = 0; v < NV; ++v) {
+        float o[E];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float2 g = mul2(dy[q][v].pair(i), w[v].pair(i)), p = fma2(g, rstd2[q], fma2(x[q][v].pair(i), slope2, rest2));
+          o[2 * i] = p.x;
+          o[2 * i + 1] = p.y;
+        }
+        Vals<BX, E> out;
+        out.set(o);
+        put_row<BX, A>(out, to + q * row_bytes, c[v], nv[v], cols);
       }
-      Oct<BX> oct;
-      oct.set(o);
-      put_row<BX, A>(oct, to, c[v], nv[v], a.cols);
     }
   }
   if (!sums) return;
@@ -440,43 +569,47 @@ __global__ void __launch_bounds__(WARP ? WARPS * 32 : 512) grad_kernel(const __g
     // the warps' sums, a warp's after the other's, in shared memory
     wait_copies<0>();
     __syncthreads();
-    float* sh = reinterpret_cast<float*>(smem);   // [2][NV * 256]
+    float* sh = reinterpret_cast<float*>(smem);   // [2][NV * 32 * E]
     for (int k = 0; k < WARPS; ++k) {
       if ((int)(threadIdx.x >> 5) == k) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float* p = sh + c[v] + e;
-            const float x0 = e & 1 ? dw[v][e >> 1].y : dw[v][e >> 1].x, x1 = e & 1 ? db[v][e >> 1].y : db[v][e >> 1].x;
-            p[0] = k ? __fadd_rn(p[0], x0) : x0;
-            p[NV * 256] = k ? __fadd_rn(p[NV * 256], x1) : x1;
+          for (int i = 0; i < P; ++i) {
+            float2* p = reinterpret_cast<float2*>(sh + c[v]) + i;
+            float2* q = reinterpret_cast<float2*>(sh + NV * 32 * E + c[v]) + i;
+            *p = k ? add2(*p, dw[v][i]) : dw[v][i];
+            *q = k ? add2(*q, db[v][i]) : db[v][i];
           }
       }
       __syncthreads();
     }
-    for (int64_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
+    for (int i = threadIdx.x; i < cols; i += blockDim.x) {
       part[i] = sh[i];
-      part[a.cols + i] = sh[NV * 256 + i];
+      part[cols + i] = sh[NV * 32 * E + i];
     }
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < nv[v]) {
-          part[c[v] + e] = e & 1 ? dw[v][e >> 1].y : dw[v][e >> 1].x;
-          part[a.cols + c[v] + e] = e & 1 ? db[v][e >> 1].y : db[v][e >> 1].x;
+      for (int i = 0; i < P; ++i) {
+        float* p = part + c[v] + 2 * i;
+        if (2 * i + 1 < nv[v] && (cols & 1) == 0) {
+          *reinterpret_cast<float2*>(p) = dw[v][i];
+          *reinterpret_cast<float2*>(p + cols) = db[v][i];
+        } else {
+          if (2 * i < nv[v]) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
+          if (2 * i + 1 < nv[v]) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
         }
+      }
   }
 }
 
 // Rows that no CTA's registers hold: dx from two reads of a row, dw and db by columns.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_dx_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int vec, int wvec) {
-  __shared__ float red[2][64];
+  __shared__ float red[2][32];
   const float inv = __fdiv_rn(1.0f, (float)a.cols);
-  int round = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const float mean = __ldg(a.stats + 2 * r), rstd = __ldg(a.stats + 2 * r + 1);
     float t[2] = {0.0f, 0.0f};
@@ -495,7 +628,7 @@ __global__ void __launch_bounds__(1024) wide_dx_kernel(const __grid_constant__ a
         t[1] = __fmaf_rn(g, __fmul_rn(__fsub_rn(x.at(e), mean), rstd), t[1]);
       }
     }
-    row_sum<false, 2>(t, red, round);
+    wide_sum<2>(t, red);
     const float m1 = __fmul_rn(t[0], inv), m2 = __fmul_rn(t[1], inv);
     for (int64_t c = threadIdx.x * 8; c < a.cols; c += 8192) {
       const int nv = a.cols - c < 8 ? (int)(a.cols - c) : 8;
@@ -613,12 +746,13 @@ int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, cuda
   return grid;
 }
 
-template <bool BX, bool BW, int NV, bool WARP>
+template <bool BX, bool BW, int NV, int MAX_THREADS>
 int64_t forward_variant(const advopt_layer_norm_args& a, bool vec, int wvec, cudaStream_t s) {
+  constexpr bool WARP = MAX_THREADS == 32;
   const int threads = WARP ? WARPS * 32 : block_threads(a.cols);
   const int64_t most = WARP ? ceil_div(a.rows, WARPS) : a.rows;
-  if (vec) return launch<forward_kernel<BX, BW, NV, WARP, true>>(a, wvec, threads, Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16, most, s);
-  return launch<forward_kernel<BX, BW, NV, WARP, false>>(a, wvec, threads, Rows<BX, NV, false, FWD_STAGES>::slots_of(threads) * 16, most, s);
+  if (vec) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16, most, s);
+  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, Rows<BX, NV, false, FWD_STAGES>::slots_of(threads) * 16, most, s);
 }
 
 template <bool BX, bool BW>
@@ -627,20 +761,22 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   const int wvec = aligned16(a.weight) && aligned16(a.bias);
   int64_t n = 1;
   if (a.cols > MOST) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-  else if (a.cols <= 256) n = forward_variant<BX, BW, 1, true>(a, vec, wvec, s);
-  else if (a.cols <= 512) n = forward_variant<BX, BW, 2, true>(a, vec, wvec, s);
-  else if (a.cols <= WARP_MOST) n = forward_variant<BX, BW, 4, true>(a, vec, wvec, s);
-  else n = forward_variant<BX, BW, 2, false>(a, vec, wvec, s);
+  else if (a.cols <= 256) n = forward_variant<BX, BW, BX ? 1 : 2, 32>(a, vec, wvec, s);
+  else if (a.cols <= 512) n = forward_variant<BX, BW, BX ? 2 : 4, 32>(a, vec, wvec, s);
+  else if (a.cols <= WARP_MOST) n = forward_variant<BX, BW, BX ? 4 : 8, 32>(a, vec, wvec, s);
+  else if (a.cols <= 4096) n = forward_variant<BX, BW, BX ? 2 : 4, 256>(a, vec, wvec, s);
+  else n = forward_variant<BX, BW, BX ? 2 : 4, 512>(a, vec, wvec, s);
   const cudaError_t e = cudaGetLastError();
   return n < 0 ? set_error(ADVOPT_E_CUDA, "advopt_layer_norm: the kernel's attributes") : check_cuda(e, "advopt_layer_norm");
 }
 
-template <bool BX, bool BW, int NV, bool WARP>
+template <bool BX, bool BW, int NV, int MAX_THREADS>
 int64_t grad_variant(const advopt_layer_norm_grad_args& a, bool vec, int wvec, cudaStream_t s) {
-  const int threads = WARP ? WARPS * 32 : block_threads(a.cols);
+  const int threads = MAX_THREADS == 32 ? WARPS * 32 : block_threads(a.cols);
   const int64_t most = grad_ctas(a.rows, a.cols);
-  if (vec) return launch<grad_kernel<BX, BW, NV, WARP, true>>(a, wvec, threads, 2 * Rows<BX, NV, true, GRAD_STAGES>::slots_of(threads) * 16, most, s);
-  return launch<grad_kernel<BX, BW, NV, WARP, false>>(a, wvec, threads, 2 * Rows<BX, NV, false, GRAD_STAGES>::slots_of(threads) * 16, most, s);
+  constexpr int arrays = 2 * grad_rows(BX, MAX_THREADS == 32);
+  if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, arrays * Rows<BX, NV, true, GRAD_STAGES>::slots_of(threads) * 16, most, s);
+  return launch<grad_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, arrays * Rows<BX, NV, false, GRAD_STAGES>::slots_of(threads) * 16, most, s);
 }
 
 template <bool BX, bool BW>
@@ -654,13 +790,15 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
     if (a.dx) wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
     if (a.work) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
   } else if (a.cols <= 256) {
-    parts = grad_variant<BX, BW, 1, true>(a, vec, wvec, s);
+    parts = grad_variant<BX, BW, BX ? 1 : 2, 32>(a, vec, wvec, s);
   } else if (a.cols <= 512) {
-    parts = grad_variant<BX, BW, 2, true>(a, vec, wvec, s);
+    parts = grad_variant<BX, BW, BX ? 2 : 4, 32>(a, vec, wvec, s);
   } else if (a.cols <= WARP_MOST) {
-    parts = grad_variant<BX, BW, 4, true>(a, vec, wvec, s);
+    parts = grad_variant<BX, BW, BX ? 4 : 8, 32>(a, vec, wvec, s);
+  } else if (a.cols <= 4096) {
+    parts = grad_variant<BX, BW, BX ? 2 : 4, 256>(a, vec, wvec, s);
   } else {
-    parts = grad_variant<BX, BW, 2, false>(a, vec, wvec, s);
+    parts = grad_variant<BX, BW, BX ? 2 : 4, 512>(a, vec, wvec, s);
   }
   if (parts > 0 && a.work)
     finish_kernel<BW><<<dim3((unsigned)ceil_div(a.cols, 32), 2), FINISH_WARPS * 32, 0, s>>>(a.dweight, a.dbias, static_cast<const float*>(a.work),
