@@ -167,7 +167,7 @@ EMBEDDING_ARGS_BYTES = 80
 EMBEDDING_GRAD_ARGS_BYTES = 80
 LAYER_NORM_ARGS_BYTES = 80
 LAYER_NORM_GRAD_ARGS_BYTES = 104
-TOKEN_LOGPROBS_ARGS_BYTES = 104
+TOKEN_LOGPROBS_ARGS_BYTES = 112
 POLICY_LOSS_ARGS_BYTES = 184
 PREFERENCE_LOSS_ARGS_BYTES = 112
 
@@ -234,6 +234,7 @@ def lib():
             "advopt_layer_norm": ([P, P], ctypes.c_int),
             "advopt_layer_norm_grad_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
             "advopt_layer_norm_grad": ([P, P], ctypes.c_int),
+            "advopt_token_logprobs_work": ([ctypes.c_int64, ctypes.c_int64, I32], ctypes.c_int64),
             "advopt_token_logprobs": ([P, P], ctypes.c_int),
             "advopt_token_logprobs_grad": ([P, P, P, P], ctypes.c_int),
             "advopt_policy_loss_work": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_int64),
@@ -283,7 +284,7 @@ def exported_symbols():
             "advopt_enable_peer", "advopt_copy_async", "advopt_spectral_step", "advopt_dropout",
             "advopt_fp8_quantize", "advopt_col_sum", "advopt_fp8_gemm", "advopt_embedding", "advopt_embedding_grad_work",
             "advopt_embedding_grad", "advopt_layer_norm", "advopt_layer_norm_grad_work", "advopt_layer_norm_grad",
-            "advopt_token_logprobs", "advopt_token_logprobs_grad", "advopt_policy_loss_work", "advopt_policy_loss",
+            "advopt_token_logprobs_work", "advopt_token_logprobs", "advopt_token_logprobs_grad", "advopt_policy_loss_work", "advopt_policy_loss",
             "advopt_policy_loss_grad", "advopt_preference_loss_work", "advopt_preference_loss",
             "advopt_preference_loss_grad"]
 

@@ -15,7 +15,7 @@ from ._device import dtype_code, empty_as, on_device, raw_stream, refuse_tangent
 from .embeddings import INDEX_ERRORS, index_bytes
 
 # advopt_token_logprobs_args, advopt_policy_loss_args, advopt_preference_loss_args
-_LOGPROBS = struct.Struct("<QQQQQqqqqqqiifi")
+_LOGPROBS = struct.Struct("<QQQQQQqqqqqqiifi")
 _POLICY = struct.Struct("<QQQQQQQQQQQqqqqqqqddfffiii")
 _PREFERENCE = struct.Struct("<QQQQQQQqqqqqffii")
 
@@ -41,18 +41,27 @@ def _strided(logits):
     return logits, max(1, logits.shape[1]), logits.stride(0), logits.stride(1)
 
 
-def _logprobs_args(out, stats, logits, tokens, temperature, ignore, err):
+@functools.lru_cache(maxsize=1024)
+def _logprobs_work(rows, vocab, dtype):
+    return L.lib().advopt_token_logprobs_work(rows, vocab, dtype)
+
+
+def _logprobs_args(out, stats, work, logits, tokens, temperature, ignore, dtype, err):
     x, inner, outer_pitch, pitch = _strided(logits)
     # x is returned too: a copy must outlive the launch
-    return x, _LOGPROBS.pack(_ptr(out), _ptr(stats), x.data_ptr(), tokens.data_ptr(), err, inner, outer_pitch, pitch, tokens.numel(),
-                             logits.shape[-1], ignore, dtype_code(logits.dtype), tokens.element_size(), temperature, 0)
+    return x, _LOGPROBS.pack(out, stats, x.data_ptr(), tokens.data_ptr(), err, work, inner, outer_pitch, pitch, tokens.numel(),
+                             logits.shape[-1], ignore, dtype, tokens.element_size(), temperature, 0)
 
 
-def _token_logprobs(logits, tokens, temperature, ignore, keep):
+def _token_logprobs(logits, tokens, temperature, ignore, dtype, keep):
+    """(log-probabilities, {m, 1 / s} of the rows if `keep`)"""
+    R = tokens.numel()
     out = logits.new_empty(tokens.shape, dtype=torch.float32)
-    stats = logits.new_empty(tokens.numel(), 2, dtype=torch.float32) if keep else None
+    stats = logits.new_empty(R, 2, dtype=torch.float32) if keep else None
+    size = _logprobs_work(R, logits.shape[-1], dtype)
+    work = logits.new_empty(size, dtype=torch.uint8) if size else None
     with on_device(logits.device):
-        x, args = _logprobs_args(out, stats, logits, tokens, temperature, ignore, INDEX_ERRORS.pointer())
+        x, args = _logprobs_args(out.data_ptr(), _ptr(stats), _ptr(work), logits, tokens, temperature, ignore, dtype, INDEX_ERRORS.pointer())
         rc = L.lib().advopt_token_logprobs(args, raw_stream(logits.device))
     if rc:
         L.check(rc, "advopt_token_logprobs")
@@ -61,7 +70,7 @@ def _token_logprobs(logits, tokens, temperature, ignore, keep):
 
 def _logprobs_backward(ctx, dlp):
     logits, tokens, stats = ctx.saved_tensors
-    x_dtype, x_shape, t_dtype, temperature, ignore = ctx.call
+    x_dtype, x_shape, t_dtype, temperature, ignore, dtype = ctx.call
     dev = dlp.device
     if logits.dtype is not x_dtype or logits.shape != x_shape or logits.device != dev:
         saved(logits, "logits", x_dtype, x_shape, dev)   # raises
@@ -70,7 +79,7 @@ def _logprobs_backward(ctx, dlp):
     dlp = dlp.contiguous()
     dx = empty_as(logits)
     with on_device(dev):
-        x, args = _logprobs_args(None, stats, logits, tokens, temperature, ignore, 0)
+        x, args = _logprobs_args(0, stats.data_ptr(), 0, logits, tokens, temperature, ignore, dtype, 0)
         rc = L.lib().advopt_token_logprobs_grad(dx.data_ptr(), dlp.data_ptr(), args, raw_stream(dev))
     if rc:
         L.check(rc, "advopt_token_logprobs_grad")
@@ -83,9 +92,9 @@ _logprobs_backward_once = once_differentiable(_logprobs_backward)
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call):   # a tuple: torch looks at every argument of its own
-        tokens, temperature, ignore = call
-        out, stats = _token_logprobs(logits, tokens, temperature, ignore, True)
-        ctx.call = logits.dtype, logits.shape, tokens.dtype, temperature, ignore
+        tokens, temperature, ignore, dtype = call
+        out, stats = _token_logprobs(logits, tokens, temperature, ignore, dtype, True)
+        ctx.call = logits.dtype, logits.shape, tokens.dtype, temperature, ignore, dtype
         ctx.save_for_backward(logits, tokens, stats)
         return out
 
@@ -116,18 +125,18 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     index_bytes("token_logprobs: tokens", tokens)
     if not logits.is_cuda or tokens.device != logits.device:
         raise NotImplementedError("token_logprobs: tensors must live on one CUDA device (no CPU fallback)")
-    dtype_code(logits.dtype)
+    dtype = dtype_code(logits.dtype)
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"token_logprobs: the temperature must be between 1e-30 and 1e30, got {temperature}")
-    if not 0 < logits.shape[-1] < 1 << 31:
-        raise ValueError("token_logprobs: rows of 1 to 2^31 - 1 logits")
+    if not 0 < logits.shape[-1] < 1 << 31 or tokens.numel() >= 1 << 31:
+        raise ValueError("token_logprobs: fewer than 2^31 tokens, rows of 1 to 2^31 - 1 logits")
     refuse_tangents("token_logprobs", logits)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogprobs.apply(logits, (tokens, temperature, int(ignore_index)))
-    return _token_logprobs(logits, tokens, temperature, int(ignore_index), False)[0]
+        return _TokenLogprobs.apply(logits, (tokens, temperature, int(ignore_index), dtype))
+    return _token_logprobs(logits, tokens, temperature, int(ignore_index), dtype, False)[0]
 
 
 # ---- losses ----

@@ -766,27 +766,30 @@ int advopt_layer_norm_grad(const advopt_layer_norm_grad_args* args, void* stream
  * and k = tokens[r].  Row r = (a, b) with b < inner starts at a * ld_outer +
  * b * ld_inner.  A token `ignore` gives 0; any other outside [0, vocab) NaN,
  * and sets *err (or NULL) to 1.  stats (or NULL) receives {largest logit,
- * sum of exp((logit - largest) / temperature)}. */
+ * 1 / sum of exp((logit - largest) / temperature)}.  `work`:
+ * advopt_token_logprobs_work(rows, vocab, dtype) bytes, 8-byte aligned. */
 typedef struct advopt_token_logprobs_args {
   float* logprobs;          /* [rows]                                          */
   float* stats;             /* [rows][2]                                       */
   const void* logits;
   const void* tokens;       /* contiguous, int32 or int64                      */
   int32_t* err;
+  void* work;
   int64_t inner;
   int64_t ld_outer;         /* elements                                        */
   int64_t ld_inner;
-  int64_t rows;
-  int64_t vocab;            /* below 2^31                                      */
+  int64_t rows;             /* below 2^31, as vocab                            */
+  int64_t vocab;
   int64_t ignore;
   int32_t dtype;            /* ADVOPT_DT_*: logits                             */
   int32_t token_bytes;      /* 4 or 8                                          */
   float temperature;        /* positive                                        */
   int32_t pad;
 } advopt_token_logprobs_args;
+int64_t advopt_token_logprobs_work(int64_t rows, int64_t vocab, int32_t dtype);
 int advopt_token_logprobs(const advopt_token_logprobs_args* args, void* stream);
 
-/* dlogits [rows][vocab] (contiguous, in the logits' dtype) = dlogprobs[r] /
+/* dlogits [rows][vocab] (contiguous, 16-byte aligned, in the logits' dtype) = dlogprobs[r] /
  * temperature * ((j == k) - p_j); rows with dlogprobs[r] == 0 and rows whose
  * token is `ignore` are zeros and are not read.  Of args: logits, tokens,
  * stats (as the forward call left them) and the sizes. */

@@ -43,7 +43,7 @@ OK = {
     "advopt_layer_norm": dict(y=4096, x=4096, weight=0, bias=0, stats=0, ldx=8, rows=4, cols=8, eps=1e-5, x_dtype=1, w_dtype=0, pad=0),
     "advopt_layer_norm_grad": dict(dx=4096, dweight=4096, dbias=4096, dy=4096, x=4096, weight=4096, stats=4096, work=4096, lddy=8, ldx=8, rows=4, cols=8,
                                    x_dtype=1, w_dtype=0),
-    "advopt_token_logprobs": dict(out=4096, stats=0, logits=4096, tokens=4096, err=0, inner=4, ld_outer=0, ld_inner=8, rows=4, vocab=8, ignore=-100,
+    "advopt_token_logprobs": dict(out=4096, stats=0, logits=4096, tokens=4096, err=0, work=0, inner=4, ld_outer=0, ld_inner=8, rows=4, vocab=8, ignore=-100,
                                   dtype=1, token_bytes=8, temperature=1.0, pad=0),
     "advopt_policy_loss": dict(loss=4096, kl=4096, clipped=4096, slope=0, scale=4096, logprobs=4096, old=4096, ref=0, advantages=4096, mask=0, work=4096, ld_logprobs=8,
                                ld_old=8, ld_ref=0, ld_adv=-1, ld_mask=0, rows=4, cols=8, log_high=0.2, log_low=-0.2, clip_low=0.2, clip_high=0.2,
@@ -69,7 +69,7 @@ BAD = [
     ("advopt_token_logprobs", dict(rows=-1)), ("advopt_token_logprobs", dict(vocab=0)), ("advopt_token_logprobs", dict(vocab=BIG)),
     ("advopt_token_logprobs", dict(inner=0)), ("advopt_token_logprobs", dict(token_bytes=3)), ("advopt_token_logprobs", dict(temperature=0.0)),
     ("advopt_token_logprobs", dict(temperature=NAN)), ("advopt_token_logprobs", dict(temperature=float("inf"))), ("advopt_token_logprobs", dict(dtype=9)),
-    ("advopt_token_logprobs", dict(out=0)), ("advopt_token_logprobs", dict(logits=0)), ("advopt_token_logprobs", dict(stats=4100)),
+    ("advopt_token_logprobs", dict(out=0)), ("advopt_token_logprobs", dict(vocab=50257)), ("advopt_token_logprobs", dict(vocab=50257, work=4100)), ("advopt_token_logprobs", dict(logits=0)), ("advopt_token_logprobs", dict(stats=4100)),
     ("advopt_policy_loss", dict(rows=-1)), ("advopt_policy_loss", dict(rows=BIG)), ("advopt_policy_loss", dict(loss=0)), ("advopt_policy_loss", dict(kl=0)), ("advopt_policy_loss", dict(clipped=0)),
     ("advopt_policy_loss", dict(scale=0)), ("advopt_policy_loss", dict(work=0)), ("advopt_policy_loss", dict(work=4104)),
     ("advopt_policy_loss", dict(ld_old=7)), ("advopt_policy_loss", dict(ld_adv=7)), ("advopt_policy_loss", dict(mask=4096, ld_mask=7)),
@@ -101,7 +101,7 @@ def test_gradient_entries_refuse_before_they_launch():
     from advanced_optimizers_b200 import losses
     lib = L.lib()
     args = losses._LOGPROBS.pack(*{**OK["advopt_token_logprobs"], "stats": 4096}.values())
-    for bad in ((0, 4096, args), (4096, 0, args), (4096, 4096, None), (4096, 4096, losses._LOGPROBS.pack(*OK["advopt_token_logprobs"].values()))):
+    for bad in ((0, 4096, args), (4104, 4096, args), (4096, 0, args), (4096, 4096, None), (4096, 4096, losses._LOGPROBS.pack(*OK["advopt_token_logprobs"].values()))):
         assert lib.advopt_token_logprobs_grad(*bad, None) == -1
     good = [4096, 4096, 4096, 4096, 4, 8, 0]
     for at, v in ((0, 0), (1, 0), (2, 0), (3, 0), (4, -1), (5, BIG), (6, 7)):
@@ -117,6 +117,8 @@ def test_work_sizes():
     assert lib.advopt_embedding_grad_work(0, 8, 0) == 0
     assert lib.advopt_embedding_grad_work(33, 8, 1) == 4 * 144 + 5 * 2 * 8 * 4
     assert lib.advopt_embedding_grad_work(1 << 17, 8, 0) == 4 * (4 << 17) + (1 << 12) * 2 * 8 * 4
+    assert lib.advopt_token_logprobs_work(5, 2048, 1) == 0 and lib.advopt_token_logprobs_work(5, 2049, 1) == 5 * 2 * 8
+    assert lib.advopt_token_logprobs_work(5, 1024, 0) == 0 and lib.advopt_token_logprobs_work(5, 8193, 0) == 5 * 9 * 8
     assert lib.advopt_policy_loss_work(3, 1025) == 3 * 9 * 16 and lib.advopt_policy_loss_work(3, 0) == 0
     assert lib.advopt_policy_loss_work(3000, 1025) == 3000 * 2 * 16
     assert lib.advopt_preference_loss_work(3, 1024) == 6 * 8 * 8 + 6 * 16 and lib.advopt_preference_loss_work(3, 0) == 6 * 16
