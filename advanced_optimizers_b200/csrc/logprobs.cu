@@ -9,9 +9,9 @@
 // Both are bound by HBM; an exponential an element is the next limit (16 a
 // clock and SM, 4.6e12 a second; bf16 logits arrive at 3.3e12).
 //
-// The lanes of a warp take 4 KB of a row at once, all of it on its way before
-// the first element is looked at, and the warp ends: no loop, no barrier, and
-// the warps behind it keep HBM busy meanwhile (a read with an exponential and
+// The lanes of a warp take 6 KB of a row at once (backward 4), all of it on its
+// way before the first element is looked at, and the warp ends: no loop, no
+// barrier, and the warps behind it keep HBM busy meanwhile (a read with an exponential and
 // a maximum an element: 144 us for 4096 x 128256 bf16; with a CTA that walks
 // along a row, however its loads were scheduled, 172 to 201).  Parts of longer
 // rows are joined by a second launch; rows up to 1 KB share a warp.
@@ -30,6 +30,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 struct Args {
@@ -99,13 +105,29 @@ __device__ __forceinline__ uint32_t head_of(const void* p, uint32_t n) {
   return h < n ? h : n;
 }
 
+// The largest element, NaN left out; bf16 ones two at a time.
+template <bool BF16, int U>
+__device__ __forceinline__ float largest(const Vec<BF16> (&v)[U]) {
+  if constexpr (BF16) {
+    uint32_t m = 0xFF80FF80u;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = max_bf16x2(max_bf16x2(max_bf16x2(v[u].q.x, v[u].q.y), max_bf16x2(v[u].q.z, v[u].q.w)), m);
+    return fmaxf(u2f(m << 16), u2f(m & 0xFFFF0000u));
+  } else {
+    float m = NEG_INF;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(fmaxf(fmaxf(v[u].at(0), v[u].at(1)), fmaxf(v[u].at(2), v[u].at(3))), m);
+    return m;
+  }
+}
+
 constexpr int THREADS = 256;
 
 // L lanes take U vectors of 16 bytes each of a row at once: 512 bytes, 1 KB, or
-// 4 KB, which are a part of a longer row.
-template <int L>
+// 6 KB (backward 4), which are a part of a longer row.
+template <int L, bool BACK>
 struct Share {
-  static constexpr int U = L == 32 ? 8 : 4, VECS = L * U;
+  static constexpr int U = L == 32 ? (BACK ? 8 : 12) : 4, VECS = L * U;
 };
 
 // Their running maximum and sum of part `part` of a row; the first part's
@@ -113,20 +135,22 @@ struct Share {
 // behind its last one.
 template <bool BF16, int L>
 __device__ __forceinline__ void scan(Run& run, const void* row, uint32_t n, float c, int lane, uint32_t part) {
-  constexpr int E = Vec<BF16>::E, U = Share<L>::U;
+  constexpr int E = Vec<BF16>::E, U = Share<L, false>::U;
   const uint32_t head = head_of<BF16>(row, n), vecs = (n - head) / E, tail = head + vecs * E;
   const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(row) + head * (BF16 ? 2 : 4));
-  const uint32_t i = part * Share<L>::VECS + lane;
-  const uint4 nothing = BF16 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
-                             : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);   // -infinity
+  const uint32_t i = part * Share<L, false>::VECS + lane;
   Vec<BF16> v[U];
+  p += i;
+  if (part * Share<L, false>::VECS + Share<L, false>::VECS <= vecs) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) v[u].q = i + u * L < vecs ? __ldg(p + i + u * L) : nothing;
-  float top = NEG_INF;
+    for (int u = 0; u < U; ++u) v[u].q = __ldg(p + u * L);
+  } else {
+    const uint4 nothing = BF16 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
+                               : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);   // -infinity
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = fmaxf(top, v[u].at(e));
+    for (int u = 0; u < U; ++u) v[u].q = i + u * L < vecs ? __ldg(p + u * L) : nothing;
+  }
+  const float top = largest<BF16, U>(v);
   run.m = top;
   const float2 b = splat2(-Run::base(top));
   float2 s = make_float2(0.0f, 0.0f);
@@ -192,7 +216,7 @@ struct Place {
 };
 
 template <bool BF16, int L>
-__global__ void __launch_bounds__(THREADS) forward_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_constant__ Args a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & (L - 1);
   const Place at = Place::of<L>(a);
@@ -252,7 +276,7 @@ __device__ __forceinline__ uint4 shifted_load(const unsigned char* p) {
 
 template <bool BF16, int L>
 __global__ void __launch_bounds__(THREADS) grad_kernel(void* dlogits, const float* dlp, const __grid_constant__ Args a) {
-  constexpr int E = Vec<BF16>::E, SIZE = BF16 ? 2 : 4, U = Share<L>::U;
+  constexpr int E = Vec<BF16>::E, SIZE = BF16 ? 2 : 4, U = Share<L, true>::U;
   const int lane = threadIdx.x & (L - 1);
   const Place at = Place::of<L>(a);
   if (at.r >= a.rows) return;
@@ -262,7 +286,7 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(void* dlogits, const floa
   const bool zero = g == 0.0f || token == a.ignore;
   unsigned char* out = static_cast<unsigned char*>(dlogits) + at.r * a.vocab * SIZE;
   const uint32_t n = a.vocab, head = head_of<BF16>(out, n), vecs = (n - head) / E, tail = head + vecs * E;
-  const uint32_t i0 = at.part * Share<L>::VECS + lane;
+  const uint32_t i0 = at.part * Share<L, true>::VECS + lane;
   uint4* to = reinterpret_cast<uint4*>(out + head * SIZE);
   const unsigned char* in = static_cast<const unsigned char*>(row_of<BF16>(a, at.r));
   if (zero) {
@@ -333,7 +357,8 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(void* dlogits, const floa
 }
 
 // Parts of a row, 1 where a group of lanes has all of it.
-inline int64_t parts_of(int64_t bytes) { return ceil_div(bytes, Share<32>::VECS * 16); }
+template <bool BACK>
+inline int64_t parts_of(int64_t bytes) { return ceil_div(bytes, Share<32, BACK>::VECS * 16); }
 
 template <class K, class... A>
 cudaError_t launch(K kernel, int lanes, int64_t groups, bool behind, cudaStream_t s, const A&... args) {
@@ -352,8 +377,8 @@ cudaError_t launch(K kernel, int lanes, int64_t groups, bool behind, cudaStream_
 template <bool BF16>
 cudaError_t forward(const Args& a, cudaStream_t s) {
   const int64_t bytes = (int64_t)a.vocab * (BF16 ? 2 : 4);
-  if (bytes <= Share<8>::VECS * 16) return launch(forward_kernel<BF16, 8>, 8, a.rows, false, s, a);
-  if (bytes <= Share<16>::VECS * 16) return launch(forward_kernel<BF16, 16>, 16, a.rows, false, s, a);
+  if (bytes <= Share<8, false>::VECS * 16) return launch(forward_kernel<BF16, 8>, 8, a.rows, false, s, a);
+  if (bytes <= Share<16, false>::VECS * 16) return launch(forward_kernel<BF16, 16>, 16, a.rows, false, s, a);
   const cudaError_t e = launch(forward_kernel<BF16, 32>, 32, a.rows * a.parts, false, s, a);
   if (e != cudaSuccess || a.parts == 1) return e;
   return a.parts <= 16 ? launch(join_kernel<BF16, 8>, 8, a.rows, true, s, a) : launch(join_kernel<BF16, 32>, 32, a.rows, true, s, a);
@@ -362,8 +387,8 @@ cudaError_t forward(const Args& a, cudaStream_t s) {
 template <bool BF16>
 cudaError_t grad(void* dlogits, const float* dlp, const Args& a, cudaStream_t s) {
   const int64_t bytes = (int64_t)a.vocab * (BF16 ? 2 : 4);
-  if (bytes <= Share<8>::VECS * 16) return launch(grad_kernel<BF16, 8>, 8, a.rows, false, s, dlogits, dlp, a);
-  if (bytes <= Share<16>::VECS * 16) return launch(grad_kernel<BF16, 16>, 16, a.rows, false, s, dlogits, dlp, a);
+  if (bytes <= Share<8, true>::VECS * 16) return launch(grad_kernel<BF16, 8>, 8, a.rows, false, s, dlogits, dlp, a);
+  if (bytes <= Share<16, true>::VECS * 16) return launch(grad_kernel<BF16, 16>, 16, a.rows, false, s, dlogits, dlp, a);
   return launch(grad_kernel<BF16, 32>, 32, a.rows * a.parts, false, s, dlogits, dlp, a);
 }
 
@@ -373,14 +398,14 @@ const char* check(const advopt_token_logprobs_args* a) {
       (a->token_bytes != 4 && a->token_bytes != 8) || !(a->temperature > 0.0f) || a->temperature > 3e38f)
     return "token_logprobs: bad arguments";
   if (!known_dtype(a->dtype)) return "token_logprobs: float32 and bfloat16 logits are supported";
-  if (a->rows * parts_of(a->vocab * bytes_of(a->dtype)) >= (int64_t)1 << 33) return "token_logprobs: too many logits";   // 2^31 CTAs of eight warps: 32 TB
+  if (a->rows * parts_of<true>(a->vocab * bytes_of(a->dtype)) >= (int64_t)1 << 33) return "token_logprobs: too many logits";   // 2^31 CTAs of eight warps: 32 TB
   if (a->rows && (!a->logits || !a->tokens || reinterpret_cast<uintptr_t>(a->stats) % 8)) return "token_logprobs: null or unaligned pointer";
   return nullptr;
 }
-Args args_of(const advopt_token_logprobs_args& a) {
+Args args_of(const advopt_token_logprobs_args& a, int64_t parts) {
   const double inv = 1.0 / (double)a.temperature;
   return {a.logprobs, a.stats, static_cast<float2*>(a.work), a.logits, a.tokens, a.err, a.inner, a.ld_outer, a.ld_inner, a.rows, a.ignore, (uint32_t)a.vocab,
-          (uint32_t)parts_of(a.vocab * bytes_of(a.dtype)),          a.token_bytes == 8, (float)(inv * 1.4426950408889634), (float)inv};
+          (uint32_t)parts,          a.token_bytes == 8, (float)(inv * 1.4426950408889634), (float)inv};
 }
 
 }  // namespace lp
@@ -389,7 +414,7 @@ Args args_of(const advopt_token_logprobs_args& a) {
 using namespace advopt;
 
 extern "C" int64_t advopt_token_logprobs_work(int64_t rows, int64_t vocab, int32_t dtype) {
-  const int64_t parts = rows <= 0 || vocab <= 0 ? 0 : lp::parts_of(vocab * bytes_of(dtype));
+  const int64_t parts = rows <= 0 || vocab <= 0 ? 0 : lp::parts_of<false>(vocab * bytes_of(dtype));
   return parts > 1 ? rows * parts * 8 : 0;
 }
 
@@ -399,8 +424,8 @@ extern "C" int advopt_token_logprobs(const advopt_token_logprobs_args* a, void* 
   if (!a->logprobs || (advopt_token_logprobs_work(a->rows, a->vocab, a->dtype) && (!a->work || reinterpret_cast<uintptr_t>(a->work) % 8)))
     return set_error(ADVOPT_E_INVALID, "token_logprobs: null output or workspace");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return check_cuda(a->dtype == ADVOPT_DT_BF16 ? lp::forward<true>(lp::args_of(*a), s) : lp::forward<false>(lp::args_of(*a), s),
-                    "advopt_token_logprobs");
+  const lp::Args q = lp::args_of(*a, lp::parts_of<false>(a->vocab * bytes_of(a->dtype)));
+  return check_cuda(a->dtype == ADVOPT_DT_BF16 ? lp::forward<true>(q, s) : lp::forward<false>(q, s), "advopt_token_logprobs");
 }
 
 extern "C" int advopt_token_logprobs_grad(void* dlogits, const float* dlogprobs, const advopt_token_logprobs_args* a, void* stream) {
@@ -409,7 +434,7 @@ extern "C" int advopt_token_logprobs_grad(void* dlogits, const float* dlogprobs,
   if (!dlogits || !aligned16(dlogits) || !dlogprobs || !a->stats)
     return set_error(ADVOPT_E_INVALID, "token_logprobs_grad: null or unaligned pointer");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return check_cuda(a->dtype == ADVOPT_DT_BF16 ? lp::grad<true>(dlogits, dlogprobs, lp::args_of(*a), s)
-                                               : lp::grad<false>(dlogits, dlogprobs, lp::args_of(*a), s),
+  const lp::Args q = lp::args_of(*a, lp::parts_of<true>(a->vocab * bytes_of(a->dtype)));
+  return check_cuda(a->dtype == ADVOPT_DT_BF16 ? lp::grad<true>(dlogits, dlogprobs, q, s) : lp::grad<false>(dlogits, dlogprobs, q, s),
                     "advopt_token_logprobs_grad");
 }

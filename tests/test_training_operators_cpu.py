@@ -117,8 +117,8 @@ def test_work_sizes():
     assert lib.advopt_embedding_grad_work(0, 8, 0) == 0
     assert lib.advopt_embedding_grad_work(33, 8, 1) == 4 * 144 + 5 * 2 * 8 * 4
     assert lib.advopt_embedding_grad_work(1 << 17, 8, 0) == 4 * (4 << 17) + (1 << 12) * 2 * 8 * 4
-    assert lib.advopt_token_logprobs_work(5, 2048, 1) == 0 and lib.advopt_token_logprobs_work(5, 2049, 1) == 5 * 2 * 8
-    assert lib.advopt_token_logprobs_work(5, 1024, 0) == 0 and lib.advopt_token_logprobs_work(5, 8193, 0) == 5 * 9 * 8
+    assert lib.advopt_token_logprobs_work(5, 3000, 1) == 0 and lib.advopt_token_logprobs_work(5, 3200, 1) == 5 * 2 * 8
+    assert lib.advopt_token_logprobs_work(5, 1536, 0) == 0 and lib.advopt_token_logprobs_work(5, 8193, 0) == 5 * 6 * 8
     assert lib.advopt_policy_loss_work(3, 1025) == 3 * 9 * 16 and lib.advopt_policy_loss_work(3, 0) == 0
     assert lib.advopt_policy_loss_work(3000, 1025) == 3000 * 2 * 16
     assert lib.advopt_preference_loss_work(3, 1024) == 6 * 8 * 8 + 6 * 16 and lib.advopt_preference_loss_work(3, 0) == 6 * 16
