@@ -492,6 +492,68 @@ __global__ void __launch_bounds__(JOIN * 32) join_kernel(const __grid_constant__
   }
 }
 
+// ---- few tokens: one launch, no order ----
+// A CTA takes a run of rows of dw, finds among the ids which of them occur,
+// and writes the others' zeros.  A warp then takes a row that occurs and 16
+// bytes a lane, and adds the row's tokens as they come.
+constexpr int FEW = 256;
+constexpr int FEW_BYTES = 32768;       // of dw a CTA at most, about
+
+template <bool BF16>
+__global__ void __launch_bounds__(FEW) few_kernel(const __grid_constant__ Grad g, uint32_t rows, uint32_t wide, int vec) {
+  constexpr int E = Cols<BF16>::E;
+  __shared__ uint32_t ids[FEW];
+  __shared__ uint32_t met[FEW_BYTES / 2 / 32];   // a bit for each of the CTA's rows
+  __shared__ uint32_t list[FEW], found;          // the rows that occur
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t first = blockIdx.x * rows, here = g.vocab - first < rows ? g.vocab - first : rows;
+  for (uint32_t i = threadIdx.x; i < (here + 31) / 32; i += FEW) met[i] = 0;
+  const uint32_t key = threadIdx.x < g.tokens ? key_of(g.ids, g.wide, threadIdx.x, g.vocab, g.padding) : g.vocab;
+  ids[threadIdx.x] = key;
+  if (threadIdx.x == 0) found = 0;
+  __syncthreads();
+  const uint32_t mine = key - first;
+  if (key < g.vocab && mine < here && !(atomicOr(&met[mine >> 5], 1u << (mine & 31)) >> (mine & 31) & 1u))
+    list[atomicAdd(&found, 1u)] = mine;   // in any order: each row's sum is its own
+  __syncthreads();
+  // `wide` vectors a row
+  const float zero[E] = {};
+  for (uint32_t u = threadIdx.x; u < here * wide; u += FEW) {
+    const uint32_t row = u / wide;
+    const int64_t c = (int64_t)(u - row * wide) * E;
+    if (!(met[row >> 5] >> (row & 31) & 1u)) write_row<BF16>(g, first + row, c, g.width - c < E ? (int)(g.width - c) : E, vec, zero);
+  }
+  const uint32_t chunks = (wide + 31) / 32;
+  for (uint32_t u = warp; u < found * chunks; u += FEW / 32) {
+    const uint32_t row = first + list[u / chunks];
+    const int64_t c = ((int64_t)(u % chunks) * 32 + lane) * E;
+    const int nv = c >= g.width ? 0 : g.width - c < E ? (int)(g.width - c) : E;
+    float acc[E] = {};
+    for (uint32_t t0 = 0; t0 < g.tokens; t0 += 32) {
+      uint32_t with = __ballot_sync(0xffffffffu, ids[t0 + lane] == row);   // beyond the last token: vocab
+      while (with) {
+        Cols<BF16> v[4];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (with) {
+            v[i].get(g.dy, (int64_t)(t0 + __ffs(with) - 1) * g.width + c, nv, vec);
+            with &= with - 1;
+            n = i + 1;
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], v[i].at(e));
+          }
+      }
+    }
+    if (nv) write_row<BF16>(g, row, c, nv, vec, acc);
+  }
+}
+inline bool is_few(int64_t tokens) { return tokens <= FEW; }
+
 struct Work {
   int64_t list, part, bytes;   // bytes of one of the four lists, where the partial sums begin, all
 };
@@ -540,12 +602,18 @@ int grad(const advopt_embedding_grad_args& a, cudaStream_t s) {
   g.scale = a.scale;
   g.passes = 1;
   while (a.vocab >> (g.passes * BITS)) ++g.passes;   // the keys are 0 .. vocab
+  if (is_few(a.tokens)) {
+    const int64_t row = a.width * (BF16 ? 2 : 4), wide = ceil_div(a.width, Cols<BF16>::E);
+    // two CTAs an SM, of 512 bytes to 32 KB each
+    int64_t share = a.vocab * row / (2 * 148);
+    share = share < 512 ? 512 : share < FEW_BYTES ? share : FEW_BYTES;
+    const int64_t rows = row >= share ? 1 : share / row;
+    const int vec = aligned16(a.dy) && a.width % Cols<BF16>::E == 0;
+    few_kernel<BF16><<<(unsigned)ceil_div(a.vocab, rows), FEW, 0, s>>>(g, (uint32_t)rows, (uint32_t)wide, vec);
+    return check_cuda(cudaGetLastError(), "advopt_embedding_grad");
+  }
   const int64_t bytes = a.vocab * a.width * (BF16 ? 2 : 4), zeros = ceil_div(bytes, FILL_THREADS * FILL * 16);
   const char* where = "advopt_embedding_grad";
-  if (a.tokens == 0) {
-    zero_kernel<BF16><<<(unsigned)zeros, FILL_THREADS, 0, s>>>(a.dweight, bytes);
-    return check_cuda(cudaGetLastError(), where);
-  }
   cudaError_t e = cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_SMEM);
   if (e != cudaSuccess) return check_cuda(e, where);
   order_kernel<<<CLUSTER, SORT_THREADS, SORT_SMEM, s>>>(g);
@@ -596,7 +664,7 @@ extern "C" int advopt_embedding(const advopt_embedding_args* a, void* stream) {
 }
 
 extern "C" int64_t advopt_embedding_grad_work(int64_t tokens, int64_t width, int32_t dtype) {
-  return tokens <= 0 || width <= 0 ? 0 : emb::work_of(tokens, width, emb::chunk_of(tokens, width, bytes_of(dtype))).bytes;
+  return emb::is_few(tokens) || width <= 0 ? 0 : emb::work_of(tokens, width, emb::chunk_of(tokens, width, bytes_of(dtype))).bytes;
 }
 
 extern "C" int advopt_embedding_grad(const advopt_embedding_grad_args* a, void* stream) {
@@ -606,7 +674,8 @@ extern "C" int advopt_embedding_grad(const advopt_embedding_grad_args* a, void* 
   if (!known_dtype(a->dtype))
     return set_error(ADVOPT_E_UNSUPPORTED, "advopt_embedding_grad: float32 and bfloat16 are supported");
   if (a->vocab == 0 || a->width == 0) return ADVOPT_OK;
-  if (!a->dweight || !aligned16(a->dweight) || (a->tokens && (!a->dy || !a->ids || !a->work || !aligned16(a->work))))
+  if (!a->dweight || !aligned16(a->dweight) || (a->tokens && (!a->dy || !a->ids)) ||
+      (!emb::is_few(a->tokens) && (!a->work || !aligned16(a->work))))
     return set_error(ADVOPT_E_INVALID, "advopt_embedding_grad: null or unaligned pointer");
   const int64_t chunks = ceil_div(a->tokens, 8);
   if (a->vocab > ((int64_t)1 << 43) / a->width || chunks * ceil_div(a->width, 128) / emb::SUM_WARPS >= emb::LIMIT - 1)

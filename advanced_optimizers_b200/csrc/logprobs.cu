@@ -15,6 +15,8 @@
 // a maximum an element: 144 us for 4096 x 128256 bf16; with a CTA that walks
 // along a row, however its loads were scheduled, 172 to 201).  Parts of longer
 // rows are joined by a second launch; rows up to 1 KB share a warp.
+#include <cooperative_groups.h>
+
 #include "advopt.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -231,6 +233,48 @@ __global__ void __launch_bounds__(THREADS, 4) forward_kernel(const __grid_consta
   else finish<BF16>(a, at.r, token, run);
 }
 
+// A cluster per row, for as many rows as there are SMs: they are bound by
+// latency, which a second launch and its buffer would add to.
+constexpr int CLUSTER = 8, WARPS = THREADS / 32;
+
+template <bool BF16>
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(THREADS) row_kernel(const __grid_constant__ Args a) {
+  namespace cg = cooperative_groups;
+  __shared__ float2 red[WARPS], whole;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = cluster.block_rank();
+  const int64_t r = blockIdx.x / CLUSTER, token = token_of(a, r);
+  if (token == a.ignore) {   // of all the cluster's CTAs
+    if (rank == 0 && threadIdx.x == 0) ignored(a, r);
+    return;
+  }
+  Run run;
+  for (uint32_t part = rank * WARPS + warp; part < a.parts; part += CLUSTER * WARPS) {
+    Run more;
+    scan<BF16, 32>(more, row_of<BF16>(a, r), a.vocab, a.c, lane, part);
+    run.join(more.m, more.s, a.c);
+  }
+  join_lanes<32>(run, a.c);
+  if (lane == 0) red[warp] = make_float2(run.m, run.s);
+  __syncthreads();
+  if (warp == 0) {
+    run.m = red[lane & (WARPS - 1)].x;
+    run.s = red[lane & (WARPS - 1)].y;
+    join_lanes<WARPS>(run, a.c);
+    if (lane == 0) whole = make_float2(run.m, run.s);
+  }
+  cluster.sync();
+  if (rank == 0 && warp == 0) {
+    const float2 t = *cluster.map_shared_rank(&whole, lane & (CLUSTER - 1));
+    run.m = t.x;
+    run.s = t.y;
+    join_lanes<CLUSTER>(run, a.c);
+    if (lane == 0) finish<BF16>(a, r, token, run);
+  }
+  cluster.sync();   // no CTA ends while its sums are read
+}
+
 // L lanes per row join its parts.
 template <bool BF16, int L>
 __global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ Args a) {
@@ -360,6 +404,9 @@ __global__ void __launch_bounds__(THREADS) grad_kernel(void* dlogits, const floa
 template <bool BACK>
 inline int64_t parts_of(int64_t bytes) { return ceil_div(bytes, Share<32, BACK>::VECS * 16); }
 
+// Whether each row is one cluster's.
+inline bool alone(int64_t rows, int64_t parts) { return parts > 1 && rows <= 148; }
+
 template <class K, class... A>
 cudaError_t launch(K kernel, int lanes, int64_t groups, bool behind, cudaStream_t s, const A&... args) {
   cudaLaunchAttribute at;
@@ -379,6 +426,10 @@ cudaError_t forward(const Args& a, cudaStream_t s) {
   const int64_t bytes = (int64_t)a.vocab * (BF16 ? 2 : 4);
   if (bytes <= Share<8, false>::VECS * 16) return launch(forward_kernel<BF16, 8>, 8, a.rows, false, s, a);
   if (bytes <= Share<16, false>::VECS * 16) return launch(forward_kernel<BF16, 16>, 16, a.rows, false, s, a);
+  if (alone(a.rows, a.parts)) {
+    row_kernel<BF16><<<(unsigned)(a.rows * CLUSTER), THREADS, 0, s>>>(a);
+    return cudaGetLastError();
+  }
   const cudaError_t e = launch(forward_kernel<BF16, 32>, 32, a.rows * a.parts, false, s, a);
   if (e != cudaSuccess || a.parts == 1) return e;
   return a.parts <= 16 ? launch(join_kernel<BF16, 8>, 8, a.rows, true, s, a) : launch(join_kernel<BF16, 32>, 32, a.rows, true, s, a);
@@ -415,7 +466,7 @@ using namespace advopt;
 
 extern "C" int64_t advopt_token_logprobs_work(int64_t rows, int64_t vocab, int32_t dtype) {
   const int64_t parts = rows <= 0 || vocab <= 0 ? 0 : lp::parts_of<false>(vocab * bytes_of(dtype));
-  return parts > 1 ? rows * parts * 8 : 0;
+  return parts > 1 && !lp::alone(rows, parts) ? rows * parts * 8 : 0;
 }
 
 extern "C" int advopt_token_logprobs(const advopt_token_logprobs_args* a, void* stream) {

@@ -57,10 +57,11 @@ def _backward(ctx, dy):
     dy = dy.contiguous()
     T = ids.numel()
     dw = dy.new_empty(V, C)
-    work = dy.new_empty(_work_bytes(T, C, dtype), dtype=torch.uint8)
+    size = _work_bytes(T, C, dtype)
+    work = dy.new_empty(size, dtype=torch.uint8) if size else None
     with on_device(dev):
         rc = L.lib().advopt_embedding_grad(_GRAD.pack(
-            dw.data_ptr(), dy.data_ptr(), ids.data_ptr(), work.data_ptr(), T, V, C, padding, dtype, ids.element_size(), scale, 0),
+            dw.data_ptr(), dy.data_ptr(), ids.data_ptr(), 0 if work is None else work.data_ptr(), T, V, C, padding, dtype, ids.element_size(), scale, 0),
             raw_stream(dev))
     if rc:
         L.check(rc, "advopt_embedding_grad")

@@ -84,9 +84,9 @@ def logprobs(logits, tokens, temperature, ignore):
     far = torch.where(z.isinf(), 0.0, (m - z).abs())
     # A term has its exponential's error (2^-22) and three roundings of its argument.  A lane's sum is rescaled, which is an exponential and
     # roundings more, at most twice for what lies ahead of and behind the row's 16-byte boundaries, once when its lanes join, then with each
-    # part of 6 KB of its row that a lane joins (two of up to 16, or one in 32 of more) and once more.  The sums' trees are 66 deep at most:
-    # 48 of a lane's pairs, their join, two, five steps, two or more parts, five steps.
-    rel = (8 + V / 32768) * (2.0 ** -22 + 4 * U) + 66 * U + (3 * U * (far * e).sum(1, keepdim=True) / s)
+    # part of 6 KB of its row that a lane joins (two of up to 16, or one in 32 of more) and twice more.  The sums' trees are 72 deep at most:
+    # 48 of a lane's pairs, their join, two, five steps, two or more parts, twice five steps.
+    rel = (9 + V / 32768) * (2.0 ** -22 + 4 * U) + 72 * U + (3 * U * (far * e).sum(1, keepdim=True) / s)
     bad = (t < 0) | (t >= V)
     zt = z.gather(1, t.clamp(0, V - 1)[:, None])
     lp = zt - m - s.log()

@@ -38,7 +38,7 @@ def check(ids, w, dy, scale=1.0, padding=None):
 
 
 @pytest.mark.parametrize("dtype", [B, F])
-@pytest.mark.parametrize("T,V,C", [(1, 1, 1), (1, 7, 8), (31, 5, 3), (32, 33, 264), (33, 512, 256), (100, 511, 129), (1000, 513, 20), (2049, 300, 64),
+@pytest.mark.parametrize("T,V,C", [(1, 1, 1), (1, 7, 8), (31, 5, 3), (32, 33, 264), (33, 512, 256), (100, 511, 129), (1000, 513, 20), (2049, 300, 64), (256, 20000, 5), (256, 70, 520),
                                    (4096, 50304, 72), (9001, 1000, 136), (70000, 262145, 8), (257, 100, 5003)])
 def test_embedding_and_gradient(T, V, C, dtype):
     ids, w, dy = make(T, V, C, dtype)
@@ -116,9 +116,10 @@ def test_infinities_stay_in_their_rows():
 
 
 @pytest.mark.parametrize("dtype", [B, F])
-def test_repeats_bit_for_bit_on_other_streams_and_in_graphs(dtype):
+@pytest.mark.parametrize("T", [200, 20000])
+def test_repeats_bit_for_bit_on_other_streams_and_in_graphs(T, dtype):
     import advanced_optimizers_b200 as A
-    ids, w, dy = make(20000, 400, 264, dtype)
+    ids, w, dy = make(T, 400, 264, dtype)
     leaf = w.requires_grad_()
     run = lambda: torch.autograd.grad(A.embedding(ids, leaf, padding_idx=3), leaf, dy)[0]  # noqa: E731
     want = run()
@@ -142,19 +143,20 @@ def test_repeats_bit_for_bit_on_other_streams_and_in_graphs(dtype):
     ref.close(out, *ref.embedding_grad(ids, dy, 400, 1.0, 3), dtype)
 
 
-def test_more_than_2_to_32_elements():
+@pytest.mark.parametrize("repeat", [1, 100])
+def test_more_than_2_to_32_elements(repeat):
     import advanced_optimizers_b200 as A
     V, C = 70000, 65536
     w = torch.zeros(V, C, dtype=B, device="cuda")
-    ids = torch.tensor([0, V - 1, 65537, V - 1], device="cuda")
+    ids = torch.tensor([0, V - 1, 65537, V - 1], device="cuda").repeat(repeat)
     w[V - 1], w[65537] = 3.0, 5.0
     leaf = w.requires_grad_()
     y = A.embedding(ids, leaf)
-    assert y.float().mean(1).tolist() == [0.0, 3.0, 5.0, 3.0]
+    assert y.float().mean(1).tolist() == [0.0, 3.0, 5.0, 3.0] * repeat
     dw, = torch.autograd.grad(y, leaf, torch.ones_like(y))
-    assert [float(dw[i].float().mean()) for i in (0, 1, 65537, V - 2, V - 1)] == [1.0, 0.0, 1.0, 0.0, 2.0]
+    assert [float(dw[i].float().mean()) for i in (0, 1, 65537, V - 2, V - 1)] == [n * repeat for n in (1.0, 0.0, 1.0, 0.0, 2.0)]
     total = sum(float(part.float().sum()) for part in dw.split(10000))
-    assert total == 4.0 * C
+    assert total == 4.0 * C * repeat
 
 
 def test_hooks_on_saved_tensors_and_other_derivatives():

@@ -58,7 +58,7 @@ BAD = [
     ("advopt_embedding", dict(weight=0)), ("advopt_embedding", dict(ids=0)),
     ("advopt_embedding_grad", dict(tokens=-1)), ("advopt_embedding_grad", dict(vocab=BIG)), ("advopt_embedding_grad", dict(width=-3)),
     ("advopt_embedding_grad", dict(dtype=3)), ("advopt_embedding_grad", dict(id_bytes=1)), ("advopt_embedding_grad", dict(dweight=0)),
-    ("advopt_embedding_grad", dict(dweight=4100)), ("advopt_embedding_grad", dict(work=4104)), ("advopt_embedding_grad", dict(work=0)),
+    ("advopt_embedding_grad", dict(dweight=4100)), ("advopt_embedding_grad", dict(tokens=300, work=4104)), ("advopt_embedding_grad", dict(tokens=300, work=0)),
     ("advopt_embedding_grad", dict(dy=0)), ("advopt_embedding_grad", dict(tokens=(1 << 31) - 1, width=(1 << 31) - 1)),
     ("advopt_layer_norm", dict(rows=-1)), ("advopt_layer_norm", dict(cols=BIG)), ("advopt_layer_norm", dict(ldx=7)), ("advopt_layer_norm", dict(eps=-1.0)),
     ("advopt_layer_norm", dict(eps=NAN)), ("advopt_layer_norm", dict(x_dtype=2)), ("advopt_layer_norm", dict(w_dtype=5)), ("advopt_layer_norm", dict(x=0)),
@@ -69,7 +69,7 @@ BAD = [
     ("advopt_token_logprobs", dict(rows=-1)), ("advopt_token_logprobs", dict(vocab=0)), ("advopt_token_logprobs", dict(vocab=BIG)),
     ("advopt_token_logprobs", dict(inner=0)), ("advopt_token_logprobs", dict(token_bytes=3)), ("advopt_token_logprobs", dict(temperature=0.0)),
     ("advopt_token_logprobs", dict(temperature=NAN)), ("advopt_token_logprobs", dict(temperature=float("inf"))), ("advopt_token_logprobs", dict(dtype=9)),
-    ("advopt_token_logprobs", dict(out=0)), ("advopt_token_logprobs", dict(vocab=50257)), ("advopt_token_logprobs", dict(vocab=50257, work=4100)), ("advopt_token_logprobs", dict(logits=0)), ("advopt_token_logprobs", dict(stats=4100)),
+    ("advopt_token_logprobs", dict(out=0)), ("advopt_token_logprobs", dict(rows=200, vocab=50257)), ("advopt_token_logprobs", dict(rows=200, vocab=50257, work=4100)), ("advopt_token_logprobs", dict(logits=0)), ("advopt_token_logprobs", dict(stats=4100)),
     ("advopt_policy_loss", dict(rows=-1)), ("advopt_policy_loss", dict(rows=BIG)), ("advopt_policy_loss", dict(loss=0)), ("advopt_policy_loss", dict(kl=0)), ("advopt_policy_loss", dict(clipped=0)),
     ("advopt_policy_loss", dict(scale=0)), ("advopt_policy_loss", dict(work=0)), ("advopt_policy_loss", dict(work=4104)),
     ("advopt_policy_loss", dict(ld_old=7)), ("advopt_policy_loss", dict(ld_adv=7)), ("advopt_policy_loss", dict(mask=4096, ld_mask=7)),
@@ -114,11 +114,11 @@ def test_gradient_entries_refuse_before_they_launch():
 def test_work_sizes():
     from advanced_optimizers_b200 import _lib as L
     lib = L.lib()
-    assert lib.advopt_embedding_grad_work(0, 8, 0) == 0
-    assert lib.advopt_embedding_grad_work(33, 8, 1) == 4 * 144 + 5 * 2 * 8 * 4
+    assert lib.advopt_embedding_grad_work(0, 8, 0) == 0 and lib.advopt_embedding_grad_work(256, 8, 0) == 0
+    assert lib.advopt_embedding_grad_work(257, 8, 1) == 4 * 1040 + 33 * 2 * 8 * 4
     assert lib.advopt_embedding_grad_work(1 << 17, 8, 0) == 4 * (4 << 17) + (1 << 12) * 2 * 8 * 4
-    assert lib.advopt_token_logprobs_work(5, 3000, 1) == 0 and lib.advopt_token_logprobs_work(5, 3200, 1) == 5 * 2 * 8
-    assert lib.advopt_token_logprobs_work(5, 1536, 0) == 0 and lib.advopt_token_logprobs_work(5, 8193, 0) == 5 * 6 * 8
+    assert lib.advopt_token_logprobs_work(500, 3000, 1) == 0 and lib.advopt_token_logprobs_work(500, 3200, 1) == 500 * 2 * 8
+    assert lib.advopt_token_logprobs_work(148, 8193, 0) == 0 and lib.advopt_token_logprobs_work(149, 8193, 0) == 149 * 6 * 8
     assert lib.advopt_policy_loss_work(3, 1025) == 3 * 9 * 16 and lib.advopt_policy_loss_work(3, 0) == 0
     assert lib.advopt_policy_loss_work(3000, 1025) == 3000 * 2 * 16
     assert lib.advopt_preference_loss_work(3, 1024) == 6 * 8 * 8 + 6 * 16 and lib.advopt_preference_loss_work(3, 0) == 6 * 16
