@@ -81,14 +81,20 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[4 * N]) {
   __syncthreads();
 }
 
-// A thread's columns: NV vectors of 16 bytes of x, `width` threads' apart.
-template <bool BF16, int NV>
-__device__ __forceinline__ void columns(int cols, int width, int lane, int (&c)[NV], int (&nv)[NV]) {
+// A thread's columns: NV vectors of 16 bytes of x, each warp's (or CTA's) next
+// to one another.  nv: how many of a vector's elements there are.  Where rows do
+// not start on 16-byte boundaries (A false), a warp's first lane repeats the
+// vector ahead of the warp's, whose last elements the next lane stores; it
+// counts for no sum (count).
+template <bool BF16, int NV, bool A>
+__device__ __forceinline__ void columns(int cols, bool warp_rows, int (&c)[NV], int (&nv)[NV], int (&count)[NV]) {
   constexpr int E = BF16 ? 8 : 4;
+  const int lane = threadIdx.x & 31, warp = warp_rows ? 0 : threadIdx.x >> 5, warps = warp_rows ? 1 : blockDim.x >> 5;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    c[v] = (v * width + lane) * E;
-    nv[v] = c[v] >= cols ? 0 : cols - c[v] < E ? cols - c[v] : E;
+    c[v] = (A ? (v * warps + warp) * 32 + lane : (v * warps + warp) * 31 + lane - 1) * E;
+    nv[v] = c[v] < 0 || c[v] >= cols ? 0 : cols - c[v] < E ? cols - c[v] : E;
+    count[v] = A || lane ? nv[v] : 0;
   }
 }
 
@@ -214,7 +220,7 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 5; ++i) t[i] = by4 ? s[i + 1] : s[i];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[v].w[i] = BF16 && by2 ? __funnelshift_r(t[i], t[i + 1], 16) : t[i];
+        for (int i = 0; i < 4; ++i) x[v].w[i] = BF16 ? __funnelshift_r(t[i], t[i + 1], by2 ? 16 : 0) : t[i];
         if (nv[v] < E) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -236,20 +242,18 @@ __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_
 
 // A thread's 16 bytes at column c of an output row.  Where rows do not start on
 // 16-byte boundaries (A false), a lane stores the aligned 16 bytes that its
-// elements begin in, with the lane before's last ones, and by itself only
-// elements whose 16 bytes no lane has whole.  All lanes take part.
+// elements begin in, with the lane before's last ones; only a row's first and
+// last ones are not whole.  All lanes take part.
 template <bool BF16, bool A>
 __device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsigned char* row, int c, int nv, int cols) {
   constexpr int SIZE = BF16 ? 2 : 4, E = 16 / SIZE;
-  unsigned char* p = row + c * SIZE;
+  unsigned char* p = row + (int64_t)c * SIZE;
   if (A) {
     if (nv) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
     return;
   }
   const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
-  if (o == 0 && nv == E) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
-  const int k = (int)o / SIZE, lane = threadIdx.x & 31;
-  const bool whole = lane > 0 && nv == E, next = lane < 31 && c + 2 * E <= cols;
+  uint32_t g[5];
   if (o) {
     uint32_t t[8];   // the previous lane's words, then this lane's
 #pragma unroll
@@ -259,24 +263,31 @@ __device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsig
     }
     const uint32_t back = 16u - o;
     const bool by8 = back & 8, by4 = back & 4, by2 = back & 2;
-    uint32_t u[6], g[5];
+    uint32_t u[6];
 #pragma unroll
     for (int i = 0; i < 6; ++i) u[i] = by8 ? t[i + 2] : t[i];
 #pragma unroll
     for (int i = 0; i < 5; ++i) g[i] = by4 ? u[i + 1] : u[i];
-    if (BF16 && by2) {
+    if (BF16) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = __funnelshift_r(g[i], g[i + 1], 16);
+      for (int i = 0; i < 4; ++i) g[i] = __funnelshift_r(g[i], g[i + 1], by2 ? 16 : 0);
     }
-    if (whole) *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = x.w[i];
   }
-  if (o ? whole && next : nv == E) return;
+  if ((threadIdx.x & 31) == 0) return;
+  const int first = c - (int)o / SIZE;   // of the row's elements in g
+  if (first >= 0 && first + E <= cols) {
+    *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
+  } else {
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (e < nv && (e < E - k ? !whole || !o : !next)) {
-      if (BF16) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(x.w[(e >> 1) & 3] >> (16 * (e & 1)));
-      else reinterpret_cast<uint32_t*>(p)[e] = x.w[e & 3];
-    }
+    for (int e = 0; e < E; ++e)
+      if (first + e >= 0 && first + e < cols) {
+        if (BF16) reinterpret_cast<uint16_t*>(p - o)[e] = (uint16_t)(g[(e >> 1) & 3] >> (16 * (e & 1)));
+        else reinterpret_cast<uint32_t*>(p - o)[e] = g[e & 3];
+      }
+  }
 }
 
 constexpr int FWD_STAGES = 4, GRAD_STAGES = 3;
@@ -288,9 +299,9 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
   constexpr bool WARP = MAX_THREADS == 32;
   extern __shared__ uint4 smem[];
   __shared__ float4 red[2][4];
-  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
-  int c[NV], nv[NV];
-  columns<BX, NV>(cols, width, lane, c, nv);
+  const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
+  int c[NV], nv[NV], count[NV];
+  columns<BX, NV, A>(cols, WARP, c, nv, count);
   constexpr int S = FWD_STAGES, E = BX ? 8 : 4, P = E / 2;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : 1);
   int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if (nv[v]) {
+      if (count[v]) {
 #pragma unroll
         for (int i = 0; i < P; ++i) s = add2(s, x[v][i]);
       }
@@ -339,7 +350,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
     s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (nv[v] == E) {
+      if (count[v] == E) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 d = add2(x[v][i], splat2(-mean));
@@ -349,8 +360,8 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 d = add2(x[v][i], splat2(-mean));
-          if (2 * i < nv[v]) s.x = __fmaf_rn(d.x, d.x, s.x);
-          if (2 * i + 1 < nv[v]) s.y = __fmaf_rn(d.y, d.y, s.y);
+          if (2 * i < count[v]) s.x = __fmaf_rn(d.x, d.x, s.x);
+          if (2 * i + 1 < count[v]) s.y = __fmaf_rn(d.y, d.y, s.y);
         }
       }
     }
@@ -443,9 +454,9 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
   constexpr int S = GRAD_STAGES, E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, WARP);
   extern __shared__ uint4 smem[];
   __shared__ float4 red[2][8 * RI];
-  const int width = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
-  int c[NV], nv[NV];
-  columns<BX, NV>(cols, width, lane, c, nv);
+  const int cols = (int)a.cols;
+  int c[NV], nv[NV], count[NV];
+  columns<BX, NV, A>(cols, WARP, c, nv, count);
   const bool sums = a.work != nullptr;
   using R = Rows<BX, NV, A, S>;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : RI);
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
       if (here[q]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          if (nv[v] == E) {
+          if (count[v] == E) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
@@ -524,13 +535,13 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
               dw[v][i] = fma2(d, h, dw[v][i]);
               db[v][i] = add2(db[v][i], d);
             }
-          } else if (!A) {
+          } else if (!A && count[v]) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
               s1 = add2(s1, g);   // dy is 0 behind the row's end; h, of a mean that may be infinite, is left out there
-              if (2 * i < nv[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
-              if (2 * i + 1 < nv[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
+              if (2 * i < count[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
+              if (2 * i + 1 < count[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
               db[v][i] = add2(db[v][i], d);
             }
           }
@@ -576,6 +587,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
         for (int v = 0; v < NV; ++v)
 #pragma unroll
           for (int i = 0; i < P; ++i) {
+            if (!A && count[v] == 0) break;
             float2* p = reinterpret_cast<float2*>(sh + c[v]) + i;
             float2* q = reinterpret_cast<float2*>(sh + NV * 32 * E + c[v]) + i;
             *p = k ? add2(*p, dw[v][i]) : dw[v][i];
@@ -594,12 +606,12 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         float* p = part + c[v] + 2 * i;
-        if (2 * i + 1 < nv[v] && (cols & 1) == 0) {
+        if (2 * i + 1 < count[v] && (cols & 1) == 0) {
           *reinterpret_cast<float2*>(p) = dw[v][i];
           *reinterpret_cast<float2*>(p + cols) = db[v][i];
         } else {
-          if (2 * i < nv[v]) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
-          if (2 * i + 1 < nv[v]) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
+          if (2 * i < count[v]) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
+          if (2 * i + 1 < count[v]) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
         }
       }
   }
@@ -716,14 +728,25 @@ __global__ void __launch_bounds__(FINISH_WARPS * 32) finish_kernel(void* dweight
 }
 
 // ---- variants ----
-constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold
-constexpr int64_t WARP_MOST = 1024; // and a warp's
+constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold (a few hundred fewer of unaligned rows)
 constexpr int64_t SMS = 148;
 
-inline int block_threads(int64_t cols) { return (int)ceil_div(cols, 2 * 8 * 32) * 32; }
+// Vectors per thread and threads of a row: a warp's where it holds the row in
+// `one`, `one` * 2 or `one` * 4 vectors a lane, else a CTA's with `one` * 2.
+struct Variant {
+  int vectors, threads;             // threads: 32, or a CTA's; 0: too wide
+};
+inline Variant variant_of(int64_t cols, bool bf16, bool aligned) {
+  const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = aligned ? 32 : 31;
+  const int64_t slots = ceil_div(cols, e) + (aligned ? 0 : 1);   // unaligned rows end in 16 bytes more
+  for (int n = one; n <= 4 * one; n *= 2)
+    if (slots <= n * lanes) return {n, 32};
+  const int64_t threads = ceil_div(slots, 2 * one * lanes) * 32;
+  return {2 * one, threads <= 512 ? (int)threads : 0};
+}
 // CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows at least where that leaves one for each SM.
 inline int64_t grad_ctas(int64_t rows, int64_t cols) {
-  const int64_t units = cols <= WARP_MOST ? ceil_div(rows, WARPS) : rows;
+  const int64_t units = cols <= 1024 ? ceil_div(rows, WARPS) : rows;
   const int64_t few = ceil_div(units, 4) > SMS ? ceil_div(units, 4) : SMS, most = 8 * SMS;
   const int64_t n = few < most ? few : most;
   return units < n ? units : n;
@@ -747,9 +770,9 @@ int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, cuda
 }
 
 template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t forward_variant(const advopt_layer_norm_args& a, bool vec, int wvec, cudaStream_t s) {
+int64_t forward_variant(const advopt_layer_norm_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
   constexpr bool WARP = MAX_THREADS == 32;
-  const int threads = WARP ? WARPS * 32 : block_threads(a.cols);
+  const int threads = WARP ? WARPS * 32 : row_threads;
   const int64_t most = WARP ? ceil_div(a.rows, WARPS) : a.rows;
   if (vec) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16, most, s);
   return launch<forward_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, Rows<BX, NV, false, FWD_STAGES>::slots_of(threads) * 16, most, s);
@@ -759,20 +782,22 @@ template <bool BX, bool BW>
 int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   const bool vec = aligned16(a.x) && aligned16(a.y) && a.cols % 8 == 0 && a.ldx * (BX ? 2 : 4) % 16 == 0;
   const int wvec = aligned16(a.weight) && aligned16(a.bias);
+  constexpr int N = BX ? 1 : 2;
+  const Variant v = variant_of(a.cols, BX, vec);
   int64_t n = 1;
-  if (a.cols > MOST) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-  else if (a.cols <= 256) n = forward_variant<BX, BW, BX ? 1 : 2, 32>(a, vec, wvec, s);
-  else if (a.cols <= 512) n = forward_variant<BX, BW, BX ? 2 : 4, 32>(a, vec, wvec, s);
-  else if (a.cols <= WARP_MOST) n = forward_variant<BX, BW, BX ? 4 : 8, 32>(a, vec, wvec, s);
-  else if (a.cols <= 4096) n = forward_variant<BX, BW, BX ? 2 : 4, 256>(a, vec, wvec, s);
-  else n = forward_variant<BX, BW, BX ? 2 : 4, 512>(a, vec, wvec, s);
+  if (a.cols > MOST || v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+  else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
+  else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+  else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
+  else n = forward_variant<BX, BW, N, 32>(a, 32, vec, wvec, s);
   const cudaError_t e = cudaGetLastError();
   return n < 0 ? set_error(ADVOPT_E_CUDA, "advopt_layer_norm: the kernel's attributes") : check_cuda(e, "advopt_layer_norm");
 }
 
 template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t grad_variant(const advopt_layer_norm_grad_args& a, bool vec, int wvec, cudaStream_t s) {
-  const int threads = MAX_THREADS == 32 ? WARPS * 32 : block_threads(a.cols);
+int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
+  const int threads = MAX_THREADS == 32 ? WARPS * 32 : row_threads;
   const int64_t most = grad_ctas(a.rows, a.cols);
   constexpr int arrays = 2 * grad_rows(BX, MAX_THREADS == 32);
   if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, arrays * Rows<BX, NV, true, GRAD_STAGES>::slots_of(threads) * 16, most, s);
@@ -784,21 +809,23 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
   const bool vec = aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) && a.cols % 8 == 0 && a.ldx * (BX ? 2 : 4) % 16 == 0 &&
                    a.lddy * (BX ? 2 : 4) % 16 == 0;
   const int wvec = aligned16(a.weight);
+  constexpr int N = BX ? 1 : 2;
+  const Variant v = variant_of(a.cols, BX, vec);
   int64_t parts = 0;
-  if (a.cols > MOST) {
+  if (a.cols > MOST || v.threads == 0) {
     parts = wide_parts(a.rows);
     if (a.dx) wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
     if (a.work) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
-  } else if (a.cols <= 256) {
-    parts = grad_variant<BX, BW, BX ? 1 : 2, 32>(a, vec, wvec, s);
-  } else if (a.cols <= 512) {
-    parts = grad_variant<BX, BW, BX ? 2 : 4, 32>(a, vec, wvec, s);
-  } else if (a.cols <= WARP_MOST) {
-    parts = grad_variant<BX, BW, BX ? 4 : 8, 32>(a, vec, wvec, s);
-  } else if (a.cols <= 4096) {
-    parts = grad_variant<BX, BW, BX ? 2 : 4, 256>(a, vec, wvec, s);
+  } else if (v.threads > 256) {
+    parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+  } else if (v.threads > 32) {
+    parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
+  } else if (v.vectors == 4 * N) {
+    parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+  } else if (v.vectors == 2 * N) {
+    parts = grad_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
   } else {
-    parts = grad_variant<BX, BW, BX ? 2 : 4, 512>(a, vec, wvec, s);
+    parts = grad_variant<BX, BW, N, 32>(a, 32, vec, wvec, s);
   }
   if (parts > 0 && a.work)
     finish_kernel<BW><<<dim3((unsigned)ceil_div(a.cols, 32), 2), FINISH_WARPS * 32, 0, s>>>(a.dweight, a.dbias, static_cast<const float*>(a.work),
