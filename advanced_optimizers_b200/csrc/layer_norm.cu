@@ -10,6 +10,7 @@
 // thread holds, over all rows its CTA takes; the CTAs' sums are added in order
 // by a second launch, so that results repeat bit for bit.
 #include <atomic>
+#include <type_traits>
 
 #include "advopt.h"
 #include "capi_internal.h"
@@ -20,6 +21,7 @@ namespace advopt {
 namespace ln {
 
 constexpr int WARPS = 8;      // rows at a time of a CTA whose warps take a row each
+constexpr int PAYLOAD = 30;   // lanes of a warp whose vectors are its own, of unaligned rows
 
 // Sums of N values (1, 2 or 4) over the warp: lane l gets value l / (32 / N).
 // Two values are halved with one exchange, so that N cost little more than one.
@@ -84,17 +86,42 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[4 * N]) {
 // A thread's columns: NV vectors of 16 bytes of x, each warp's (or CTA's) next
 // to one another.  nv: how many of a vector's elements there are.  Where rows do
 // not start on 16-byte boundaries (A false), a warp's first lane repeats the
-// vector ahead of the warp's, whose last elements the next lane stores; it
-// counts for no sum (count).
+// vector ahead of the warp's, whose last elements the next lane stores, and its
+// last lane the one behind, whose first ones the lane before reads; they count
+// for no sum (count).
 template <bool BF16, int NV, bool A>
 __device__ __forceinline__ void columns(int cols, bool warp_rows, int (&c)[NV], int (&nv)[NV], int (&count)[NV]) {
   constexpr int E = BF16 ? 8 : 4;
   const int lane = threadIdx.x & 31, warp = warp_rows ? 0 : threadIdx.x >> 5, warps = warp_rows ? 1 : blockDim.x >> 5;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    c[v] = (A ? (v * warps + warp) * 32 + lane : (v * warps + warp) * 31 + lane - 1) * E;
+    c[v] = (A ? (v * warps + warp) * 32 + lane : (v * warps + warp) * PAYLOAD + lane - 1) * E;
     nv[v] = c[v] < 0 || c[v] >= cols ? 0 : cols - c[v] < E ? cols - c[v] : E;
-    count[v] = A || lane ? nv[v] : 0;
+    count[v] = A || (lane > 0 && lane <= PAYLOAD) ? nv[v] : 0;
+  }
+}
+
+// Whether a row ends within one of the warp's vectors.
+template <bool BF16, int NV, bool A>
+__device__ __forceinline__ bool warp_ragged(const int (&nv)[NV]) {
+  bool some = false;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) some |= nv[v] > 0 && nv[v] < (BF16 ? 8 : 4);
+  return !A && __any_sync(0xffffffffu, some);
+}
+
+// Words k .. k + 4 of eight, shifted by `bits` (0 or 16): 16 bytes from byte 4 k + bits / 8 on.  k and bits are the warp's.
+__device__ __forceinline__ void cut(const uint32_t (&t)[8], uint32_t k, uint32_t bits, uint32_t (&w)[4]) {
+  const auto from = [&](auto at) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(t[at.value + i], t[at.value + i + 1], bits);
+  };
+  if (k < 2) {
+    if (k == 0) from(std::integral_constant<int, 0>());
+    else from(std::integral_constant<int, 1>());
+  } else {
+    if (k == 2) from(std::integral_constant<int, 2>());
+    else from(std::integral_constant<int, 3>());
   }
 }
 
@@ -158,15 +185,12 @@ __device__ __forceinline__ void weights(Oct<BW>& w, const void* p, float absent,
 // that only its own copies have to be waited for.  Rows that do not start on a
 // 16-byte boundary (A false) are copied from the boundary before: each 16
 // bytes hold an element of the row, and a thread's elements then reach into
-// the ones behind its own, which are the next lane's (the last lane copies
-// them too).
+// the next lane's.
 template <bool BF16, int NV, bool A, int S>
 struct Rows {
   static constexpr int E = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
   using X = Vals<BF16, E>;
-  // Shared memory, 16 bytes each: [S][NV][threads], then [S][NV][warps].
-  uint4* own;                                       // this thread's, of stage 0
-  uint4* last;                                      // this warp's
+  uint4* own;                                       // this thread's of stage 0; shared memory is [S][NV][threads]
   const unsigned char* ahead;                       // the next row to be copied
   const unsigned char* now;                         // and to be read (A false)
   int64_t stride;                                   // bytes from a row to the one that follows here
@@ -174,11 +198,10 @@ struct Rows {
   uint32_t at[NV];                                  // this thread's vectors, in bytes
   int to, from;                                     // stages
 
-  // 16-byte slots of a CTA
-  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * (threads + (A ? 0 : threads / 32)); }
+  // 16-byte slots of a CTA; the last lane of all reads one behind its own
+  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * threads + (A ? 0 : 1); }
   __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t row, int64_t step, int cols, const int (&c)[NV]) {
     own = smem + threadIdx.x;
-    last = smem + S * NV * blockDim.x + (threadIdx.x >> 5);
     ahead = now = static_cast<const unsigned char*>(p) + row * ld * SIZE;
     stride = step * ld * SIZE;
     bytes = (uint32_t)cols * SIZE;
@@ -195,16 +218,16 @@ struct Rows {
       const uint32_t o = A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(ahead) & 15u, end = bytes + o;
       const unsigned char* p = ahead - o;
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
+      for (int v = 0; v < NV; ++v)
         if (at[v] < end) copy(own + (to * NV + v) * (int)blockDim.x, p + at[v]);
-        if (!A && (threadIdx.x & 31) == 31 && at[v] + 16 < end) copy(last + (to * NV + v) * (int)(blockDim.x >> 5), p + at[v] + 16);
-      }
     }
     ahead += stride;
     to = to == S - 1 ? 0 : to + 1;
   }
-  // The next row's elements, zeros behind its end in a vector that it ends in.  All lanes take part; the copies have been waited for.
-  __device__ __forceinline__ void get(X (&x)[NV], const int (&nv)[NV]) {
+  // The next row's elements, zeros behind its end in a vector that it ends in
+  // (`ragged`: the warp has one).  All lanes take part; the copies have been waited for.
+  __device__ __forceinline__ void get(X (&x)[NV], const int (&nv)[NV], bool ragged) {
+    const uint32_t o = A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(now) & 15u;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const uint4* slot = own + (from * NV + v) * (int)blockDim.x;
@@ -212,23 +235,19 @@ struct Rows {
       if (A) {
         x[v].w[0] = q.x; x[v].w[1] = q.y; x[v].w[2] = q.z; x[v].w[3] = q.w;   // behind the row's end: anything
       } else {
-        const uint4 n = (threadIdx.x & 31) == 31 ? last[(from * NV + v) * (int)(blockDim.x >> 5)] : slot[1];
-        const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(now) & 15u;
-        const bool by8 = o & 8, by4 = o & 4, by2 = o & 2;
-        const uint32_t s[6] = {by8 ? q.z : q.x, by8 ? q.w : q.y, by8 ? n.x : q.z, by8 ? n.y : q.w, by8 ? n.z : n.x, by8 ? n.w : n.y};
-        uint32_t t[5];
-#pragma unroll
-        for (int i = 0; i < 5; ++i) t[i] = by4 ? s[i + 1] : s[i];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[v].w[i] = BF16 ? __funnelshift_r(t[i], t[i + 1], by2 ? 16 : 0) : t[i];
-        if (nv[v] < E) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (BF16) x[v].w[i] &= (2 * i < nv[v] ? 0xFFFFu : 0u) | (2 * i + 1 < nv[v] ? 0xFFFF0000u : 0u);
-            else x[v].w[i] = i < nv[v] ? x[v].w[i] : 0u;
-          }
-        }
+        const uint4 n = slot[1];
+        const uint32_t t[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
+        cut(t, o >> 2, o & 2 ? 16 : 0, x[v].w);
       }
+    }
+    if (!A && ragged) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (BF16) x[v].w[i] &= (2 * i < nv[v] ? 0xFFFFu : 0u) | (2 * i + 1 < nv[v] ? 0xFFFF0000u : 0u);
+          else x[v].w[i] = i < nv[v] ? x[v].w[i] : 0u;
+        }
     }
     now += stride;
     from = from == S - 1 ? 0 : from + 1;
@@ -253,37 +272,26 @@ __device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsig
     return;
   }
   const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
-  uint32_t g[5];
+  uint32_t t[8], g[4];   // the previous lane's words, then this lane's
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = __shfl_up_sync(0xffffffffu, x.w[i], 1);
+    t[4 + i] = x.w[i];
+  }
   if (o) {
-    uint32_t t[8];   // the previous lane's words, then this lane's
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      t[i] = __shfl_up_sync(0xffffffffu, x.w[i], 1);
-      t[4 + i] = x.w[i];
-    }
     const uint32_t back = 16u - o;
-    const bool by8 = back & 8, by4 = back & 4, by2 = back & 2;
-    uint32_t u[6];
-#pragma unroll
-    for (int i = 0; i < 6; ++i) u[i] = by8 ? t[i + 2] : t[i];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) g[i] = by4 ? u[i + 1] : u[i];
-    if (BF16) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) g[i] = __funnelshift_r(g[i], g[i + 1], by2 ? 16 : 0);
-    }
+    cut(t, back >> 2, back & 2 ? 16 : 0, g);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) g[i] = x.w[i];
   }
-  if ((threadIdx.x & 31) == 0) return;
-  const int first = c - (int)o / SIZE;   // of the row's elements in g
-  if (first >= 0 && first + E <= cols) {
-    *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
-  } else {
+  const int lane = threadIdx.x & 31, first = c - (int)o / SIZE;   // of the row's elements in g
+  const bool payload = lane > 0 && lane <= PAYLOAD, whole = first >= 0 && first + E <= cols;
+  if (payload && whole) *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
+  if (__any_sync(0xffffffffu, payload && !whole && first < cols)) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (first + e >= 0 && first + e < cols) {
+      if (payload && !whole && first + e >= 0 && first + e < cols) {
         if (BF16) reinterpret_cast<uint16_t*>(p - o)[e] = (uint16_t)(g[(e >> 1) & 3] >> (16 * (e & 1)));
         else reinterpret_cast<uint32_t*>(p - o)[e] = g[e & 3];
       }
@@ -302,6 +310,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
   int c[NV], nv[NV], count[NV];
   columns<BX, NV, A>(cols, WARP, c, nv, count);
+  const bool ragged = warp_ragged<BX, NV, A>(nv);
   constexpr int S = FWD_STAGES, E = BX ? 8 : 4, P = E / 2;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : 1);
   int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
@@ -328,7 +337,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
     float2 x[NV][P];
     {
       Vals<BX, E> raw[NV];
-      rows.get(raw, nv);
+      rows.get(raw, nv, ragged);
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
           const float2 d = add2(x[v][i], splat2(-mean));
           s = fma2(d, d, s);
         }
-      } else if (!A) {
+      } else if (!A && count[v]) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 d = add2(x[v][i], splat2(-mean));
@@ -457,6 +466,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
   const int cols = (int)a.cols;
   int c[NV], nv[NV], count[NV];
   columns<BX, NV, A>(cols, WARP, c, nv, count);
+  const bool ragged = warp_ragged<BX, NV, A>(nv);
   const bool sums = a.work != nullptr;
   using R = Rows<BX, NV, A, S>;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : RI);
@@ -503,8 +513,8 @@ __global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS ==
     Vals<BX, E> x[RI][NV], dy[RI][NV];
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
-      xs[q].get(x[q], nv);
-      dys[q].get(dy[q], nv);
+      xs[q].get(x[q], nv, ragged);
+      dys[q].get(dy[q], nv, ragged);
     }
     if (!A) __syncwarp();
     // into the stage that was read a round ago
@@ -737,7 +747,7 @@ struct Variant {
   int vectors, threads;             // threads: 32, or a CTA's; 0: too wide
 };
 inline Variant variant_of(int64_t cols, bool bf16, bool aligned) {
-  const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = aligned ? 32 : 31;
+  const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = aligned ? 32 : PAYLOAD;
   const int64_t slots = ceil_div(cols, e) + (aligned ? 0 : 1);   // unaligned rows end in 16 bytes more
   for (int n = one; n <= 4 * one; n *= 2)
     if (slots <= n * lanes) return {n, 32};
