@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 // ---- the gradients ----
 // RI rows of a CTA (adjacent ones) share a round of sums.
 template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 256 ? 2 : 1)
+__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 512 || NV > 4 ? 1 : 2)
     grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
   constexpr int S = GRAD_STAGES, E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, WARP);
@@ -742,14 +742,14 @@ constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold (a fe
 constexpr int64_t SMS = 148;
 
 // Vectors per thread and threads of a row: a warp's where it holds the row in
-// `one`, `one` * 2 or `one` * 4 vectors a lane, else a CTA's with `one` * 2.
+// `one` to `most` * `one` vectors a lane, else a CTA's with `one` * 2.
 struct Variant {
   int vectors, threads;             // threads: 32, or a CTA's; 0: too wide
 };
-inline Variant variant_of(int64_t cols, bool bf16, bool aligned) {
+inline Variant variant_of(int64_t cols, bool bf16, bool aligned, int most) {
   const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = aligned ? 32 : PAYLOAD;
   const int64_t slots = ceil_div(cols, e) + (aligned ? 0 : 1);   // unaligned rows end in 16 bytes more
-  for (int n = one; n <= 4 * one; n *= 2)
+  for (int n = one; n <= most * one; n += one)
     if (slots <= n * lanes) return {n, 32};
   const int64_t threads = ceil_div(slots, 2 * one * lanes) * 32;
   return {2 * one, threads <= 512 ? (int)threads : 0};
@@ -793,12 +793,13 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   const bool vec = aligned16(a.x) && aligned16(a.y) && a.cols % 8 == 0 && a.ldx * (BX ? 2 : 4) % 16 == 0;
   const int wvec = aligned16(a.weight) && aligned16(a.bias);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, vec);
+  const Variant v = variant_of(a.cols, BX, vec, 4);
   int64_t n = 1;
   if (a.cols > MOST || v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
   else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
   else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
   else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+  else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, 32, vec, wvec, s);
   else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
   else n = forward_variant<BX, BW, N, 32>(a, 32, vec, wvec, s);
   const cudaError_t e = cudaGetLastError();
@@ -820,7 +821,7 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
                    a.lddy * (BX ? 2 : 4) % 16 == 0;
   const int wvec = aligned16(a.weight);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, vec);
+  const Variant v = variant_of(a.cols, BX, vec, BX ? 3 : 4);   // bf16 rows of four vectors a lane would leave an SM eight warps
   int64_t parts = 0;
   if (a.cols > MOST || v.threads == 0) {
     parts = wide_parts(a.rows);
@@ -831,7 +832,9 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
   } else if (v.threads > 32) {
     parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
   } else if (v.vectors == 4 * N) {
-    parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+    if constexpr (!BX) parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+  } else if (v.vectors == 3 * N) {
+    parts = grad_variant<BX, BW, 3 * N, 32>(a, 32, vec, wvec, s);
   } else if (v.vectors == 2 * N) {
     parts = grad_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
   } else {
