@@ -197,15 +197,17 @@ struct Rows {
   uint32_t bytes;                                   // of a row
   uint32_t at[NV];                                  // this thread's vectors, in bytes
   int to, from;                                     // stages
+  int behind;                                       // the next lane's slot; the last lane, which needs none, takes its own
 
-  // 16-byte slots of a CTA; the last lane of all reads one behind its own
-  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * threads + (A ? 0 : 1); }
+  // 16-byte slots of a CTA
+  __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * threads; }
   __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t row, int64_t step, int cols, const int (&c)[NV]) {
     own = smem + threadIdx.x;
     ahead = now = static_cast<const unsigned char*>(p) + row * ld * SIZE;
     stride = step * ld * SIZE;
     bytes = (uint32_t)cols * SIZE;
     to = from = 0;
+    behind = (threadIdx.x & 31) == 31 ? 0 : 1;
 #pragma unroll
     for (int v = 0; v < NV; ++v) at[v] = (uint32_t)c[v] * SIZE;
   }
@@ -235,7 +237,7 @@ struct Rows {
       if (A) {
         x[v].w[0] = q.x; x[v].w[1] = q.y; x[v].w[2] = q.z; x[v].w[3] = q.w;   // behind the row's end: anything
       } else {
-        const uint4 n = slot[1];
+        const uint4 n = slot[behind];
         const uint32_t t[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
         cut(t, o >> 2, o & 2 ? 16 : 0, x[v].w);
       }

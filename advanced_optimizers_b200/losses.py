@@ -131,12 +131,15 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
         raise ValueError(f"token_logprobs: the temperature must be between 1e-30 and 1e30, got {temperature}")
     if not 0 < logits.shape[-1] < 1 << 31 or tokens.numel() >= 1 << 31:
         raise ValueError("token_logprobs: fewer than 2^31 tokens, rows of 1 to 2^31 - 1 logits")
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"token_logprobs: ignore_index must fit 64 bits, got {ignore_index}")
     refuse_tangents("token_logprobs", logits)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogprobs.apply(logits, (tokens, temperature, int(ignore_index), dtype))
-    return _token_logprobs(logits, tokens, temperature, int(ignore_index), dtype, False)[0]
+        return _TokenLogprobs.apply(logits, (tokens, temperature, ignore_index, dtype))
+    return _token_logprobs(logits, tokens, temperature, ignore_index, dtype, False)[0]
 
 
 # ---- losses ----

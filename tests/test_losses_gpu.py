@@ -350,6 +350,33 @@ def test_losses_repeat_on_other_streams_and_in_graphs(R, C):
     assert all(same(o, want) for o in outs)
 
 
+@pytest.mark.parametrize("R,V", [(5, 50257), (300, 9001), (200, 70001), (400, 40), (200, 900)])
+def test_logprobs_of_every_variant_in_a_graph(R, V):
+    """Two graphs of the same call in turn, each with its own buffers, on inputs that changed since their capture."""
+    import advanced_optimizers_b200 as A
+    x, t, g = case(R, V, B)
+    leaf = x.requires_grad_()
+
+    def run():
+        lp = A.token_logprobs(leaf, t, temperature=0.9)
+        return [lp.detach(), *torch.autograd.grad(lp, leaf, g)]
+
+    run()
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run())
+    with torch.no_grad():
+        x.mul_(1.25)
+        t.copy_(t.flip(0))
+    t[::7] = IGNORE
+    for graph in graphs * 2:
+        graph.replay()
+    want = run()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
 def test_gradients_against_differences():
     """The kernels' own difference quotients along a direction, within their rounding and the 64-bit quotients' truncation."""
     import advanced_optimizers_b200 as A

@@ -153,6 +153,7 @@ def test_refusals_behind_the_device_check(monkeypatch):
         (ValueError, "temperature", lambda: A.token_logprobs(x, ids, temperature=0)),
         (ValueError, "temperature", lambda: A.token_logprobs(x, ids, temperature=NAN)),
         (ValueError, "rows of 1", lambda: A.token_logprobs(x[:, :0], ids)),
+        (ValueError, "64 bits", lambda: A.token_logprobs(x, ids, ignore_index=1 << 63)),
         (NotImplementedError, "not supported", lambda: A.policy_loss(h, h, h)),
         (ValueError, "dtype", lambda: A.policy_loss(x, h, x)),
         (ValueError, "shape", lambda: A.policy_loss(x, x[:, :7], x)),
