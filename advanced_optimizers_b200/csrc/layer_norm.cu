@@ -304,7 +304,7 @@ constexpr int FWD_STAGES = 4, GRAD_STAGES = 3;
 __host__ __device__ constexpr int grad_rows(bool bf16, bool warp) { return bf16 && !warp ? 2 : 1; }
 
 template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 512 ? 2 : MAX_THREADS == 256 ? 4 : 1)
+__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 ? 1 : MAX_THREADS == 256 ? (A ? 4 : 3) : 2)
     forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
   extern __shared__ uint4 smem[];
@@ -798,7 +798,8 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   const Variant v = variant_of(a.cols, BX, vec, 4);
   int64_t n = 1;
   if (a.cols > MOST || v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+  else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v.threads, vec, wvec, s);
   else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
   else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
   else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, 32, vec, wvec, s);
