@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 // ---- the gradients ----
 // RI rows of a CTA (adjacent ones) share a round of sums.
 template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 512 ? 512 : 256, MAX_THREADS == 512 || NV > 4 ? 1 : 2)
+__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS > 256 || (MAX_THREADS == 32 && NV > 4) ? 1 : 2)
     grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
   constexpr int S = GRAD_STAGES, E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, WARP);
@@ -786,8 +786,9 @@ int64_t forward_variant(const advopt_layer_norm_args& a, int row_threads, bool v
   constexpr bool WARP = MAX_THREADS == 32;
   const int threads = WARP ? WARPS * 32 : row_threads;
   const int64_t most = WARP ? ceil_div(a.rows, WARPS) : a.rows;
-  if (vec) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16, most, s);
-  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, Rows<BX, NV, false, FWD_STAGES>::slots_of(threads) * 16, most, s);
+  const int smem = Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16;
+  if (vec) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, smem, most, s);
+  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, smem, most, s);
 }
 
 template <bool BX, bool BW>
@@ -813,9 +814,9 @@ template <bool BX, bool BW, int NV, int MAX_THREADS>
 int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
   const int threads = MAX_THREADS == 32 ? WARPS * 32 : row_threads;
   const int64_t most = grad_ctas(a.rows, a.cols);
-  constexpr int arrays = 2 * grad_rows(BX, MAX_THREADS == 32);
-  if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, arrays * Rows<BX, NV, true, GRAD_STAGES>::slots_of(threads) * 16, most, s);
-  return launch<grad_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, arrays * Rows<BX, NV, false, GRAD_STAGES>::slots_of(threads) * 16, most, s);
+  const int smem = 2 * grad_rows(BX, MAX_THREADS == 32) * Rows<BX, NV, true, GRAD_STAGES>::slots_of(threads) * 16;
+  if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, smem, most, s);
+  return launch<grad_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, smem, most, s);
 }
 
 template <bool BX, bool BW>
@@ -830,8 +831,10 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
     parts = wide_parts(a.rows);
     if (a.dx) wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
     if (a.work) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
-  } else if (v.threads > 256) {
+  } else if (v.threads > 384) {
     parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+  } else if (v.threads > 256) {
+    parts = grad_variant<BX, BW, 2 * N, 384>(a, v.threads, vec, wvec, s);
   } else if (v.threads > 32) {
     parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
   } else if (v.vectors == 4 * N) {
