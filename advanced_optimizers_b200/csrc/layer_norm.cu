@@ -3,12 +3,15 @@
 //   dx = rstd * (g - mean of g - h * mean of g h), dw = sum of dy h, db = sum of dy.
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and
-// writes dx, each once.  A row stays in the registers of one warp (up to 1024
-// columns) or one CTA (up to 8192), so the variance is that of the
-// differences from the mean, in float32, without a second read.  Wider rows
-// are read again (from L2).  dw and db are summed down the columns that a
-// thread holds, over all rows its CTA takes; the CTAs' sums are added in order
-// by a second launch, so that results repeat bit for bit.
+// writes dx, each once (16384 x 4096 bf16: 47 and 78 us for 41 and 61 of HBM's;
+// the second is bound by its instructions at 16 warps an SM, 25 an element).
+// A row stays in the registers of one warp (up to 1024 columns) or one CTA (up
+// to 16384), so the variance is that of the differences from the mean, in
+// float32, without a second read.  Wider rows are read again (from L2).  dw
+// and db are summed down the columns that a thread holds, over all rows its CTA
+// takes (up to 8192 columns, else by a kernel of their own that reads again);
+// the CTAs' sums are added in order by one more launch, so that results repeat
+// bit for bit.
 #include <atomic>
 #include <type_traits>
 
@@ -47,41 +50,42 @@ __device__ __forceinline__ float warp_sums(float (&v)[N]) {
   return a;
 }
 
-// Sums of N values over the warp or the CTA (up to 16 warps); every thread gets
-// them.  `red` has room for two rounds, so that one barrier a round is enough;
-// what it holds for warps that are not there is 0 (clear_sums).
-template <bool WARP, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float4 (*red)[4 * N], int& round) {
+// Sums of N values over the warp (Q = 0) or the CTA of up to 4 Q warps; every
+// thread gets them.  `red` has room for two rounds, so that one barrier a round
+// is enough; what it holds for warps that are not there is 0 (clear_sums).
+template <int N, int Q>
+__device__ __forceinline__ void row_sum(float (&v)[N], float4 (*red)[Q ? Q * N : 1], int& round) {
   const float a = warp_sums<N>(v);
-  if constexpr (WARP) {
+  if constexpr (Q == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = N == 1 ? a : __shfl_sync(0xffffffffu, a, i * (32 / N));
   } else {
     float4* r = red[round];
     round ^= 1;
     const int lane = threadIdx.x & 31;
-    if (lane % (32 / N) == 0) reinterpret_cast<float*>(r + lane / (32 / N) * 4)[threadIdx.x >> 5] = a;
+    if (lane % (32 / N) == 0) reinterpret_cast<float*>(r + lane / (32 / N) * Q)[threadIdx.x >> 5] = a;
     __syncthreads();
-    const bool many = blockDim.x > 256;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float4 q = r[i * 4], p = r[i * 4 + 1];
-      v[i] = __fadd_rn(__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w)), __fadd_rn(__fadd_rn(p.x, p.y), __fadd_rn(p.z, p.w)));
-    }
-    if (many) {
+      float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float4 q = r[i * 4 + 2], p = r[i * 4 + 3];
-        v[i] = __fadd_rn(v[i], __fadd_rn(__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w)), __fadd_rn(__fadd_rn(p.x, p.y), __fadd_rn(p.z, p.w))));
+      for (int k = 0; k < Q; ++k) {
+        const float4 q = r[i * Q + k];
+        s = add2(s, add2(make_float2(q.x, q.y), make_float2(q.z, q.w)));
       }
+      v[i] = __fadd_rn(s.x, s.y);
     }
   }
 }
-template <int N>
-__device__ __forceinline__ void clear_sums(float4 (*red)[4 * N]) {
-  if (threadIdx.x < 2 * 4 * N) red[threadIdx.x / (4 * N)][threadIdx.x % (4 * N)] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  __syncthreads();
+template <int N, int Q>
+__device__ __forceinline__ void clear_sums(float4 (*red)[Q ? Q * N : 1]) {
+  if constexpr (Q > 0) {
+    for (int i = threadIdx.x; i < 2 * Q * N; i += blockDim.x) red[i / (Q * N)][i % (Q * N)] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __syncthreads();
+  }
 }
+// Q of a kernel for rows of up to `threads` threads (32: a warp's).
+__host__ __device__ constexpr int quads(int threads) { return threads == 32 ? 0 : threads / 128; }
 
 // A thread's columns: NV vectors of 16 bytes of x, each warp's (or CTA's) next
 // to one another.  nv: how many of a vector's elements there are.  Where rows do
@@ -304,14 +308,15 @@ __device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsig
 // 48 (4096 x 8192 float32), three backward 87 where two take 84 (16384 x 4096 bf16; float32 70 and 72).
 constexpr int FWD_STAGES = 3;
 __host__ __device__ constexpr int grad_stages(bool bf16) { return bf16 ? 2 : 3; }
-__host__ __device__ constexpr int grad_rows(bool bf16, bool warp) { return bf16 && !warp ? 2 : 1; }
+__host__ __device__ constexpr int grad_rows(bool bf16, int max_threads) { return bf16 && max_threads > 32 && max_threads < 1024 ? 2 : 1; }
 
 template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 ? 1 : MAX_THREADS == 256 ? (A ? 4 : 3) : 2)
+__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 || MAX_THREADS == 1024 ? 1 : MAX_THREADS == 256 ? (A ? 4 : 3) : 2)
     forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
+  constexpr int Q = quads(MAX_THREADS);
   extern __shared__ uint4 smem[];
-  __shared__ float4 red[2][4];
+  __shared__ float4 red[2][Q ? Q : 1];
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
   int c[NV], nv[NV], count[NV];
   columns<BX, NV, A>(cols, WARP, c, nv, count);
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     rows.issue(r + s * step < a.rows);
     commit_copies();
   }
-  if (!WARP) clear_sums<1>(red);
+  clear_sums<1, Q>(red);
   Vals<BW, E> w[NV], b[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
         for (int i = 0; i < P; ++i) s = add2(s, x[v][i]);
       }
     float t[1] = {__fadd_rn(s.x, s.y)};
-    row_sum<WARP, 1>(t, red, round);
+    row_sum<1, Q>(t, red, round);
     const float mean = __fmul_rn(t[0], inv);
     s = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
       }
     }
     t[0] = __fadd_rn(s.x, s.y);
-    row_sum<WARP, 1>(t, red, round);
+    row_sum<1, Q>(t, red, round);
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(t[0], inv, a.eps)));
     const float2 rstd2 = splat2(rstd), shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
     if (a.stats && lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
@@ -465,14 +470,15 @@ template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
 __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS > 256 || (MAX_THREADS == 32 && NV > 4) ? 1 : 2)
     grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
-  constexpr int S = grad_stages(BX), E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, WARP);
+  constexpr int S = grad_stages(BX), E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, MAX_THREADS), Q = quads(MAX_THREADS);
+  constexpr bool SUMS = MAX_THREADS < 1024;   // of more threads, the registers do not hold the columns' sums
   extern __shared__ uint4 smem[];
-  __shared__ float4 red[2][8 * RI];
+  __shared__ float4 red[2][Q ? Q * 2 * RI : 1];
   const int cols = (int)a.cols;
   int c[NV], nv[NV], count[NV];
   columns<BX, NV, A>(cols, WARP, c, nv, count);
   const bool ragged = warp_ragged<BX, NV, A>(nv);
-  const bool sums = a.work != nullptr;
+  const bool sums = SUMS && a.work != nullptr;
   using R = Rows<BX, NV, A, S>;
   const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : RI);
   int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x * RI;
@@ -492,7 +498,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     }
     commit_copies();
   }
-  if (!WARP) clear_sums<2 * RI>(red);
+  clear_sums<2 * RI, Q>(red);
   Vals<BW, E> w[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) w[v].weights(a.weight, 1.0f, c[v], nv[v], wvec);
@@ -547,8 +553,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
               const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
               s1 = add2(s1, g);
               s2 = fma2(g, h, s2);
-              dw[v][i] = fma2(d, h, dw[v][i]);
-              db[v][i] = add2(db[v][i], d);
+              if (SUMS) dw[v][i] = fma2(d, h, dw[v][i]), db[v][i] = add2(db[v][i], d);
             }
           } else if (!A && count[v]) {
 #pragma unroll
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
               s1 = add2(s1, g);   // dy is 0 behind the row's end; h, of a mean that may be infinite, is left out there
               if (2 * i < count[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
               if (2 * i + 1 < count[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
-              db[v][i] = add2(db[v][i], d);
+              if (SUMS) db[v][i] = add2(db[v][i], d);
             }
           }
         }
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
       t[2 * q + 1] = __fadd_rn(s2.x, s2.y);
     }
     if (!a.dx) continue;
-    row_sum<WARP, 2 * RI>(t, red, round);
+    row_sum<2 * RI, Q>(t, red, round);
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
       if (!here[q]) continue;
@@ -632,7 +637,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
   }
 }
 
-// Rows that no CTA's registers hold: dx from two reads of a row, dw and db by columns.
+// Rows that no CTA's registers hold, and float32 ones of more than 8192 columns: dx from two reads of a row.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_dx_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int vec, int wvec) {
   __shared__ float red[2][32];
@@ -743,7 +748,7 @@ __global__ void __launch_bounds__(FINISH_WARPS * 32) finish_kernel(void* dweight
 }
 
 // ---- variants ----
-constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold (a few hundred fewer of unaligned rows)
+constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold with their sums (a few hundred fewer of unaligned rows)
 constexpr int64_t SMS = 148;
 
 // Vectors per thread and threads of a row: a warp's where it holds the row in
@@ -757,7 +762,7 @@ inline Variant variant_of(int64_t cols, bool bf16, bool aligned, int most) {
   for (int n = one; n <= most * one; n += one)
     if (slots <= n * lanes) return {n, 32};
   const int64_t threads = ceil_div(slots, 2 * one * lanes) * 32;
-  return {2 * one, threads <= 512 ? (int)threads : 0};
+  return {2 * one, threads <= 1024 ? (int)threads : 0};
 }
 // CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows at least where that leaves one for each SM.
 inline int64_t grad_ctas(int64_t rows, int64_t cols) {
@@ -801,7 +806,8 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   constexpr int N = BX ? 1 : 2;
   const Variant v = variant_of(a.cols, BX, vec, 4);
   int64_t n = 1;
-  if (a.cols > MOST || v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+  if (v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+  else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v.threads, vec, wvec, s);
   else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
   else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v.threads, vec, wvec, s);
   else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
@@ -816,8 +822,8 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
 template <bool BX, bool BW, int NV, int MAX_THREADS>
 int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
   const int threads = MAX_THREADS == 32 ? WARPS * 32 : row_threads;
-  const int64_t most = grad_ctas(a.rows, a.cols);
-  const int smem = 2 * grad_rows(BX, MAX_THREADS == 32) * Rows<BX, NV, true, grad_stages(BX)>::slots_of(threads) * 16;
+  const int64_t most = MAX_THREADS < 1024 ? grad_ctas(a.rows, a.cols) : a.rows;
+  const int smem = 2 * grad_rows(BX, MAX_THREADS) * Rows<BX, NV, true, grad_stages(BX)>::slots_of(threads) * 16;
   if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, smem, most, s);
   return launch<grad_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, smem, most, s);
 }
@@ -830,10 +836,16 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
   constexpr int N = BX ? 1 : 2;
   const Variant v = variant_of(a.cols, BX, vec, BX ? 3 : 4);   // bf16 rows of four vectors a lane would leave an SM eight warps
   int64_t parts = 0;
-  if (a.cols > MOST || v.threads == 0) {
+  if (a.cols > MOST || v.threads == 0 || v.threads > 512) {
     parts = wide_parts(a.rows);
-    if (a.dx) wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-    if (a.work) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
+    // float32 rows of that width would not fit shared memory twice
+    if (a.dx && BX && v.threads) {
+      if constexpr (BX)
+        if (grad_variant<BX, BW, 2 * N, 1024>(a, v.threads, vec, wvec, s) < 0) parts = -1;
+    } else if (a.dx) {
+      wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+    }
+    if (a.work && parts > 0) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
   } else if (v.threads > 384) {
     parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
   } else if (v.threads > 256) {
