@@ -1,16 +1,19 @@
 // Token embedding: y_t = scale * W[id_t], and its gradient
 // dW_v = scale * sum of dy_t over the tokens t with id_t = v.
 //
-// Forward: a gather, bound by HBM (touched rows read once, y written once).
+// Forward: a gather, bound by HBM (touched rows read once, y written once: 8192
+// x 4096 bf16 17.7 us).
 //
 // Gradient: bound by HBM too (dy read once, every row of dW written once, of
-// which most are zeros).  The tokens are put in order of their ids first (a
-// stable radix sort, so that the order of a row's sum follows from the ids
-// alone); then each warp takes 32 tokens of that order for 256 columns and
-// sums and writes, from registers, the rows that begin among them.  A row
-// that fills a whole such chunk, and so may be of any length, leaves a float32
-// partial sum in each of its chunks, and a third launch adds these up in
-// order.  No atomics: results repeat bit for bit.
+// which most are zeros: 8192 x 4096 of 128256 bf16 172 us, 140 of them for 1.05
+// GB of zeros).  The tokens are put in order of their ids first (a stable radix
+// sort, so that the order of a row's sum follows from the ids alone); then each
+// warp takes 8 or 32 tokens of that order, for 16 bytes a lane, and sums and
+// writes, from registers, the rows that begin among them (25 us).  A row that
+// fills a whole such chunk, and so may be of any length, leaves a float32
+// partial sum in each of its chunks, and a further launch adds these up in
+// order (7 us).  No float atomics: results repeat bit for bit.  Few tokens take
+// one launch that compares instead of sorting.
 #include <cooperative_groups.h>
 
 #include "advopt.h"
@@ -101,14 +104,6 @@ constexpr int AHEAD = 8;               // tokens of a lane whose loads are on th
 constexpr int SORT_SMEM = (SORT_WARPS * BINS + 2 * BINS + SORT_WARPS) * 4;
 constexpr int FILL_THREADS = 512, FILL = 4;   // 16-byte stores of a thread that writes zeros
 
-// One cluster sorts, beside the kernel that writes the zeros: the sort reads and
-// writes a few hundred KB that stay in L2, and takes less time than the zeros
-// of a large table.
-//
-// A pass: every warp counts the digits of its contiguous share,
-// the counts are summed over the digits, CTAs and warps before it, and the
-// warp walks its share again, in order, and places each token behind those of
-// its digit that came before.
 // The lanes of `live` with this lane's digit, bit by bit (65536 tokens of a
 // vocabulary of 50257: 36 us for the sort, with __match_any_sync 42).
 __device__ __forceinline__ uint32_t peers_of(uint32_t d, uint32_t live) {
@@ -122,6 +117,14 @@ __device__ __forceinline__ uint32_t peers_of(uint32_t d, uint32_t live) {
   return peers;
 }
 
+// One cluster sorts, beside the kernel that writes the zeros: the sort reads and
+// writes a few hundred KB that stay in L2, and takes less time than the zeros
+// of a large table (16 us for 8192 tokens, two passes).
+//
+// A pass: every warp counts the digits of its contiguous share, the counts are
+// summed over the digits, CTAs and warps before it, and the warp walks its share
+// again, in order, and places each token behind those of its digit that came
+// before.
 __device__ __forceinline__ void sort_cluster(const Grad& g, uint32_t* sm) {
   cg::cluster_group cluster = cg::this_cluster();
   uint32_t* hist = sm;                                  // [SORT_WARPS][BINS]
