@@ -3,7 +3,7 @@
 //   dx = rstd * (g - mean of g - h * mean of g h), dw = sum of dy h, db = sum of dy.
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and
-// writes dx, each once (16384 x 4096 bf16: 47 and 78 us for 41 and 61 of HBM's;
+// writes dx, each once (16384 x 4096 bf16: 46 and 77 us for 41 and 61 of HBM's;
 // the second is bound by its instructions at 16 warps an SM, 25 an element).
 // A row stays in the registers of one warp (up to 1024 columns) or one CTA (up
 // to 16384), so the variance is that of the differences from the mean, in
@@ -13,7 +13,9 @@
 // the CTAs' sums are added in order by one more launch, so that results repeat
 // bit for bit.
 #include <atomic>
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "advopt.h"
 #include "capi_internal.h"
@@ -85,34 +87,72 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[Q ? Q * N : 1]) {
   }
 }
 // Q of a kernel for rows of up to `threads` threads (32: a warp's).
-__host__ __device__ constexpr int quads(int threads) { return threads == 32 ? 0 : threads / 128; }
+__host__ __device__ constexpr int quads(int threads) { return threads == 32 ? 0 : (threads + 127) / 128; }
+
+// How rows lie.  ALIGNED: all on 16-byte boundaries.  PHASE: all of a pass's
+// tensors lie the same way, and a thread's rows are eight apart, so that they
+// all begin at the same place between two boundaries; it takes the 16 bytes
+// between boundaries as they are, with the columns that these hold.  SHIFT:
+// anything else; what is read is shifted into place, and so is what is written.
+// Timed, PHASE against SHIFT: 10000 x 5003 bf16 48 us forward for 73 and 95
+// backward for 100, float32 68 for 100 and 110 for 154, 16384 x 999 float32 24
+// for 44 and 38 for 81; aligned rows of 5000 take 40 and 70 in bf16.
+constexpr int ALIGNED = 0, PHASE = 1, SHIFT = 2;
 
 // A thread's columns: NV vectors of 16 bytes of x, each warp's (or CTA's) next
-// to one another.  nv: how many of a vector's elements there are.  Where rows do
-// not start on 16-byte boundaries (A false), a warp's first lane repeats the
-// vector ahead of the warp's, whose last elements the next lane stores, and its
-// last lane the one behind, whose first ones the lane before reads; they count
-// for no sum (count).
-template <bool BF16, int NV, bool A>
-__device__ __forceinline__ void columns(int cols, bool warp_rows, int (&c)[NV], int (&nv)[NV], int (&count)[NV]) {
-  constexpr int E = BF16 ? 8 : 4;
-  const int lane = threadIdx.x & 31, warp = warp_rows ? 0 : threadIdx.x >> 5, warps = warp_rows ? 1 : blockDim.x >> 5;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    c[v] = (A ? (v * warps + warp) * 32 + lane : (v * warps + warp) * PAYLOAD + lane - 1) * E;
-    nv[v] = c[v] < 0 || c[v] >= cols ? 0 : cols - c[v] < E ? cols - c[v] : E;
-    count[v] = A || (lane > 0 && lane <= PAYLOAD) ? nv[v] : 0;
+// to one another.  PHASE: `k` elements ahead of the row share its first 16
+// bytes.  SHIFT: a warp's first lane repeats the vector ahead of the warp's,
+// whose last elements the next lane stores, and its last lane the one behind,
+// whose first ones the lane before reads; they are in no sum.
+template <bool BF16, int NV, int MODE>
+struct Columns {
+  static constexpr int E = BF16 ? 8 : 4;
+  static constexpr uint32_t WHOLE = (1u << E) - 1;
+  static_assert(NV * E <= 32, "a bit for each element");
+  int first, each;                                  // vector v begins at first + v * each
+  uint32_t row, mine;                               // a bit for each element: of the row, and to be summed by this thread
+  uint32_t ragged;                                  // a bit for each vector: the row begins or ends within one of the warp's
+  __device__ __forceinline__ int c(int v) const { return first + v * each; }
+  __device__ __forceinline__ uint32_t bits(int v) const { return row >> (v * E) & WHOLE; }
+  __device__ __forceinline__ bool whole(int v) const { return (mine >> (v * E) & WHOLE) == WHOLE; }
+  __device__ __forceinline__ bool some(int v) const { return (mine >> (v * E) & WHOLE) != 0; }
+  __device__ __forceinline__ bool has(int v, int e) const { return mine >> (v * E + e) & 1u; }
+  // The same, for a branch in the loop over rows: volatile, since what follows from the bits would be worked out ahead of
+  // the loop and take more registers than there are.
+  __device__ __forceinline__ static uint32_t here(uint32_t bits) {
+    uint32_t b;
+    asm volatile("mov.b32 %0, %1;" : "=r"(b) : "r"(bits));
+    return b;
   }
-}
-
-// Whether a row ends within one of the warp's vectors.
-template <bool BF16, int NV, bool A>
-__device__ __forceinline__ bool warp_ragged(const int (&nv)[NV]) {
-  bool some = false;
+  __device__ __forceinline__ void init(int cols, bool warp_rows, int k) {
+    const int lane = threadIdx.x & 31, warp = warp_rows ? 0 : threadIdx.x >> 5, warps = warp_rows ? 1 : blockDim.x >> 5;
+    constexpr int LANES = MODE == SHIFT ? PAYLOAD : 32;
+    first = (warp * LANES + lane - (MODE == SHIFT ? 1 : 0)) * E - (MODE == PHASE ? k : 0);
+    each = warps * LANES * E;
+    row = ragged = 0;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) some |= nv[v] > 0 && nv[v] < (BF16 ? 8 : 4);
-  return !A && __any_sync(0xffffffffu, some);
-}
+    for (int v = 0; v < NV; ++v) {
+      uint32_t q = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) q |= c(v) + e >= 0 && c(v) + e < cols ? 1u << e : 0u;
+      if (MODE != ALIGNED && __any_sync(0xffffffffu, q && q != WHOLE)) ragged |= 1u << v;
+      row |= q << (v * E);
+    }
+    mine = MODE == SHIFT && (lane == 0 || lane > PAYLOAD) ? 0u : row;
+  }
+  // Zeros in those of vectors v (N of them) that are outside the row, where the row begins or ends in one of the warp's.
+  template <class X, int N>
+  __device__ __forceinline__ void clear(int v, X* const (&x)[N]) const {
+    if (MODE == ALIGNED || !(ragged >> v & 1u)) return;
+    const uint32_t bits = here(row) >> (v * E);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = BF16 ? (bits >> (2 * i) & 1u ? 0xFFFFu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xFFFF0000u : 0u) : bits >> i & 1u ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+      for (int n = 0; n < N; ++n) x[n]->w[i] &= m;
+    }
+  }
+};
 
 // Words k .. k + 4 of eight, shifted by `bits` (0 or 16): 16 bytes from byte 4 k + bits / 8 on.  k and bits are the warp's.
 __device__ __forceinline__ void cut(const uint32_t (&t)[8], uint32_t k, uint32_t bits, uint32_t (&w)[4]) {
@@ -146,8 +186,8 @@ struct Vals {
       else w[i] = f2u(v[i]);
     }
   }
-  // `absent` where there are no weights; zeros behind the row's end
-  __device__ __forceinline__ void weights(const void* p, float absent, int c, int nv, bool vec) {
+  // `absent` where there are no weights; zeros outside the row; vec: 8-byte aligned
+  __device__ __forceinline__ void weights(const void* p, float absent, int c, uint32_t bits, bool vec) {
     if (!p) {
       float v[E];
 #pragma unroll
@@ -155,7 +195,7 @@ struct Vals {
       set(v);
       return;
     }
-    if (vec && nv == E) {
+    if (vec && bits == (1u << E) - 1) {
       const uint2* q = reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p) + (int64_t)c * (BF16 ? 2 : 4));
 #pragma unroll
       for (int i = 0; i < W / 2; ++i) {
@@ -168,7 +208,7 @@ struct Vals {
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      v[e] = e >= nv ? 0.0f : BF16 ? bf16_to_f(__ldg(static_cast<const uint16_t*>(p) + c + e)) : __ldg(static_cast<const float*>(p) + c + e);
+      v[e] = !(bits >> e & 1u) ? 0.0f : BF16 ? bf16_to_f(__ldg(static_cast<const uint16_t*>(p) + c + e)) : __ldg(static_cast<const float*>(p) + c + e);
     set(v);
   }
 };
@@ -187,33 +227,36 @@ __device__ __forceinline__ void weights(Oct<BW>& w, const void* p, float absent,
 // ---- rows on their way through shared memory ----
 // A thread copies the 16 bytes that it will read itself, several rows ahead, so
 // that only its own copies have to be waited for.  Rows that do not start on a
-// 16-byte boundary (A false) are copied from the boundary before: each 16
-// bytes hold an element of the row, and a thread's elements then reach into
-// the next lane's.
-template <bool BF16, int NV, bool A, int S>
+// 16-byte boundary are copied from the boundary before: each 16 bytes hold an
+// element of the row.  SHIFT: a thread's elements then reach into the next
+// lane's.
+template <bool BF16, int NV, int MODE, int S>
 struct Rows {
   static constexpr int E = BF16 ? 8 : 4, SIZE = BF16 ? 2 : 4;
   using X = Vals<BF16, E>;
   uint4* own;                                       // this thread's of stage 0; shared memory is [S][NV][threads]
   const unsigned char* ahead;                       // the next row to be copied
-  const unsigned char* now;                         // and to be read (A false)
+  const unsigned char* now;                         // and to be read (SHIFT)
   int64_t stride;                                   // bytes from a row to the one that follows here
   uint32_t bytes;                                   // of a row
-  uint32_t at[NV];                                  // this thread's vectors, in bytes
+  uint32_t at, each;                                // this thread's first vector, in bytes from the boundary, and from one to the next
   int to, from;                                     // stages
   int behind;                                       // the next lane's slot; the last lane, which needs none, takes its own
 
   // 16-byte slots of a CTA
   __host__ __device__ static constexpr int slots_of(int threads) { return S * NV * threads; }
-  __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t row, int64_t step, int cols, const int (&c)[NV]) {
+  __device__ __forceinline__ void init(uint4* smem, const void* p, int64_t ld, int64_t row, int64_t step, int cols, const Columns<BF16, NV, MODE>& c) {
     own = smem + threadIdx.x;
     ahead = now = static_cast<const unsigned char*>(p) + row * ld * SIZE;
     stride = step * ld * SIZE;
     bytes = (uint32_t)cols * SIZE;
     to = from = 0;
     behind = (threadIdx.x & 31) == 31 ? 0 : 1;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) at[v] = (uint32_t)c[v] * SIZE;
+    const uint32_t o = MODE == PHASE ? (uint32_t)reinterpret_cast<uintptr_t>(ahead) & 15u : 0u;
+    ahead -= o;                                     // PHASE: from here on the boundary's
+    bytes += o;
+    at = (uint32_t)(c.first * SIZE) + o;
+    each = (uint32_t)(c.each * SIZE);
   }
   __device__ __forceinline__ static void copy(uint4* slot, const unsigned char* p) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot)), "l"(p) : "memory");
@@ -221,39 +264,29 @@ struct Rows {
   // The next row, if it is there.
   __device__ __forceinline__ void issue(bool there) {
     if (there) {
-      const uint32_t o = A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(ahead) & 15u, end = bytes + o;
+      const uint32_t o = MODE == SHIFT ? (uint32_t)reinterpret_cast<uintptr_t>(ahead) & 15u : 0u, end = bytes + o;
       const unsigned char* p = ahead - o;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (at[v] < end) copy(own + (to * NV + v) * (int)blockDim.x, p + at[v]);
+        if (at + v * each < end) copy(own + (to * NV + v) * (int)blockDim.x, p + (at + v * each));
     }
     ahead += stride;
     to = to == S - 1 ? 0 : to + 1;
   }
-  // The next row's elements, zeros behind its end in a vector that it ends in
-  // (`ragged`: the warp has one).  All lanes take part; the copies have been waited for.
-  __device__ __forceinline__ void get(X (&x)[NV], const int (&nv)[NV], bool ragged) {
-    const uint32_t o = A ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(now) & 15u;
+  // The next row's elements, anything outside it.  All lanes take part; the copies have been waited for.
+  __device__ __forceinline__ void get(X (&x)[NV]) {
+    const uint32_t o = MODE == SHIFT ? (uint32_t)reinterpret_cast<uintptr_t>(now) & 15u : 0u;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const uint4* slot = own + (from * NV + v) * (int)blockDim.x;
       const uint4 q = *slot;
-      if (A) {
-        x[v].w[0] = q.x; x[v].w[1] = q.y; x[v].w[2] = q.z; x[v].w[3] = q.w;   // behind the row's end: anything
-      } else {
+      if (MODE == SHIFT) {
         const uint4 n = slot[behind];
         const uint32_t t[8] = {q.x, q.y, q.z, q.w, n.x, n.y, n.z, n.w};
         cut(t, o >> 2, o & 2 ? 16 : 0, x[v].w);
+      } else {
+        x[v].w[0] = q.x; x[v].w[1] = q.y; x[v].w[2] = q.z; x[v].w[3] = q.w;
       }
-    }
-    if (!A && ragged) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (BF16) x[v].w[i] &= (2 * i < nv[v] ? 0xFFFFu : 0u) | (2 * i + 1 < nv[v] ? 0xFFFF0000u : 0u);
-          else x[v].w[i] = i < nv[v] ? x[v].w[i] : 0u;
-        }
     }
     now += stride;
     from = from == S - 1 ? 0 : from + 1;
@@ -265,67 +298,105 @@ __device__ __forceinline__ void wait_copies() {
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// A thread's 16 bytes at column c of an output row.  Where rows do not start on
-// 16-byte boundaries (A false), a lane stores the aligned 16 bytes that its
-// elements begin in, with the lane before's last ones; only a row's first and
-// last ones are not whole.  All lanes take part.
-template <bool BF16, bool A>
-__device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsigned char* row, int c, int nv, int cols) {
+// A thread's vector v of an output row.  SHIFT: a lane stores the aligned 16
+// bytes that its elements begin in, with the lane before's last ones.  Only a
+// row's first and last 16 bytes are not whole.  All lanes take part.
+template <bool BF16, int NV, int MODE>
+__device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsigned char* row, const Columns<BF16, NV, MODE>& col, int v, int cols) {
   constexpr int SIZE = BF16 ? 2 : 4, E = 16 / SIZE;
-  unsigned char* p = row + (int64_t)c * SIZE;
-  if (A) {
-    if (nv) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
-    return;
-  }
-  const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
-  uint32_t t[8], g[4];   // the previous lane's words, then this lane's
+  unsigned char* p = row + (int64_t)col.c(v) * SIZE;
+  if constexpr (MODE == ALIGNED) {
+    if (col.some(v)) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+  } else if constexpr (MODE == PHASE) {
+    if (col.whole(v)) *reinterpret_cast<uint4*>(p) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+    if ((col.ragged >> v & 1u) && !col.whole(v) && col.some(v)) {
+      const uint32_t bits = col.here(col.row) >> (v * E);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    t[i] = __shfl_up_sync(0xffffffffu, x.w[i], 1);
-    t[4 + i] = x.w[i];
-  }
-  if (o) {
-    const uint32_t back = 16u - o;
-    cut(t, back >> 2, back & 2 ? 16 : 0, g);
+      for (int e = 0; e < E; ++e)
+        if (bits >> e & 1u) {
+          if (BF16) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(x.w[(e >> 1) & 3] >> (16 * (e & 1)));
+          else reinterpret_cast<uint32_t*>(p)[e] = x.w[e & 3];
+        }
+    }
   } else {
+    const uint32_t o = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+    uint32_t t[8], g[4];   // the previous lane's words, then this lane's
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = x.w[i];
-  }
-  const int lane = threadIdx.x & 31, first = c - (int)o / SIZE;   // of the row's elements in g
-  const bool payload = lane > 0 && lane <= PAYLOAD, whole = first >= 0 && first + E <= cols;
-  if (payload && whole) *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
-  if (__any_sync(0xffffffffu, payload && !whole && first < cols)) {
+    for (int i = 0; i < 4; ++i) {
+      t[i] = __shfl_up_sync(0xffffffffu, x.w[i], 1);
+      t[4 + i] = x.w[i];
+    }
+    if (o) {
+      const uint32_t back = 16u - o;
+      cut(t, back >> 2, back & 2 ? 16 : 0, g);
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (payload && !whole && first + e >= 0 && first + e < cols) {
-        if (BF16) reinterpret_cast<uint16_t*>(p - o)[e] = (uint16_t)(g[(e >> 1) & 3] >> (16 * (e & 1)));
-        else reinterpret_cast<uint32_t*>(p - o)[e] = g[e & 3];
-      }
+      for (int i = 0; i < 4; ++i) g[i] = x.w[i];
+    }
+    const int lane = threadIdx.x & 31, first = col.c(v) - (int)o / SIZE;   // of the row's elements in g
+    const bool payload = lane > 0 && lane <= PAYLOAD, whole = first >= 0 && first + E <= cols;
+    if (payload && whole) *reinterpret_cast<uint4*>(p - o) = make_uint4(g[0], g[1], g[2], g[3]);
+    if (__any_sync(0xffffffffu, payload && !whole && first < cols)) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (payload && !whole && first + e >= 0 && first + e < cols) {
+          if (BF16) reinterpret_cast<uint16_t*>(p - o)[e] = (uint16_t)(g[(e >> 1) & 3] >> (16 * (e & 1)));
+          else reinterpret_cast<uint32_t*>(p - o)[e] = g[e & 3];
+        }
+    }
   }
 }
+
+// The rows of a CTA (or warp): from `first` on, `each` apart within a round, `step` from round to round.  PHASE: a CTA's
+// all begin at one place, so eight CTAs make a group (fewer where there are fewer rows); SUMS:
+// also those of its warps.
+template <int MODE, bool WARP, int RI, bool SUMS>
+struct Walk {
+  int64_t first, each, step;
+  __device__ __forceinline__ Walk() {
+    const int64_t warp = WARP ? threadIdx.x >> 5 : 0;
+    if (MODE == PHASE && (SUMS || !WARP)) {
+      constexpr int64_t ROWS = (WARP ? WARPS : RI) * 8;
+      first = (int64_t)(blockIdx.x / 8) * ROWS + warp * 8 + blockIdx.x % 8;
+      each = 8;
+      step = (gridDim.x < 8 ? 1 : gridDim.x / 8) * ROWS;
+    } else {
+      constexpr int64_t ROWS = WARP ? WARPS : RI;
+      first = (int64_t)blockIdx.x * ROWS + warp;
+      each = 1;
+      step = (int64_t)gridDim.x * ROWS;
+    }
+  }
+};
 
 // Stages: rows of a thread on their way, and the one that it reads.  Timed: four forward cost 60 us where three take
 // 48 (4096 x 8192 float32), three backward 87 where two take 84 (16384 x 4096 bf16; float32 70 and 72).
 constexpr int FWD_STAGES = 3;
 __host__ __device__ constexpr int grad_stages(bool bf16) { return bf16 ? 2 : 3; }
-__host__ __device__ constexpr int grad_rows(bool bf16, int max_threads) { return bf16 && max_threads > 32 && max_threads < 1024 ? 2 : 1; }
+// Rows of a CTA that share a round of sums: two of bf16, but one where the fewer registers let two CTAs run on an SM: 320
+// threads and 384 of aligned rows (10000 x 5000: 86 -> 69 us, x 6000: 101 -> 91; unaligned ones of 320 gained nothing).
+__host__ __device__ constexpr bool two_ctas(bool bf16, int max_threads, int mode) { return bf16 && mode == ALIGNED && (max_threads == 320 || max_threads == 384); }
+__host__ __device__ constexpr int grad_rows(bool bf16, int max_threads, int mode) {
+  return bf16 && max_threads > 32 && max_threads < 1024 && !two_ctas(bf16, max_threads, mode) ? 2 : 1;
+}
 
-template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 || MAX_THREADS == 1024 ? 1 : MAX_THREADS == 256 ? (A ? 4 : 3) : 2)
+template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE>
+__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 || MAX_THREADS == 1024 ? 1 : MAX_THREADS == 256 ? (MODE == ALIGNED ? 4 : 3) : 2)
     forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
   constexpr int Q = quads(MAX_THREADS);
   extern __shared__ uint4 smem[];
   __shared__ float4 red[2][Q ? Q : 1];
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
-  int c[NV], nv[NV], count[NV];
-  columns<BX, NV, A>(cols, WARP, c, nv, count);
-  const bool ragged = warp_ragged<BX, NV, A>(nv);
   constexpr int S = FWD_STAGES, E = BX ? 8 : 4, P = E / 2;
-  const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : 1);
-  int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  Rows<BX, NV, A, S> rows;
-  rows.init(smem, a.x, a.ldx, r, step, cols, c);
+  const Walk<MODE, WARP, 1, false> walk;
+  const int64_t step = walk.step;
+  int64_t r = walk.first;
+  unsigned char* to = static_cast<unsigned char*>(a.y) + r * cols * (BX ? 2 : 4);
+  Columns<BX, NV, MODE> col;
+  col.init(cols, WARP, (int)(reinterpret_cast<uintptr_t>(to) & 15) / (BX ? 2 : 4));
+  Rows<BX, NV, MODE, S> rows;
+  rows.init(smem, a.x, a.ldx, r, step, cols, col);
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
     rows.issue(r + s * step < a.rows);
@@ -335,31 +406,35 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
   Vals<BW, E> w[NV], b[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    w[v].weights(a.weight, 1.0f, c[v], nv[v], wvec);
-    b[v].weights(a.bias, 0.0f, c[v], nv[v], wvec);
+    w[v].weights(a.weight, 1.0f, col.c(v), col.bits(v), MODE != PHASE && wvec);
+    b[v].weights(a.bias, 0.0f, col.c(v), col.bits(v), MODE != PHASE && wvec);
   }
   const float inv = __fdiv_rn(1.0f, (float)cols);
-  unsigned char* to = static_cast<unsigned char*>(a.y) + r * cols * (BX ? 2 : 4);
   int round = 0;
   for (; r < a.rows; r += step, to += step * cols * (BX ? 2 : 4)) {
     wait_copies<S - 2>();
-    if (!A) __syncwarp();   // the next lane's copies are read too
+    if (MODE == SHIFT) __syncwarp();   // the next lane's copies are read too
     float2 x[NV][P];
     {
       Vals<BX, E> raw[NV];
-      rows.get(raw, nv, ragged);
+      rows.get(raw);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        Vals<BX, E>* const all[1] = {&raw[v]};
+        col.clear(v, all);
+      }
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < P; ++i) x[v][i] = raw[v].pair(i);
     }
-    if (!A) __syncwarp();
+    if (MODE == SHIFT) __syncwarp();
     rows.issue(r + (S - 1) * step < a.rows);   // into the stage that was read a row ago
     commit_copies();
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if (count[v]) {
+      if (col.some(v)) {
 #pragma unroll
         for (int i = 0; i < P; ++i) s = add2(s, x[v][i]);
       }
@@ -369,18 +444,19 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (count[v] == E) {
+      if (col.whole(v)) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 d = add2(x[v][i], splat2(-mean));
           s = fma2(d, d, s);
         }
-      } else if (!A && count[v]) {
+      } else if (MODE != ALIGNED && col.some(v)) {
+        const uint32_t bits = col.here(col.mine) >> (v * E);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const float2 d = add2(x[v][i], splat2(-mean));
-          if (2 * i < count[v]) s.x = __fmaf_rn(d.x, d.x, s.x);
-          if (2 * i + 1 < count[v]) s.y = __fmaf_rn(d.y, d.y, s.y);
+          if (bits >> (2 * i) & 1u) s.x = __fmaf_rn(d.x, d.x, s.x);
+          if (bits >> (2 * i + 1) & 1u) s.y = __fmaf_rn(d.y, d.y, s.y);
         }
       }
     }
@@ -400,7 +476,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
       }
       Vals<BX, E> o;
       o.set(y);
-      put_row<BX, A>(o, to, c[v], nv[v], cols);
+      put_row<BX, NV, MODE>(o, to, col, v, cols);
     }
   }
 }
@@ -465,34 +541,34 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 }
 
 // ---- the gradients ----
-// RI rows of a CTA (adjacent ones) share a round of sums.
-template <bool BX, bool BW, int NV, int MAX_THREADS, bool A>
-__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS > 256 || (MAX_THREADS == 32 && NV > 4) ? 1 : 2)
+// RI rows of a CTA share a round of sums.
+template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE>
+__global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_THREADS > 256 && !two_ctas(BX, MAX_THREADS, MODE)) || (MAX_THREADS == 32 && NV > 4) ? 1 : 2)
     grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
-  constexpr int S = grad_stages(BX), E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, MAX_THREADS), Q = quads(MAX_THREADS);
+  constexpr int S = grad_stages(BX), E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, MAX_THREADS, MODE), Q = quads(MAX_THREADS);
   constexpr bool SUMS = MAX_THREADS < 1024;   // of more threads, the registers do not hold the columns' sums
   extern __shared__ uint4 smem[];
   __shared__ float4 red[2][Q ? Q * 2 * RI : 1];
   const int cols = (int)a.cols;
-  int c[NV], nv[NV], count[NV];
-  columns<BX, NV, A>(cols, WARP, c, nv, count);
-  const bool ragged = warp_ragged<BX, NV, A>(nv);
   const bool sums = SUMS && a.work != nullptr;
-  using R = Rows<BX, NV, A, S>;
-  const int64_t step = (int64_t)gridDim.x * (WARP ? WARPS : RI);
-  int64_t r = WARP ? (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5) : (int64_t)blockIdx.x * RI;
+  using R = Rows<BX, NV, MODE, S>;
+  const Walk<MODE, WARP, RI, true> walk;
+  const int64_t step = walk.step, each = walk.each;
+  int64_t r = walk.first;
+  Columns<BX, NV, MODE> col;
+  col.init(cols, WARP, (int)((reinterpret_cast<uintptr_t>(a.x) + r * a.ldx * (BX ? 2 : 4)) & 15) / (BX ? 2 : 4));
   R xs[RI], dys[RI];
 #pragma unroll
   for (int q = 0; q < RI; ++q) {
-    xs[q].init(smem + 2 * q * R::slots_of(blockDim.x), a.x, a.ldx, r + q, step, cols, c);
-    dys[q].init(smem + (2 * q + 1) * R::slots_of(blockDim.x), a.dy, a.lddy, r + q, step, cols, c);
+    xs[q].init(smem + 2 * q * R::slots_of(blockDim.x), a.x, a.ldx, r + q * each, step, cols, col);
+    dys[q].init(smem + (2 * q + 1) * R::slots_of(blockDim.x), a.dy, a.lddy, r + q * each, step, cols, col);
   }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) {
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
-      const bool there = r + s * step + q < a.rows;
+      const bool there = r + s * step + q * each < a.rows;
       xs[q].issue(there);
       dys[q].issue(there);
     }
@@ -501,7 +577,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
   clear_sums<2 * RI, Q>(red);
   Vals<BW, E> w[NV];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) w[v].weights(a.weight, 1.0f, c[v], nv[v], wvec);
+  for (int v = 0; v < NV; ++v) w[v].weights(a.weight, 1.0f, col.c(v), col.bits(v), MODE != PHASE && wvec);
   float2 dw[NV][P], db[NV][P];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
@@ -516,22 +592,27 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     bool here[RI];
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
-      here[q] = q == 0 || r + q < a.rows;
-      if (here[q]) st[q] = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + q)));
+      here[q] = q == 0 || r + q * each < a.rows;
+      if (here[q]) st[q] = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + q * each)));
     }
     wait_copies<S - 2>();
-    if (!A) __syncwarp();   // the next lane's copies are read too
+    if (MODE == SHIFT) __syncwarp();   // the next lane's copies are read too
     Vals<BX, E> x[RI][NV], dy[RI][NV];
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
-      xs[q].get(x[q], nv, ragged);
-      dys[q].get(dy[q], nv, ragged);
+      xs[q].get(x[q]);
+      dys[q].get(dy[q]);
     }
-    if (!A) __syncwarp();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      Vals<BX, E>* const all[4] = {&x[0][v], &dy[0][v], &x[RI - 1][v], &dy[RI - 1][v]};   // of one row: the same twice
+      col.clear(v, all);
+    }
+    if (MODE == SHIFT) __syncwarp();
     // into the stage that was read a round ago
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
-      const bool there = r + (S - 1) * step + q < a.rows;
+      const bool there = r + (S - 1) * step + q * each < a.rows;
       xs[q].issue(there);
       dys[q].issue(there);
     }
@@ -547,22 +628,13 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
       if (here[q]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          if (count[v] == E) {
+          if (col.some(v)) {   // x and dy are 0 where a vector is outside its row; h is not a number there only where all of a row's are
 #pragma unroll
             for (int i = 0; i < P; ++i) {
               const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
               s1 = add2(s1, g);
               s2 = fma2(g, h, s2);
               if (SUMS) dw[v][i] = fma2(d, h, dw[v][i]), db[v][i] = add2(db[v][i], d);
-            }
-          } else if (!A && count[v]) {
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-              const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
-              s1 = add2(s1, g);   // dy is 0 behind the row's end; h, of a mean that may be infinite, is left out there
-              if (2 * i < count[v]) s2.x = __fmaf_rn(g.x, h.x, s2.x), dw[v][i].x = __fmaf_rn(d.x, h.x, dw[v][i].x);
-              if (2 * i + 1 < count[v]) s2.y = __fmaf_rn(g.y, h.y, s2.y), dw[v][i].y = __fmaf_rn(d.y, h.y, dw[v][i].y);
-              if (SUMS) db[v][i] = add2(db[v][i], d);
             }
           }
         }
@@ -590,48 +662,50 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
         }
         Vals<BX, E> out;
         out.set(o);
-        put_row<BX, A>(out, to + q * row_bytes, c[v], nv[v], cols);
+        put_row<BX, NV, MODE>(out, to + q * each * row_bytes, col, v, cols);
       }
     }
   }
   if (!sums) return;
   float* part = static_cast<float*>(a.work) + (int64_t)blockIdx.x * 2 * a.cols;
   if constexpr (WARP) {
-    // the warps' sums, a warp's after the other's, in shared memory
+    // the warps' sums through shared memory, all of the same columns: [WARPS][2][NV * P][32], added in the warps' order
     wait_copies<0>();
     __syncthreads();
-    float* sh = reinterpret_cast<float*>(smem);   // [2][NV * 32 * E]
-    for (int k = 0; k < WARPS; ++k) {
-      if ((int)(threadIdx.x >> 5) == k) {
+    constexpr int ALL = 2 * NV * P;
+    static_assert(WARPS * ALL * 32 * 8 <= 2 * R::slots_of(WARPS * 32) * 16, "the rows' shared memory");
+    float2* sh = reinterpret_cast<float2*>(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v)
 #pragma unroll
-          for (int i = 0; i < P; ++i) {
-            if (!A && count[v] == 0) break;
-            float2* p = reinterpret_cast<float2*>(sh + c[v]) + i;
-            float2* q = reinterpret_cast<float2*>(sh + NV * 32 * E + c[v]) + i;
-            *p = k ? add2(*p, dw[v][i]) : dw[v][i];
-            *q = k ? add2(*q, db[v][i]) : db[v][i];
-          }
+      for (int i = 0; i < P; ++i) {
+        sh[(warp * ALL + v * P + i) * 32 + lane] = dw[v][i];
+        sh[(warp * ALL + NV * P + v * P + i) * 32 + lane] = db[v][i];
       }
-      __syncthreads();
-    }
-    for (int i = threadIdx.x; i < cols; i += blockDim.x) {
-      part[i] = sh[i];
-      part[cols + i] = sh[NV * 32 * E + i];
+    __syncthreads();
+    for (int j = warp; j < ALL; j += WARPS) {
+      float2 t = sh[j * 32 + lane];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) t = add2(t, sh[(k * ALL + j) * 32 + lane]);
+      const int m = j % (NV * P), c = col.first + m / P * col.each + m % P * 2;
+      float* p = part + j / (NV * P) * cols + c;
+      if (MODE == SHIFT && (lane == 0 || lane > PAYLOAD)) continue;
+      if (c >= 0 && c < cols) p[0] = t.x;
+      if (c + 1 >= 0 && c + 1 < cols) p[1] = t.y;
     }
   } else {
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        float* p = part + c[v] + 2 * i;
-        if (2 * i + 1 < count[v] && (cols & 1) == 0) {
+        float* p = part + col.c(v) + 2 * i;
+        if (MODE != PHASE && col.has(v, 2 * i + 1) && (cols & 1) == 0) {
           *reinterpret_cast<float2*>(p) = dw[v][i];
           *reinterpret_cast<float2*>(p + cols) = db[v][i];
         } else {
-          if (2 * i < count[v]) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
-          if (2 * i + 1 < count[v]) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
+          if (col.has(v, 2 * i)) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
+          if (col.has(v, 2 * i + 1)) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
         }
       }
   }
@@ -756,9 +830,9 @@ constexpr int64_t SMS = 148;
 struct Variant {
   int vectors, threads;             // threads: 32, or a CTA's; 0: too wide
 };
-inline Variant variant_of(int64_t cols, bool bf16, bool aligned, int most) {
-  const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = aligned ? 32 : PAYLOAD;
-  const int64_t slots = ceil_div(cols, e) + (aligned ? 0 : 1);   // unaligned rows end in 16 bytes more
+inline Variant variant_of(int64_t cols, bool bf16, int mode, int most) {
+  const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = mode == SHIFT ? PAYLOAD : 32;
+  const int64_t slots = ceil_div(cols, e) + (mode == ALIGNED ? 0 : 1);   // unaligned rows end in 16 bytes more
   for (int n = one; n <= most * one; n += one)
     if (slots <= n * lanes) return {n, 32};
   const int64_t threads = ceil_div(slots, 2 * one * lanes) * 32;
@@ -766,7 +840,8 @@ inline Variant variant_of(int64_t cols, bool bf16, bool aligned, int most) {
 }
 // CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows at least where that leaves one for each SM.
 inline int64_t grad_ctas(int64_t rows, int64_t cols) {
-  const int64_t units = cols <= 1024 ? ceil_div(rows, WARPS) : rows;
+  int64_t units = cols <= 1024 ? ceil_div(rows, WARPS) : rows;
+  if (units < 8) units = rows < 8 ? rows : 8;   // one for each place that a row may begin at
   const int64_t few = ceil_div(units, 4) > SMS ? ceil_div(units, 4) : SMS, most = 8 * SMS;
   const int64_t n = few < most ? few : most;
   return units < n ? units : n;
@@ -775,7 +850,7 @@ inline int64_t wide_parts(int64_t rows) { return rows < 8 * 32 ? ceil_div(rows, 
 
 // Launches a persistent kernel with as many CTAs as fit the SMs, `most` at most; the number of CTAs, or -1.
 template <auto KERNEL, class Arg>
-int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, cudaStream_t s) {
+int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, bool by_eight, cudaStream_t s) {
   static std::atomic<int> resident[33];   // this kernel's, by warps
   // for the current device, whichever that is
   if (smem > 47 * 1024 && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
@@ -784,82 +859,107 @@ int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, cuda
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem) != cudaSuccess || n < 1) return -1;
     resident[threads / 32].store(n, std::memory_order_relaxed);
   }
-  const int64_t grid = n * SMS < most ? n * SMS : most;
+  int64_t grid = n * SMS < most ? n * SMS : most;
+  if (by_eight && grid > 8) grid -= grid % 8;
   KERNEL<<<(unsigned)grid, threads, smem, s>>>(a, wvec);
   return grid;
 }
 
+// How the rows of matrices with these first addresses and pitches (elements) lie.
+inline int mode_of(int64_t cols, int size, std::initializer_list<std::pair<const void*, int64_t>> all) {
+  const int e = 16 / size;
+  const auto first = *all.begin();
+  bool aligned = cols % 8 == 0, same = true;
+  for (const auto& m : all) {
+    aligned = aligned && aligned16(m.first) && m.second % e == 0;
+    same = same && (reinterpret_cast<uintptr_t>(m.first) - reinterpret_cast<uintptr_t>(first.first)) % 16 == 0 && (m.second - first.second) % e == 0;
+  }
+  return aligned ? ALIGNED : same ? PHASE : SHIFT;
+}
+
 template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t forward_variant(const advopt_layer_norm_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
+int64_t forward_variant(const advopt_layer_norm_args& a, int row_threads, int mode, int wvec, cudaStream_t s) {
   constexpr bool WARP = MAX_THREADS == 32;
   const int threads = WARP ? WARPS * 32 : row_threads;
   const int64_t most = WARP ? ceil_div(a.rows, WARPS) : a.rows;
-  const int smem = Rows<BX, NV, true, FWD_STAGES>::slots_of(threads) * 16;
-  if (vec) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, smem, most, s);
-  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, smem, most, s);
+  const int smem = Rows<BX, NV, ALIGNED, FWD_STAGES>::slots_of(threads) * 16;
+  if (mode == ALIGNED) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, ALIGNED>>(a, wvec, threads, smem, most, false, s);
+  if (mode == PHASE) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, PHASE>>(a, wvec, threads, smem, most, !WARP, s);
+  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, SHIFT>>(a, wvec, threads, smem, most, false, s);
 }
 
 template <bool BX, bool BW>
 int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
-  const bool vec = aligned16(a.x) && aligned16(a.y) && a.cols % 8 == 0 && a.ldx * (BX ? 2 : 4) % 16 == 0;
+  const int mode = mode_of(a.cols, BX ? 2 : 4, {{a.x, a.rows > 1 ? a.ldx : a.cols}, {a.y, a.cols}});
+  const bool vec = mode == ALIGNED;
   const int wvec = aligned16(a.weight) && aligned16(a.bias);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, vec, 4);
+  const Variant v = variant_of(a.cols, BX, mode, 4);
   int64_t n = 1;
   if (v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-  else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v.threads, vec, wvec, s);
-  else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
-  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v.threads, vec, wvec, s);
-  else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
-  else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
-  else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, 32, vec, wvec, s);
-  else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
-  else n = forward_variant<BX, BW, N, 32>(a, 32, vec, wvec, s);
+  else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v.threads, mode, wvec, s);
+  else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, mode, wvec, s);
+  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v.threads, mode, wvec, s);
+  else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, mode, wvec, s);
+  else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, mode, wvec, s);
+  else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, 32, mode, wvec, s);
+  else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, 32, mode, wvec, s);
+  else n = forward_variant<BX, BW, N, 32>(a, 32, mode, wvec, s);
   const cudaError_t e = cudaGetLastError();
   return n < 0 ? set_error(ADVOPT_E_CUDA, "advopt_layer_norm: the kernel's attributes") : check_cuda(e, "advopt_layer_norm");
 }
 
 template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, bool vec, int wvec, cudaStream_t s) {
-  const int threads = MAX_THREADS == 32 ? WARPS * 32 : row_threads;
-  const int64_t most = MAX_THREADS < 1024 ? grad_ctas(a.rows, a.cols) : a.rows;
-  const int smem = 2 * grad_rows(BX, MAX_THREADS) * Rows<BX, NV, true, grad_stages(BX)>::slots_of(threads) * 16;
-  if (vec) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, true>>(a, wvec, threads, smem, most, s);
-  return launch<grad_kernel<BX, BW, NV, MAX_THREADS, false>>(a, wvec, threads, smem, most, s);
+int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, int mode, int wvec, cudaStream_t s) {
+  constexpr bool WARP = MAX_THREADS == 32;
+  const int threads = WARP ? WARPS * 32 : row_threads;
+  const int64_t ctas = WARP && mode != PHASE ? ceil_div(a.rows, WARPS) : a.rows, parts = grad_ctas(a.rows, a.cols);
+  const int64_t most = MAX_THREADS == 1024 || ctas < parts ? ctas : parts;
+  const auto bytes = [&](int rows) { return 2 * rows * Rows<BX, NV, ALIGNED, grad_stages(BX)>::slots_of(threads) * 16; };
+  if (mode == ALIGNED) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, ALIGNED>>(a, wvec, threads, bytes(grad_rows(BX, MAX_THREADS, ALIGNED)), most, false, s);
+  if constexpr (MAX_THREADS != 320) {
+    const int smem = bytes(grad_rows(BX, MAX_THREADS, SHIFT));
+    if (mode == PHASE) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, PHASE>>(a, wvec, threads, smem, most, true, s);
+    return launch<grad_kernel<BX, BW, NV, MAX_THREADS, SHIFT>>(a, wvec, threads, smem, most, false, s);
+  }
+  return -1;
 }
 
 template <bool BX, bool BW>
 int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
-  const bool vec = aligned16(a.x) && aligned16(a.dy) && aligned16(a.dx) && a.cols % 8 == 0 && a.ldx * (BX ? 2 : 4) % 16 == 0 &&
-                   a.lddy * (BX ? 2 : 4) % 16 == 0;
+  const int64_t ldx = a.rows > 1 ? a.ldx : a.cols, lddy = a.rows > 1 ? a.lddy : a.cols;
+  const int mode = a.dx ? mode_of(a.cols, BX ? 2 : 4, {{a.x, ldx}, {a.dy, lddy}, {a.dx, a.cols}}) : mode_of(a.cols, BX ? 2 : 4, {{a.x, ldx}, {a.dy, lddy}});
+  const bool vec = mode == ALIGNED;
   const int wvec = aligned16(a.weight);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, vec, BX ? 3 : 4);   // bf16 rows of four vectors a lane would leave an SM eight warps
+  const Variant v = variant_of(a.cols, BX, mode, BX ? 3 : 4);   // bf16 rows of four vectors a lane would leave an SM eight warps
   int64_t parts = 0;
   if (a.cols > MOST || v.threads == 0 || v.threads > 512) {
     parts = wide_parts(a.rows);
     // float32 rows of that width would not fit shared memory twice
     if (a.dx && BX && v.threads) {
       if constexpr (BX)
-        if (grad_variant<BX, BW, 2 * N, 1024>(a, v.threads, vec, wvec, s) < 0) parts = -1;
+        if (grad_variant<BX, BW, 2 * N, 1024>(a, v.threads, mode, wvec, s) < 0) parts = -1;
     } else if (a.dx) {
       wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
     }
     if (a.work && parts > 0) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
   } else if (v.threads > 384) {
-    parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, vec, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, mode, wvec, s);
+  } else if (BX && mode == ALIGNED && v.threads > 256 && v.threads <= 320) {
+    if constexpr (BX) parts = grad_variant<BX, BW, 2 * N, 320>(a, v.threads, mode, wvec, s);
   } else if (v.threads > 256) {
-    parts = grad_variant<BX, BW, 2 * N, 384>(a, v.threads, vec, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 384>(a, v.threads, mode, wvec, s);
   } else if (v.threads > 32) {
-    parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, vec, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, mode, wvec, s);
   } else if (v.vectors == 4 * N) {
-    if constexpr (!BX) parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, vec, wvec, s);
+    if constexpr (!BX) parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, mode, wvec, s);
   } else if (v.vectors == 3 * N) {
-    parts = grad_variant<BX, BW, 3 * N, 32>(a, 32, vec, wvec, s);
+    parts = grad_variant<BX, BW, 3 * N, 32>(a, 32, mode, wvec, s);
   } else if (v.vectors == 2 * N) {
-    parts = grad_variant<BX, BW, 2 * N, 32>(a, 32, vec, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 32>(a, 32, mode, wvec, s);
   } else {
-    parts = grad_variant<BX, BW, N, 32>(a, 32, vec, wvec, s);
+    parts = grad_variant<BX, BW, N, 32>(a, 32, mode, wvec, s);
   }
   if (parts > 0 && a.work)
     finish_kernel<BW><<<dim3((unsigned)ceil_div(a.cols, 32), 2), FINISH_WARPS * 32, 0, s>>>(a.dweight, a.dbias, static_cast<const float*>(a.work),

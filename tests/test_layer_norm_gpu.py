@@ -191,3 +191,20 @@ def test_hooks_on_saved_tensors_and_other_derivatives():
         for args in ((dual(x), w, b), (x, dual(w), b), (x, w, dual(b))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 A.layer_norm(*args)
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("R", [1, 5, 7, 8, 9, 15, 17, 40, 600])
+@pytest.mark.parametrize("C", [1, 5, 331, 1001, 1003, 5003, 6007])
+def test_rows_between_boundaries(C, R, dtype):
+    """Rows that begin anywhere between two 16-byte boundaries: alike in x, y, dy and dx, or each in their own way."""
+    x, w, b, dy = make(R, C, dtype, dtype)
+
+    def placed(t, pitch, offset):
+        flat = torch.full((R * pitch + offset + 8,), float("nan"), dtype=dtype, device="cuda")   # outside the rows
+        v = flat.as_strided((R, C), (pitch, 1), offset)
+        v.copy_(t)
+        return v
+
+    for px, ox, pd, od in ((C, 0, C, 0), (C + 8, 0, C + 16, 8), (C, 0, C + 1, 0), (C, 3, C, 1), (C + 2, 1, C + 2, 1)):
+        check(placed(x, px, ox), w, b, placed(dy, pd, od))
