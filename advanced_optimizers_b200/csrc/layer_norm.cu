@@ -5,13 +5,15 @@
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and
 // writes dx, each once (16384 x 4096 bf16: 46 and 77 us for 41 and 61 of HBM's;
 // the second is bound by its instructions at 16 warps an SM, 25 an element).
-// A row stays in the registers of one warp (up to 1024 columns) or one CTA (up
-// to 16384), so the variance is that of the differences from the mean, in
-// float32, without a second read.  Wider rows are read again (from L2).  dw
-// and db are summed down the columns that a thread holds, over all rows its CTA
-// takes (up to 8192 columns, else by a kernel of their own that reads again);
-// the CTAs' sums are added in order by one more launch, so that results repeat
-// bit for bit.
+// A row stays in the registers of one warp (up to 1024 columns), one CTA (up to
+// 16384 forward, 8192 backward) or a cluster of up to eight (up to 65536), so
+// the variance is that of the differences from the mean, in float32, without a
+// second read.  Wider rows are read again (from L2).  dw and db are summed down
+// the columns that a thread holds, over all rows its CTA takes (of the widest
+// rows by a kernel of their own that reads again); the CTAs' sums are added in
+// order by one more launch, so that results repeat bit for bit.
+#include <cooperative_groups.h>
+
 #include <atomic>
 #include <initializer_list>
 #include <type_traits>
@@ -21,6 +23,8 @@
 #include "capi_internal.h"
 #include "common.cuh"
 #include "rows.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace advopt {
 namespace ln {
@@ -86,6 +90,41 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[Q ? Q * N : 1]) {
     __syncthreads();
   }
 }
+// A CTA's place in a cluster of up to 8 that share a row (1 without one), and the row's sums over them.  Timed against two
+// reads of a row and a third for dw and db, backward: 4096 x 16384 bf16 150 -> 117 us, 8192 x 12288 230 -> 168, 2048 x
+// 16384 float32 169 -> 84, 4000 x 12005 float32 492 -> 143; forward, beyond 16384 columns, against three reads: 1024 x
+// 32768 float32 86 -> 70, 1000 x 40001 bf16 172 -> 76, 1024 x 65536 bf16 89 -> 109.
+constexpr int MOST_CTAS = 8;
+template <bool CLUSTER, int N>
+struct Team {
+  uint32_t ctas, rank;
+  __device__ __forceinline__ Team() : ctas(1), rank(0) {
+    if constexpr (CLUSTER) {
+      ctas = cg::this_cluster().num_blocks();
+      rank = cg::this_cluster().block_rank();
+    }
+  }
+  // Of the CTA's sums v, which all its threads hold; added in the CTAs' order.  `all` has room for two rounds: a CTA writes
+  // a round's place again only after a barrier that the others reach when they have read it.
+  __device__ __forceinline__ void sum(float (&v)[N], float (*all)[MOST_CTAS][N], int& round) const {
+    if constexpr (CLUSTER) {
+      cg::cluster_group cluster = cg::this_cluster();
+      float (*p)[N] = all[round];
+      round ^= 1;
+      if (threadIdx.x < ctas) {
+        float* to = cluster.map_shared_rank(p[rank], threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) to[i] = v[i];
+      }
+      cluster.sync();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = p[0][i];
+      for (uint32_t k = 1; k < ctas; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], p[k][i]);
+    }
+  }
+};
 // Q of a kernel for rows of up to `threads` threads (32: a warp's).
 __host__ __device__ constexpr int quads(int threads) { return threads == 32 ? 0 : (threads + 127) / 128; }
 
@@ -124,10 +163,10 @@ struct Columns {
     asm volatile("mov.b32 %0, %1;" : "=r"(b) : "r"(bits));
     return b;
   }
-  __device__ __forceinline__ void init(int cols, bool warp_rows, int k) {
+  __device__ __forceinline__ void init(int cols, bool warp_rows, int rank, int k) {
     const int lane = threadIdx.x & 31, warp = warp_rows ? 0 : threadIdx.x >> 5, warps = warp_rows ? 1 : blockDim.x >> 5;
     constexpr int LANES = MODE == SHIFT ? PAYLOAD : 32;
-    first = (warp * LANES + lane - (MODE == SHIFT ? 1 : 0)) * E - (MODE == PHASE ? k : 0);
+    first = ((rank * NV * warps + warp) * LANES + lane - (MODE == SHIFT ? 1 : 0)) * E - (MODE == PHASE ? k : 0);
     each = warps * LANES * E;
     row = ragged = 0;
 #pragma unroll
@@ -347,24 +386,24 @@ __device__ __forceinline__ void put_row(const Vals<BF16, BF16 ? 8 : 4>& x, unsig
   }
 }
 
-// The rows of a CTA (or warp): from `first` on, `each` apart within a round, `step` from round to round.  PHASE: a CTA's
+// The rows of a CTA (a warp, a cluster): from `first` on, `each` apart within a round, `step` from round to round.  PHASE: a CTA's
 // all begin at one place, so eight CTAs make a group (fewer where there are fewer rows); SUMS:
 // also those of its warps.
 template <int MODE, bool WARP, int RI, bool SUMS>
 struct Walk {
   int64_t first, each, step;
-  __device__ __forceinline__ Walk() {
+  __device__ __forceinline__ Walk(uint32_t cta, uint32_t ctas) {
     const int64_t warp = WARP ? threadIdx.x >> 5 : 0;
     if (MODE == PHASE && (SUMS || !WARP)) {
       constexpr int64_t ROWS = (WARP ? WARPS : RI) * 8;
-      first = (int64_t)(blockIdx.x / 8) * ROWS + warp * 8 + blockIdx.x % 8;
+      first = (int64_t)(cta / 8) * ROWS + warp * 8 + cta % 8;
       each = 8;
-      step = (gridDim.x < 8 ? 1 : gridDim.x / 8) * ROWS;
+      step = (ctas < 8 ? 1 : ctas / 8) * ROWS;
     } else {
       constexpr int64_t ROWS = WARP ? WARPS : RI;
-      first = (int64_t)blockIdx.x * ROWS + warp;
+      first = (int64_t)cta * ROWS + warp;
       each = 1;
-      step = (int64_t)gridDim.x * ROWS;
+      step = (int64_t)ctas * ROWS;
     }
   }
 };
@@ -377,10 +416,10 @@ __host__ __device__ constexpr int grad_stages(bool bf16) { return bf16 ? 2 : 3; 
 // threads and 384 of aligned rows (10000 x 5000: 86 -> 69 us, x 6000: 101 -> 91; unaligned ones of 320 gained nothing).
 __host__ __device__ constexpr bool two_ctas(bool bf16, int max_threads, int mode) { return bf16 && mode == ALIGNED && (max_threads == 320 || max_threads == 384); }
 __host__ __device__ constexpr int grad_rows(bool bf16, int max_threads, int mode) {
-  return bf16 && max_threads > 32 && max_threads < 1024 && !two_ctas(bf16, max_threads, mode) ? 2 : 1;
+  return bf16 && max_threads > 32 && !two_ctas(bf16, max_threads, mode) ? 2 : 1;
 }
 
-template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE>
+template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THREADS == 32 || MAX_THREADS == 1024 ? 1 : MAX_THREADS == 256 ? (MODE == ALIGNED ? 4 : 3) : 2)
     forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
@@ -389,12 +428,14 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
   __shared__ float4 red[2][Q ? Q : 1];
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, cols = (int)a.cols;
   constexpr int S = FWD_STAGES, E = BX ? 8 : 4, P = E / 2;
-  const Walk<MODE, WARP, 1, false> walk;
+  __shared__ float all[2][MOST_CTAS][1];
+  const Team<CLUSTER, 1> team;
+  const Walk<MODE, WARP, 1, false> walk(blockIdx.x / team.ctas, gridDim.x / team.ctas);
   const int64_t step = walk.step;
   int64_t r = walk.first;
   unsigned char* to = static_cast<unsigned char*>(a.y) + r * cols * (BX ? 2 : 4);
   Columns<BX, NV, MODE> col;
-  col.init(cols, WARP, (int)(reinterpret_cast<uintptr_t>(to) & 15) / (BX ? 2 : 4));
+  col.init(cols, WARP, (int)team.rank, (int)(reinterpret_cast<uintptr_t>(to) & 15) / (BX ? 2 : 4));
   Rows<BX, NV, MODE, S> rows;
   rows.init(smem, a.x, a.ldx, r, step, cols, col);
 #pragma unroll
@@ -403,6 +444,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     commit_copies();
   }
   clear_sums<1, Q>(red);
+  if constexpr (CLUSTER) cg::this_cluster().sync();   // all its CTAs are there
   Vals<BW, E> w[NV], b[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
@@ -410,7 +452,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     b[v].weights(a.bias, 0.0f, col.c(v), col.bits(v), MODE != PHASE && wvec);
   }
   const float inv = __fdiv_rn(1.0f, (float)cols);
-  int round = 0;
+  int round = 0, team_round = 0;
   for (; r < a.rows; r += step, to += step * cols * (BX ? 2 : 4)) {
     wait_copies<S - 2>();
     if (MODE == SHIFT) __syncwarp();   // the next lane's copies are read too
@@ -440,6 +482,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
       }
     float t[1] = {__fadd_rn(s.x, s.y)};
     row_sum<1, Q>(t, red, round);
+    team.sum(t, all, team_round);
     const float mean = __fmul_rn(t[0], inv);
     s = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -462,9 +505,10 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     }
     t[0] = __fadd_rn(s.x, s.y);
     row_sum<1, Q>(t, red, round);
+    team.sum(t, all, team_round);
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(t[0], inv, a.eps)));
     const float2 rstd2 = splat2(rstd), shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
-    if (a.stats && lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
+    if (a.stats && lane == 0 && team.rank == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float y[E];
@@ -495,7 +539,7 @@ __device__ __forceinline__ void wide_sum(float (&v)[N], float (*red)[32]) {
   __syncthreads();
 }
 
-// Rows that no CTA's registers hold: read three times.
+// Rows that no cluster's registers hold: read three times.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int vec, int wvec) {
   __shared__ float red[1][32];
@@ -542,22 +586,22 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
 
 // ---- the gradients ----
 // RI rows of a CTA share a round of sums.
-template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE>
+template <bool BX, bool BW, int NV, int MAX_THREADS, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_THREADS > 256 && !two_ctas(BX, MAX_THREADS, MODE)) || (MAX_THREADS == 32 && NV > 4) ? 1 : 2)
     grad_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int wvec) {
   constexpr bool WARP = MAX_THREADS == 32;
   constexpr int S = grad_stages(BX), E = BX ? 8 : 4, P = E / 2, RI = grad_rows(BX, MAX_THREADS, MODE), Q = quads(MAX_THREADS);
-  constexpr bool SUMS = MAX_THREADS < 1024;   // of more threads, the registers do not hold the columns' sums
   extern __shared__ uint4 smem[];
   __shared__ float4 red[2][Q ? Q * 2 * RI : 1];
   const int cols = (int)a.cols;
-  const bool sums = SUMS && a.work != nullptr;
   using R = Rows<BX, NV, MODE, S>;
-  const Walk<MODE, WARP, RI, true> walk;
+  __shared__ float all[2][MOST_CTAS][2 * RI];
+  const Team<CLUSTER, 2 * RI> team;
+  const Walk<MODE, WARP, RI, true> walk(blockIdx.x / team.ctas, gridDim.x / team.ctas);
   const int64_t step = walk.step, each = walk.each;
   int64_t r = walk.first;
   Columns<BX, NV, MODE> col;
-  col.init(cols, WARP, (int)((reinterpret_cast<uintptr_t>(a.x) + r * a.ldx * (BX ? 2 : 4)) & 15) / (BX ? 2 : 4));
+  col.init(cols, WARP, (int)team.rank, (int)((reinterpret_cast<uintptr_t>(a.x) + r * a.ldx * (BX ? 2 : 4)) & 15) / (BX ? 2 : 4));
   R xs[RI], dys[RI];
 #pragma unroll
   for (int q = 0; q < RI; ++q) {
@@ -575,6 +619,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
     commit_copies();
   }
   clear_sums<2 * RI, Q>(red);
+  if constexpr (CLUSTER) cg::this_cluster().sync();   // all its CTAs are there
   Vals<BW, E> w[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) w[v].weights(a.weight, 1.0f, col.c(v), col.bits(v), MODE != PHASE && wvec);
@@ -586,7 +631,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
   const float inv = __fdiv_rn(1.0f, (float)cols);
   const int64_t row_bytes = (int64_t)cols * (BX ? 2 : 4);
   unsigned char* to = static_cast<unsigned char*>(a.dx) + r * row_bytes;
-  int round = 0;
+  int round = 0, team_round = 0;
   for (; r < a.rows; r += step, to += step * row_bytes) {
     float2 st[RI];
     bool here[RI];
@@ -634,7 +679,8 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
               const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
               s1 = add2(s1, g);
               s2 = fma2(g, h, s2);
-              if (SUMS) dw[v][i] = fma2(d, h, dw[v][i]), db[v][i] = add2(db[v][i], d);
+              dw[v][i] = fma2(d, h, dw[v][i]);
+              db[v][i] = add2(db[v][i], d);
             }
           }
         }
@@ -644,6 +690,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
     }
     if (!a.dx) continue;
     row_sum<2 * RI, Q>(t, red, round);
+    team.sum(t, all, team_round);
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
       if (!here[q]) continue;
@@ -666,8 +713,8 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
       }
     }
   }
-  if (!sums) return;
-  float* part = static_cast<float*>(a.work) + (int64_t)blockIdx.x * 2 * a.cols;
+  if (!a.work) return;
+  float* part = static_cast<float*>(a.work) + (int64_t)(blockIdx.x / team.ctas) * 2 * a.cols;
   if constexpr (WARP) {
     // the warps' sums through shared memory, all of the same columns: [WARPS][2][NV * P][32], added in the warps' order
     wait_copies<0>();
@@ -711,7 +758,7 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
   }
 }
 
-// Rows that no CTA's registers hold, and float32 ones of more than 8192 columns: dx from two reads of a row.
+// Rows that no cluster's registers hold: dx from two reads of a row.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_dx_kernel(const __grid_constant__ advopt_layer_norm_grad_args a, int vec, int wvec) {
   __shared__ float red[2][32];
@@ -823,20 +870,26 @@ __global__ void __launch_bounds__(FINISH_WARPS * 32) finish_kernel(void* dweight
 
 // ---- variants ----
 constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold with their sums (a few hundred fewer of unaligned rows)
+constexpr int64_t MOST_OF_CLUSTER = MOST * MOST_CTAS;
 constexpr int64_t SMS = 148;
 
-// Vectors per thread and threads of a row: a warp's where it holds the row in
-// `one` to `most` * `one` vectors a lane, else a CTA's with `one` * 2.
+// Vectors per thread, and threads and CTAs of a row: a warp's where it holds
+// the row in `one` to `most` * `one` vectors a lane, else a CTA's of up to
+// `threads` with `one` * 2, else those of a cluster: of up to 256 threads each
+// where eight CTAs do, so that two share an SM (8192 x 12288 bf16 backward: 162 us
+// where two of 384 threads take 193), else of up to 512.
 struct Variant {
-  int vectors, threads;             // threads: 32, or a CTA's; 0: too wide
+  int vectors, threads, ctas;       // threads: 32, or a CTA's; ctas: 0: too wide
 };
-inline Variant variant_of(int64_t cols, bool bf16, int mode, int most) {
+inline Variant variant_of(int64_t cols, bool bf16, int mode, int most, int threads) {
   const int e = bf16 ? 8 : 4, one = bf16 ? 1 : 2, lanes = mode == SHIFT ? PAYLOAD : 32;
   const int64_t slots = ceil_div(cols, e) + (mode == ALIGNED ? 0 : 1);   // unaligned rows end in 16 bytes more
   for (int n = one; n <= most * one; n += one)
-    if (slots <= n * lanes) return {n, 32};
-  const int64_t threads = ceil_div(slots, 2 * one * lanes) * 32;
-  return {2 * one, threads <= 1024 ? (int)threads : 0};
+    if (slots <= n * lanes) return {n, 32, 1};
+  const int64_t warps = ceil_div(slots, (int64_t)2 * one * lanes);
+  if (warps * 32 <= threads) return {2 * one, (int)warps * 32, 1};
+  const int64_t ctas = warps <= 8 * MOST_CTAS ? ceil_div(warps, 8) : MOST_CTAS, each = ceil_div(warps, ctas) * 32;
+  return each <= 512 ? Variant{2 * one, (int)each, (int)ctas} : Variant{2 * one, 0, 0};
 }
 // CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows at least where that leaves one for each SM.
 inline int64_t grad_ctas(int64_t rows, int64_t cols) {
@@ -846,23 +899,40 @@ inline int64_t grad_ctas(int64_t rows, int64_t cols) {
   const int64_t n = few < most ? few : most;
   return units < n ? units : n;
 }
+// Clusters of the gradient kernel at most: of three CTAs or more, two an SM.
+inline int64_t grad_clusters(int64_t rows) { return rows < 2 * SMS / 3 ? rows : 2 * SMS / 3; }
 inline int64_t wide_parts(int64_t rows) { return rows < 8 * 32 ? ceil_div(rows, 8) : 32; }
 
-// Launches a persistent kernel with as many CTAs as fit the SMs, `most` at most; the number of CTAs, or -1.
+// Launches a persistent kernel with as many CTAs (clusters of `ctas`) as fit the SMs, `most` at most; their number, or -1.
 template <auto KERNEL, class Arg>
-int64_t launch(const Arg& a, int wvec, int threads, int smem, int64_t most, bool by_eight, cudaStream_t s) {
-  static std::atomic<int> resident[33];   // this kernel's, by warps
+int64_t launch(const Arg& a, int wvec, int threads, int ctas, int smem, int64_t most, bool by_eight, cudaStream_t s) {
+  static std::atomic<int> resident[33][MOST_CTAS + 1];   // of this kernel on all SMs, by warps and ctas
   // for the current device, whichever that is
   if (smem > 47 * 1024 && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
-  int n = resident[threads / 32].load(std::memory_order_relaxed);
+  cudaLaunchConfig_t c = {};
+  cudaLaunchAttribute cluster = {};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)ctas;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  c.gridDim = dim3((unsigned)ctas);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = (size_t)smem;
+  c.stream = s;
+  c.attrs = &cluster;
+  c.numAttrs = ctas > 1;
+  std::atomic<int>& known = resident[threads / 32][ctas];
+  int n = known.load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem) != cudaSuccess || n < 1) return -1;
-    resident[threads / 32].store(n, std::memory_order_relaxed);
+    const cudaError_t e = ctas > 1 ? cudaOccupancyMaxActiveClusters(&n, KERNEL, &c) : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem);
+    if (e != cudaSuccess || n < 1) return -1;
+    if (ctas == 1) n *= (int)SMS;
+    known.store(n, std::memory_order_relaxed);
   }
-  int64_t grid = n * SMS < most ? n * SMS : most;
+  int64_t grid = n < most ? n : most;
   if (by_eight && grid > 8) grid -= grid % 8;
-  KERNEL<<<(unsigned)grid, threads, smem, s>>>(a, wvec);
-  return grid;
+  if (by_eight && grid < 8 && grid < most) return -1;   // a CTA (cluster) for each place that a row may begin at
+  c.gridDim.x = (unsigned)(grid * ctas);
+  return cudaLaunchKernelEx(&c, KERNEL, a, wvec) == cudaSuccess ? grid : -1;
 }
 
 // How the rows of matrices with these first addresses and pitches (elements) lie.
@@ -877,15 +947,15 @@ inline int mode_of(int64_t cols, int size, std::initializer_list<std::pair<const
   return aligned ? ALIGNED : same ? PHASE : SHIFT;
 }
 
-template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t forward_variant(const advopt_layer_norm_args& a, int row_threads, int mode, int wvec, cudaStream_t s) {
+template <bool BX, bool BW, int NV, int MAX_THREADS, bool CLUSTER = false>
+int64_t forward_variant(const advopt_layer_norm_args& a, const Variant& v, int mode, int wvec, cudaStream_t s) {
   constexpr bool WARP = MAX_THREADS == 32;
-  const int threads = WARP ? WARPS * 32 : row_threads;
+  const int threads = WARP ? WARPS * 32 : v.threads;
   const int64_t most = WARP ? ceil_div(a.rows, WARPS) : a.rows;
   const int smem = Rows<BX, NV, ALIGNED, FWD_STAGES>::slots_of(threads) * 16;
-  if (mode == ALIGNED) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, ALIGNED>>(a, wvec, threads, smem, most, false, s);
-  if (mode == PHASE) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, PHASE>>(a, wvec, threads, smem, most, !WARP, s);
-  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, SHIFT>>(a, wvec, threads, smem, most, false, s);
+  if (mode == ALIGNED) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, ALIGNED, CLUSTER>>(a, wvec, threads, v.ctas, smem, most, false, s);
+  if (mode == PHASE) return launch<forward_kernel<BX, BW, NV, MAX_THREADS, PHASE, CLUSTER>>(a, wvec, threads, v.ctas, smem, most, !WARP, s);
+  return launch<forward_kernel<BX, BW, NV, MAX_THREADS, SHIFT, CLUSTER>>(a, wvec, threads, v.ctas, smem, most, false, s);
 }
 
 template <bool BX, bool BW>
@@ -894,33 +964,35 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   const bool vec = mode == ALIGNED;
   const int wvec = aligned16(a.weight) && aligned16(a.bias);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, mode, 4);
+  const Variant v = variant_of(a.cols, BX, mode, 4, 1024);
   int64_t n = 1;
-  if (v.threads == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-  else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v.threads, mode, wvec, s);
-  else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v.threads, mode, wvec, s);
-  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v.threads, mode, wvec, s);
-  else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v.threads, mode, wvec, s);
-  else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, 32, mode, wvec, s);
-  else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, 32, mode, wvec, s);
-  else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, 32, mode, wvec, s);
-  else n = forward_variant<BX, BW, N, 32>(a, 32, mode, wvec, s);
+  if (v.ctas == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+  else if (v.ctas > 1 && v.threads > 256) n = forward_variant<BX, BW, 2 * N, 512, true>(a, v, mode, wvec, s);
+  else if (v.ctas > 1) n = forward_variant<BX, BW, 2 * N, 256, true>(a, v, mode, wvec, s);
+  else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v, mode, wvec, s);
+  else if (v.threads > 384) n = forward_variant<BX, BW, 2 * N, 512>(a, v, mode, wvec, s);
+  else if (v.threads > 256) n = forward_variant<BX, BW, 2 * N, 384>(a, v, mode, wvec, s);
+  else if (v.threads > 32) n = forward_variant<BX, BW, 2 * N, 256>(a, v, mode, wvec, s);
+  else if (v.vectors == 4 * N) n = forward_variant<BX, BW, 4 * N, 32>(a, v, mode, wvec, s);
+  else if (v.vectors == 3 * N) n = forward_variant<BX, BW, 3 * N, 32>(a, v, mode, wvec, s);
+  else if (v.vectors == 2 * N) n = forward_variant<BX, BW, 2 * N, 32>(a, v, mode, wvec, s);
+  else n = forward_variant<BX, BW, N, 32>(a, v, mode, wvec, s);
   const cudaError_t e = cudaGetLastError();
   return n < 0 ? set_error(ADVOPT_E_CUDA, "advopt_layer_norm: the kernel's attributes") : check_cuda(e, "advopt_layer_norm");
 }
 
-template <bool BX, bool BW, int NV, int MAX_THREADS>
-int64_t grad_variant(const advopt_layer_norm_grad_args& a, int row_threads, int mode, int wvec, cudaStream_t s) {
+template <bool BX, bool BW, int NV, int MAX_THREADS, bool CLUSTER = false>
+int64_t grad_variant(const advopt_layer_norm_grad_args& a, const Variant& v, int mode, int wvec, cudaStream_t s) {
   constexpr bool WARP = MAX_THREADS == 32;
-  const int threads = WARP ? WARPS * 32 : row_threads;
-  const int64_t ctas = WARP && mode != PHASE ? ceil_div(a.rows, WARPS) : a.rows, parts = grad_ctas(a.rows, a.cols);
-  const int64_t most = MAX_THREADS == 1024 || ctas < parts ? ctas : parts;
+  const int threads = WARP ? WARPS * 32 : v.threads;
+  const int64_t ctas = WARP && mode != PHASE ? ceil_div(a.rows, WARPS) : a.rows, parts = CLUSTER ? grad_clusters(a.rows) : grad_ctas(a.rows, a.cols);
+  const int64_t most = ctas < parts ? ctas : parts;
   const auto bytes = [&](int rows) { return 2 * rows * Rows<BX, NV, ALIGNED, grad_stages(BX)>::slots_of(threads) * 16; };
-  if (mode == ALIGNED) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, ALIGNED>>(a, wvec, threads, bytes(grad_rows(BX, MAX_THREADS, ALIGNED)), most, false, s);
+  if (mode == ALIGNED) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, ALIGNED, CLUSTER>>(a, wvec, threads, v.ctas, bytes(grad_rows(BX, MAX_THREADS, ALIGNED)), most, false, s);
   if constexpr (MAX_THREADS != 320) {
     const int smem = bytes(grad_rows(BX, MAX_THREADS, SHIFT));
-    if (mode == PHASE) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, PHASE>>(a, wvec, threads, smem, most, true, s);
-    return launch<grad_kernel<BX, BW, NV, MAX_THREADS, SHIFT>>(a, wvec, threads, smem, most, false, s);
+    if (mode == PHASE) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, PHASE, CLUSTER>>(a, wvec, threads, v.ctas, smem, most, true, s);
+    return launch<grad_kernel<BX, BW, NV, MAX_THREADS, SHIFT, CLUSTER>>(a, wvec, threads, v.ctas, smem, most, false, s);
   }
   return -1;
 }
@@ -932,34 +1004,30 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
   const bool vec = mode == ALIGNED;
   const int wvec = aligned16(a.weight);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, mode, BX ? 3 : 4);   // bf16 rows of four vectors a lane would leave an SM eight warps
+  const Variant v = variant_of(a.cols, BX, mode, BX ? 3 : 4, 512);   // bf16 rows of four vectors a lane would leave an SM eight warps
   int64_t parts = 0;
-  if (a.cols > MOST || v.threads == 0 || v.threads > 512) {
+  if (v.ctas == 0) {
     parts = wide_parts(a.rows);
-    // float32 rows of that width would not fit shared memory twice
-    if (a.dx && BX && v.threads) {
-      if constexpr (BX)
-        if (grad_variant<BX, BW, 2 * N, 1024>(a, v.threads, mode, wvec, s) < 0) parts = -1;
-    } else if (a.dx) {
-      wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
-    }
-    if (a.work && parts > 0) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
+    if (a.dx) wide_dx_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+    if (a.work) wide_sums_kernel<BX><<<dim3((unsigned)ceil_div(a.cols, 256), (unsigned)parts), 256, 0, s>>>(a, vec);
+  } else if (v.ctas > 1) {
+    parts = v.threads > 256 ? grad_variant<BX, BW, 2 * N, 512, true>(a, v, mode, wvec, s) : grad_variant<BX, BW, 2 * N, 256, true>(a, v, mode, wvec, s);
   } else if (v.threads > 384) {
-    parts = grad_variant<BX, BW, 2 * N, 512>(a, v.threads, mode, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 512>(a, v, mode, wvec, s);
   } else if (BX && mode == ALIGNED && v.threads > 256 && v.threads <= 320) {
-    if constexpr (BX) parts = grad_variant<BX, BW, 2 * N, 320>(a, v.threads, mode, wvec, s);
+    if constexpr (BX) parts = grad_variant<BX, BW, 2 * N, 320>(a, v, mode, wvec, s);
   } else if (v.threads > 256) {
-    parts = grad_variant<BX, BW, 2 * N, 384>(a, v.threads, mode, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 384>(a, v, mode, wvec, s);
   } else if (v.threads > 32) {
-    parts = grad_variant<BX, BW, 2 * N, 256>(a, v.threads, mode, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 256>(a, v, mode, wvec, s);
   } else if (v.vectors == 4 * N) {
-    if constexpr (!BX) parts = grad_variant<BX, BW, 4 * N, 32>(a, 32, mode, wvec, s);
+    if constexpr (!BX) parts = grad_variant<BX, BW, 4 * N, 32>(a, v, mode, wvec, s);
   } else if (v.vectors == 3 * N) {
-    parts = grad_variant<BX, BW, 3 * N, 32>(a, 32, mode, wvec, s);
+    parts = grad_variant<BX, BW, 3 * N, 32>(a, v, mode, wvec, s);
   } else if (v.vectors == 2 * N) {
-    parts = grad_variant<BX, BW, 2 * N, 32>(a, 32, mode, wvec, s);
+    parts = grad_variant<BX, BW, 2 * N, 32>(a, v, mode, wvec, s);
   } else {
-    parts = grad_variant<BX, BW, N, 32>(a, 32, mode, wvec, s);
+    parts = grad_variant<BX, BW, N, 32>(a, v, mode, wvec, s);
   }
   if (parts > 0 && a.work)
     finish_kernel<BW><<<dim3((unsigned)ceil_div(a.cols, 32), 2), FINISH_WARPS * 32, 0, s>>>(a.dweight, a.dbias, static_cast<const float*>(a.work),
@@ -992,7 +1060,7 @@ extern "C" int advopt_layer_norm(const advopt_layer_norm_args* a, void* stream) 
 
 extern "C" int64_t advopt_layer_norm_grad_work(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (cols > ln::MOST ? ln::wide_parts(rows) : ln::grad_ctas(rows, cols)) * 2 * cols * 4;
+  return (cols > ln::MOST_OF_CLUSTER ? ln::wide_parts(rows) : cols > ln::MOST ? ln::grad_clusters(rows) : ln::grad_ctas(rows, cols)) * 2 * cols * 4;
 }
 
 extern "C" int advopt_layer_norm_grad(const advopt_layer_norm_grad_args* a, void* stream) {

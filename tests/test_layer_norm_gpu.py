@@ -208,3 +208,23 @@ def test_rows_between_boundaries(C, R, dtype):
 
     for px, ox, pd, od in ((C, 0, C, 0), (C + 8, 0, C + 16, 8), (C, 0, C + 1, 0), (C, 3, C, 1), (C + 2, 1, C + 2, 1)):
         check(placed(x, px, ox), w, b, placed(dy, pd, od))
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(B, B), (F, F), (F, B)])
+@pytest.mark.parametrize("R,C", [(1, 8193), (200, 12288), (190, 12001), (700, 16384), (7, 16385), (40, 20011), (100, 33000), (20, 50000), (17, 65536), (9, 65537),
+                                 (6, 70001), (40, 131072)])
+def test_wide_rows(R, C, dtype, wdtype):
+    """Rows that take two, four and eight CTAs, and wider ones."""
+    check(*make(R, C, dtype, wdtype))
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("R", [1, 7, 9, 33])
+@pytest.mark.parametrize("C", [8195, 12001, 30011, 61000, 61447, 66666])
+def test_wide_rows_between_boundaries(C, R, dtype):
+    x, w, b, dy = make(R, C, dtype, dtype)
+    for px, ox, pd, od in ((C, 0, C + 16, 8), (C + 1, 1, C, 2)):
+        xs, dys = (torch.full((R * p + o + 8,), float("nan"), dtype=dtype, device="cuda").as_strided((R, C), (p, 1), o) for p, o in ((px, ox), (pd, od)))
+        xs.copy_(x)
+        dys.copy_(dy)
+        check(xs, w, b, dys)
