@@ -3,7 +3,7 @@
 //   dx = rstd * (g - mean of g - h * mean of g h), dw = sum of dy h, db = sum of dy.
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and
-// writes dx, each once (16384 x 4096 bf16: 46 and 77 us for 41 and 61 of HBM's;
+// writes dx, each once (16384 x 4096 bf16: 46 and 74 us for 41 and 61 of HBM's;
 // the second is bound by its instructions at 16 warps an SM, 25 an element).
 // A row stays in the registers of one warp (up to 1024 columns), one CTA (up to
 // 16384 forward, 8192 backward) or a cluster of up to eight (up to 65536), so
@@ -133,9 +133,9 @@ __host__ __device__ constexpr int quads(int threads) { return threads == 32 ? 0 
 // all begin at the same place between two boundaries; it takes the 16 bytes
 // between boundaries as they are, with the columns that these hold.  SHIFT:
 // anything else; what is read is shifted into place, and so is what is written.
-// Timed, PHASE against SHIFT: 10000 x 5003 bf16 48 us forward for 73 and 95
-// backward for 100, float32 68 for 100 and 110 for 154, 16384 x 999 float32 24
-// for 44 and 38 for 81; aligned rows of 5000 take 40 and 70 in bf16.
+// Timed, PHASE against SHIFT: 10000 x 5003 bf16 47 us forward for 73 and 91
+// backward for 100, float32 69 for 100 and 107 for 154, 16384 x 999 float32 24
+// for 44 and 38 for 81; aligned rows of 5000 take 40 and 67 in bf16.
 constexpr int ALIGNED = 0, PHASE = 1, SHIFT = 2;
 
 // A thread's columns: NV vectors of 16 bytes of x, each warp's (or CTA's) next
@@ -155,7 +155,6 @@ struct Columns {
   __device__ __forceinline__ uint32_t bits(int v) const { return row >> (v * E) & WHOLE; }
   __device__ __forceinline__ bool whole(int v) const { return (mine >> (v * E) & WHOLE) == WHOLE; }
   __device__ __forceinline__ bool some(int v) const { return (mine >> (v * E) & WHOLE) != 0; }
-  __device__ __forceinline__ bool has(int v, int e) const { return mine >> (v * E + e) & 1u; }
   // The same, for a branch in the loop over rows: volatile, since what follows from the bits would be worked out ahead of
   // the loop and take more registers than there are.
   __device__ __forceinline__ static uint32_t here(uint32_t bits) {
@@ -742,19 +741,28 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
       if (c + 1 >= 0 && c + 1 < cols) p[1] = t.y;
     }
   } else {
+    // in the columns' order through shared memory, so that whole sectors are written; two words in 34 are left free against bank conflicts
+    // (1000 x 5003 bf16: 12 us where each thread's own stores took 16)
+    wait_copies<0>();
+    float* sh = reinterpret_cast<float*>(smem);
+    const auto place = [](int i) { return i + (i >> 5) * 2; };
+    constexpr int LANES = MODE == SHIFT ? PAYLOAD : 32;
+    const int lane31 = threadIdx.x & 31, span = NV * (int)(blockDim.x >> 5) * LANES * E;
+    const int begin = col.first - ((int)(threadIdx.x >> 5) * LANES + lane31 - (MODE == SHIFT ? 1 : 0)) * E;   // the CTA's first column
+    static_assert(NV * E * 4 * 17 / 16 <= 2 * RI * S * NV * 16, "the rows' shared memory");
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int k = 0; k < 2; ++k) {
+      __syncthreads();
+      if (MODE != SHIFT || (lane31 > 0 && lane31 <= PAYLOAD)) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        float* p = part + col.c(v) + 2 * i;
-        if (MODE != PHASE && col.has(v, 2 * i + 1) && (cols & 1) == 0) {
-          *reinterpret_cast<float2*>(p) = dw[v][i];
-          *reinterpret_cast<float2*>(p + cols) = db[v][i];
-        } else {
-          if (col.has(v, 2 * i)) p[0] = dw[v][i].x, p[cols] = db[v][i].x;
-          if (col.has(v, 2 * i + 1)) p[1] = dw[v][i].y, p[cols + 1] = db[v][i].y;
-        }
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int i = 0; i < P; ++i) *reinterpret_cast<float2*>(sh + place(col.c(v) - begin + 2 * i)) = k ? db[v][i] : dw[v][i];
       }
+      __syncthreads();
+      for (int j = threadIdx.x; j < span; j += blockDim.x)
+        if (begin + j >= 0 && begin + j < cols) part[k * cols + begin + j] = sh[place(j)];
+    }
   }
 }
 
