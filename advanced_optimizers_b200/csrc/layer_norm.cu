@@ -93,7 +93,7 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[Q ? Q * N : 1]) {
 // A CTA's place in a cluster of up to 8 that share a row (1 without one), and the row's sums over them.  Timed against two
 // reads of a row and a third for dw and db, backward: 4096 x 16384 bf16 150 -> 117 us, 8192 x 12288 230 -> 168, 2048 x
 // 16384 float32 169 -> 84, 4000 x 12005 float32 492 -> 143; forward, beyond 16384 columns, against three reads: 1024 x
-// 32768 float32 86 -> 70, 1000 x 40001 bf16 172 -> 76, 1024 x 65536 bf16 89 -> 109.
+// 32768 float32 86 -> 70, 1000 x 40001 bf16 172 -> 76.
 constexpr int MOST_CTAS = 8;
 template <bool CLUSTER, int N>
 struct Team {
@@ -538,7 +538,7 @@ __device__ __forceinline__ void wide_sum(float (&v)[N], float (*red)[32]) {
   __syncthreads();
 }
 
-// Rows that no cluster's registers hold: read three times.
+// Rows that no cluster's registers hold, and many aligned bf16 ones: read three times.
 template <bool BX, bool BW>
 __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constant__ advopt_layer_norm_args a, int vec, int wvec) {
   __shared__ float red[1][32];
@@ -974,7 +974,10 @@ int forward(const advopt_layer_norm_args& a, cudaStream_t s) {
   constexpr int N = BX ? 1 : 2;
   const Variant v = variant_of(a.cols, BX, mode, 4, 1024);
   int64_t n = 1;
-  if (v.ctas == 0) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
+  // many aligned bf16 rows: reading them thrice costs less than the clusters' barriers (1024 x 65536: 91 us for 109, 3276 x
+  // 20480 94 for 94; float32 171 for 143, 188 for 129; 25 x 65536 bf16 12.6 for 6.8)
+  const bool again = v.ctas == 0 || (BX && vec && v.ctas > 1 && a.rows > 2 * SMS);
+  if (again) wide_forward_kernel<BX, BW><<<(unsigned)(a.rows < 2 * SMS ? a.rows : 2 * SMS), 1024, 0, s>>>(a, vec, wvec);
   else if (v.ctas > 1 && v.threads > 256) n = forward_variant<BX, BW, 2 * N, 512, true>(a, v, mode, wvec, s);
   else if (v.ctas > 1) n = forward_variant<BX, BW, 2 * N, 256, true>(a, v, mode, wvec, s);
   else if (v.threads > 512) n = forward_variant<BX, BW, 2 * N, 1024>(a, v, mode, wvec, s);

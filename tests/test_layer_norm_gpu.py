@@ -228,3 +228,9 @@ def test_wide_rows_between_boundaries(C, R, dtype):
         xs.copy_(x)
         dys.copy_(dy)
         check(xs, w, b, dys)
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("R", [296, 297, 400])
+def test_many_wide_rows(R, dtype):
+    check(*make(R, 17408, dtype, dtype))
