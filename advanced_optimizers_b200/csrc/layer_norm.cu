@@ -3,15 +3,16 @@
 //   dx = rstd * (g - mean of g - h * mean of g h), dw = sum of dy h, db = sum of dy.
 //
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and
-// writes dx, each once (16384 x 4096 bf16: 46 and 74 us for 41 and 61 of HBM's;
-// the second is bound by its instructions at 16 warps an SM, 25 an element).
-// A row stays in the registers of one warp (up to 1024 columns), one CTA (up to
-// 16384 forward, 8192 backward) or a cluster of up to eight (up to 65536), so
-// the variance is that of the differences from the mean, in float32, without a
-// second read.  Wider rows are read again (from L2).  dw and db are summed down
-// the columns that a thread holds, over all rows its CTA takes (of the widest
-// rows by a kernel of their own that reads again); the CTAs' sums are added in
-// order by one more launch, so that results repeat bit for bit.
+// writes dx, each once (16384 x 4096 bf16: 45 and 76 us for 41 and 61 of HBM's;
+// the second is bound by its instructions at 16 warps an SM, 26 an element).
+// A row stays in the registers of one warp (up to 1024 columns; bf16 backward
+// 768), one CTA (up to 16384 forward, 8192 backward) or a cluster of up to eight
+// (up to 65536), so the variance is that of the differences from the mean, in
+// float32, without a second read; h is rstd times these differences.  Wider rows
+// are read again (from L2).  dw and db are summed down the columns that a thread
+// holds, over all rows its CTA takes (of the widest rows by a kernel of their own
+// that reads again); the CTAs' sums are added in order by one more launch, so
+// that results repeat bit for bit.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -89,6 +90,12 @@ __device__ __forceinline__ void clear_sums(float4 (*red)[Q ? Q * N : 1]) {
     for (int i = threadIdx.x; i < 2 * Q * N; i += blockDim.x) red[i / (Q * N)][i % (Q * N)] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __syncthreads();
   }
+}
+// A row's mean from its sum and 1 / cols: the product, and what is left of the sum (exact in one fma) once more, so that the mean is exact where
+// it is a float.
+__device__ __forceinline__ float mean_of(float sum, float cols, float inv) {
+  const float m = __fmul_rn(sum, inv);
+  return __fmaf_rn(__fmaf_rn(-m, cols, sum), inv, m);
 }
 // A CTA's place in a cluster of up to 8 that share a row (1 without one), and the row's sums over them.  Timed against two
 // reads of a row and a third for dw and db, backward: 4096 x 16384 bf16 150 -> 117 us, 8192 x 12288 230 -> 168, 2048 x
@@ -217,6 +224,10 @@ struct Vals {
     else return u2f(w[e]);
   }
   __device__ __forceinline__ float2 pair(int i) const { return make_float2(at(2 * i), at(2 * i + 1)); }
+  __device__ __forceinline__ void set_pair(int i, float2 v) {   // of float32
+    w[2 * i] = f2u(v.x);
+    w[2 * i + 1] = f2u(v.y);
+  }
   __device__ __forceinline__ void set(const float (&v)[E]) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -412,7 +423,8 @@ struct Walk {
 constexpr int FWD_STAGES = 3;
 __host__ __device__ constexpr int grad_stages(bool bf16) { return bf16 ? 2 : 3; }
 // Rows of a CTA that share a round of sums: two of bf16, but one where the fewer registers let two CTAs run on an SM: 320
-// threads and 384 of aligned rows (10000 x 5000: 86 -> 69 us, x 6000: 101 -> 91; unaligned ones of 320 gained nothing).
+// threads and 384 of aligned rows (10000 x 5000: 86 -> 69 us, x 6000: 101 -> 91, and with the statistics read ahead 61 and 75; unaligned ones
+// of 320 gained nothing).
 __host__ __device__ constexpr bool two_ctas(bool bf16, int max_threads, int mode) { return bf16 && mode == ALIGNED && (max_threads == 320 || max_threads == 384); }
 __host__ __device__ constexpr int grad_rows(bool bf16, int max_threads, int mode) {
   return bf16 && max_threads > 32 && !two_ctas(bf16, max_threads, mode) ? 2 : 1;
@@ -482,23 +494,23 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     float t[1] = {__fadd_rn(s.x, s.y)};
     row_sum<1, Q>(t, red, round);
     team.sum(t, all, team_round);
-    const float mean = __fmul_rn(t[0], inv);
+    const float mean = mean_of(t[0], (float)cols, inv);
     s = make_float2(0.0f, 0.0f);
+    // x - mean from here on: x rstd - (mean rstd), with the product rounded, is off by another 2^-24 |mean| rstd, where the difference is exact
+    // for x near the mean (rows of one value become 0)
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[v][i] = add2(x[v][i], splat2(-mean));
       if (col.whole(v)) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-          const float2 d = add2(x[v][i], splat2(-mean));
-          s = fma2(d, d, s);
-        }
+        for (int i = 0; i < P; ++i) s = fma2(x[v][i], x[v][i], s);
       } else if (MODE != ALIGNED && col.some(v)) {
         const uint32_t bits = col.here(col.mine) >> (v * E);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float2 d = add2(x[v][i], splat2(-mean));
-          if (bits >> (2 * i) & 1u) s.x = __fmaf_rn(d.x, d.x, s.x);
-          if (bits >> (2 * i + 1) & 1u) s.y = __fmaf_rn(d.y, d.y, s.y);
+          if (bits >> (2 * i) & 1u) s.x = __fmaf_rn(x[v][i].x, x[v][i].x, s.x);
+          if (bits >> (2 * i + 1) & 1u) s.y = __fmaf_rn(x[v][i].y, x[v][i].y, s.y);
         }
       }
     }
@@ -506,14 +518,14 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, MAX_THR
     row_sum<1, Q>(t, red, round);
     team.sum(t, all, team_round);
     const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(t[0], inv, a.eps)));
-    const float2 rstd2 = splat2(rstd), shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
+    const float2 rstd2 = splat2(rstd);
     if (a.stats && lane == 0 && team.rank == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(mean, rstd);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       float y[E];
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        const float2 h = fma2(x[v][i], rstd2, shift2), q = fma2(h, w[v].pair(i), b[v].pair(i));
+        const float2 h = mul2(x[v][i], rstd2), q = fma2(h, w[v].pair(i), b[v].pair(i));
         y[2 * i] = q.x;
         y[2 * i + 1] = q.y;
       }
@@ -552,7 +564,7 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const __grid_constan
       for (int e = 0; e < 8; ++e) t[0] = __fadd_rn(t[0], x.at(e));
     }
     wide_sum<1>(t, red);
-    const float mean = __fmul_rn(t[0], inv);
+    const float mean = mean_of(t[0], (float)a.cols, inv);
     t[0] = 0.0f;
     for (int64_t c = threadIdx.x * 8; c < a.cols; c += 8192) {
       const int nv = a.cols - c < 8 ? (int)(a.cols - c) : 8;
@@ -631,14 +643,22 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
   const int64_t row_bytes = (int64_t)cols * (BX ? 2 : 4);
   unsigned char* to = static_cast<unsigned char*>(a.dx) + r * row_bytes;
   int round = 0, team_round = 0;
+  // The next row's statistics are on their way too where a round is one row of bf16 or a cluster's.  Timed with and without, bf16: 10000 x 5000 61 and 79 us, x 6000 75 and 90,
+  // 65536 x 768 55 and 60; rounds of two rows, which hide one another's, lose by it (16384 x 4096 84 and 76), float32 ones of no cluster now and then (32768 x
+  // 700 55 and 50, 4096 x 1021 26 and 32).
+  constexpr bool AHEAD = RI == 1 && (BX || CLUSTER);
+  float2 next = make_float2(0.0f, 0.0f);
+  if (AHEAD && r < a.rows) next = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * r));
   for (; r < a.rows; r += step, to += step * row_bytes) {
     float2 st[RI];
     bool here[RI];
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
       here[q] = q == 0 || r + q * each < a.rows;
-      if (here[q]) st[q] = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + q * each)));
+      if (AHEAD) st[q] = next;
+      else if (here[q]) st[q] = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + q * each)));
     }
+    if (AHEAD && r + step < a.rows) next = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * (r + step)));
     wait_copies<S - 2>();
     if (MODE == SHIFT) __syncwarp();   // the next lane's copies are read too
     Vals<BX, E> x[RI][NV], dy[RI][NV];
@@ -668,14 +688,19 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
       float2 s1 = make_float2(0.0f, 0.0f), s2 = s1;
       const float mean = st[q].x, rstd = st[q].y;
       rstd2[q] = splat2(rstd);
-      const float2 shift2 = splat2(-__fmul_rn(mean, rstd));   // h = x rstd - mean rstd
+      if constexpr (!BX) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int i = 0; i < P; ++i) x[q][v].set_pair(i, add2(x[q][v].pair(i), splat2(-mean)));   // also what the next lane stores
+      }
       if (here[q]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           if (col.some(v)) {   // x and dy are 0 where a vector is outside its row; h is not a number there only where all of a row's are
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-              const float2 h = fma2(x[q][v].pair(i), rstd2[q], shift2), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
+              const float2 xm = BX ? add2(x[q][v].pair(i), splat2(-mean)) : x[q][v].pair(i), h = mul2(xm, rstd2[q]), d = dy[q][v].pair(i), g = mul2(d, w[v].pair(i));
               s1 = add2(s1, g);
               s2 = fma2(g, h, s2);
               dw[v][i] = fma2(d, h, dw[v][i]);
@@ -693,10 +718,12 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
       if (!here[q]) continue;
-      // dx = rstd g - rstd m2 h - rstd m1, with h = x rstd - mean rstd
+      // dx = rstd g - rstd m2 h - rstd m1, with h = (x - mean) rstd.  float32 rows have kept x - mean; of bf16 ones, which would take registers for it,
+      // slope times the mean is rounded once with the rest: their spread is at least 2^-8 / sqrt(cols) of their mean, or nothing (and m2 is 0
+      // with h), so that this is off by 2^-16 of rstd g at most.
       const float mean = st[q].x, rstd = st[q].y, m1 = __fmul_rn(t[2 * q], inv), m2 = __fmul_rn(t[2 * q + 1], inv);
       const float slope = -__fmul_rn(__fmul_rn(rstd, rstd), m2);
-      const float2 slope2 = splat2(slope), rest2 = splat2(-__fmaf_rn(rstd, m1, __fmul_rn(slope, mean)));
+      const float2 slope2 = splat2(slope), rest2 = splat2(-(BX ? __fmaf_rn(rstd, m1, __fmul_rn(slope, mean)) : __fmul_rn(rstd, m1)));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float o[E];

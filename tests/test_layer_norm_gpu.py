@@ -234,3 +234,38 @@ def test_wide_rows_between_boundaries(C, R, dtype):
 @pytest.mark.parametrize("R", [296, 297, 400])
 def test_many_wide_rows(R, dtype):
     check(*make(R, 17408, dtype, dtype))
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("C", [1, 8, 100, 500, 768, 1000, 1024, 1030, 4096, 5003, 8192, 10000, 16384, 20000, 32768, 40001, 65536, 70000])
+def test_rows_of_one_value(C, dtype):
+    """Their sum is exact (values of eight bits or fewer), so their mean and every difference from it are: y is the bias and dweight 0."""
+    import advanced_optimizers_b200 as A
+    values = torch.tensor([3.296875, 100.0, -1000.0, 5.0, 0.001953125 * 211, -77.0, 1.0, 2.0 ** 20], dtype=dtype, device="cuda")
+    x = values[:, None].repeat(1, C).requires_grad_()
+    _, w, b, dy = make(8, C, dtype, dtype)
+    w.requires_grad_()
+    for eps in (1e-5, 1e-12):
+        y = A.layer_norm(x, w, b, eps)
+        assert torch.equal(y, b.expand_as(y))
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        ref.close(dx, *ref.LayerNorm(torch.zeros_like(x), w.detach(), b, eps).backward(dy)[0], dtype)
+        assert bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("C", [256, 1000, 1024, 1031, 4096, 5000, 5003, 8192, 12288, 16384])
+def test_a_mean_far_from_zero(C):
+    """Rows of integers around their mean, whose sums are below 2^24: mean and differences are exact, and the results within the bounds of
+    the rows without the mean."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    half = torch.randint(-2, 3, (16, C // 2), generator=g, device="cuda").float()
+    d = torch.cat([half, -half, torch.zeros(16, C % 2, device="cuda")], 1)
+    mean = 1000.0 + torch.arange(16, device="cuda")[:, None]
+    _, w, b, dy = make(16, C, F, F)
+    import advanced_optimizers_b200 as A
+    leaves = [t.requires_grad_() for t in (d + mean, w, b)]
+    o = ref.LayerNorm(d, w.detach(), b.detach(), 1e-5)
+    y = A.layer_norm(*leaves)
+    ref.close(y, *o.forward(), F)
+    for got, want in zip(torch.autograd.grad(y, leaves, dy), o.backward(dy)):
+        ref.close(got, *want, F)
