@@ -718,18 +718,18 @@ __global__ void __launch_bounds__(MAX_THREADS == 32 ? 256 : MAX_THREADS, (MAX_TH
 #pragma unroll
     for (int q = 0; q < RI; ++q) {
       if (!here[q]) continue;
-      // dx = rstd g - rstd m2 h - rstd m1, with h = (x - mean) rstd.  float32 rows have kept x - mean; of bf16 ones, which would take registers for it,
-      // slope times the mean is rounded once with the rest: their spread is at least 2^-8 / sqrt(cols) of their mean, or nothing (and m2 is 0
-      // with h), so that this is off by 2^-16 of rstd g at most.
+      // dx = rstd (g - m1 - m2 rstd (x - mean)); the square of rstd, which may be beyond float32, appears nowhere.  float32 rows have kept x - mean; of
+      // bf16 ones, which would take registers for it, slope times the mean is rounded with the rest: their spread is at least 2^-8 /
+      // sqrt(cols) of their mean, or nothing (and m2 is 0 with h), so that this is off by 2^-15 of rstd g at most.
       const float mean = st[q].x, rstd = st[q].y, m1 = __fmul_rn(t[2 * q], inv), m2 = __fmul_rn(t[2 * q + 1], inv);
-      const float slope = -__fmul_rn(__fmul_rn(rstd, rstd), m2);
-      const float2 slope2 = splat2(slope), rest2 = splat2(-(BX ? __fmaf_rn(rstd, m1, __fmul_rn(slope, mean)) : __fmul_rn(rstd, m1)));
+      const float slope = -__fmul_rn(rstd, m2);
+      const float2 slope2 = splat2(slope), rest2 = splat2(-__fmul_rn(rstd, BX ? __fmaf_rn(slope, mean, m1) : m1));
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float o[E];
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float2 g = mul2(dy[q][v].pair(i), w[v].pair(i)), p = fma2(g, rstd2[q], fma2(x[q][v].pair(i), slope2, rest2));
+          const float2 g = mul2(dy[q][v].pair(i), w[v].pair(i)), p = fma2(fma2(x[q][v].pair(i), slope2, g), rstd2[q], rest2);
           o[2 * i] = p.x;
           o[2 * i + 1] = p.y;
         }

@@ -269,3 +269,27 @@ def test_a_mean_far_from_zero(C):
     ref.close(y, *o.forward(), F)
     for got, want in zip(torch.autograd.grad(y, leaves, dy), o.backward(dy)):
         ref.close(got, *want, F)
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("C", [40, 701, 4096, 5003, 9000])
+def test_tiny_rows_without_eps(C, dtype):
+    """Rows of a spread of 2^-66: 1 / var is beyond float32, rstd, its square root, and the gradient are not.  Half of a row is one value
+    and half another, so that its sums are exact."""
+    import advanced_optimizers_b200 as A
+    x = torch.zeros(9, C, dtype=dtype, device="cuda")
+    x[:, : C // 2], x[:, C // 2 : C // 2 * 2] = 2.0 ** -66, -(2.0 ** -66)
+    _, w, b, dy = make(9, C, dtype, dtype)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    o = ref.LayerNorm(x.detach(), w.detach(), b.detach(), 0.0)
+    # the squares, 2^-132, are denormal numbers of 17 bits: the sum of the squares is exact, its mean off by 2^-18 of it
+    rel = 2.0 ** -18
+    y = A.layer_norm(*leaves, 0.0)
+    want, slack = o.forward()
+    ref.close(y, want, slack + rel * (o.h * o.w).abs(), dtype)
+    (dx, ox), (dw, ow), (db, ob) = o.backward(dy)
+    g = torch.autograd.grad(y, leaves, dy)
+    size = o.rstd * (dy.double() * o.w).abs().amax(1, keepdim=True) * 3   # of dx's terms: |h| is about 1
+    ref.close(g[0], dx, ox + 3 * rel * size, dtype)
+    ref.close(g[1], dw, ow + rel * (dy.double() * o.h).abs().sum(0), dtype)
+    ref.close(g[2], db, ob, dtype)
