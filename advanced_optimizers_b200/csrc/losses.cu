@@ -172,9 +172,9 @@ __device__ __forceinline__ float4 policy_unit(const Policy& q, int64_t r, int64_
       float kl = 0.0f, e1;
       if (a.ref) {
         kl_of(__fsub_rn(ref[i], p[i]), kl, e1);
-        slope[i] = __fmaf_rn(-a.kl_weight, e1, slope[i]);
+        if (a.kl_weight != 0.0f) slope[i] = __fmaf_rn(-a.kl_weight, e1, slope[i]);   // else kl is reported alone, and may be infinite
       }
-      loss = __fadd_rn(loss, __fmaf_rn(a.kl_weight, kl, -gain));
+      loss = __fadd_rn(loss, a.kl_weight != 0.0f ? __fmaf_rn(a.kl_weight, kl, -gain) : -gain);
       kls = __fadd_rn(kls, kl);
       clips += clipped ? 1.0f : 0.0f;
       count += 1.0f;

@@ -438,3 +438,21 @@ def test_hooks_on_saved_tensors_and_other_derivatives():
                      lambda: A.preference_loss(dual(lp)), lambda: A.token_logprobs(dual(x), t)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("dtype", [B, F])
+@pytest.mark.parametrize("R,C", [(3, 40), (3, 41), (70, 3000)])
+def test_a_reference_without_weight_changes_nothing(R, C, dtype):
+    """kl_weight = 0: the KL term is only reported, and where it is beyond float32 neither the loss nor a gradient sees it."""
+    import advanced_optimizers_b200 as A
+    lp, old, refp = policy_case(R, C, dtype)
+    refp[0, 3], refp[1, 0], lp[2, 5] = 100.0, 3e4, -INF
+    adv, mask = rand(R, C, seed=9, dtype=dtype), answers(R, C)
+    mask[0, 3] = mask[1, 0] = mask[2, 5] = True
+    leaf = lp.requires_grad_()
+    for average in ("tokens", "sequences"):
+        plain, seen = A.policy_loss(leaf, old, adv, mask, average=average), A.policy_loss(leaf, old, adv, mask, ref_logprobs=refp, average=average)
+        assert bool(plain.loss.isfinite()) and torch.equal(seen.loss, plain.loss) and torch.equal(seen.clip_fraction, plain.clip_fraction)
+        a, b = (torch.autograd.grad(r.loss, leaf)[0] for r in (plain, seen))
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+        assert not bool(seen.kl.isfinite())
