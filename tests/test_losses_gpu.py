@@ -456,3 +456,16 @@ def test_a_reference_without_weight_changes_nothing(R, C, dtype):
         a, b = (torch.autograd.grad(r.loss, leaf)[0] for r in (plain, seen))
         assert bool(a.isfinite().all()) and torch.equal(a, b)
         assert not bool(seen.kl.isfinite())
+
+
+def test_ratios_beyond_float32():
+    """e^d A is 0 where the advantage is, and a number of its own where e^d alone has left float32."""
+    d = torch.tensor([[87.0, 88.5, 89.0, 95.0, 100.0, 150.0, 176.0, 250.0, 700.0], [88.0, 88.8, 90.0, 100.0, 120.0, 0.1, -3.0, -300.0, 0.0]], device="cuda")
+    old = torch.full_like(d, -1.0)
+    old[0, -2:], old[1, 7] = -800.0, 0.0
+    adv = torch.zeros_like(d)
+    check_policy(old + d, old, adv, None, None)
+    check_policy(old + d, old, adv[:, 0], None, None, average="sequences")
+    adv[1] = torch.tensor([-1.0, -1e-3, -1e-4, -1e-8, -1e-20, -1.0, -1.0, -1.0, -1.0], device="cuda")
+    check_policy(old + d, old, adv, None, None)
+    check_policy(old + d, old, adv, None, old + d, kl_weight=0.1)
