@@ -331,8 +331,7 @@ __device__ __forceinline__ void preference_finish(const Preference& q) {
   const advopt_preference_loss_args& a = q.a;
   __shared__ double red[32][1];
   const float2* units = static_cast<const float2*>(a.work);
-  // the rewards, in double, over the units' sums that they came from; a row's
-  // tokens in its slope
+  // a row's reward, in double, and its tokens (1 for a sum), behind the units' sums
   each_row<2>(2 * a.pairs, q.per_row, [&](double (&s)[2], int64_t u) {
     const float2 v = units[u];
     s[0] += v.x; s[1] += v.y;
@@ -347,7 +346,7 @@ __device__ __forceinline__ void preference_finish(const Preference& q) {
   for (int64_t i = threadIdx.x; i < a.pairs; i += FINISH) {
     const double2 c = rows[i], j = rows[i + a.pairs];
     const double h = c.x - j.x, e = a.smoothing;
-    t[0] += (1.0 - e) * softplus(-h) + e * softplus(h);
+    t[0] += (e < 1.0 ? (1.0 - e) * softplus(-h) : 0.0) + (e > 0.0 ? e * softplus(h) : 0.0);   // infinite without weight: nothing
     if (a.slope) {
       const double k = (double)a.beta / (double)a.pairs * (e - 1.0 / (1.0 + exp(h)));   // -(1 - e) sig(-h) + e sig(h)
       a.slope[i] = (float)(k / c.y);

@@ -469,3 +469,21 @@ def test_ratios_beyond_float32():
     adv[1] = torch.tensor([-1.0, -1e-3, -1e-4, -1e-8, -1e-20, -1.0, -1.0, -1.0, -1.0], device="cuda")
     check_policy(old + d, old, adv, None, None)
     check_policy(old + d, old, adv, None, old + d, kl_weight=0.1)
+
+
+def test_preference_of_impossible_sequences():
+    """A term without weight is left out: a rejected sequence of probability 0 costs nothing, a chosen one is infinite."""
+    import advanced_optimizers_b200 as A
+    lp = torch.full((4, 40), -1.0, device="cuda")
+    lp[2, 7] = -INF   # rejected
+    for e, want in ((0.0, 0.6931471805599453 / 2), (0.1, INF), (1.0, INF)):
+        leaf = lp.clone().requires_grad_()
+        r = A.preference_loss(leaf, label_smoothing=e)
+        assert float(r.loss) == want if want == INF else abs(float(r.loss) - want) <= 2 * ref.U
+        g, = torch.autograd.grad(r.loss, leaf)
+        assert bool(g.isfinite().all()) and (e > 0 or bool((g[[0, 2]] == 0).all()))
+        chosen = torch.cat([lp[2:], lp[:2]]).requires_grad_()   # the other way round
+        r = A.preference_loss(chosen, label_smoothing=1 - e)
+        assert float(r.loss) == want if want == INF else abs(float(r.loss) - want) <= 2 * ref.U
+        g, = torch.autograd.grad(r.loss, chosen)
+        assert bool(g.isfinite().all()) and (e > 0 or bool((g[[0, 2]] == 0).all()))
