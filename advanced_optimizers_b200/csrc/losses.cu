@@ -135,11 +135,9 @@ __device__ __forceinline__ bool beyond(float p, float old, float d, double borde
 
 // e^d adv.  Where e^d is about to leave float32 (88.7) its root is a factor twice; an advantage of 0 stays 0 for any number d.
 __device__ __forceinline__ float gain_of(float d, float adv) {
-  if (d > 88.0f && d < __builtin_huge_valf()) {
-    const float root = expf(__fmul_rn(0.5f, d));
-    return adv == 0.0f ? 0.0f : __fmul_rn(__fmul_rn(root, adv), root);
-  }
-  return __fmul_rn(expf(d), adv);
+  const bool far = d > 88.0f;
+  const float e = expf(far ? __fmul_rn(0.5f, d) : d), gain = __fmul_rn(e, adv);
+  return !far ? gain : adv == 0.0f && d < __builtin_huge_valf() ? 0.0f : __fmul_rn(gain, e);
 }
 
 // ---- the policy loss ----
