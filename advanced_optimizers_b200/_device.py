@@ -111,9 +111,11 @@ class ErrorWord:
     def __init__(self, message="an earlier kernel reported an error"):
         self.message = message
         self.word = self.view = None
+        self.devices = set()   # whose kernels may set it
         self.lock = threading.Lock()
 
-    def pointer(self) -> int:
+    def pointer(self, device=None) -> int:
+        """For a launch on `device`."""
         if self.word is None:
             if torch.cuda.is_current_stream_capturing():
                 return 0   # no allocation of pinned memory during a capture
@@ -124,6 +126,8 @@ class ErrorWord:
                     self.word = word
         if self.view[0]:
             self.raise_()
+        if device is not None:
+            self.devices.add(device)
         return self.word.data_ptr()
 
     def raise_(self):
@@ -131,8 +135,9 @@ class ErrorWord:
         raise L.AdvOptError(self.message)
 
     def check(self):
-        """Waits for the GPU and raises what it reported."""
-        torch.cuda.synchronize()
+        """Waits for the GPUs that may report, whichever is the current one, and raises what they reported."""
+        for device in list(self.devices):
+            torch.cuda.synchronize(device)
         if self.word is not None and self.view[0]:
             self.raise_()
 

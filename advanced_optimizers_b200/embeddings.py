@@ -19,7 +19,7 @@ INDEX_ERRORS = ErrorWord("an earlier embedding or token_logprobs call met an ind
 
 
 def check_index_errors():
-    """Waits for the GPU and raises if an `embedding` or `token_logprobs` call
+    """Waits for the GPUs of earlier calls and raises if an `embedding` or `token_logprobs` call
     met an index outside its table (otherwise the process's next such call
     raises, on whichever thread or device).  Calls captured before the
     process's first eager one have no word to report to."""
@@ -43,7 +43,7 @@ def _gather(ids, weight, scale, dtype):
     y = weight.new_empty(*ids.shape, C)
     with on_device(weight.device):
         rc = L.lib().advopt_embedding(_FORWARD.pack(
-            y.data_ptr(), w.data_ptr(), ids.data_ptr(), INDEX_ERRORS.pointer(), ld, ids.numel(), V, C, dtype, ids.element_size(), scale, 0),
+            y.data_ptr(), w.data_ptr(), ids.data_ptr(), INDEX_ERRORS.pointer(weight.device), ld, ids.numel(), V, C, dtype, ids.element_size(), scale, 0),
             raw_stream(weight.device))
     if rc:
         L.check(rc, "advopt_embedding")

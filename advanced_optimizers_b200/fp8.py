@@ -31,7 +31,7 @@ _ERR = ErrorWord("an earlier fp8 product gave up waiting for its copies (bounded
 
 
 def check_fp8_errors():
-    """Waits for the GPU and raises if an fp8 product's bounded wait gave up (a
+    """Waits for the GPUs of earlier products and raises if an fp8 product's bounded wait gave up (a
     guard that is not expected to fire; otherwise the process's next product
     raises, on whichever thread or device).  Products captured before the
     process's first eager one have no word to report to."""
@@ -200,7 +200,7 @@ def _product(a, b, k, a_code, b_code, a_square, b_square, out, bias=None, residu
     m, n = out.shape
     rc = L.lib().advopt_fp8_gemm(_GEMM.pack(
         *a, *b, out.data_ptr(), n, 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), n,
-        m, n, k, a_code, b_code, a_square, b_square, dtype_code(out.dtype), variant, _ERR.pointer(), *drop),
+        m, n, k, a_code, b_code, a_square, b_square, dtype_code(out.dtype), variant, _ERR.pointer(out.device), *drop),
         raw_stream(out.device))
     if rc:
         L.check(rc, "advopt_fp8_gemm")

@@ -61,7 +61,7 @@ def _token_logprobs(logits, tokens, temperature, ignore, dtype, keep):
     size = _logprobs_work(R, logits.shape[-1], dtype)
     work = logits.new_empty(size, dtype=torch.uint8) if size else None
     with on_device(logits.device):
-        x, args = _logprobs_args(out.data_ptr(), _ptr(stats), _ptr(work), logits, tokens, temperature, ignore, dtype, INDEX_ERRORS.pointer())
+        x, args = _logprobs_args(out.data_ptr(), _ptr(stats), _ptr(work), logits, tokens, temperature, ignore, dtype, INDEX_ERRORS.pointer(logits.device))
         rc = L.lib().advopt_token_logprobs(args, raw_stream(logits.device))
     if rc:
         L.check(rc, "advopt_token_logprobs")

@@ -206,3 +206,35 @@ def test_rows_that_are_read_as_they_lie():
         for r in range(t[..., 0].numel()):
             at = r // inner * outer + r % inner * pitch
             assert torch.equal(got.as_strided((t.shape[-1],), (1,), got.storage_offset() + at), t.reshape(-1, t.shape[-1])[r])
+
+
+def test_every_gpu_that_may_report_an_error_is_waited_for(monkeypatch):
+    """Two GPUs' calls share a word: a check with either of them current waits for both."""
+    import numpy as np
+    from advanced_optimizers_b200 import _device, embeddings, fp8
+
+    class Word:
+        array = np.zeros(1, dtype=np.int32)
+        numpy = lambda self: self.array  # noqa: E731
+        data_ptr = lambda self: self.array.ctypes.data  # noqa: E731
+
+    waited = []
+
+    def synchronize(device=None):
+        waited.append(device)
+        if device == torch.device("cuda", 1):
+            Word.array[0] = 1   # its kernel reports while it is waited for
+
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: Word())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "synchronize", synchronize)
+    for module, name, check in ((embeddings, "INDEX_ERRORS", embeddings.check_index_errors), (fp8, "_ERR", fp8.check_fp8_errors)):
+        word = _device.ErrorWord()
+        monkeypatch.setattr(module, name, word)
+        check()   # nothing to wait for
+        for index in (0, 1, 0):
+            assert word.pointer(torch.device("cuda", index)) == Word.array.ctypes.data
+        del waited[:]
+        with pytest.raises(_device.L.AdvOptError):
+            check()
+        assert set(waited) == {torch.device("cuda", 0), torch.device("cuda", 1)} and Word.array[0] == 0
