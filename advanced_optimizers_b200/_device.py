@@ -4,6 +4,7 @@ for device memory and streams."""
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import threading
 
 import numpy as np
@@ -28,6 +29,11 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.bfloat16:
         return 1
     raise NotImplementedError(f"parameter dtype {dt} is not supported (float32 and bfloat16 are)")
+
+
+def as_float32(v: float) -> float:
+    """v as the kernels get it; infinite beyond float32."""
+    return ctypes.c_float(v).value
 
 
 def refuse_tangents(what: str, *tensors):

@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._device import ErrorWord, dtype_code, on_device, raw_stream, refuse_tangents, rows_of, saved
+from ._device import ErrorWord, as_float32, dtype_code, on_device, raw_stream, refuse_tangents, rows_of, saved
 
 # advopt_embedding_args, advopt_embedding_grad_args
 _FORWARD = struct.Struct("<QQQQqqqqiifi")
@@ -107,8 +107,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, pa
     dtype = dtype_code(weight.dtype)
     V, C = weight.shape
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"embedding: the scale must be finite, got {scale}")
+    if not math.isfinite(as_float32(scale)):
+        raise ValueError(f"embedding: the scale must be finite in float32, got {scale}")
     if max(V, C, ids.numel()) >= 1 << 31:
         raise ValueError("embedding: fewer than 2^31 ids, rows and columns")
     padding = -1

@@ -9,7 +9,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._device import dtype_code, empty_as, on_device, raw_stream, refuse_tangents, rows_of, saved
+from ._device import as_float32, dtype_code, empty_as, on_device, raw_stream, refuse_tangents, rows_of, saved
 
 # advopt_layer_norm_args, advopt_layer_norm_grad_args
 _FORWARD = struct.Struct("<QQQQQqqqfiii")
@@ -110,8 +110,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"layer_norm: weight and bias share a dtype, got {weight.dtype} and {bias.dtype}")
     eps = float(eps)
-    if not (eps >= 0 and math.isfinite(eps)):
-        raise ValueError(f"layer_norm: eps must be finite and not negative, got {eps}")
+    eps32 = as_float32(eps)
+    if not (eps >= 0 and math.isfinite(eps32) and (eps32 > 0 or eps == 0)):
+        raise ValueError(f"layer_norm: eps must be 0 or a positive number of float32, got {eps}")
     if C == 0 or C >= 1 << 31:
         raise ValueError(f"layer_norm: rows of 1 to 2^31 - 1 elements, got {C}")
     refuse_tangents("layer_norm", x, weight, bias)

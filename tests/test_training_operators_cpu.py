@@ -238,3 +238,15 @@ def test_every_gpu_that_may_report_an_error_is_waited_for(monkeypatch):
         with pytest.raises(_device.L.AdvOptError):
             check()
         assert set(waited) == {torch.device("cuda", 0), torch.device("cuda", 1)} and Word.array[0] == 0
+
+
+def test_numbers_that_float32_does_not_hold_are_refused(monkeypatch):
+    import advanced_optimizers_b200 as A
+    _on_gpu(monkeypatch)
+    x, ids = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    for scale in (1e39, -1e39, 3.4028236e38):
+        with pytest.raises(ValueError, match="scale"):
+            A.embedding(ids, x, scale=scale)
+    for eps in (1e39, 1e-50):   # the second would act as 0
+        with pytest.raises(ValueError, match="eps"):
+            A.layer_norm(x, eps=eps)
