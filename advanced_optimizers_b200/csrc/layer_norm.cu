@@ -904,8 +904,6 @@ __global__ void __launch_bounds__(FINISH_WARPS * 32) finish_kernel(void* dweight
 }
 
 // ---- variants ----
-constexpr int64_t MOST = 8192;      // columns that a CTA's registers hold with their sums (a few hundred fewer of unaligned rows)
-constexpr int64_t MOST_OF_CLUSTER = MOST * MOST_CTAS;
 constexpr int64_t SMS = 148;
 
 // Vectors per thread, and threads and CTAs of a row: a warp's where it holds
@@ -926,9 +924,12 @@ inline Variant variant_of(int64_t cols, bool bf16, int mode, int most, int threa
   const int64_t ctas = warps <= 8 * MOST_CTAS ? ceil_div(warps, 8) : MOST_CTAS, each = ceil_div(warps, ctas) * 32;
   return each <= 512 ? Variant{2 * one, (int)each, (int)ctas} : Variant{2 * one, 0, 0};
 }
-// CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows at least where that leaves one for each SM.
-inline int64_t grad_ctas(int64_t rows, int64_t cols) {
-  int64_t units = cols <= 1024 ? ceil_div(rows, WARPS) : rows;
+// The gradient's: bf16 rows of four vectors a lane would leave an SM eight warps.
+inline Variant grad_variant_of(int64_t cols, bool bf16, int mode) { return variant_of(cols, bf16, mode, bf16 ? 3 : 4, 512); }
+// CTAs of the gradient kernel at most: each leaves a row of partial sums, so a CTA takes four rows (a row a warp: rounds of eight) at least where
+// that leaves one for each SM.
+inline int64_t grad_ctas(int64_t rows, bool warp_rows) {
+  int64_t units = warp_rows ? ceil_div(rows, WARPS) : rows;
   if (units < 8) units = rows < 8 ? rows : 8;   // one for each place that a row may begin at
   const int64_t few = ceil_div(units, 4) > SMS ? ceil_div(units, 4) : SMS, most = 8 * SMS;
   const int64_t n = few < most ? few : most;
@@ -937,6 +938,10 @@ inline int64_t grad_ctas(int64_t rows, int64_t cols) {
 // Clusters of the gradient kernel at most: of three CTAs or more, two an SM.
 inline int64_t grad_clusters(int64_t rows) { return rows < 2 * SMS / 3 ? rows : 2 * SMS / 3; }
 inline int64_t wide_parts(int64_t rows) { return rows < 8 * 32 ? ceil_div(rows, 8) : 32; }
+// Rows of partial sums of a variant at most.
+inline int64_t parts_of(int64_t rows, const Variant& v) {
+  return v.ctas == 0 ? wide_parts(rows) : v.ctas > 1 ? grad_clusters(rows) : grad_ctas(rows, v.threads == 32);
+}
 
 // Launches a persistent kernel with as many CTAs (clusters of `ctas`) as fit the SMs, `most` at most; their number, or -1.
 template <auto KERNEL, class Arg>
@@ -1023,7 +1028,7 @@ template <bool BX, bool BW, int NV, int MAX_THREADS, bool CLUSTER = false>
 int64_t grad_variant(const advopt_layer_norm_grad_args& a, const Variant& v, int mode, int wvec, cudaStream_t s) {
   constexpr bool WARP = MAX_THREADS == 32;
   const int threads = WARP ? WARPS * 32 : v.threads;
-  const int64_t ctas = WARP && mode != PHASE ? ceil_div(a.rows, WARPS) : a.rows, parts = CLUSTER ? grad_clusters(a.rows) : grad_ctas(a.rows, a.cols);
+  const int64_t ctas = WARP && mode != PHASE ? ceil_div(a.rows, WARPS) : a.rows, parts = parts_of(a.rows, v);
   const int64_t most = ctas < parts ? ctas : parts;
   const auto bytes = [&](int rows) { return 2 * rows * Rows<BX, NV, ALIGNED, grad_stages(BX)>::slots_of(threads) * 16; };
   if (mode == ALIGNED) return launch<grad_kernel<BX, BW, NV, MAX_THREADS, ALIGNED, CLUSTER>>(a, wvec, threads, v.ctas, bytes(grad_rows(BX, MAX_THREADS, ALIGNED)), most, false, s);
@@ -1042,7 +1047,7 @@ int grad(const advopt_layer_norm_grad_args& a, cudaStream_t s) {
   const bool vec = mode == ALIGNED;
   const int wvec = aligned16(a.weight);
   constexpr int N = BX ? 1 : 2;
-  const Variant v = variant_of(a.cols, BX, mode, BX ? 3 : 4, 512);   // bf16 rows of four vectors a lane would leave an SM eight warps
+  const Variant v = grad_variant_of(a.cols, BX, mode);
   int64_t parts = 0;
   if (v.ctas == 0) {
     parts = wide_parts(a.rows);
@@ -1098,7 +1103,13 @@ extern "C" int advopt_layer_norm(const advopt_layer_norm_args* a, void* stream) 
 
 extern "C" int64_t advopt_layer_norm_grad_work(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (cols > ln::MOST_OF_CLUSTER ? ln::wide_parts(rows) : cols > ln::MOST ? ln::grad_clusters(rows) : ln::grad_ctas(rows, cols)) * 2 * cols * 4;
+  int64_t parts = 0;   // whatever the rows' type and alignment
+  for (const bool bf16 : {false, true})
+    for (const int mode : {ln::ALIGNED, ln::PHASE, ln::SHIFT}) {
+      const int64_t n = ln::parts_of(rows, ln::grad_variant_of(cols, bf16, mode));
+      parts = parts < n ? n : parts;
+    }
+  return parts * 2 * cols * 4;
 }
 
 extern "C" int advopt_layer_norm_grad(const advopt_layer_norm_grad_args* a, void* stream) {

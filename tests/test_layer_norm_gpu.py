@@ -293,3 +293,11 @@ def test_tiny_rows_without_eps(C, dtype):
     ref.close(g[0], dx, ox + 3 * rel * size, dtype)
     ref.close(g[1], dw, ow + rel * (dy.double() * o.h).abs().sum(0), dtype)
     ref.close(g[2], db, ob, dtype)
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(B, B), (B, F), (F, F)])
+@pytest.mark.parametrize("R,C", [(256, 1024), (1000, 776), (4097, 1024), (515, 1001), (600, 713), (300, 1023)])
+def test_rows_of_up_to_1024_columns_that_a_cta_takes(R, C, dtype, wdtype):
+    check(*make(R, C, dtype, wdtype))
+    x, w, b, dy = make(R, C + 1, dtype, wdtype)
+    check(x[:, 1:], w[1:], b[1:], dy[:, :-1])

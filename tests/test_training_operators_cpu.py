@@ -250,3 +250,17 @@ def test_numbers_that_float32_does_not_hold_are_refused(monkeypatch):
     for eps in (1e39, 1e-50):   # the second would act as 0
         with pytest.raises(ValueError, match="eps"):
             A.layer_norm(x, eps=eps)
+
+
+def test_layer_norm_s_sums_have_room_for_every_way_to_take_a_row():
+    """A row of partial sums for each CTA: eight rows a CTA where warps take them, whatever their type and alignment, else one, until there
+    is a CTA for each SM; then four times as many rows; never more than 1184."""
+    from advanced_optimizers_b200 import _lib as L
+    parts = lambda rows, cols: L.lib().advopt_layer_norm_grad_work(rows, cols) / (2 * cols * 4)  # noqa: E731
+    for cols in (769, 776, 1000, 1023, 1024, 1032, 2048):
+        assert [parts(r, cols) for r in (1, 7, 100, 148, 500, 1000, 4096, 100000)] == [1, 7, 100, 148, 148, 250, 1024, 1184]
+    for cols in (1, 500, 700):
+        assert [parts(r, cols) for r in (1, 7, 100, 1000, 4096, 100000)] == [1, 7, 13, 125, 148, 1184]
+    for cols in (8193, 16384, 65536):
+        assert [parts(r, cols) for r in (1, 98, 5000)] == [1, 98, 98]
+    assert [parts(r, 70001) for r in (1, 100, 5000)] == [1, 13, 32]
