@@ -223,3 +223,35 @@ def test_index_error_of_a_captured_call_is_reported():
     with pytest.raises(A.embeddings.L.AdvOptError, match="outside its table"):
         A.check_index_errors()
     assert bool(y[3].isnan().all())
+
+
+@pytest.mark.parametrize("S,T,V,C,H", [(4, 17, 61, 48, 96), (6, 130, 1003, 200, 256)])
+def test_a_model_s_policy_gradients_near_its_reference(S, T, V, C, H):
+    """As above, with old log-probabilities near the model's own, as a trainer has them, so that every term is a number; none of the ratios is
+    within 0.08 of a border of the clipping (log 1.2 and log 0.8)."""
+    p = {k: v.requires_grad_() for k, v in weights(V, C, H).items()}
+    q = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    ids, mask, _, adv = batch(S, T, V)
+    logits = plain_model(q, ids)
+    lp = torch.log_softmax(logits.detach()[:, :-1], -1).gather(-1, ids[:, 1:, None])[..., 0]
+    apart = torch.tensor([-0.5, -0.1, 0.0, 0.1, 0.3], dtype=D, device="cuda")[torch.arange(S * (T - 1), device="cuda") % 5].view(S, T - 1)
+    old = torch.cat([torch.zeros(S, 1, dtype=D, device="cuda"), lp - apart], 1).float()
+    want = plain_loss(logits, ids, mask, old, adv, "policy")
+    loss = loss_of(model(p, ids), ids, mask, old, adv, "policy")
+    for k, g, w in zip(p, torch.autograd.grad(loss, list(p.values())), torch.autograd.grad(want, list(q.values()))):
+        assert float(w.norm()) > 0 and float((g.double() - w).norm()) <= 1e-4 * float(w.norm()), k
+
+
+@pytest.mark.parametrize("S,T,V", [(4, 17, 61), (3, 9, 1003), (40, 30, 5003)])
+def test_shifted_tokens_of_whole_logits(S, T, V):
+    """The last place ignored: the same log-probabilities and gradients as of the logits without it, and zeros there."""
+    import advanced_optimizers_b200 as A
+    ids, mask, _, _ = batch(S, T, V)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randn(S, T, V, generator=g, device="cuda", dtype=B).requires_grad_()
+    tokens = torch.full_like(ids, IGNORE)
+    tokens[:, :-1] = torch.where(mask[:, 1:], ids[:, 1:], IGNORE)
+    d = torch.randn(S, T, generator=g, device="cuda")
+    lp, cut = A.token_logprobs(logits, tokens), A.token_logprobs(logits[:, :-1], tokens[:, :-1])
+    assert torch.equal(lp[:, :-1], cut) and bool((lp[:, -1] == 0).all())
+    assert torch.equal(torch.autograd.grad(lp, logits, d)[0], torch.autograd.grad(cut, logits, d[:, :-1].contiguous())[0])
