@@ -111,7 +111,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
 
     logits [..., V] float32 or bfloat16, tokens [...] int32 or int64, on one
     CUDA device.  Logits with up to two leading dimensions are read as they lie
-    where a row's elements are consecutive (so `logits[:, :-1]` is not copied).
+    where a row's elements are consecutive (so `logits[:, :-1]` is not copied;
+    torch's gradient of that slice is, and shifted tokens with the last place
+    ignored need neither).
     Sums are float32; infinities and NaN act as in the formula (a logit of -inf
     has probability 0).  A token `ignore_index` gives 0 and its row is neither
     read nor given a gradient.  In the backward pass rows whose incoming
@@ -252,6 +254,7 @@ def policy_loss(logprobs: torch.Tensor, old_logprobs: torch.Tensor, advantages: 
 
       loss = mean of -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_weight (exp(q) - q - 1)
 
+    kl_weight   0: the KL term is only reported, whatever its size
     average     "tokens": the mean over all tokens; "sequences": the mean over
                 the sequences with a token of the means over their tokens.  With
                 no token at all the loss is 0.
