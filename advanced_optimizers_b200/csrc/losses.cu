@@ -133,11 +133,10 @@ __device__ __forceinline__ bool beyond(float p, float old, float d, double borde
   return ABOVE ? e > border : e < border;
 }
 
-// e^d adv.  Where e^d is about to leave float32 (88.7) its root is a factor twice; an advantage of 0 stays 0 for any number d.
-__device__ __forceinline__ float gain_of(float d, float adv) {
-  const bool far = d > 88.0f;
-  const float e = expf(far ? __fmul_rn(0.5f, d) : d), gain = __fmul_rn(e, adv);
-  return !far ? gain : adv == 0.0f && d < __builtin_huge_valf() ? 0.0f : __fmul_rn(gain, e);
+// e^d adv where e^d is about to leave float32 (e^88.7) or has: its root is a factor twice; an advantage of 0 stays 0 for any number d.
+__device__ __forceinline__ float far_gain(float d, float adv) {
+  const float root = expf(__fmul_rn(0.5f, d));
+  return adv == 0.0f && d < __builtin_huge_valf() ? 0.0f : __fmul_rn(__fmul_rn(root, adv), root);
 }
 
 // ---- the policy loss ----
@@ -174,7 +173,8 @@ __device__ __forceinline__ float4 policy_unit(const Policy& q, int64_t r, int64_
       const float d = __fsub_rn(p[i], old[i]);
       const bool clipped = adv[i] > 0.0f ? beyond<true>(p[i], old[i], d, a.log_high, q.high32)
                                          : adv[i] < 0.0f && beyond<false>(p[i], old[i], d, a.log_low, q.low32);
-      const float gain = clipped ? __fmul_rn(adv[i] > 0.0f ? high : low, adv[i]) : gain_of(d, adv[i]);
+      const float gain = d > 88.0f && !clipped ? far_gain(d, adv[i])   // a branch that hardly any warp takes: selects cost 29.7 us where it costs 28.4
+                                               : __fmul_rn(clipped ? adv[i] > 0.0f ? high : low : expf(d), adv[i]);
       slope[i] = clipped ? 0.0f : -gain;
       float kl = 0.0f, e1;
       if (a.ref) {
